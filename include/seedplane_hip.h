@@ -383,6 +383,92 @@ int sp_library_release(void);
 int sp_op_draft_link(const int32_t *tokens_dev, int32_t n_branches, int32_t level, int32_t *canon_dev,
                      uint64_t *masks_dev, int32_t *rows_dev, void *hip_stream);
 
+/* ---------------------------------------------------------------- paged K/V cache: rotation, append, attention
+ * No counterpart in the reference, whose cache is one tensor per sequence (qwen_engine.py:18-29) and whose rotary embedding
+ * is the half layout without scaling (qwen_engine.py:94-103); sp_op_rotate and sp_op_paged_append generalise its _rope and
+ * cache copy (qwen_engine.py:121-125), sp_op_paged_attention its attention (qwen_engine.py:126-135).
+ * Strides are in elements of their array.  All calls are asynchronous on hip_stream, allocate nothing, keep no state (the plan
+ * is the caller's) and may be captured into a graph. */
+enum { SP_DT_F32 = 0, SP_DT_F16 = 1, SP_DT_BF16 = 2, SP_DT_E4M3 = 3 /* OCP e4m3, no infinities, largest 448 */ };
+enum { SP_ROPE_HALF = 0 /* pairs (j, j + rot_dim/2) */, SP_ROPE_INTERLEAVED = 1 /* pairs (2j, 2j + 1) */ };
+
+typedef struct sp_rotary {
+    const double *inv_freq_dev;   /* device [rot_dim / 2]: radians per position of each pair                       */
+    int32_t rot_dim;              /* the first rot_dim values of a head rotate (even), the rest passes through     */
+    int32_t layout;               /* SP_ROPE_*                                                                     */
+    float factor;                 /* on cosines and sines (1; the attention factor of a scaled table)              */
+    int32_t reserved0;
+} sp_rotary;
+
+/* out[r][h] = x[r][h] rotated at position pos_dev[r] (int32, any sign: negated positions undo a rotation of factor 1 and are
+ * its gradient).  dtype (SP_DT_F32 / F16 / BF16) is that of x and out, whose values of a head lie side by side: row r, head h
+ * starts at r * row + h * head.  out may be x itself (same strides); otherwise they must not overlap. */
+int sp_op_rotate(const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t n_heads, int32_t head_dim, const void *x_dev,
+                 int64_t x_row, int64_t x_head, void *out_dev, int64_t out_row, int64_t out_head, const int32_t *pos_dev,
+                 void *hip_stream);
+
+/* One layer's paged cache: pages [n_pages] of [n_kv_heads][page_size][head_dim] values, page_stride elements apart (the same
+ * for keys and values).  A sequence's position p lies in row p % page_size of page table[seq][p / page_size].  e4m3 caches hold
+ * value / scale with a positive fp32 scale per K/V head, for keys and for values. */
+typedef struct sp_paged_kv {
+    void *k_dev, *v_dev;
+    const float *k_scale_dev, *v_scale_dev;   /* device [n_kv_heads], SP_DT_E4M3 only (NULL otherwise) */
+    int64_t page_stride;
+    int32_t dtype;                            /* SP_DT_F16, SP_DT_BF16 or SP_DT_E4M3 */
+    int32_t n_pages, page_size, n_kv_heads, head_dim;
+    int32_t reserved0;
+} sp_paged_kv;
+
+/* Appends n_rows new tokens: row r's keys (rotated at pos_dev[r] unless rotary is NULL) and values go to position at_dev[r] of
+ * sequence seq_dev[r], and with q_dev its n_heads query heads are rotated into q_out_dev (dtype q_out_dtype; q_dev itself
+ * with the same type and strides, or memory apart from the inputs).  table_dev is int32 [n_seq][max_pages].  A row whose seq, position or page entry is out of range (e.g. seq -1:
+ * padding) writes nothing, not its queries either.  dtype: of q, k and v (F32, F16 or BF16).  Values too large for an e4m3
+ * cache saturate at 448 scales, NaN stays NaN.  Two rows of one call must not name the same position of a sequence. */
+int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t n_heads,
+                       const void *q_dev, int64_t q_row, int64_t q_head, const void *k_dev, int64_t k_row, int64_t k_head,
+                       const void *v_dev, int64_t v_row, int64_t v_head, const int32_t *pos_dev, const int32_t *seq_dev,
+                       const int32_t *at_dev, const int32_t *table_dev, int32_t n_seq, int32_t max_pages, void *q_out_dev,
+                       int32_t q_out_dtype, int64_t q_out_row, int64_t q_out_head, void *hip_stream);
+
+/* The plan of a batch's attention, kept by the caller over the layers of a step: which block reads which keys for which
+ * queries.  max_rows: most query rows (tokens) of a batch, max_seqs: most sequences.  head_dim 64 or 128, at most 32 query
+ * heads per K/V head.  A plan belongs to the device that is current at its creation; calls on one plan must not overlap. */
+typedef struct sp_attn_plan sp_attn_plan;
+int sp_attn_plan_create(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_rows, int32_t max_seqs,
+                        sp_attn_plan **out);
+/* Waits for the plan's own copies; the caller has waited for the calls that use it. */
+void sp_attn_plan_destroy(sp_attn_plan *plan);
+/* Lengths of the next batch (host arrays): sequence s has q_len[s] query rows, the last of its kv_len[s] cached positions:
+ * its query i sees positions 0 .. kv_len[s] - q_len[s] + i (none where that is negative: the output row is zeros).  Sequences
+ * in order; their query rows lie one after the other.  Groups (n_groups 0: none) are runs of group_size sequences whose page
+ * tables name the same rows for positions 0 .. group_shared - 1, which are then read once for the group (through the table of
+ * its first sequence with queries); of a group whose first query stands earlier, only the positions before that query.  The
+ * tables are copied to the device on hip_stream: later sp_op_paged_attention calls must follow on it.  SP_ESTATE in a stream
+ * capture; a captured sp_op_paged_attention reads the tables of the last set before each replay. */
+int sp_attn_plan_set(sp_attn_plan *plan, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len, int32_t n_groups,
+                     const int32_t *group_size, const int32_t *group_shared, void *hip_stream);
+/* Host only, for inspection: the items of one kind (0, 1, 2: row tiles of 32, 64, 128 rows) that sp_attn_plan_set makes of these
+ * lengths, as 8 int32 each: first token, tokens, K/V head, sequence, first position, end, position seen by the first token (2^30:
+ * all), first record or -1; and per token 8 int32: base, parts, tile and index of its records of the shared and of its own
+ * positions (pairs).  items and token_recs may be NULL. */
+int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len,
+                       int32_t n_groups, const int32_t *group_size, const int32_t *group_shared, int32_t kind, int32_t capacity,
+                       int32_t *items, int32_t *n_items, int32_t *token_recs, int64_t *n_records);
+/* Bytes of sp_op_paged_attention's workspace, for every batch within max_rows. */
+size_t sp_attn_plan_workspace(const sp_attn_plan *plan);
+
+/* out = softmax(scale q k^T) v over the positions each query sees, for the batch of the plan's last set.  q and out: n_rows
+ * rows of the plan's n_heads heads, dtype SP_DT_F16 or SP_DT_BF16 (a cache of the same type, or e4m3), 16 / 8 byte aligned rows
+ * and heads; rows behind the plan's last are left as they are.  lse_dev (may be NULL): fp32 [n_rows][n_heads], the natural
+ * logarithm of each row's sum of exponentials (-infinity for a row that sees nothing).  table_dev: int32 [n_seq][max_pages];
+ * entries of positions at or behind a sequence's length are not read, an entry outside [0, n_pages) hides its positions.  What
+ * the pool holds outside the positions read does not matter (NaN included).  scale must be positive.  workspace_dev: see
+ * above; calls that overlap (other streams, graphs replayed side by side) need a workspace each. */
+int sp_op_paged_attention(const sp_attn_plan *plan, const sp_paged_kv *kv, int32_t dtype, int32_t n_rows, const void *q_dev,
+                          int64_t q_row, int64_t q_head, const int32_t *table_dev, int32_t n_seq, int32_t max_pages, float scale,
+                          void *out_dev, int64_t out_row, int64_t out_head, float *lse_dev, void *workspace_dev,
+                          void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,8 @@ SP_FMT_F32, SP_FMT_F16, SP_FMT_Q8, SP_FMT_Q4 = range(4)
  SP_T_GATE_UP, SP_T_DOWN) = range(10)
 SP_F_LOGITS, SP_F_ARGMAX, SP_F_GRAPH, SP_F_PERSISTENT, SP_F_UNFUSED, SP_F_FEED, SP_F_CHAIN = 1, 2, 4, 8, 16, 32, 64
 SP_F_DEVCOLS = 128
+SP_DT_F32, SP_DT_F16, SP_DT_BF16, SP_DT_E4M3 = range(4)
+SP_ROPE_HALF, SP_ROPE_INTERLEAVED = 0, 1
 
 # Every function the header declares, with its ctypes signature.
 c_int, c_int32, c_size_t, c_uint64, c_float = ctypes.c_int, ctypes.c_int32, ctypes.c_size_t, ctypes.c_uint64, ctypes.c_float
@@ -39,6 +41,17 @@ class Token(ctypes.Structure):
 
 
 assert ctypes.sizeof(Token) == 40
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [('inv_freq', c_void_p), ('rot_dim', c_int32), ('layout', c_int32), ('factor', c_float), ('reserved0', c_int32)]
+
+
+class PagedKVDesc(ctypes.Structure):
+    _fields_ = [('k', c_void_p), ('v', c_void_p), ('k_scale', c_void_p), ('v_scale', c_void_p), ('page_stride', c_int64),
+                ('dtype', c_int32), ('n_pages', c_int32), ('page_size', c_int32), ('n_kv_heads', c_int32), ('head_dim', c_int32),
+                ('reserved0', c_int32)]
+
 
 # the same layout as a numpy structured dtype (columns built in bulk)
 TOKEN_DTYPE = np.dtype([(name, np.int32 if ctype is c_int32 else np.uint64) for name, ctype in Token._fields_])
@@ -99,6 +112,19 @@ SIGNATURES = {
                                        c_int32, c_void_p, c_void_p, c_void_p]),
     'sp_op_draft_link': (c_int, [c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
     'sp_engine_set_device_columns': (c_int, [c_void_p, c_void_p, c_void_p]),
+    'sp_op_rotate': (c_int, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                             c_void_p, c_void_p]),
+    'sp_op_paged_append': (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                   c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
+                                   c_void_p, c_int32, c_int64, c_int64, c_void_p]),
+    'sp_attn_plan_create': (c_int, [c_int32, c_int32, c_int32, c_int32, c_int32, ctypes.POINTER(c_void_p)]),
+    'sp_attn_plan_destroy': (None, [c_void_p]),
+    'sp_attn_plan_set': (c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
+    'sp_attn_plan_items': (c_int, [c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_int32,
+                                   c_void_p, c_void_p, c_void_p, c_void_p]),
+    'sp_attn_plan_workspace': (c_size_t, [c_void_p]),
+    'sp_op_paged_attention': (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_int32,
+                                      c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     'sp_library_release': (c_int, []),
     'sp_engine_kv_layer': (c_int, [c_void_p, c_int32, ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p)]),
 }

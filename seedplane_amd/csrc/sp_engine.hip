@@ -26,6 +26,7 @@
 #include "sp_decode1.h"
 #include "sp_gemv.h"
 #include "sp_gemv1.h"
+#include "sp_host.h"
 #include "sp_order.h"
 #include "sp_pack.h"
 #include "sp_sample.h"
@@ -34,39 +35,6 @@
 namespace {
 
 thread_local std::string g_err;
-
-struct Fail {
-    int code;
-    std::string msg;
-};
-
-#define HIPCHK(expr)                                                                                     \
-    do {                                                                                                 \
-        hipError_t _e = (expr);                                                                          \
-        if (_e != hipSuccess)                                                                            \
-            throw Fail{SP_EHIP, std::string(#expr) + ": " + hipGetErrorString(_e)};                      \
-    } while (0)
-
-inline void require(bool ok, int code, const std::string &msg) {
-    if (!ok) throw Fail{code, msg};
-}
-// A literal message builds its string only on failure (per-column checks run on every call).
-inline void require(bool ok, int code, const char *msg) {
-    if (!ok) throw Fail{code, msg};
-}
-
-template <class T>
-T *dev_alloc(size_t count, uint64_t *acct = nullptr) {
-    void *p = nullptr;
-    if (count == 0) count = 1;
-    hipError_t e = hipMalloc(&p, count * sizeof(T));
-    if (e != hipSuccess) throw Fail{SP_ENOMEM, "hipMalloc of " + std::to_string(count * sizeof(T)) + " bytes failed: " + hipGetErrorString(e)};
-    if (acct) *acct += count * sizeof(T);
-    return (T *)p;
-}
-inline void dev_free(void *p) {
-    if (p) (void)hipFree(p);
-}
 
 // ------------------------------------------------------------------------------------------- packed matrix on HBM
 struct DevMat {
@@ -1502,6 +1470,8 @@ int guarded(sp_engine *e, F &&fn) {
     }
 }
 }  // namespace
+
+std::string &sp_call_error() { return g_err; }
 
 extern "C" {
 

@@ -1,0 +1,342 @@
+"""Paged K/V cache operators on MI355X: rotary embedding, append, and attention over pages with shared prefixes.
+
+For servers that hold their K/V in pages rather than in `Qwen2Engine`'s rings, and for other models than Qwen2: rotary layouts
+and scaled position tables, fp16 / bf16 / e4m3 caches, head ratios up to 32.  A page holds `page_size` positions of one
+sequence for every K/V head; a table (int32 [sequences, most pages]) names each sequence's pages in order.  Sequences that
+start with the same tokens may name the same pages, and `AttentionPlan` then reads those once for all of them:
+
+    rotary = Rotary.from_config(config)                     # 'rope_scaling' honoured
+    kv = PagedKV.allocate(n_pages, 64, kv_heads, head_dim)  # one layer's pages
+    plan = AttentionPlan(heads, kv_heads, head_dim, max_rows=256, max_seqs=256)
+    # one step: the plan once, then for every layer
+    plan.set(q_lens, kv_lens, groups=[(sequences, shared_positions), ...])
+    q = kv.append(k, v, seq, pos, table, rotary=rotary, q=q)
+    out = plan.run(q, kv, table)
+
+Every call runs on torch's current stream of its tensors' device, allocates nothing on the device except outputs that are not
+given, and may be captured into a graph (`AttentionPlan.set` may not; a captured `run` follows later `set` calls).  The
+reference has none of this (its cache is one tensor per sequence, seedplane/qwen_engine.py:18-29); the operators generalise
+its _rope, cache copy and attention (qwen_engine.py:94-103, 121-135).
+"""
+import ctypes
+import math
+import weakref
+
+import numpy as np
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.SP_DT_F32, torch.float16: _lib.SP_DT_F16, torch.bfloat16: _lib.SP_DT_BF16,
+           torch.float8_e4m3fn: _lib.SP_DT_E4M3}
+E4M3_MAX = 448.0
+
+
+def rotary_frequencies(rot_dim, theta=10000.0, scaling=None, length=None):
+    """Angle per position of the rot_dim / 2 pairs (float64 tensor) and the factor on cosines and sines, for a
+    `rope_scaling` entry of a Hugging Face config.json: rope_type (or type) 'default', 'linear', 'dynamic' (NTK: for `length`
+    positions), 'yarn' or 'llama3' with their usual keys."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError('rot_dim must be even and positive')
+    j = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    inv = 1.0 / theta ** (j / rot_dim)
+    s = scaling or {}
+    kind = s.get('rope_type', s.get('type', 'default'))
+    if kind in ('default', None):
+        return inv, 1.0
+    if kind not in ('linear', 'dynamic', 'yarn', 'llama3'):
+        raise ValueError(f'unknown rope scaling {kind!r}')
+    factor = float(s['factor'])
+    if factor < 1:
+        raise ValueError('the scaling factor must be at least 1')
+    if kind == 'linear':
+        return inv / factor, 1.0
+    original = s.get('original_max_position_embeddings')
+    if not original:
+        raise ValueError(f'{kind} scaling needs original_max_position_embeddings')
+    if kind == 'dynamic':
+        if rot_dim < 4:
+            raise ValueError('dynamic scaling needs rot_dim of at least 4')
+        grown = max(length or original, original)
+        base = theta * (factor * grown / original - (factor - 1)) ** (rot_dim / (rot_dim - 2))
+        return 1.0 / base ** (j / rot_dim), 1.0
+    turns = original * inv / (2 * math.pi)                  # turns of each pair over the original length
+    if kind == 'llama3':
+        low, high = float(s['low_freq_factor']), float(s['high_freq_factor'])
+        keep = ((turns - low) / (high - low)).clamp(0, 1)   # 1: short waves, kept; 0: long ones, slowed by the factor
+        return inv * (keep + (1 - keep) / factor), 1.0
+    # YaRN: kept above beta_fast turns, slowed below beta_slow, a ramp over the pair's index between
+    def index_at(n):
+        return rot_dim * math.log(original / (n * 2 * math.pi)) / (2 * math.log(theta))
+    lo, hi = index_at(s.get('beta_fast') or 32), index_at(s.get('beta_slow') or 1)
+    if s.get('truncate', True):
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, rot_dim - 1)
+    slowed = ((torch.arange(rot_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+    def grade(m):
+        return 1.0 if factor <= 1 else 0.1 * m * math.log(factor) + 1.0
+    attention = s.get('attention_factor')
+    if attention is None:
+        m, m_all = s.get('mscale'), s.get('mscale_all_dim')
+        attention = grade(m) / grade(m_all) if m and m_all else grade(1)
+    return inv * (1 - slowed) + inv / factor * slowed, float(attention)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _device(device):
+    d = torch.device('cuda' if device in ('hip', None) else device)
+    if d.type != 'cuda':
+        raise ValueError('seedplane_amd runs on a ROCm GPU device ("cuda"/"hip")')
+    return torch.device('cuda', torch.cuda.current_device() if d.index is None else d.index)
+
+
+def _call(fn, device, *args):
+    """One library call with `device` current."""
+    if torch.cuda.current_device() == device.index:
+        _lib.check(fn(*args, _stream(device)))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, _stream(device)))
+
+
+def _heads(x, name, device, heads=None, hd=None):
+    """A [rows, heads, head_dim] GPU tensor with values of a head side by side; returns its dtype code."""
+    if x.dim() != 3 or x.device != device:
+        raise ValueError(f'{name} must be a [rows, heads, head_dim] tensor on {device}')
+    if x.stride(2) != 1 and x.shape[2] > 1:
+        raise ValueError(f'the values of a head of {name} must lie side by side')
+    if (heads is not None and x.shape[1] != heads) or (hd is not None and x.shape[2] != hd):
+        raise ValueError(f'{name} has heads {tuple(x.shape[1:])}, expected {(heads, hd)}')
+    if x.dtype not in _DTYPES or x.dtype == torch.float8_e4m3fn:
+        raise ValueError(f'{name} must be fp32, fp16 or bf16')
+    return _DTYPES[x.dtype]
+
+
+def _ints(x, name, device, n=None):
+    """A contiguous int32 GPU tensor of n entries (None: any); returns its address."""
+    if x.dtype != torch.int32 or x.device != device or not x.is_contiguous():
+        raise ValueError(f'{name} must be a contiguous int32 tensor on {device}')
+    if n is not None and (x.dim() != 1 or x.shape[0] != n):
+        raise ValueError(f'{name} must have one entry per row')
+    return x.data_ptr()
+
+
+def _apart(out, *ins):
+    """Refuse an output whose memory another operand reads."""
+    def span(t):
+        a = t.data_ptr()
+        return a, a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    if not out.numel():
+        return
+    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError('the output has rows or heads on top of each other')
+    lo, hi = span(out)
+    for t in ins:
+        if t.numel():
+            a, b = span(t)
+            if a < hi and lo < b:
+                raise ValueError('the output overlaps an input')
+
+
+class Rotary:
+    """A rotary position table on a device: `layout` 'half' (pairs j, j + rot_dim/2) or 'interleaved' (2j, 2j + 1), over the
+    first `rot_dim` values of a head (default: all)."""
+
+    def __init__(self, head_dim, theta=10000.0, rot_dim=None, layout='half', scaling=None, length=None, device='cuda'):
+        if layout not in ('half', 'interleaved'):
+            raise ValueError("layout must be 'half' or 'interleaved'")
+        self.head_dim, self.rot_dim, self.layout = int(head_dim), int(rot_dim or head_dim), layout
+        if self.rot_dim > self.head_dim:
+            raise ValueError('rot_dim exceeds head_dim')
+        self.inv_freq, self.factor = rotary_frequencies(self.rot_dim, theta, scaling, length)
+        _lib.require_gpu()
+        self.lib = _lib.load()
+        self.device = _device(device)
+        self._inv = self.inv_freq.to(self.device)
+        self.desc = _lib.RotaryDesc(self._inv.data_ptr(), self.rot_dim,
+                                    _lib.SP_ROPE_HALF if layout == 'half' else _lib.SP_ROPE_INTERLEAVED, self.factor, 0)
+        self._ref = ctypes.addressof(self.desc)
+
+    @classmethod
+    def from_config(cls, config, layout='half', length=None, device='cuda'):
+        """From a Hugging Face config.json dictionary (rope_theta, rope_scaling or rope_parameters, partial_rotary_factor)."""
+        hd = config.get('head_dim') or config['hidden_size'] // config['num_attention_heads']
+        p = config.get('rope_parameters') or {}
+        scaling = config.get('rope_scaling') or (p if p.get('rope_type', 'default') != 'default' else None)
+        if scaling and not scaling.get('original_max_position_embeddings'):
+            scaling = dict(scaling, original_max_position_embeddings=config.get('max_position_embeddings'))
+        rot = int(hd * (config.get('partial_rotary_factor') or p.get('partial_rotary_factor') or 1.0))
+        return cls(hd, config.get('rope_theta', p.get('rope_theta', 10000.0)), rot, layout, scaling, length, device)
+
+    def apply(self, x, positions, out=None):
+        """x [rows, heads, head_dim] rotated at int32 `positions` [rows] (any sign; with factor 1, negated positions undo the
+        rotation and give its gradient).  `out` may be x."""
+        dt = _heads(x, 'x', self.device, hd=self.head_dim)
+        pos = _ints(positions, 'positions', self.device, x.shape[0])
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        else:
+            if out.shape != x.shape or out.dtype != x.dtype:
+                raise ValueError('out must have the shape and type of x')
+            _heads(out, 'out', self.device)
+            if out.data_ptr() != x.data_ptr() or out.stride() != x.stride():
+                _apart(out, x)
+            elif any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+                raise ValueError('the output has rows or heads on top of each other')
+        _call(self.lib.sp_op_rotate, self.device, self._ref, dt, x.shape[0], x.shape[1], self.head_dim, x.data_ptr(), x.stride(0),
+              x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), pos)
+        return out
+
+
+class PagedKV:
+    """One layer's pages: `k` and `v` [n_pages, kv_heads, page_size, head_dim], fp16, bf16 or float8_e4m3fn; pages may lie
+    further apart than their size (the same for both).  An e4m3 cache holds value / scale, with fp32 scales per K/V head."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
+            raise ValueError('k and v must be [n_pages, kv_heads, page_size, head_dim] of one shape, type, device and layout')
+        if k.dtype not in _DTYPES or k.dtype == torch.float32:
+            raise ValueError('the cache must be fp16, bf16 or float8_e4m3fn')
+        n, nkv, page, hd = k.shape
+        if 0 in k.shape or k.stride()[1:] != (page * hd, hd, 1) or (n > 1 and k.stride(0) < nkv * page * hd):
+            raise ValueError('a page must be contiguous and pages must not overlap')
+        e4m3 = k.dtype == torch.float8_e4m3fn
+        for s in (k_scale, v_scale):
+            if (s is not None) != e4m3:
+                raise ValueError('an e4m3 cache has k_scale and v_scale, others have none')
+            if s is not None and (s.shape != (nkv,) or s.dtype != torch.float32 or s.device != k.device or not s.is_contiguous()):
+                raise ValueError('scales must be fp32 [kv_heads] on the device of the cache')
+        _lib.require_gpu()
+        self.lib = _lib.load()
+        self.device = k.device
+        if self.device.type != 'cuda':
+            raise ValueError('seedplane_amd runs on a ROCm GPU device ("cuda"/"hip")')
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, nkv, page, hd
+        self.dtype = k.dtype
+        stride = k.stride(0) if n > 1 else nkv * page * hd
+        self.desc = _lib.PagedKVDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if e4m3 else None,
+                                     v_scale.data_ptr() if e4m3 else None, stride, _DTYPES[k.dtype], n, page, nkv, hd, 0)
+        self._ref = ctypes.addressof(self.desc)
+
+    @classmethod
+    def allocate(cls, n_pages, page_size, n_kv_heads, head_dim, dtype=torch.float16, k_scale=None, v_scale=None, device='cuda'):
+        shape, device = (n_pages, n_kv_heads, page_size, head_dim), _device(device)
+        return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device), k_scale, v_scale)
+
+    def append(self, k, v, seq, pos, table, rotary=None, q=None, q_out=None, rotary_pos=None):
+        """New tokens into the pages: row r's keys and values k[r], v[r] [kv_heads, head_dim] at position pos[r] of sequence
+        seq[r] (int32 [rows]; a row with seq -1, or whose position has no page, writes nothing).  With `rotary` the keys turn by
+        rotary_pos (default: pos) on the way, and the queries q [rows, heads, head_dim] into q_out (default: a new tensor of q's
+        type; may be q itself), which is returned."""
+        dt = _heads(k, 'k', self.device, self.n_kv_heads, self.head_dim)
+        if _heads(v, 'v', self.device, self.n_kv_heads, self.head_dim) != dt or v.shape != k.shape:
+            raise ValueError('k and v must have one shape and type')
+        rows = k.shape[0]
+        if table.dim() != 2 or 0 in table.shape:
+            raise ValueError('table must be [sequences, most pages]')
+        s, p, t = (_ints(seq, 'seq', self.device, rows), _ints(pos, 'pos', self.device, rows), _ints(table, 'table', self.device))
+        turn = p if rotary_pos is None else _ints(rotary_pos, 'rotary_pos', self.device, rows)
+        if rotary is not None and (rotary.head_dim != self.head_dim or rotary.device != self.device):
+            raise ValueError('the rotary table is of another head_dim or device')
+        qa = (None, 0, 0)
+        qo = (None, 0, 0, 0)
+        nh = 0
+        if q is not None:
+            if _heads(q, 'q', self.device, hd=self.head_dim) != dt or q.shape[0] != rows:
+                raise ValueError('q must have the rows and the type of k')
+            nh = q.shape[1]
+            if q_out is None:
+                # rows that write nothing are zeros in a new tensor
+                q_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+            else:
+                if q_out.shape != q.shape:
+                    raise ValueError('q_out must have the shape of q')
+                if q_out.data_ptr() != q.data_ptr() or q_out.stride() != q.stride() or q_out.dtype != q.dtype:
+                    _apart(q_out, q, k, v)
+            qa = (q.data_ptr(), q.stride(0), q.stride(1))
+            qo = (q_out.data_ptr(), _heads(q_out, 'q_out', self.device), q_out.stride(0), q_out.stride(1))
+        elif q_out is not None:
+            raise ValueError('q_out without q')
+        if rows:
+            _call(self.lib.sp_op_paged_append, self.device, self._ref, None if rotary is None else rotary._ref, dt, rows, nh, *qa,
+                  k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), turn, s, p, t, table.shape[0],
+                  table.shape[1], *qo)
+        return q_out
+
+
+class AttentionPlan:
+    """Attention over pages for batches of up to `max_rows` query tokens of up to `max_seqs` sequences; head_dim 64 or 128."""
+
+    def __init__(self, n_heads, n_kv_heads, head_dim, max_rows, max_seqs, device='cuda'):
+        _lib.require_gpu()
+        self.lib = _lib.load()
+        self.device = _device(device)
+        self.n_heads, self.n_kv_heads, self.head_dim = int(n_heads), int(n_kv_heads), int(head_dim)
+        self.max_rows, self.max_seqs = int(max_rows), int(max_seqs)
+        h = ctypes.c_void_p()
+        with torch.cuda.device(self.device):
+            _lib.check(self.lib.sp_attn_plan_create(self.n_heads, self.n_kv_heads, self.head_dim, self.max_rows, self.max_seqs,
+                                                    ctypes.byref(h)))
+        self.h = h
+        self._finalizer = weakref.finalize(self, self.lib.sp_attn_plan_destroy, h)
+        self._ws = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+        self._scale = 1.0 / math.sqrt(self.head_dim)
+        self.rows = 0
+
+    @property
+    def workspace_bytes(self):
+        """Bytes of a workspace for run(): calls that overlap each other need one each."""
+        return int(self.lib.sp_attn_plan_workspace(self.h))
+
+    def set(self, q_lens, kv_lens, groups=None):
+        """The next batch (host integers): sequence s has q_lens[s] query tokens, the last of its kv_lens[s] cached positions.
+        groups: (sequences, shared positions) of each run of sequences whose tables name the same pages for their first positions;
+        None: nothing is shared."""
+        q = np.ascontiguousarray(q_lens, dtype=np.int32)
+        kv = np.ascontiguousarray(kv_lens, dtype=np.int32)
+        if q.ndim != 1 or q.shape != kv.shape:
+            raise ValueError('q_lens and kv_lens must have one entry per sequence')
+        size = shared = None
+        n = 0
+        if groups is not None:
+            g = np.ascontiguousarray(groups, dtype=np.int32).reshape(-1, 2)
+            size, shared, n = np.ascontiguousarray(g[:, 0]), np.ascontiguousarray(g[:, 1]), len(g)
+            if n == 0 and len(q):
+                raise ValueError('the groups do not cover the sequences')
+        _call(self.lib.sp_attn_plan_set, self.device, self.h, len(q), q.ctypes.data, kv.ctypes.data, n,
+              None if size is None else size.ctypes.data, None if shared is None else shared.ctypes.data)
+        self.rows = int(q.sum())
+        return self
+
+    def run(self, q, kv, table, out=None, lse=None, scale=None, workspace=None):
+        """Attention of q [rows, heads, head_dim] (fp16 or bf16) over the pages of `kv`; returns `out` (default: a new tensor,
+        zeros behind the plan's rows).  lse: fp32 [rows, heads], filled with the logarithm of each row's sum of exponentials."""
+        dt = _heads(q, 'q', self.device, self.n_heads, self.head_dim)
+        if kv.device != self.device:
+            raise ValueError('the cache is on another device')
+        if table.dim() != 2:
+            raise ValueError('table must be [sequences, most pages]')
+        t = _ints(table, 'table', self.device)
+        if out is None:
+            new = torch.empty if q.shape[0] == self.rows else torch.zeros
+            out = new(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            if out.shape != q.shape or out.dtype != q.dtype:
+                raise ValueError('out must have the shape and type of q')
+            _heads(out, 'out', self.device)
+            _apart(out, q, kv.k, kv.v)
+        if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != self.device
+                                or not lse.is_contiguous()):
+            raise ValueError('lse must be a contiguous fp32 [rows, heads] tensor')
+        ws = self._ws if workspace is None else workspace
+        if workspace is not None and (ws.device != self.device or not ws.is_contiguous()
+                                      or ws.numel() * ws.element_size() < self._ws.numel()):
+            raise ValueError('the workspace is too small or on another device')
+        _call(self.lib.sp_op_paged_attention, self.device, self.h, kv._ref, dt, q.shape[0], q.data_ptr(), q.stride(0), q.stride(1),
+              t, table.shape[0], table.shape[1], self._scale if scale is None else float(scale), out.data_ptr(), out.stride(0),
+              out.stride(1), None if lse is None else lse.data_ptr(), ws.data_ptr())
+        return out
