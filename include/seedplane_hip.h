@@ -447,12 +447,12 @@ void sp_attn_plan_destroy(sp_attn_plan *plan);
  * capture; a captured sp_op_paged_attention reads the tables of the last set before each replay. */
 int sp_attn_plan_set(sp_attn_plan *plan, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len, int32_t n_groups,
                      const int32_t *group_size, const int32_t *group_shared, void *hip_stream);
-/* Host only, for inspection: the items of one kind (0, 1, 2: row tiles of 32, 64, 128 rows) that sp_attn_plan_set makes of these
- * lengths, as 8 int32 each: first token, tokens, K/V head, sequence, first position, end, position seen by the first token (2^30:
- * all), first record or -1; and per token 8 int32: base, parts, tile and index of its records of the shared and of its own
+/* Host only, for inspection: the items that sp_attn_plan_set makes of these lengths, as 12 int32 each: first token, tokens, K/V
+ * head, sequence, first position, end, position seen by the first token (2^30: all), first record or -1, kind (row tile of
+ * 32 << kind rows), three reserved; and per token 8 int32: base, parts, tile and index of its records of the shared and of its own
  * positions (pairs).  items and token_recs may be NULL. */
 int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len,
-                       int32_t n_groups, const int32_t *group_size, const int32_t *group_shared, int32_t kind, int32_t capacity,
+                       int32_t n_groups, const int32_t *group_size, const int32_t *group_shared, int32_t capacity,
                        int32_t *items, int32_t *n_items, int32_t *token_recs, int64_t *n_records);
 /* Bytes of sp_op_paged_attention's workspace, for every batch within max_rows. */
 size_t sp_attn_plan_workspace(const sp_attn_plan *plan);

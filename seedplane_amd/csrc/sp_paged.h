@@ -38,7 +38,7 @@ struct AttnArgs {
     int NH, G;
     float scale;                      // of the scores, times log2(e)
     const Item *items;
-    const int *n_items;
+    const int *n_items;               // NULL: one block per item
     float *po;                        // records: [rows][HD] unnormalised outputs
     float2 *ml;                       // [rows] (m in log2 units, l)
 };
@@ -76,12 +76,11 @@ __device__ __forceinline__ int piece_swap(int k) {
 }
 
 // One 16-byte global-to-LDS copy per lane: lane i's 16 bytes at g land at LDS byte address lds + 16 i.  Inline asm so that the
-// compiler does not make every LDS read wait for the copies in flight; copies_landed waits for them.  The hardware needs one
+// compiler does not make every LDS read wait for the copies in flight; copies_wait counts them.  The hardware needs one
 // wait state between the scalar write of M0 (the LDS address) and the copy.
 __device__ __forceinline__ void copy_to_lds(const void *g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds) : "memory");
 }
-__device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // The other half's value of lane ^ 32, combined.
@@ -94,275 +93,414 @@ __device__ __forceinline__ float half_sum(float v) {
     return __uint_as_float(r.x) + __uint_as_float(r.y);
 }
 
+// LDS of a block: tiles (64 KiB), which the join over key waves reuses, the pool rows of the next TABLE_KEYS positions, the
+// key waves' (m, l).  Two blocks share a CU (8 waves: one block's loads and exponentials beside the other's matrix products).
+constexpr float LAZY = 8.f;
+constexpr int TABLE_KEYS = 2048;
+constexpr int TILE_SMEM = 65536;
+struct AttnShared {                                                    // beside the tiles
+    uint32_t rows[TABLE_KEYS];                                         // pool row of each position (0 where there is none)
+    uint32_t seen[TABLE_KEYS / 32];                                    // which positions exist
+    float2 ml[4][32];
+};
+
 template <bool KV8, int HD, int WM>
 struct AttnTile {
     static constexpr int WK = 4 / WM;                                  // waves over keys
-    static constexpr int KT = WM == 4 ? 64 : 32;                       // keys of a tile (of one group of WM waves)
     static constexpr int RB = HD * (KV8 ? 1 : 2), NCH = RB / 16;       // bytes and pieces of a row
+    static constexpr int KT = WM == 2 || (WM == 1 && RB == 256) ? 32 : 64;      // keys of a tile (of one group of WM waves)
+    static constexpr int STAGES = WM == 1 ? 1 : 2;
     static constexpr int TILE = KT * RB;                               // bytes of a tile's keys (and of its values)
-    static constexpr int COPIES = KT * NCH / 64 / WM;                  // copies per wave, of keys and of values
+    static constexpr int ALL = KT * NCH / 64;                          // copies of a tile's keys, and of its values
+    static constexpr int COPIES = ALL < WM ? 1 : ALL / WM;             // ... of a wave (of the first ALL waves, if fewer)
     static constexpr int JOIN = (WK - 1) * WM * 32 * HD * 4;           // LDS of the join over the key waves
-    static constexpr int SMEM = WK * 2 * 2 * TILE > JOIN ? WK * 2 * 2 * TILE : JOIN;
-    static_assert(COPIES >= 1 && COPIES * 64 * WM == KT * NCH, "whole copies");
+    static_assert(ALL >= 1 && (ALL < WM || ALL % WM == 0), "whole copies");
+    static_assert(WK * STAGES * 2 * TILE <= TILE_SMEM && JOIN <= TILE_SMEM, "LDS plan");
+    static_assert(TABLE_KEYS % (WK * KT) == 0, "whole rounds of the row table");
 };
 
+// x, of which the compiler knows nothing: what is computed from it stays where it is written.  Addresses of copies and of rare
+// paths would otherwise be kept in registers over the loops, which need theirs for the accumulators.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 template <class T, bool KV8, int HD, int WM>
-__global__ void __launch_bounds__(256, WM == 1 ? 1 : 2) k_paged_attn(AttnArgs a) {
+__device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsigned char *smem, AttnShared &sh) {
     typedef AttnTile<KV8, HD, WM> TL;
     typedef Mma<T> M;
     typedef typename M::frag frag;
     constexpr int KT = TL::KT, RB = TL::RB, NCH = TL::NCH, WK = TL::WK, NS = HD / 16, ND = HD / 32, SUB = KT / 32;
     constexpr int RPC = 64 / NCH;                                      // rows of one copy
-    extern __shared__ __align__(1024) unsigned char smem[];
-    __shared__ float2 ml_s[4][32];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;                          // the lane's query row; its half of every 8 keys
     const int rw = wv % WM, kw = wv / WM;
-    unsigned char *const buf0 = smem + kw * (4 * TL::TILE);            // [2 stages][keys, values] of this key wave
+    unsigned char *const buf0 = smem + kw * (TL::STAGES * 2 * TL::TILE);       // [stage][keys, values] of this key wave
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
         (uint32_t)(size_t)((__attribute__((address_space(3))) unsigned char *)buf0));
 
-    // reads of a tile: key row `col`, its piece for head-dim step s at kbase ^ (step bytes); values by transpose reads
+    const int row = rw * 32 + col;
+    // (a captured call may meet tables set later: its own sizes bound every access)
+    const bool live = row < w.ntok * a.G && w.tok0 + row / a.G < a.rows;
+    const int tok = live ? row / a.G : 0, hh = live ? row - tok * a.G : 0;
+    frag qf[NS];
+    {
+        const T *q = (const T *)a.q + (int64_t)min(w.tok0 + tok, a.rows - 1) * a.q_row + (int64_t)(w.kvh * a.G + hh) * a.q_head + 8 * h;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qf[s] = *(const frag *)(q + 16 * s);
+    }
+    // the row sees positions < lim; rows behind the tile's last compute along and are never stored
+    const int lim = live ? min(w.k1, w.pos0 + tok + 1) : w.k1;
+    int lo = lim, hi = live ? lim : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o)); hi = max(hi, __shfl_xor(hi, o)); }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    const float sc = KV8 ? a.scale * a.ks[w.kvh] : a.scale;
+
     const int swz = piece_swap<NCH>(col);
-    const int krow = col * RB;
-    const int kbase = KV8 ? (swz << 4) | (h << 3) : ((h ^ swz) << 4);
     const int tg = (lane >> 4) & 1, ti = lane & 15;                    // which 16 of 32 dims; lane within them
 
-    for (int it = blockIdx.x; it < *a.n_items; it += gridDim.x) {
-        const Item w = a.items[it];
-        const int nt = (w.k1 - w.k0 + KT - 1) / KT, ni = (nt + WK - 1) / WK;
-        const int row = rw * 32 + col;
-        // (a captured call may meet tables set later: its own sizes bound every access)
-        const bool live = row < w.ntok * a.G && w.tok0 + row / a.G < a.rows;
-        const int tok = live ? row / a.G : 0, hh = live ? row - tok * a.G : 0;
-        // the row sees positions < lim; rows behind the tile's last compute along and are never stored
-        const int lim = live ? min(w.k1, w.pos0 + tok + 1) : w.k1;
-        int lo = lim, hi = live ? lim : 0;
+    f32x16 o[ND];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o)); hi = max(hi, __shfl_xor(hi, o)); }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = __builtin_amdgcn_readfirstlane(hi);
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[d][j] = 0.f;
+    float m = -INFINITY, l = 0.f;                                      // m in log2 units; l of the lane's own keys
 
-        frag qf[NS];
-        {
-            const T *q = (const T *)a.q + (int64_t)min(w.tok0 + tok, a.rows - 1) * a.q_row + (int64_t)(w.kvh * a.G + hh) * a.q_head + 8 * h;
+    // copies of tile t of the row table (this wave's share) to LDS address `to`, keys or values.  Row kr of the tile is copied by
+    // lanes of copy kr / RPC; the swap of its pieces is the lane's own, xor one that the copy alone decides.
+    const int copy0 = rw * TL::COPIES * RPC + lane / NCH;
+    const uint32_t piece0 = (uint32_t)((lane % NCH) ^ piece_swap<NCH>(copy0)) << 4;
+    auto rows_of = [&](int t, uint32_t *r) {
+        const uint32_t *rows = sh.rows + t * KT + copy0;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) qf[s] = *(const frag *)(q + 16 * s);
+        for (int c = 0; c < TL::COPIES; ++c) r[c] = rows[c * RPC];
+    };
+    auto copy_row = [&](const uint8_t *pool, const uint32_t *r, uint32_t to, int c) {
+        if (TL::ALL < WM && rw >= TL::ALL) return;
+        const uint32_t piece = opaque(piece0);
+        copy_to_lds(pool + ((uint64_t)r[c] * RB + (piece ^ (uint32_t)(piece_swap<NCH>(c * RPC) << 4))), to + (rw * TL::COPIES + c) * 1024);
+    };
+    auto copy_tile = [&](const uint8_t *pool, int t, uint32_t to) {
+        uint32_t r[TL::COPIES];
+        rows_of(t, r);
+#pragma unroll
+        for (int c = 0; c < TL::COPIES; ++c) copy_row(pool, r, to, c);
+    };
+    // which of 32 positions exist (block b of the row table)
+    auto seen_of = [&](int b) -> uint32_t { return __builtin_amdgcn_readfirstlane(sh.seen[b]); };
+    // values without a position are row 0 of the pool: zeros instead, so that a weight of 0 stays 0 (each wave its own copies)
+    auto clear_values = [&](unsigned char *vb, int t, uint32_t all) {
+        if (all == ~0u || (TL::ALL < WM && rw >= TL::ALL)) return;
+        const int ln = opaque(lane);
+#pragma unroll 1
+        for (int c = 0; c < TL::COPIES; ++c) {
+            const int n = rw * TL::COPIES + c, kr = n * RPC + ln / NCH;
+            if (!((sh.seen[t * SUB + kr / 32] >> (kr & 31)) & 1)) *(u32x4 *)(vb + n * 1024 + ln * 16) = (u32x4){0, 0, 0, 0};
         }
-        const float sc = KV8 ? a.scale * a.ks[w.kvh] : a.scale;
+        lds_wait();
+    };
+    // 32 keys at a time: scores (kb: their rows), then maxima, weights, outputs (vb: their rows)
+    int ka[NS], va[2][ND];                                             // LDS offsets of the lane's operands
+#pragma unroll
+    for (int p = 0; p < NS; ++p) ka[p] = KV8 ? col * RB + (((swz ^ p) << 4) | (h << 3)) : col * RB + ((h ^ swz ^ (2 * p)) << 4);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+        if constexpr (KV8) {
+            const int rr = ti >> 1, key = 8 * (rr >> 2) + 4 * h + (rr & 3);
+            va[0][d] = va[1][d] = key * RB + (((2 * d + tg) ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
+        } else {
+            const int key = 4 * h + (ti >> 2), c = 4 * d + 2 * tg + ((ti >> 1) & 1);
+            va[0][d] = key * RB + ((c ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
+            va[1][d] = (key + 8) * RB + ((c ^ piece_swap<NCH>(key + 8)) << 4) + ((ti & 1) << 3);
+        }
+    }
+    auto key_frag = [&](const unsigned char *kb, int p) -> frag {
+        if constexpr (KV8) return from_e4m3<T>(*(const u32x2 *)(kb + ka[p]));
+        else return *(const frag *)(kb + ka[p]);
+    };
+    auto value_frag = [&](const unsigned char *vb, int y, int d) -> frag {         // keys 16 y .. + 15
+        if constexpr (KV8) {
+            return from_e4m3<T>(__builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (__attribute__((address_space(3))) i32x2 *)(vb + 16 * y * RB + va[0][d]))));
+        } else {
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vb + 16 * y * RB + va[0][d]));
+            const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vb + 16 * y * RB + va[1][d]));
+            const u32x2 xx = __builtin_bit_cast(u32x2, x), zz = __builtin_bit_cast(u32x2, z);
+            return __builtin_bit_cast(frag, (u32x4){xx.x, xx.y, zz.x, zz.y});
+        }
+    };
+    auto scores = [&](const unsigned char *kb, f32x16 &s) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = 0.f;
+        frag kf[NS];
+#pragma unroll
+        for (int p = 0; p < NS; ++p) kf[p] = key_frag(kb, p);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int p = 0; p < NS; ++p) s = M::run(kf[p], qf[p], s);
+    };
+    // masks the scores of positions t0 .. t0 + 31 and brings the running maximum up to date; returns the exponent's base
+    auto maxima = [&](f32x16 &s, int t0, uint32_t seen) -> float {
+        if (t0 + 32 > lo || seen != ~0u) {
+            const uint32_t mine = seen >> (4 * h);
+            const int left = lim - t0 - 4 * h;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int kk = 8 * (j / 4) + j % 4;
+                s[j] = kk < left && ((mine >> kk) & 1) ? s[j] : -INFINITY;
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+        mx = fmaxf(m, half_max(mx) * sc);
+        // weights are taken from the base m, which follows the maximum only when that has grown by more than 2^8: up to there
+        // they fit every type, and the outputs need no rescaling.  (A row that has seen nothing stays empty.)
+        if (__any(mx > m + LAZY)) {
+            const float keep = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mx);
+            l *= keep;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[d][j] *= keep;
+            m = mx;
+        }
+        return m == -INFINITY ? 0.f : m;
+    };
+    frag pf[2];
+    auto weights = [&](const f32x16 &s, float base) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float p = __builtin_amdgcn_exp2f(s[j] * sc - base);
+            l += p;
+            pf[j / 8][j % 8] = (T)p;
+        }
+    };
+    auto outputs = [&](const unsigned char *vb) {
+        frag vf[2][ND];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) vf[y][d] = value_frag(vb, y, d);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] = M::run(vf[y][d], pf[y], o[d]);
+    };
 
-        // the page of key `lane` of tile i of this key wave: entry loaded one tile ahead
-        const int *table = a.table + (int64_t)w.seq * a.max_pages;
-        auto key_of = [&](int i) { return w.k0 + (kw + i * WK) * KT + (lane & (KT - 1)); };
-        auto entry_of = [&](int i) {
-            const int key = key_of(i), page = key / a.page_size;
-            return key < w.k1 && w.seq < a.n_seq && page < a.max_pages ? table[page] : -1;
-        };
-        // copies tile i to stage st; returns which of its positions exist
-        auto stage = [&](int i, int entry, int st) -> uint64_t {
-            const int key = key_of(i);
-            const bool ok = key < w.k1 && entry >= 0 && entry < a.n_pages;
-            const uint32_t r = ok ? (uint32_t)entry * a.page_rows + (uint32_t)(w.kvh * a.page_size + key % a.page_size) : 0u;
-#pragma unroll
-            for (int c = 0; c < TL::COPIES; ++c) {
-                const int n = rw * TL::COPIES + c, kr = n * RPC + lane / NCH;      // row of the tile
-                const uint32_t src = __shfl(r, kr);
-                const uint64_t off = (uint64_t)src * RB + (((lane % NCH) ^ piece_swap<NCH>(kr)) << 4);
-                const uint32_t to = lds0 + st * (2 * TL::TILE) + n * 1024;
-                copy_to_lds(a.k + off, to);
-                copy_to_lds(a.v + off, to + TL::TILE);
+    const int *table = a.table + (int64_t)w.seq * a.max_pages;
+    for (int c0 = w.k0; c0 < w.k1; c0 += TABLE_KEYS) {
+        // the pool rows of the next positions, NO_ROW where there is none
+        if (c0 != w.k0) lds_barrier();
+        const int tid = opaque(threadIdx.x);
+#pragma unroll 1
+        for (int j = tid; j < TABLE_KEYS && c0 + j - tid < w.k1 + 64; j += 256) {  // (a tile past the end reads up to 63 rows past it)
+            const int key = c0 + j, page = key / a.page_size;
+            uint32_t r = 0;
+            bool ok = false;
+            if (key < w.k1 && w.seq < a.n_seq && page < a.max_pages) {
+                const int e = table[page];
+                ok = e >= 0 && e < a.n_pages;
+                if (ok) r = (uint32_t)e * a.page_rows + (uint32_t)(w.kvh * a.page_size + key - page * a.page_size);
             }
-            return KT == 64 ? __ballot(ok) : __ballot(ok) | 0xffffffff00000000ull;
-        };
-        // rows without a position hold row 0 of the pool: zeros instead, so that 0 x value stays 0
-        auto clear = [&](int st, uint64_t seen) {
-            if (seen == ~0ull) return;
+            sh.rows[j] = r;
+            const uint64_t b = __ballot(ok);
+            if ((tid & 63) == 0) *(uint64_t *)&sh.seen[j / 32] = b;
+        }
+        lds_barrier();
+        // the queries have landed: inside the loops the compiler must not wait for them, which would wait for the copies too
 #pragma unroll
-            for (int c = 0; c < TL::COPIES; ++c) {
-                const int n = rw * TL::COPIES + c, kr = n * RPC + lane / NCH;
-                if (!((seen >> kr) & 1)) {
-                    unsigned char *d = buf0 + st * (2 * TL::TILE) + n * 1024 + lane * 16;
-                    *(u32x4 *)d = (u32x4){0, 0, 0, 0};
-                    *(u32x4 *)(d + TL::TILE) = (u32x4){0, 0, 0, 0};
-                }
+        for (int p = 0; p < NS; ++p) asm volatile("" : "+v"(qf[p]));
+        const int nt = (min(w.k1 - c0, TABLE_KEYS) + KT - 1) / KT;     // tiles; this key wave's are kw, kw + WK ..
+        if constexpr (WM == 1) {
+            // a wave of its own: one tile, keys and values copied apart, so that the next keys are on their way while the
+            // values are awaited and used
+            unsigned char *const kb = buf0, *const vb = buf0 + TL::TILE;
+            const int n = min(nt, (max(hi - c0, 0) + KT - 1) / KT);    // tiles behind the last seen position are skipped
+            if (kw < n) {
+                copy_tile(a.k, kw, lds0);
+                copy_tile(a.v, kw, lds0 + TL::TILE);
             }
-        };
-
-        f32x16 o[ND];
+            for (int t = kw; t < n; t += WK) {
+                const bool more = t + WK < n;
+                copies_wait<TL::COPIES>();
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) o[d][j] = 0.f;
-        float m = -INFINITY, l = 0.f;                                  // m in raw scores; l of the lane's own keys
-
-        int entry = entry_of(0);
-        uint64_t next = stage(0, entry, 0);
-        entry = entry_of(1);
-        for (int i = 0; i < ni; ++i) {
-            const int st = i & 1;
-            const uint64_t seen = next;
-            copies_landed();
-            clear(st, seen);
-            if constexpr (WM > 1) lds_barrier();
-            else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (i + 1 < ni) {
-                const int e = entry;
-                entry = entry_of(i + 2);
-                next = stage(i + 1, e, st ^ 1);
-            }
-            const int t0 = w.k0 + (kw + i * WK) * KT;                  // the tile's first position
-            if (t0 >= hi) continue;
-            const unsigned char *kb = buf0 + st * (2 * TL::TILE), *vb = kb + TL::TILE;
-            f32x16 s[SUB];
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) s[u][j] = 0.f;
-#pragma unroll
-                for (int p = 0; p < NS; ++p) {
-                    frag kf;
-                    if constexpr (KV8) kf = from_e4m3<T>(*(const u32x2 *)(kb + u * 32 * RB + krow + (kbase ^ (p << 4))));
-                    else kf = *(const frag *)(kb + u * 32 * RB + krow + (kbase ^ (p << 5)));
-                    s[u] = M::run(kf, qf[p], s[u]);
-                }
-            }
-            if (t0 + KT > lo || seen != ~0ull) {
-                const uint64_t mine = seen >> (4 * h);
-                const int left = lim - t0 - 4 * h;
-#pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int kk = u * 32 + 8 * (j / 4) + j % 4;
-                        s[u][j] = kk < left && ((mine >> kk) & 1) ? s[u][j] : -INFINITY;
+                for (int u = 0; u < SUB; ++u) {
+                    f32x16 s;
+                    scores(kb + u * 32 * RB, s);
+                    if (u == SUB - 1) {
+                        lds_wait();
+                        if (more) copy_tile(a.k, t + WK, lds0);
                     }
-            }
-            float mx = s[0][0];
-#pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[u][j]);
-            mx = fmaxf(m, half_max(mx));
-            const float base = mx == -INFINITY ? 0.f : mx * sc;        // a row that has seen nothing stays empty
-            if (__any(mx > m)) {
-                const float keep = __builtin_amdgcn_exp2f(m * sc - base);
-                l *= keep;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) o[d][j] *= keep;
-                m = mx;
-            }
-            frag pf[SUB * 2];
-#pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float p = __builtin_amdgcn_exp2f(s[u][j] * sc - base);
-                    l += p;
-                    pf[u * 2 + j / 8][j % 8] = (T)p;
-                }
-#pragma unroll
-            for (int y = 0; y < SUB * 2; ++y)                          // 16 keys
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    frag vf;
-                    if constexpr (KV8) {
-                        const int rr = ti >> 1, key = 16 * y + 8 * (rr >> 2) + 4 * h + (rr & 3);
-                        const int at = key * RB + (((2 * d + tg) ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
-                        vf = from_e4m3<T>(__builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                            (__attribute__((address_space(3))) i32x2 *)(vb + at))));
-                    } else {
-                        const int key = 16 * y + 4 * h + (ti >> 2), c = 4 * d + 2 * tg + ((ti >> 1) & 1);
-                        const int a0 = key * RB + ((c ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
-                        const int a1 = (key + 8) * RB + ((c ^ piece_swap<NCH>(key + 8)) << 4) + ((ti & 1) << 3);
-                        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vb + a0));
-                        const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vb + a1));
-                        const u32x2 xx = __builtin_bit_cast(u32x2, x), zz = __builtin_bit_cast(u32x2, z);
-                        vf = __builtin_bit_cast(frag, (u32x4){xx.x, xx.y, zz.x, zz.y});
+                    weights(s, maxima(s, c0 + t * KT + u * 32, seen_of(t * SUB + u)));
+                    if (u == 0) {
+                        if (more && SUB == 1) copies_wait<TL::COPIES>();
+                        else copies_wait<0>();
+                        clear_values(vb, t, SUB == 1 ? seen_of(t) : seen_of(t * SUB) & seen_of(t * SUB + SUB - 1));
                     }
-                    o[d] = M::run(vf, pf[y], o[d]);
+                    outputs(vb + u * 32 * RB);
                 }
+                lds_wait();
+                if (more) copy_tile(a.v, t + WK, lds0 + TL::TILE);
+            }
+        } else {
+            // the row waves share a tile; the next one is copied meanwhile
+            const int rounds = (nt + WK - 1) / WK;
+            copy_tile(a.k, kw, lds0);
+            copy_tile(a.v, kw, lds0 + TL::TILE);
+            uint32_t seen_next[SUB];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) seen_next[u] = seen_of(kw * SUB + u);
+            auto step = [&](int i, auto stage_of) {
+                constexpr int ST = decltype(stage_of)::value * 2 * TL::TILE;
+                const int t = i * WK + kw;
+                const bool more = i + 1 < rounds;
+                unsigned char *const kb = buf0 + ST, *const vb = kb + TL::TILE;
+                const uint32_t to = lds0 + (2 * TL::TILE - ST);
+                uint32_t seen[SUB], r[TL::COPIES];
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) seen[u] = seen_next[u];
+                if (more) {                                            // (read ahead of the barrier)
+                    rows_of(t + WK, r);
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u) seen_next[u] = seen_of((t + WK) * SUB + u);
+                }
+                copies_wait<0>();
+                clear_values(vb, t, seen[0] & seen[SUB - 1]);
+                lds_barrier();
+                // the next tile's copies are issued behind matrix products: a CU takes one in 16 cycles, and four waves that
+                // issue theirs together wait for each other
+                auto copies = [&](int part) {
+                    if (!more) return;
+#pragma unroll
+                    for (int c = part; c < TL::COPIES; c += SUB) {
+                        copy_row(a.k, r, to, c);
+                        copy_row(a.v, r, to + TL::TILE, c);
+                    }
+                };
+                if (c0 + t * KT >= hi) {
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u) copies(u);
+                    return;
+                }
+                f32x16 s[SUB];
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    scores(kb + u * 32 * RB, s[u]);
+                    copies(u);
+                }
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    weights(s[u], maxima(s[u], c0 + t * KT + u * 32, seen[u]));
+                    outputs(vb + u * 32 * RB);
+                }
+            };
+            for (int i = 0; i < rounds; i += 2) {
+                step(i, std::integral_constant<int, 0>{});
+                if (i + 1 < rounds) step(i + 1, std::integral_constant<int, 1>{});
+            }
         }
-        l = half_sum(l);
-        m = m == -INFINITY ? -INFINITY : m * sc;                       // log2 units
+    }
+    l = half_sum(l);
 
-        if constexpr (WK > 1) {
-            // the key waves of a row group joined in LDS: waves kw > 0 leave theirs, wave kw = 0 adds them in order
-            lds_barrier();
-            f32x4 *const area = (f32x4 *)smem;
-            if (h == 0) ml_s[wv][col] = make_float2(m, l);
-            if (kw > 0) {
+    if constexpr (WK > 1) {
+        // the key waves of a row group joined in LDS: waves kw > 0 leave theirs, wave kw = 0 adds them in order
+        lds_barrier();
+        f32x4 *const area = (f32x4 *)smem;
+        if (h == 0) sh.ml[wv][col] = make_float2(m, l);
+        if (kw > 0) {
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        area[(((kw - 1) * WM + rw) * (4 * ND) + d * 4 + j) * 64 + lane] =
-                            (f32x4){o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
-            }
-            lds_barrier();
-            if (kw == 0) {
-                float mm = m;
-#pragma unroll
-                for (int k = 1; k < WK; ++k) mm = fmaxf(mm, ml_s[k * WM + rw][col].x);
-                const float base = mm == -INFINITY ? 0.f : mm;
-                float f = __builtin_amdgcn_exp2f(m - base);
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) o[d][j] *= f;
-#pragma unroll
-                for (int k = 1; k < WK; ++k) {
-                    const float2 x = ml_s[k * WM + rw][col];
-                    f = __builtin_amdgcn_exp2f(x.x - base);
-                    l += x.y * f;
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const f32x4 y = area[(((k - 1) * WM + rw) * (4 * ND) + d * 4 + j) * 64 + lane];
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) o[d][4 * j + c] += y[c] * f;
-                        }
-                }
-                m = mm;
-            }
+                for (int j = 0; j < 4; ++j)
+                    area[(((kw - 1) * WM + rw) * (4 * ND) + d * 4 + j) * 64 + lane] =
+                        (f32x4){o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
         }
-        if (kw == 0 && live) {
-            const float vs = KV8 ? a.vs[w.kvh] : 1.f;
-            if (w.rec < 0) {
-                const float il = l > 0.f ? vs / l : 0.f;               // a row that sees nothing: zeros
-                const int64_t head = w.kvh * a.G + hh;
-                T *d0 = (T *)a.out + (int64_t)(w.tok0 + tok) * a.out_row + head * a.out_head + 4 * h;
+        lds_barrier();
+        if (kw == 0) {
+            float mm = m;
+#pragma unroll
+            for (int k = 1; k < WK; ++k) mm = fmaxf(mm, sh.ml[k * WM + rw][col].x);
+            const float base = mm == -INFINITY ? 0.f : mm;
+            float f = __builtin_amdgcn_exp2f(m - base);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[d][j] *= f;
+#pragma unroll
+            for (int k = 1; k < WK; ++k) {
+                const float2 x = sh.ml[k * WM + rw][col];
+                f = __builtin_amdgcn_exp2f(x.x - base);
+                l += x.y * f;
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        typedef T T4 __attribute__((ext_vector_type(4)));
-                        *(T4 *)(d0 + d * 32 + 8 * j) = (T4){(T)(o[d][4 * j] * il), (T)(o[d][4 * j + 1] * il),
-                                                            (T)(o[d][4 * j + 2] * il), (T)(o[d][4 * j + 3] * il)};
+                        const f32x4 y = area[(((k - 1) * WM + rw) * (4 * ND) + d * 4 + j) * 64 + lane];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[d][4 * j + c] += y[c] * f;
                     }
-                if (a.lse && h == 0)
-                    a.lse[(int64_t)(w.tok0 + tok) * a.NH + head] = l > 0.f ? LN2 * (m + log2f(l)) : -INFINITY;
-            } else {
-                const int64_t rec = w.rec + row;
-                float *d0 = a.po + rec * HD + 4 * h;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        *(f32x4 *)(d0 + d * 32 + 8 * j) = (f32x4){o[d][4 * j] * vs, o[d][4 * j + 1] * vs, o[d][4 * j + 2] * vs,
-                                                                  o[d][4 * j + 3] * vs};
-                if (h == 0) a.ml[rec] = make_float2(m, l);
             }
+            m = mm;
         }
-        lds_barrier();                                                 // LDS is free for the next item
+    }
+    const int row2 = rw * 32 + (opaque(lane) & 31), tok2 = row2 / a.G;
+    if (kw == 0 && row2 < w.ntok * a.G && w.tok0 + tok2 < a.rows) {
+        const int row = row2, tok = tok2, hh = row2 - tok2 * a.G;
+        const float vs = KV8 ? a.vs[w.kvh] : 1.f;
+        if (w.rec < 0) {
+            const float il = l > 0.f ? vs / l : 0.f;                   // a row that sees nothing: zeros
+            const int64_t head = w.kvh * a.G + hh;
+            T *d0 = (T *)a.out + (int64_t)(w.tok0 + tok) * a.out_row + head * a.out_head + 4 * h;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    typedef T T4 __attribute__((ext_vector_type(4)));
+                    *(T4 *)(d0 + d * 32 + 8 * j) = (T4){(T)(o[d][4 * j] * il), (T)(o[d][4 * j + 1] * il),
+                                                        (T)(o[d][4 * j + 2] * il), (T)(o[d][4 * j + 3] * il)};
+                }
+            if (a.lse && h == 0)
+                a.lse[(int64_t)(w.tok0 + tok) * a.NH + head] = l > 0.f ? LN2 * (m + log2f(l)) : -INFINITY;
+        } else {
+            const int64_t rec = w.rec + row;
+            float *d0 = a.po + rec * HD + 4 * h;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *(f32x4 *)(d0 + d * 32 + 8 * j) = (f32x4){o[d][4 * j] * vs, o[d][4 * j + 1] * vs, o[d][4 * j + 2] * vs,
+                                                              o[d][4 * j + 3] * vs};
+            if (h == 0) a.ml[rec] = make_float2(m, l);
+        }
     }
 }
 
-// The records of a token joined: one wave per (token, query head), lane i on values HD/64 i ...  Tokens whose item wrote the
-// output itself are left alone; a token without any key gets zeros (and lse -inf).
+template <class T, bool KV8, int HD>
+__global__ void __launch_bounds__(256, 2) k_paged_attn(AttnArgs a) {
+    extern __shared__ __align__(1024) unsigned char smem[];            // TILE_SMEM
+    __shared__ __align__(16) AttnShared sh;
+    const int n = a.n_items ? *a.n_items : gridDim.x;
+    for (int it = blockIdx.x; it < n; it += gridDim.x) {
+        const Item w = a.items[it];
+        if (it != (int)blockIdx.x) lds_barrier();                      // LDS is free of the item before
+        if (w.kind == 0) run_item<T, KV8, HD, 1>(a, w, smem, sh);
+        else if (w.kind == 1) run_item<T, KV8, HD, 2>(a, w, smem, sh);
+        else run_item<T, KV8, HD, 4>(a, w, smem, sh);
+    }
+}
+
+// The records of a token joined.  Tokens whose item wrote the output itself are left alone; a token without any key gets zeros
+// (and lse -inf).  WAVES waves of a block share a (token, query head): each takes every WAVES-th batch of records, two
+// (HD 128) or four (64) records per load and UNROLL loads in flight, and wave 0 adds the waves' sums in order.
 struct JoinArgs {
     const TokenRecs *toks;
     const int *n_toks;
@@ -373,42 +511,69 @@ struct JoinArgs {
     int64_t out_row, out_head;
     int rows, NH, G;
 };
-template <class T, int HD>
+template <class T, int HD, int WAVES>
 __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
-    const int tok = blockIdx.x, lane = threadIdx.x & 63;
-    const int head = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (tok >= min(*a.n_toks, a.rows) || head >= a.NH) return;
+    constexpr int LPR = HD / 4, RPL = 64 / LPR, UNROLL = 4;            // lanes per record, records per load
+    __shared__ f32x4 sum_s[4][LPR];
+    const int tok = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int head = blockIdx.y * (4 / WAVES) + wv / WAVES, part = wv % WAVES;
+    if (tok >= min(*a.n_toks, a.rows)) return;
     const TokenRecs t = a.toks[tok];
     if (t.parts[0] < 0 || t.parts[1] < 0) return;
-    const int kvh = head / a.G, hh = head - kvh * a.G, n = t.parts[0] + t.parts[1];
+    const bool live = head < a.NH;
+    const int kvh = (live ? head : 0) / a.G, hh = (live ? head : 0) - kvh * a.G, n = t.parts[0] + t.parts[1];
     auto rec_of = [&](int j) {
         const int w = j < t.parts[0] ? 0 : 1, p = w ? j - t.parts[0] : j;
         return ((int64_t)t.base[w] + (int64_t)(kvh * t.parts[w] + p) * t.tile[w] + t.i[w]) * a.G + hh;
     };
-    constexpr int D = HD / 64;
-    float M = -INFINITY, L = 0.f, acc[D] = {};
+    const int sub = lane / LPR, li = lane % LPR;
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int j0 = 0; j0 < n; j0 += 64) {
         const int cnt = min(64, n - j0);
+        f32x4 v[UNROLL];
+        auto fetch = [&](int b) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int j = (b + u * WAVES) * RPL + sub;             // (records past the last read the last again, weight 0)
+                v[u] = *(const f32x4 *)(a.po + rec_of(j0 + min(j, cnt - 1)) * HD + li * 4);
+            }
+        };
+        fetch(part);
         const float2 x = lane < cnt ? a.ml[rec_of(j0 + lane)] : make_float2(-INFINITY, 0.f);
         const float top = fmaxf(M, wave_max_dpp(x.x));
         const float base = top == -INFINITY ? 0.f : top;
         const float keep = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(x.x - base);
         L = L * keep + wave_sum_dpp(x.y * f);
-#pragma unroll
-        for (int d = 0; d < D; ++d) acc[d] *= keep;
+        acc *= keep;
         M = top;
-#pragma unroll 4
-        for (int j = 0; j < cnt; ++j) {
-            const float fj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), j));
-            const float *p = a.po + rec_of(j0 + j) * HD + lane * D;
+        for (int b = part; b * RPL < cnt; b += UNROLL * WAVES) {
+            if (b != part) fetch(b);
 #pragma unroll
-            for (int d = 0; d < D; ++d) acc[d] += p[d] * fj;
+            for (int u = 0; u < UNROLL; ++u) {
+                const int j = (b + u * WAVES) * RPL + sub;
+                const float fj = __shfl(f, min(j, 63));
+                acc += v[u] * (j < cnt ? fj : 0.f);
+            }
         }
     }
-    const float il = L > 0.f ? 1.f / L : 0.f;
-    T *o = (T *)a.out + (int64_t)tok * a.out_row + (int64_t)head * a.out_head + lane * D;
+    // the records of one load side by side, then the waves
 #pragma unroll
-    for (int d = 0; d < D; ++d) o[d] = (T)(acc[d] * il);
+    for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] += __shfl_xor(acc[c], o);
+    if constexpr (WAVES > 1) {
+        if (sub == 0) sum_s[wv][li] = acc;
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) acc += sum_s[wv + k][li];
+    }
+    if (!live || sub != 0) return;
+    const float il = L > 0.f ? 1.f / L : 0.f;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    *(T4 *)((T *)a.out + (int64_t)tok * a.out_row + (int64_t)head * a.out_head + li * 4) =
+        (T4){(T)(acc[0] * il), (T)(acc[1] * il), (T)(acc[2] * il), (T)(acc[3] * il)};
     if (a.lse && lane == 0) a.lse[(int64_t)tok * a.NH + head] = L > 0.f ? LN2 * (M + log2f(L)) : -INFINITY;
 }
 

@@ -58,6 +58,42 @@ bool wide_ok(const void *p, int dt, int64_t row, int64_t head) {
     return aligned(p, dt == SP_DT_E4M3 ? 8 : 16) && row % 8 == 0 && head % 8 == 0;
 }
 
+// The bytes of [rows][heads][hd] values at strides row and head (elements); empty where there are none.
+struct Span {
+    uintptr_t lo = 0, hi = 0, row = 0, width = 0;            // first and last + 1 byte; row stride, bytes of a row from its start
+    bool folded = false;                                     // rows or heads lie on top of each other, or run backwards
+};
+Span span_of(const void *p, int dt, int64_t rows, int64_t heads, int64_t hd, int64_t row, int64_t head) {
+    Span s;
+    const int b = bytes_of(dt);
+    s.folded = (rows > 1 && row < hd) || (heads > 1 && head < hd) ||
+               (rows > 1 && heads > 1 && row < (heads - 1) * head + hd && head < (rows - 1) * row + hd);
+    if (s.folded || !rows || !heads) return s;
+    s.lo = (uintptr_t)p;
+    s.width = ((heads - 1) * head + hd) * b;
+    s.row = row * b;
+    s.hi = s.lo + (rows - 1) * s.row + s.width;
+    return s;
+}
+// Whether two spans may share a byte: they do not where their rows have one stride and lie beside each other in it.
+bool overlap(const Span &a, const Span &b) {
+    if (a.lo >= b.hi || b.lo >= a.hi) return false;
+    if (a.row != b.row || !a.row || a.width > a.row || b.width > b.row) return true;
+    const uintptr_t off = b.lo >= a.lo ? (b.lo - a.lo) % a.row : (a.row - (a.lo - b.lo) % a.row) % a.row;
+    return off < a.width || off + b.width > a.row;
+}
+bool may_overlap(const Span &out, const void *p, int dt, int64_t rows, int64_t heads, int64_t hd, int64_t row, int64_t head) {
+    const Span in = span_of(p, dt, rows, heads, hd, row, head);
+    if (!in.folded) return overlap(out, in);
+    // rows or heads of the input repeat (stride 0, sliding windows): its outer bytes
+    const int b = bytes_of(dt);
+    const int64_t r = (rows - 1) * row, h = (heads - 1) * head;
+    const intptr_t lo = (intptr_t)p + (std::min<int64_t>(r, 0) + std::min<int64_t>(h, 0)) * b;
+    const intptr_t hi = (intptr_t)p + (std::max<int64_t>(r, 0) + std::max<int64_t>(h, 0) + hd) * b;
+    return lo < (intptr_t)out.hi && (intptr_t)out.lo < hi;
+}
+void check_output(const Span &out) { require(!out.folded, SP_EINVAL, "the output's rows or heads lie on top of each other"); }
+
 // Rows of a block and its threads: about 256 threads a block, whole rows.
 void shape_of(int per_row, int rows, int &per_block, int &threads) {
     per_block = std::max(1, std::min(rows, 256 / per_row));
@@ -87,16 +123,16 @@ void check_cache(const sp_paged_kv *kv) {
 
 struct sp_attn_plan {
     int NH = 0, NKV = 0, HD = 0, max_rows = 0, max_seqs = 0, device = 0;
-    // device block: header [16] (items of each kind, tokens), token records, items of each kind at fixed places
+    // device block: header [16] (items, tokens), items, and token records, at fixed places
     int32_t *dev = nullptr;
-    size_t tok_at = 0, item_at[KINDS] = {}, words = 0;
+    size_t tok_at = 0, item_at = 0, words = 0;
     int32_t *staging[2] = {};            // pinned images of the block, used in turn
     hipEvent_t copied[2] = {};
     bool used[2] = {};
     int turn = 0;
     // the last set()
     bool set = false, joined = false;
-    int n_items[KINDS] = {}, n_tok = 0, n_seq = 0, max_kv = 0;
+    int n_items = 0, n_tok = 0, n_seq = 0, max_kv = 0, most_parts = 0;
 
     void release() {
         for (int i = 0; i < 2; ++i) {
@@ -114,12 +150,8 @@ constexpr size_t HEADER = 16;
 // The plan's shape and where its tables lie (words).
 void lay_out(sp_attn_plan &p) {
     p.tok_at = HEADER;
-    size_t at = HEADER + (size_t)p.max_rows * (sizeof(TokenRecs) / 4);
-    for (int k = 0; k < KINDS; ++k) {
-        p.item_at[k] = at;
-        at += (size_t)items_bound(p.max_rows, p.NKV) * (sizeof(Item) / 4);
-    }
-    p.words = at;
+    p.item_at = p.tok_at + (size_t)p.max_rows * (sizeof(TokenRecs) / 4);
+    p.words = p.item_at + (size_t)items_bound(p.max_rows, p.NKV) * (sizeof(Item) / 4);
 }
 
 void check_shape(int NH, int NKV, int HD, int max_rows, int max_seqs) {
@@ -166,20 +198,20 @@ void tables_of(int NH, int NKV, int n_seq, const int32_t *q_len, const int32_t *
     }
 }
 
-template <class T, bool KV8, int HD, int WM>
-void launch_items(const AttnArgs &a, int grid, hipStream_t st) {
-    hipLaunchKernelGGL((k_paged_attn<T, KV8, HD, WM>), dim3(grid), dim3(256), (AttnTile<KV8, HD, WM>::SMEM), st, a);
-}
 template <class T, bool KV8, int HD>
-void launch_kind(int kind, const AttnArgs &a, int grid, hipStream_t st) {
-    if (kind == 0) launch_items<T, KV8, HD, 1>(a, grid, st);
-    else if (kind == 1) launch_items<T, KV8, HD, 2>(a, grid, st);
-    else launch_items<T, KV8, HD, 4>(a, grid, st);
+void launch_items(const AttnArgs &a, int grid, hipStream_t st) {
+    hipLaunchKernelGGL((k_paged_attn<T, KV8, HD>), dim3(grid), dim3(256), TILE_SMEM, st, a);
 }
 template <class T>
-void launch_typed(bool kv8, int HD, int kind, const AttnArgs &a, int grid, hipStream_t st) {
-    if (kv8) { if (HD == 128) launch_kind<T, true, 128>(kind, a, grid, st); else launch_kind<T, true, 64>(kind, a, grid, st); }
-    else { if (HD == 128) launch_kind<T, false, 128>(kind, a, grid, st); else launch_kind<T, false, 64>(kind, a, grid, st); }
+void launch_typed(bool kv8, int HD, const AttnArgs &a, int grid, hipStream_t st) {
+    if (kv8) { if (HD == 128) launch_items<T, true, 128>(a, grid, st); else launch_items<T, true, 64>(a, grid, st); }
+    else { if (HD == 128) launch_items<T, false, 128>(a, grid, st); else launch_items<T, false, 64>(a, grid, st); }
+}
+// Few records: a wave joins a (token, head); many: the block's four share it.
+template <class T, int HD>
+void launch_join(const JoinArgs &j, int tokens, int most_parts, hipStream_t st) {
+    if (most_parts > 8) hipLaunchKernelGGL((k_paged_join<T, HD, 4>), dim3(tokens, j.NH), dim3(256), 0, st, j);
+    else hipLaunchKernelGGL((k_paged_join<T, HD, 1>), dim3(tokens, (j.NH + 3) / 4), dim3(256), 0, st, j);
 }
 
 // Blocks of a captured launch, whose item counts may change between replays: each block walks the items grid by grid.
@@ -195,22 +227,32 @@ int sp_op_rotate(const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t
     return guarded([&] {
         require(dtype == SP_DT_F32 || dtype == SP_DT_F16 || dtype == SP_DT_BF16, SP_EINVAL,
                 "dtype must be SP_DT_F32, SP_DT_F16 or SP_DT_BF16");
-        require(n_rows >= 0 && n_heads >= 1 && head_dim >= 2 && head_dim <= 1024 && (int64_t)n_heads * head_dim <= (1 << 20),
-                SP_EINVAL, "n_rows must not be negative, head_dim in [2, 1024] and n_heads * head_dim at most 2^20");
+        require(n_rows >= 0 && n_heads >= 1 && head_dim >= 2 && head_dim <= 1024 && (int64_t)n_heads * head_dim < (1 << 16),
+                SP_EINVAL, "n_rows must not be negative, head_dim in [2, 1024] and n_heads * head_dim below 2^16");
         require(rotary != nullptr, SP_EINVAL, "rotary is NULL");
         const Rotation rot = rotation_of(rotary, head_dim);
         if (n_rows == 0) return;
         require(x_dev && out_dev && pos_dev, SP_EINVAL, "NULL pointer");
-        const bool in_place = x_dev == out_dev;
-        require(!in_place || (x_row == out_row && x_head == out_head), SP_EINVAL, "in place, the strides must be the same");
-        RotateArgs a{rot, x_dev, out_dev, x_row, x_head, out_row, out_head, pos_dev, n_rows, n_heads, head_dim, dtype, 1, 0, 0};
+        const bool in_place = x_dev == out_dev && x_row == out_row && x_head == out_head;
+        const Span to = span_of(out_dev, dtype, n_rows, n_heads, head_dim, out_row, out_head);
+        check_output(to);
+        require(in_place || !may_overlap(to, x_dev, dtype, n_rows, n_heads, head_dim, x_row, x_head), SP_EINVAL,
+                "the output overlaps the input");
+        RotateArgs a{};
+        a.rot = rot;
+        a.x = x_dev; a.out = out_dev;
+        a.x_row = x_row; a.x_head = x_head; a.out_row = out_row; a.out_head = out_head;
+        a.pos = pos_dev;
+        a.rows = n_rows; a.heads = n_heads;
         const bool wide = wide_ok(x_dev, dtype, x_row, x_head) && wide_ok(out_dev, dtype, out_row, out_head) &&
                           rot.rot % 16 == 0 && head_dim % 8 == 0;
         const int vec = wide ? 8 : 1;
         a.units = rot.rot / 2 / vec;
-        a.tail = in_place ? 0 : (head_dim - rot.rot) / vec;
+        a.per_head = a.units + (in_place ? 0 : (head_dim - rot.rot) / vec);
+        a.per_row = n_heads * a.per_head;
+        a.by_row = Divisor(a.per_row); a.by_head = Divisor(a.per_head); a.by_half = Divisor(rot.rot / 2);
         int threads;
-        shape_of(n_heads * (a.units + a.tail), n_rows, a.per_block, threads);
+        shape_of(a.per_row, n_rows, a.per_block, threads);
         for_input(dtype, wide, [&](auto *t, auto v) {
             hipLaunchKernelGGL((k_rotate<std::remove_pointer_t<decltype(t)>, decltype(v)::value>),
                                dim3((n_rows + a.per_block - 1) / a.per_block), dim3(threads),
@@ -230,17 +272,24 @@ int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t d
         require(dtype == SP_DT_F32 || dtype == SP_DT_F16 || dtype == SP_DT_BF16, SP_EINVAL,
                 "dtype must be SP_DT_F32, SP_DT_F16 or SP_DT_BF16");
         const int hd = kv->head_dim, nq = q_dev ? n_heads : 0;
-        require(hd <= 1024 && n_rows >= 0 && (!q_dev || n_heads >= 1) && (int64_t)(std::max(nq, 0) + 2 * (int64_t)kv->n_kv_heads) * hd <= (1 << 20),
-                SP_EINVAL, "n_rows must not be negative, head_dim at most 1024 and the values of a row at most 2^20");
+        require(hd <= 1024 && n_rows >= 0 && (!q_dev || n_heads >= 1) && (std::max(nq, 0) + 2 * (int64_t)kv->n_kv_heads) * hd < (1 << 16),
+                SP_EINVAL, "n_rows must not be negative, head_dim at most 1024 and the values of a row below 2^16");
         require((q_dev != nullptr) == (q_out_dev != nullptr), SP_EINVAL, "q_dev and q_out_dev come together");
         require(!q_dev || q_out_dtype == SP_DT_F32 || q_out_dtype == SP_DT_F16 || q_out_dtype == SP_DT_BF16, SP_EINVAL,
                 "q_out_dtype must be SP_DT_F32, SP_DT_F16 or SP_DT_BF16");
-        require(!q_dev || q_dev != q_out_dev || (q_out_dtype == dtype && q_row == q_out_row && q_head == q_out_head), SP_EINVAL,
-                "in place, the queries' type and strides must be the same");
         require(n_seq >= 1 && max_pages >= 1, SP_EINVAL, "n_seq and max_pages must be positive");
         const Rotation rot = rotation_of(rotary, hd);
         if (n_rows == 0) return;
         require(k_dev && v_dev && seq_dev && at_dev && table_dev && (!rotary || pos_dev), SP_EINVAL, "NULL pointer");
+        if (q_dev) {
+            const bool in_place = q_dev == q_out_dev && q_out_dtype == dtype && q_row == q_out_row && q_head == q_out_head;
+            const Span to = span_of(q_out_dev, q_out_dtype, n_rows, nq, hd, q_out_row, q_out_head);
+            check_output(to);
+            require((in_place || !may_overlap(to, q_dev, dtype, n_rows, nq, hd, q_row, q_head)) &&
+                        !may_overlap(to, k_dev, dtype, n_rows, kv->n_kv_heads, hd, k_row, k_head) &&
+                        !may_overlap(to, v_dev, dtype, n_rows, kv->n_kv_heads, hd, v_row, v_head),
+                    SP_EINVAL, "the rotated queries overlap an input");
+        }
         AppendArgs a{};
         a.rot = rot;
         a.q = q_dev; a.k = k_dev; a.v = v_dev;
@@ -260,8 +309,13 @@ int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t d
         a.units = rot.rot / 2 / vec;
         a.tail = (hd - rot.rot) / vec;
         a.vecs = hd / vec;
+        a.turned = (nq + a.nkv) * a.units;
+        a.rest = (nq + a.nkv) * a.tail;
+        a.per_row = a.turned + a.rest + a.nkv * a.vecs;
+        a.by_row = Divisor(a.per_row); a.by_units = Divisor(a.units); a.by_tail = Divisor(a.tail); a.by_vecs = Divisor(a.vecs);
+        a.by_half = Divisor(rot.rot / 2);
         int threads;
-        shape_of((nq + a.nkv) * (a.units + a.tail) + a.nkv * a.vecs, n_rows, a.per_block, threads);
+        shape_of(a.per_row, n_rows, a.per_block, threads);
         for_input(dtype, wide, [&](auto *t, auto v) {
             hipLaunchKernelGGL((k_append<std::remove_pointer_t<decltype(t)>, decltype(v)::value>),
                                dim3((n_rows + a.per_block - 1) / a.per_block), dim3(threads),
@@ -316,22 +370,20 @@ int sp_attn_plan_set(sp_attn_plan *p, int32_t n_seq, const int32_t *q_len, const
         if (p->used[turn]) HIPCHK(hipEventSynchronize(p->copied[turn]));
         int32_t *img = p->staging[turn];
         std::memset(img, 0, HEADER * sizeof(int32_t));
-        for (int k = 0; k < KINDS; ++k) img[k] = (int32_t)t.items[k].size();
-        img[KINDS] = (int32_t)t.toks.size();
-        auto put = [&](size_t at, const void *data, size_t bytes) {
-            if (!bytes) return;
-            std::memcpy(img + at, data, bytes);
-            HIPCHK(hipMemcpyAsync(p->dev + at, img + at, bytes, hipMemcpyHostToDevice, st));
-        };
-        p->set = false;                                  // until every table is on its way
-        // header and token records lie side by side: one copy; then the items of each kind
+        img[0] = (int32_t)t.items.size();
+        img[1] = (int32_t)t.toks.size();
+        p->set = false;                                  // until the tables are on their way
+        // header and token records lie side by side: one copy; then the items
         std::memcpy(img + p->tok_at, t.toks.data(), t.toks.size() * sizeof(TokenRecs));
+        std::memcpy(img + p->item_at, t.items.data(), t.items.size() * sizeof(Item));
         HIPCHK(hipMemcpyAsync(p->dev, img, (HEADER + t.toks.size() * (sizeof(TokenRecs) / 4)) * 4, hipMemcpyHostToDevice, st));
-        for (int k = 0; k < KINDS; ++k) put(p->item_at[k], t.items[k].data(), t.items[k].size() * sizeof(Item));
+        if (!t.items.empty())
+            HIPCHK(hipMemcpyAsync(p->dev + p->item_at, img + p->item_at, t.items.size() * sizeof(Item), hipMemcpyHostToDevice, st));
         HIPCHK(hipEventRecord(p->copied[turn], st));
         p->used[turn] = true;
         p->turn = turn ^ 1;
-        for (int k = 0; k < KINDS; ++k) p->n_items[k] = (int)t.items[k].size();
+        p->n_items = (int)t.items.size();
+        p->most_parts = t.most_parts;
         p->n_tok = (int)t.toks.size();
         p->n_seq = n_seq;
         p->max_kv = t.max_kv;
@@ -341,21 +393,21 @@ int sp_attn_plan_set(sp_attn_plan *p, int32_t n_seq, const int32_t *q_len, const
 }
 
 int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len,
-                       int32_t n_groups, const int32_t *group_size, const int32_t *group_shared, int32_t kind, int32_t capacity,
+                       int32_t n_groups, const int32_t *group_size, const int32_t *group_shared, int32_t capacity,
                        int32_t *items, int32_t *n_items, int32_t *token_recs, int64_t *n_records) {
     return guarded([&] {
         check_shape(n_heads, n_kv_heads, 64, 1, 1);
-        require(kind >= 0 && kind < KINDS && n_items, SP_EINVAL, "kind must be 0, 1 or 2, and n_items not NULL");
+        require(n_items != nullptr, SP_EINVAL, "n_items is NULL");
         check_lengths(n_seq, q_len, kv_len, n_groups, group_size, group_shared, (1 << 27) / n_heads, 65535);
         PlanTables t;
         tables_of(n_heads, n_kv_heads, n_seq, q_len, kv_len, n_groups, group_size, group_shared, t);
-        *n_items = (int32_t)t.items[kind].size();
+        *n_items = (int32_t)t.items.size();
         if (n_records) *n_records = t.records;
         if (items) {
             require(capacity >= *n_items, SP_ECAPACITY, "capacity is smaller than the number of items");
-            std::memcpy(items, t.items[kind].data(), t.items[kind].size() * sizeof(Item));
+            if (!t.items.empty()) std::memcpy(items, t.items.data(), t.items.size() * sizeof(Item));
         }
-        if (token_recs) std::memcpy(token_recs, t.toks.data(), t.toks.size() * sizeof(TokenRecs));
+        if (token_recs && !t.toks.empty()) std::memcpy(token_recs, t.toks.data(), t.toks.size() * sizeof(TokenRecs));
     });
 }
 
@@ -386,6 +438,11 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         if (p->n_tok == 0) return;
         require(q_dev && out_dev && table_dev && workspace_dev, SP_EINVAL, "NULL pointer");
         require(aligned(q_dev, 16) && q_row % 8 == 0 && q_head % 8 == 0, SP_EINVAL, "queries must be aligned to 16 bytes");
+        {
+            const Span to = span_of(out_dev, dtype, n_rows, p->NH, p->HD, out_row, out_head);
+            check_output(to);
+            require(!may_overlap(to, q_dev, dtype, n_rows, p->NH, p->HD, q_row, q_head), SP_EINVAL, "the output overlaps the queries");
+        }
         require(aligned(out_dev, 8) && out_row % 4 == 0 && out_head % 4 == 0, SP_EINVAL, "outputs must be aligned to 8 bytes");
         require(aligned(kv->k_dev, 16) && aligned(kv->v_dev, 16) && kv->page_stride * bytes_of(kv->dtype) % 16 == 0 &&
                     kv->head_dim * bytes_of(kv->dtype) % 16 == 0,
@@ -406,25 +463,24 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         a.po = (float *)workspace_dev;
         a.ml = (float2 *)(a.po + recs * p->HD);
         const bool kv8 = kv->dtype == SP_DT_E4M3;
-        for (int k = KINDS - 1; k >= 0; --k) {
-            const int grid = capturing ? CAPTURED_GRID : p->n_items[k];
-            if (!grid) continue;
-            a.items = (const Item *)(p->dev + p->item_at[k]);
-            a.n_items = p->dev + k;
-            if (dtype == SP_DT_F16) launch_typed<f16>(kv8, p->HD, k, a, grid, st);
-            else launch_typed<bf16>(kv8, p->HD, k, a, grid, st);
+        a.items = (const Item *)(p->dev + p->item_at);
+        a.n_items = capturing ? p->dev : nullptr;
+        const int grid = capturing ? CAPTURED_GRID : p->n_items;
+        if (grid) {
+            if (dtype == SP_DT_F16) launch_typed<f16>(kv8, p->HD, a, grid, st);
+            else launch_typed<bf16>(kv8, p->HD, a, grid, st);
             HIPCHK(hipGetLastError());
         }
         if (p->joined || capturing) {
-            const JoinArgs j{(const TokenRecs *)(p->dev + p->tok_at), p->dev + KINDS, a.po, a.ml, out_dev, lse_dev, out_row, out_head,
+            const JoinArgs j{(const TokenRecs *)(p->dev + p->tok_at), p->dev + 1, a.po, a.ml, out_dev, lse_dev, out_row, out_head,
                              n_rows, p->NH, a.G};
-            const dim3 grid(capturing ? std::min(n_rows, p->max_rows) : p->n_tok, (p->NH + 3) / 4);
+            const int tokens = capturing ? std::min(n_rows, p->max_rows) : p->n_tok;
             if (dtype == SP_DT_F16) {
-                if (p->HD == 128) hipLaunchKernelGGL((k_paged_join<f16, 128>), grid, dim3(256), 0, st, j);
-                else hipLaunchKernelGGL((k_paged_join<f16, 64>), grid, dim3(256), 0, st, j);
+                if (p->HD == 128) launch_join<f16, 128>(j, tokens, p->most_parts, st);
+                else launch_join<f16, 64>(j, tokens, p->most_parts, st);
             } else {
-                if (p->HD == 128) hipLaunchKernelGGL((k_paged_join<bf16, 128>), grid, dim3(256), 0, st, j);
-                else hipLaunchKernelGGL((k_paged_join<bf16, 64>), grid, dim3(256), 0, st, j);
+                if (p->HD == 128) launch_join<bf16, 128>(j, tokens, p->most_parts, st);
+                else launch_join<bf16, 64>(j, tokens, p->most_parts, st);
             }
             HIPCHK(hipGetLastError());
         }

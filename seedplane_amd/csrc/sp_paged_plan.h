@@ -22,6 +22,8 @@ struct Item {                        // one block's work
     int32_t k0, k1;                  // positions read
     int32_t pos0;                    // token tok0 + i sees positions <= pos0 + i (ALL_SEEN: every one)
     int32_t rec;                     // first record (row r of the tile leaves record rec + r), -1: the output itself
+    int32_t kind;                    // row tile of 32 << kind rows
+    int32_t reserved[3];
 };
 struct TokenRecs {                   // the records of a token: record (kvh * parts + j) * tile + i, times G, from base
     int32_t base[2], parts[2], tile[2], i[2];     // of the shared positions, of its own
@@ -29,31 +31,32 @@ struct TokenRecs {                   // the records of a token: record (kvh * pa
 constexpr int32_t ALL_SEEN = 1 << 30;
 constexpr int KINDS = 3;                                       // row tiles of 32 << kind rows
 constexpr int TILE_ROWS_OF[KINDS] = {32, 64, 128};
-constexpr int KEY_STEP[KINDS] = {128, 64, 64};                // keys a block reads per round
+constexpr int KEY_STEP = 64;                                   // parts are whole steps of keys
+// Cost of a step by kind, in units of a 128-row tile's (bound by its matrix products); the others read their keys for few rows
+// and are bound by memory.  And the fewest steps of a part: shorter ones cost more in records and latency than they spread.
+constexpr int STEP_COST[KINDS] = {1, 1, 1};
+constexpr int LEAST_STEPS[KINDS] = {2, 2, 2};
 constexpr int MAX_GROUP = 32;                                  // query heads per K/V head
 
 struct Segment {
-    int32_t tok0, ntok, seq, k0, k1, pos0, which;              // which: 0 shared, 1 own
+    int32_t tok0, ntok, seq, k0, k1, pos0, which, kind;        // which: 0 shared, 1 own
 };
 
 struct PlanTables {
-    std::vector<Item> items[KINDS];
+    std::vector<Item> items;         // the costliest first
     std::vector<TokenRecs> toks;
     bool joined = false;             // some token needs the join
+    int32_t most_parts = 0;          // most records of a token that does
     int64_t records = 0;             // rows of records
     int32_t max_kv = 0;
 };
 
-// Items of each kind the plan aims at: enough to fill 256 CUs.
-constexpr int ITEM_TARGET[KINDS] = {512, 512, 512};
-// Records at most: a kind whose tiles are cut has at most ITEM_TARGET items, one whose tiles are not leaves at most one
-// record per row and range.
-inline int64_t records_bound(int64_t rows, int n_heads) {
-    int64_t n = 2 * rows * n_heads;
-    for (int k = 0; k < KINDS; ++k) n += (int64_t)ITEM_TARGET[k] * TILE_ROWS_OF[k];
-    return n;
-}
-inline int64_t items_bound(int64_t rows, int n_kv) { return 2 * rows * n_kv + 512; }      // of one kind
+// A part has the ITEM_TARGET-th of the whole cost: two blocks on each of 256 CUs get about the same; shorter tiles fill in.
+constexpr int ITEM_TARGET = 512;
+// Most rows of records: a tile that is not cut leaves one record per row and range; the parts of those that are, each of more
+// than one part's cost, are fewer than 2 ITEM_TARGET.
+inline int64_t records_bound(int64_t rows, int n_heads) { return 2 * rows * n_heads + (int64_t)2 * ITEM_TARGET * 128; }
+inline int64_t items_bound(int64_t rows, int n_kv) { return 2 * rows * n_kv + ITEM_TARGET; }
 
 inline int kind_of(int64_t rows) { return rows <= 32 ? 0 : rows <= 64 ? 1 : 2; }
 
@@ -62,7 +65,7 @@ inline int kind_of(int64_t rows) { return rows <= 32 ? 0 : rows <= 64 ? 1 : 2; }
 inline void make_plan(int n_heads, int n_kv, int n_seq, const int32_t *q_len, const int32_t *kv_len, int n_groups,
                       const int32_t *group_size, const int32_t *group_shared, PlanTables &out) {
     const int G = n_heads / n_kv;
-    std::vector<Segment> segs[KINDS];
+    std::vector<Segment> segs;
     int32_t n_tok = 0;
     out = PlanTables{};
     auto add = [&](int32_t tok0, int32_t ntok, int32_t seq, int32_t k0, int32_t k1, int32_t pos0, int which) {
@@ -70,7 +73,7 @@ inline void make_plan(int n_heads, int n_kv, int n_seq, const int32_t *q_len, co
         for (int32_t t = 0; t < ntok; t += per) {
             const int32_t n = std::min(per, ntok - t);
             const int32_t end = which ? std::min(k1, pos0 + t + n) : k1;     // the tile's last token sees positions < end
-            if (end > k0) segs[kind].push_back({tok0 + t, n, seq, k0, end, which ? pos0 + t : ALL_SEEN, which});
+            if (end > k0) segs.push_back({tok0 + t, n, seq, k0, end, which ? pos0 + t : ALL_SEEN, which, kind});
         }
     };
     int s0 = 0;
@@ -93,69 +96,50 @@ inline void make_plan(int n_heads, int n_kv, int n_seq, const int32_t *q_len, co
         s0 += group_size[g];
     }
     out.toks.assign(n_tok, TokenRecs{});
-    for (int k = 0; k < KINDS; ++k) {
-        // the shortest part length whose parts fit the target
-        auto parts_at = [&](int64_t len) {
-            int64_t n = 0;
-            for (const Segment &s : segs[k]) n += (s.k1 - s.k0 + len - 1) / len;
-            return n * n_kv;
-        };
-        int64_t lo = 2, hi = 2;                                              // in key steps
-        int32_t longest = 0;
-        for (const Segment &s : segs[k]) longest = std::max(longest, s.k1 - s.k0);
-        hi = std::max<int64_t>(lo, (longest + KEY_STEP[k] - 1) / KEY_STEP[k]);
-        const int64_t most = std::max<int64_t>(ITEM_TARGET[k], (int64_t)segs[k].size() * n_kv);
-        while (lo < hi) {
-            const int64_t mid = (lo + hi) / 2;
-            if (parts_at(mid * KEY_STEP[k]) <= most) hi = mid;
-            else lo = mid + 1;
+    auto steps_of = [](const Segment &s) { return (int64_t)(s.k1 - s.k0 + KEY_STEP - 1) / KEY_STEP; };
+    int64_t total = 0;
+    for (const Segment &s : segs) total += steps_of(s) * STEP_COST[s.kind] * n_kv;
+    const int64_t share = (total + ITEM_TARGET - 1) / ITEM_TARGET;
+    auto parts_of = [&](const Segment &s) {
+        const int64_t len = std::max<int64_t>(LEAST_STEPS[s.kind], (share + STEP_COST[s.kind] - 1) / STEP_COST[s.kind]);
+        return (steps_of(s) + len - 1) / len;
+    };
+    for (const Segment &s : segs)
+        for (int i = 0; i < s.ntok; ++i) {
+            TokenRecs &t = out.toks[s.tok0 + i];
+            t.parts[s.which] = (int32_t)parts_of(s);
+            t.tile[s.which] = s.ntok;
+            t.i[s.which] = i;
         }
-        const int64_t len = lo * KEY_STEP[k];
-        for (const Segment &s : segs[k]) {
-            const int32_t parts = (int32_t)((s.k1 - s.k0 + len - 1) / len);
-            for (int i = 0; i < s.ntok; ++i) {
-                TokenRecs &t = out.toks[s.tok0 + i];
-                t.parts[s.which] = parts;
-                t.tile[s.which] = s.ntok;
-                t.i[s.which] = i;
-            }
-        }
-        for (const Segment &s : segs[k]) {
-            const int32_t parts = out.toks[s.tok0].parts[s.which];
-            // parts of nearly equal length, whole key steps
-            const int64_t steps = (s.k1 - s.k0 + KEY_STEP[k] - 1) / KEY_STEP[k];
-            for (int h = 0; h < n_kv; ++h)
-                for (int j = 0; j < parts; ++j) {
-                    const int32_t a = s.k0 + (int32_t)(steps * j / parts) * KEY_STEP[k];
-                    const int32_t b = j + 1 == parts ? s.k1 : s.k0 + (int32_t)(steps * (j + 1) / parts) * KEY_STEP[k];
-                    out.items[k].push_back({s.tok0, s.ntok, h, s.seq, a, b, s.pos0, 0});
-                }
-        }
-    }
     // records: a tile's block of (K/V head, part, token) rows, unless the tile's tokens have no other range or part
-    for (int k = 0; k < KINDS; ++k) {
-        size_t at = 0;
-        for (const Segment &s : segs[k]) {
-            const TokenRecs &t0 = out.toks[s.tok0];
-            const int32_t parts = t0.parts[s.which];
-            bool alone = parts == 1;
-            for (int i = 0; i < s.ntok && alone; ++i) alone = out.toks[s.tok0 + i].parts[1 - s.which] == 0;
-            const int64_t base = out.records;
-            if (alone) {
-                for (int i = 0; i < s.ntok; ++i) out.toks[s.tok0 + i].parts[s.which] = -1;     // written by its item
-            } else {
-                for (int i = 0; i < s.ntok; ++i) out.toks[s.tok0 + i].base[s.which] = (int32_t)(base / G);
-                out.records += (int64_t)n_kv * parts * s.ntok * G;
-            }
-            for (int h = 0; h < n_kv; ++h)
-                for (int j = 0; j < parts; ++j, ++at)
-                    out.items[k][at].rec = alone ? -1 : (int32_t)(base + ((int64_t)h * parts + j) * s.ntok * G);
+    for (const Segment &s : segs) {
+        const int32_t parts = out.toks[s.tok0].parts[s.which];
+        bool alone = parts == 1;
+        for (int i = 0; i < s.ntok && alone; ++i) alone = out.toks[s.tok0 + i].parts[1 - s.which] == 0;
+        const int64_t base = out.records;
+        for (int i = 0; i < s.ntok; ++i) {
+            TokenRecs &t = out.toks[s.tok0 + i];
+            if (alone) t.parts[s.which] = -1;                                // written by its item
+            else t.base[s.which] = (int32_t)(base / G);
         }
-        std::stable_sort(out.items[k].begin(), out.items[k].end(),
-                         [](const Item &x, const Item &y) { return x.k1 - x.k0 > y.k1 - y.k0; });
+        if (!alone) out.records += (int64_t)n_kv * parts * s.ntok * G;
+        const int64_t steps = steps_of(s);
+        for (int h = 0; h < n_kv; ++h)
+            for (int j = 0; j < parts; ++j) {                                // parts of nearly equal length
+                const int32_t a = s.k0 + (int32_t)(steps * j / parts) * KEY_STEP;
+                const int32_t b = j + 1 == parts ? s.k1 : s.k0 + (int32_t)(steps * (j + 1) / parts) * KEY_STEP;
+                out.items.push_back({s.tok0, s.ntok, h, s.seq, a, b, s.pos0,
+                                     alone ? -1 : (int32_t)(base + ((int64_t)h * parts + j) * s.ntok * G), s.kind, {0, 0, 0}});
+            }
     }
+    std::stable_sort(out.items.begin(), out.items.end(), [](const Item &x, const Item &y) {
+        return (int64_t)(x.k1 - x.k0) * STEP_COST[x.kind] > (int64_t)(y.k1 - y.k0) * STEP_COST[y.kind];
+    });
     for (const TokenRecs &t : out.toks)
-        out.joined |= t.parts[0] >= 0 && t.parts[1] >= 0;        // records to join, or no key at all (zeros)
+        if (t.parts[0] >= 0 && t.parts[1] >= 0) {                            // records to join, or no key at all (zeros)
+            out.joined = true;
+            out.most_parts = std::max(out.most_parts, t.parts[0] + t.parts[1]);
+        }
 }
 
 }  // namespace paged

@@ -11,6 +11,8 @@
 // takes whole rows: its threads load their values, then form the rows' (cos, sin) table in LDS, each pair once for all heads
 // (a thread per pair and head would spend more on angles than on memory), then rotate and store.
 #pragma once
+#include <algorithm>
+
 #include "sp_device.h"
 #include "../../include/seedplane_hip.h"
 
@@ -125,56 +127,68 @@ __device__ __forceinline__ void turn_unit(const Rotation &r, const float2 *cs, f
 
 constexpr int ROT_MAX_THREADS = 512;
 
+// n / d for n, d < 2^16 by a multiplication: the rounded-up reciprocal is off by less than 2^-32 d, so n times it is off by
+// less than one part of d.
+struct Divisor {
+    uint32_t inverse, d;
+    Divisor() = default;
+    explicit Divisor(int v) : inverse((uint32_t)((((uint64_t)1 << 32) + v - 1) / std::max(v, 1))), d(v) {}
+};
+__device__ __forceinline__ int operator/(int n, Divisor v) { return v.d == 1 ? n : (int)__umulhi((uint32_t)n, v.inverse); }
+
 struct RotateArgs {
     Rotation rot;
     const void *x;
     void *out;
     int64_t x_row, x_head, out_row, out_head;    // elements
     const int *pos;
-    int rows, heads, hd, dt, per_block;          // rows per block
-    int units, tail;                             // units of a head's rotated part, and vectors of its rest (0: in place)
+    int rows, heads, per_block;                  // rows per block
+    int units, per_head, per_row;                // units of a head's rotated part; with the vectors of its rest (none in place)
+    Divisor by_row, by_head, by_half;
 };
+
+// Angles of the block's rows: cs [n][rot / 2]
+__device__ __forceinline__ void turn_rows(const Rotation &rot, const int *pos, int n, Divisor by_half, float2 *cs) {
+    const int half = rot.rot >> 1;
+    for (int k = threadIdx.x; k < n * half; k += blockDim.x) {
+        const int r = k / by_half;
+        cs[k] = turn_of(rot, pos[r], k - r * half);
+    }
+}
+
+template <class T> constexpr int dtype_of() { return sizeof(T) == 4 ? SP_DT_F32 : std::is_same<T, f16>::value ? SP_DT_F16 : SP_DT_BF16; }
 
 template <class T, int VEC>
 __global__ void __launch_bounds__(ROT_MAX_THREADS) k_rotate(RotateArgs a) {
     extern __shared__ __align__(16) unsigned char rot_smem[];
-    float2 *cs = (float2 *)rot_smem;                                   // [rows of the block][rot / 2]
+    float2 *cs = (float2 *)rot_smem;
     const int row0 = blockIdx.x * a.per_block, n = min(a.per_block, a.rows - row0), half = a.rot.rot >> 1;
-    const int per_head = a.units + a.tail, per_row = per_head * a.heads, total = n * per_row;
+    const int total = n * a.per_row;
     float v1[VEC], v2[VEC];
     int at1 = 0, at2 = 0, r = 0, head = 0, u = 0;
-    const T *src = nullptr;
+    // (the unrotated rest has one vector: v2 repeats it and is not stored)
     auto fetch = [&](int i) {
-        r = i / per_row;
-        const int k = i - r * per_row;
-        head = k / per_head;
-        u = k - head * per_head;
-        src = (const T *)a.x + (int64_t)(row0 + r) * a.x_row + (int64_t)head * a.x_head;
-        if (u < a.units) {
-            unit_offsets<VEC>(a.rot, u, at1, at2);
-            load_values<T, VEC>(src + at1, v1);
-            load_values<T, VEC>(src + at2, v2);
-        } else {
-            at1 = a.rot.rot + (u - a.units) * VEC;
-            load_values<T, VEC>(src + at1, v1);
-        }
+        r = i / a.by_row;
+        const int k = i - r * a.per_row;
+        head = k / a.by_head;
+        u = k - head * a.per_head;
+        unit_offsets<VEC>(a.rot, u, at1, at2);
+        if (u >= a.units) at1 = at2 = a.rot.rot + (u - a.units) * VEC;
+        const T *src = (const T *)a.x + (int64_t)(row0 + r) * a.x_row + (int64_t)head * a.x_head;
+        load_values<T, VEC>(src + at1, v1);
+        load_values<T, VEC>(src + at2, v2);
     };
     int i = threadIdx.x;
     if (i < total) fetch(i);
-    for (int k = threadIdx.x; k < n * half; k += blockDim.x) {
-        const int rr = k / half;
-        cs[k] = turn_of(a.rot, a.pos[row0 + rr], k - rr * half);
-    }
+    turn_rows(a.rot, a.pos + row0, n, a.by_half, cs);
     __syncthreads();
     while (i < total) {
         const int64_t to = (int64_t)(row0 + r) * a.out_row + (int64_t)head * a.out_head;
         if (u < a.units) {
             turn_unit<VEC>(a.rot, cs + r * half + u * VEC, v1, v2);
-            store_values<VEC>(a.out, to + at1, a.dt, v1);
-            store_values<VEC>(a.out, to + at2, a.dt, v2);
-        } else {
-            store_values<VEC>(a.out, to + at1, a.dt, v1);
+            store_values<VEC>(a.out, to + at2, dtype_of<T>(), v2);
         }
+        store_values<VEC>(a.out, to + at1, dtype_of<T>(), v1);
         i += blockDim.x;
         if (i < total) fetch(i);
     }
@@ -192,6 +206,8 @@ struct AppendArgs {
     int n_seq, max_pages, n_pages, page_size;
     int64_t page_stride;
     int units, tail, vecs;                       // of a head: rotated units, vectors of the rest, vectors of a value
+    int turned, rest, per_row;                   // units of a row: rotated, unrotated rests of queries and keys, all
+    Divisor by_row, by_units, by_tail, by_vecs, by_half;
 };
 
 // Units of a row: the rotated parts of the query and key heads, their unrotated rests, the value heads.  A row whose
@@ -202,38 +218,37 @@ __global__ void __launch_bounds__(ROT_MAX_THREADS) k_append(AppendArgs a) {
     int64_t *dst = (int64_t *)rot_smem;                                // [rows of the block]: element offset in the pools, or -1
     float2 *cs = (float2 *)(dst + a.per_block);                        // [rows of the block][rot / 2]
     const int row0 = blockIdx.x * a.per_block, n = min(a.per_block, a.rows - row0), half = a.rot.rot >> 1;
-    const int turned = (a.nq + a.nkv) * a.units, rest = (a.nq + a.nkv) * a.tail;
-    const int per_row = turned + rest + a.nkv * a.vecs, total = n * per_row;
+    const int total = n * a.per_row;
     float v1[VEC], v2[VEC];
     int at1 = 0, at2 = 0, r = 0, head = 0, u = 0;
+    bool two = false;                                                  // a rotated unit (else v2 repeats v1 and is not stored)
     auto fetch = [&](int i) {
-        r = i / per_row;
-        int k = i - r * per_row;
+        r = i / a.by_row;
+        int k = i - r * a.per_row;
         const int64_t row = row0 + r;
         const T *src;
-        if (k < turned + rest) {
-            const bool two = k < turned;
-            k = two ? k : k - turned;
-            head = k / (two ? a.units : a.tail);
-            u = k - head * (two ? a.units : a.tail);
+        two = k < a.turned;
+        if (k < a.turned + a.rest) {
+            if (two) {
+                head = k / a.by_units;
+                u = k - head * a.units;
+                unit_offsets<VEC>(a.rot, u, at1, at2);
+            } else {
+                k -= a.turned;
+                head = k / a.by_tail;
+                at1 = at2 = a.rot.rot + (k - head * a.tail) * VEC;
+            }
             src = head < a.nq ? (const T *)a.q + row * a.q_row + (int64_t)head * a.q_head
                               : (const T *)a.k + row * a.k_row + (int64_t)(head - a.nq) * a.k_head;
-            if (two) {
-                unit_offsets<VEC>(a.rot, u, at1, at2);
-                load_values<T, VEC>(src + at2, v2);
-            } else {
-                at1 = a.rot.rot + u * VEC;
-                at2 = -1;
-            }
         } else {
-            k -= turned + rest;
-            head = k / a.vecs;
-            at1 = (k - head * a.vecs) * VEC;
+            k -= a.turned + a.rest;
+            head = k / a.by_vecs;
+            at1 = at2 = (k - head * a.vecs) * VEC;
             src = (const T *)a.v + row * a.v_row + (int64_t)head * a.v_head;
             head += a.nq + a.nkv;
-            at2 = -1;
         }
         load_values<T, VEC>(src + at1, v1);
+        load_values<T, VEC>(src + at2, v2);
     };
     int i = threadIdx.x;
     if (i < total) fetch(i);
@@ -246,19 +261,16 @@ __global__ void __launch_bounds__(ROT_MAX_THREADS) k_append(AppendArgs a) {
         }
         dst[k] = to;
     }
-    for (int k = threadIdx.x; k < n * half; k += blockDim.x) {
-        const int rr = k / half;
-        cs[k] = turn_of(a.rot, a.pos[row0 + rr], k - rr * half);
-    }
+    turn_rows(a.rot, a.pos + row0, n, a.by_half, cs);
     __syncthreads();
     while (i < total) {
         const int64_t to = dst[r];
         if (to >= 0) {
-            if (at2 >= 0) turn_unit<VEC>(a.rot, cs + r * half + u * VEC, v1, v2);
+            if (two) turn_unit<VEC>(a.rot, cs + r * half + u * VEC, v1, v2);
             if (head < a.nq) {
                 const int64_t o = (int64_t)(row0 + r) * a.qo_row + (int64_t)head * a.qo_head;
                 store_values<VEC>(a.q_out, o + at1, a.qo_dt, v1);
-                if (at2 >= 0) store_values<VEC>(a.q_out, o + at2, a.qo_dt, v2);
+                if (two) store_values<VEC>(a.q_out, o + at2, a.qo_dt, v2);
             } else {
                 const bool key = head < a.nq + a.nkv;
                 const int h = head - a.nq - (key ? 0 : a.nkv);
@@ -269,7 +281,7 @@ __global__ void __launch_bounds__(ROT_MAX_THREADS) k_append(AppendArgs a) {
                 }
                 const int64_t o = to + (int64_t)h * a.page_size * a.hd;
                 store_values<VEC>(key ? a.kc : a.vc, o + at1, a.kv_dt, v1);
-                if (at2 >= 0) store_values<VEC>(key ? a.kc : a.vc, o + at2, a.kv_dt, v2);
+                if (two) store_values<VEC>(key ? a.kc : a.vc, o + at2, a.kv_dt, v2);
             }
         }
         i += blockDim.x;

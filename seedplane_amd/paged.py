@@ -29,7 +29,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.SP_DT_F32, torch.float16: _lib.SP_DT_F16, torch.bfloat16: _lib.SP_DT_BF16,
            torch.float8_e4m3fn: _lib.SP_DT_E4M3}
-E4M3_MAX = 448.0
+_FLOATS = {t: code for t, code in _DTYPES.items() if t != torch.float8_e4m3fn}
 
 
 def rotary_frequencies(rot_dim, theta=10000.0, scaling=None, length=None):
@@ -82,8 +82,7 @@ def rotary_frequencies(rot_dim, theta=10000.0, scaling=None, length=None):
     return inv * (1 - slowed) + inv / factor * slowed, float(attention)
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _device(device):
@@ -94,51 +93,37 @@ def _device(device):
 
 
 def _call(fn, device, *args):
-    """One library call with `device` current."""
-    if torch.cuda.current_device() == device.index:
-        _lib.check(fn(*args, _stream(device)))
+    """One library call on the current stream of `device`, with that device current."""
+    i = device.index
+    if _current() == i:
+        rc = fn(*args, _raw_stream(i))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, _stream(device)))
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        _lib.check(rc)
 
 
-def _heads(x, name, device, heads=None, hd=None):
-    """A [rows, heads, head_dim] GPU tensor with values of a head side by side; returns its dtype code."""
-    if x.dim() != 3 or x.device != device:
-        raise ValueError(f'{name} must be a [rows, heads, head_dim] tensor on {device}')
-    if x.stride(2) != 1 and x.shape[2] > 1:
-        raise ValueError(f'the values of a head of {name} must lie side by side')
-    if (heads is not None and x.shape[1] != heads) or (hd is not None and x.shape[2] != hd):
-        raise ValueError(f'{name} has heads {tuple(x.shape[1:])}, expected {(heads, hd)}')
-    if x.dtype not in _DTYPES or x.dtype == torch.float8_e4m3fn:
-        raise ValueError(f'{name} must be fp32, fp16 or bf16')
-    return _DTYPES[x.dtype]
+def _heads(x, name, device, heads, hd):
+    """(dtype code, rows, row stride, head stride, address) of a [rows, heads, hd] tensor; heads None: any number."""
+    dt, s, n = _FLOATS.get(x.dtype), x.stride(), x.shape
+    if dt is None or x.device != device or len(n) != 3 or n[2] != hd or s[2] != 1 or (heads is not None and n[1] != heads):
+        raise ValueError(f'{name} must be an fp32, fp16 or bf16 tensor [rows, {"heads" if heads is None else heads}, {hd}] on '
+                         f'{device}, the values of a head side by side; got {x.dtype} {tuple(n)} with strides {s} on {x.device}')
+    return dt, n[0], s[0], s[1], x.data_ptr()
 
 
-def _ints(x, name, device, n=None):
-    """A contiguous int32 GPU tensor of n entries (None: any); returns its address."""
-    if x.dtype != torch.int32 or x.device != device or not x.is_contiguous():
-        raise ValueError(f'{name} must be a contiguous int32 tensor on {device}')
-    if n is not None and (x.dim() != 1 or x.shape[0] != n):
-        raise ValueError(f'{name} must have one entry per row')
+def _ints(x, name, device, n):
+    """The address of a contiguous int32 GPU tensor of n entries."""
+    if x.dtype != torch.int32 or x.device != device or x.shape != (n,) or (n > 1 and x.stride(0) != 1):
+        raise ValueError(f'{name} must be a contiguous int32 tensor on {device} with one entry per row')
     return x.data_ptr()
 
 
-def _apart(out, *ins):
-    """Refuse an output whose memory another operand reads."""
-    def span(t):
-        a = t.data_ptr()
-        return a, a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    if not out.numel():
-        return
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-        raise ValueError('the output has rows or heads on top of each other')
-    lo, hi = span(out)
-    for t in ins:
-        if t.numel():
-            a, b = span(t)
-            if a < hi and lo < b:
-                raise ValueError('the output overlaps an input')
+def _table(x, device):
+    if x.dtype != torch.int32 or x.device != device or x.dim() != 2 or not x.is_contiguous() or not x.numel():
+        raise ValueError(f'table must be a contiguous int32 tensor [sequences, most pages] on {device}')
+    return x.data_ptr()
 
 
 class Rotary:
@@ -174,20 +159,15 @@ class Rotary:
     def apply(self, x, positions, out=None):
         """x [rows, heads, head_dim] rotated at int32 `positions` [rows] (any sign; with factor 1, negated positions undo the
         rotation and give its gradient).  `out` may be x."""
-        dt = _heads(x, 'x', self.device, hd=self.head_dim)
-        pos = _ints(positions, 'positions', self.device, x.shape[0])
+        dt, rows, row, head, addr = _heads(x, 'x', self.device, None, self.head_dim)
+        pos = _ints(positions, 'positions', self.device, rows)
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        else:
-            if out.shape != x.shape or out.dtype != x.dtype:
-                raise ValueError('out must have the shape and type of x')
-            _heads(out, 'out', self.device)
-            if out.data_ptr() != x.data_ptr() or out.stride() != x.stride():
-                _apart(out, x)
-            elif any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
-                raise ValueError('the output has rows or heads on top of each other')
-        _call(self.lib.sp_op_rotate, self.device, self._ref, dt, x.shape[0], x.shape[1], self.head_dim, x.data_ptr(), x.stride(0),
-              x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), pos)
+            out = torch.empty_like(x)
+        elif out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError('out must have the shape and type of x')
+        _, _, o_row, o_head, o_addr = _heads(out, 'out', self.device, None, self.head_dim)
+        _call(self.lib.sp_op_rotate, self.device, self._ref, dt, rows, x.shape[1], self.head_dim, addr, row, head, o_addr, o_row,
+              o_head, pos)
         return out
 
 
@@ -232,39 +212,32 @@ class PagedKV:
         seq[r] (int32 [rows]; a row with seq -1, or whose position has no page, writes nothing).  With `rotary` the keys turn by
         rotary_pos (default: pos) on the way, and the queries q [rows, heads, head_dim] into q_out (default: a new tensor of q's
         type; may be q itself), which is returned."""
-        dt = _heads(k, 'k', self.device, self.n_kv_heads, self.head_dim)
-        if _heads(v, 'v', self.device, self.n_kv_heads, self.head_dim) != dt or v.shape != k.shape:
-            raise ValueError('k and v must have one shape and type')
-        rows = k.shape[0]
-        if table.dim() != 2 or 0 in table.shape:
-            raise ValueError('table must be [sequences, most pages]')
-        s, p, t = (_ints(seq, 'seq', self.device, rows), _ints(pos, 'pos', self.device, rows), _ints(table, 'table', self.device))
-        turn = p if rotary_pos is None else _ints(rotary_pos, 'rotary_pos', self.device, rows)
-        if rotary is not None and (rotary.head_dim != self.head_dim or rotary.device != self.device):
+        dev, nkv, hd = self.device, self.n_kv_heads, self.head_dim
+        dt, rows, k_row, k_head, k_addr = _heads(k, 'k', dev, nkv, hd)
+        v_dt, v_rows, v_row, v_head, v_addr = _heads(v, 'v', dev, nkv, hd)
+        if v_dt != dt or v_rows != rows:
+            raise ValueError('k and v must have the same rows and type')
+        s, p, t = _ints(seq, 'seq', dev, rows), _ints(pos, 'pos', dev, rows), _table(table, dev)
+        turn = p if rotary_pos is None else _ints(rotary_pos, 'rotary_pos', dev, rows)
+        if rotary is not None and (rotary.head_dim != hd or rotary.device != dev):
             raise ValueError('the rotary table is of another head_dim or device')
-        qa = (None, 0, 0)
-        qo = (None, 0, 0, 0)
-        nh = 0
         if q is not None:
-            if _heads(q, 'q', self.device, hd=self.head_dim) != dt or q.shape[0] != rows:
+            q_dt, q_rows, q_row, q_head, q_addr = _heads(q, 'q', dev, None, hd)
+            if q_dt != dt or q_rows != rows:
                 raise ValueError('q must have the rows and the type of k')
-            nh = q.shape[1]
             if q_out is None:
-                # rows that write nothing are zeros in a new tensor
-                q_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-            else:
-                if q_out.shape != q.shape:
-                    raise ValueError('q_out must have the shape of q')
-                if q_out.data_ptr() != q.data_ptr() or q_out.stride() != q.stride() or q_out.dtype != q.dtype:
-                    _apart(q_out, q, k, v)
-            qa = (q.data_ptr(), q.stride(0), q.stride(1))
-            qo = (q_out.data_ptr(), _heads(q_out, 'q_out', self.device), q_out.stride(0), q_out.stride(1))
+                q_out = torch.zeros_like(q)                    # rows that write nothing
+            elif q_out.shape != q.shape:
+                raise ValueError('q_out must have the shape of q')
+            o_dt, _, o_row, o_head, o_addr = _heads(q_out, 'q_out', dev, None, hd)
+            queries, turned, nh = (q_addr, q_row, q_head), (o_addr, o_dt, o_row, o_head), q.shape[1]
         elif q_out is not None:
             raise ValueError('q_out without q')
+        else:
+            queries, turned, nh = (None, 0, 0), (None, 0, 0, 0), 0
         if rows:
-            _call(self.lib.sp_op_paged_append, self.device, self._ref, None if rotary is None else rotary._ref, dt, rows, nh, *qa,
-                  k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), turn, s, p, t, table.shape[0],
-                  table.shape[1], *qo)
+            _call(self.lib.sp_op_paged_append, dev, self._ref, None if rotary is None else rotary._ref, dt, rows, nh, *queries,
+                  k_addr, k_row, k_head, v_addr, v_row, v_head, turn, s, p, t, table.shape[0], table.shape[1], *turned)
         return q_out
 
 
@@ -284,6 +257,7 @@ class AttentionPlan:
         self.h = h
         self._finalizer = weakref.finalize(self, self.lib.sp_attn_plan_destroy, h)
         self._ws = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=self.device)
+        self._ws_addr = self._ws.data_ptr()
         self._scale = 1.0 / math.sqrt(self.head_dim)
         self.rows = 0
 
@@ -315,28 +289,26 @@ class AttentionPlan:
     def run(self, q, kv, table, out=None, lse=None, scale=None, workspace=None):
         """Attention of q [rows, heads, head_dim] (fp16 or bf16) over the pages of `kv`; returns `out` (default: a new tensor,
         zeros behind the plan's rows).  lse: fp32 [rows, heads], filled with the logarithm of each row's sum of exponentials."""
-        dt = _heads(q, 'q', self.device, self.n_heads, self.head_dim)
-        if kv.device != self.device:
+        dev = self.device
+        dt, rows, q_row, q_head, q_addr = _heads(q, 'q', dev, self.n_heads, self.head_dim)
+        if kv.device != dev:
             raise ValueError('the cache is on another device')
-        if table.dim() != 2:
-            raise ValueError('table must be [sequences, most pages]')
-        t = _ints(table, 'table', self.device)
+        t = _table(table, dev)
         if out is None:
-            new = torch.empty if q.shape[0] == self.rows else torch.zeros
-            out = new(q.shape, dtype=q.dtype, device=q.device)
-        else:
-            if out.shape != q.shape or out.dtype != q.dtype:
-                raise ValueError('out must have the shape and type of q')
-            _heads(out, 'out', self.device)
-            _apart(out, q, kv.k, kv.v)
-        if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != self.device
+            out = torch.empty_like(q) if rows == self.rows else torch.zeros_like(q)
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError('out must have the shape and type of q')
+        _, _, o_row, o_head, o_addr = _heads(out, 'out', dev, self.n_heads, self.head_dim)
+        if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != dev
                                 or not lse.is_contiguous()):
             raise ValueError('lse must be a contiguous fp32 [rows, heads] tensor')
-        ws = self._ws if workspace is None else workspace
-        if workspace is not None and (ws.device != self.device or not ws.is_contiguous()
-                                      or ws.numel() * ws.element_size() < self._ws.numel()):
-            raise ValueError('the workspace is too small or on another device')
-        _call(self.lib.sp_op_paged_attention, self.device, self.h, kv._ref, dt, q.shape[0], q.data_ptr(), q.stride(0), q.stride(1),
-              t, table.shape[0], table.shape[1], self._scale if scale is None else float(scale), out.data_ptr(), out.stride(0),
-              out.stride(1), None if lse is None else lse.data_ptr(), ws.data_ptr())
+        if workspace is None:
+            ws = self._ws_addr
+        else:
+            if workspace.device != dev or not workspace.is_contiguous() or workspace.nbytes < self._ws.nbytes:
+                raise ValueError('the workspace is too small or on another device')
+            ws = workspace.data_ptr()
+        _call(self.lib.sp_op_paged_attention, dev, self.h, kv._ref, dt, rows, q_addr, q_row, q_head, t, table.shape[0],
+              table.shape[1], self._scale if scale is None else float(scale), o_addr, o_row, o_head,
+              None if lse is None else lse.data_ptr(), ws)
         return out

@@ -16,15 +16,12 @@ def plan(nh, nkv, q_lens, kv_lens, groups):
     g = np.array(groups if groups is not None else [], np.int32).reshape(-1, 2)
     size, shared = np.ascontiguousarray(g[:, 0]), np.ascontiguousarray(g[:, 1])
     toks = np.zeros((int(q.sum()), 8), np.int32)
-    out, recs = [], ctypes.c_int64()
-    for kind in range(3):
-        n = ctypes.c_int32()
-        args = (nh, nkv, len(q), q.ctypes.data, kv.ctypes.data, len(g), size.ctypes.data, shared.ctypes.data, kind)
-        _lib.check(lib.sp_attn_plan_items(*args, 0, None, ctypes.byref(n), None, ctypes.byref(recs)))
-        items = np.zeros((n.value, 8), np.int32)
-        _lib.check(lib.sp_attn_plan_items(*args, n.value, items.ctypes.data, ctypes.byref(n), toks.ctypes.data, None))
-        out.append(items)
-    return out, toks, recs.value
+    recs, n = ctypes.c_int64(), ctypes.c_int32()
+    args = (nh, nkv, len(q), q.ctypes.data, kv.ctypes.data, len(g), size.ctypes.data, shared.ctypes.data)
+    _lib.check(lib.sp_attn_plan_items(*args, 0, None, ctypes.byref(n), None, ctypes.byref(recs)))
+    items = np.zeros((n.value, 12), np.int32)
+    _lib.check(lib.sp_attn_plan_items(*args, n.value, items.ctypes.data, ctypes.byref(n), toks.ctypes.data, None))
+    return items, toks, recs.value
 
 
 CASES = [
@@ -47,7 +44,7 @@ CASES = [
 def test_every_seen_position_is_read_once_and_records_have_one_writer(case):
     nh, nkv, q_lens, kv_lens, groups = CASES[case]
     G = nh // nkv
-    kinds, toks, n_recs = plan(nh, nkv, q_lens, kv_lens, groups)
+    items, toks, n_recs = plan(nh, nkv, q_lens, kv_lens, groups)
     seqs = [s for s, n in enumerate(q_lens) for _ in range(n)]
     pos = [kv_lens[s] - q_lens[s] + i for s, n in enumerate(q_lens) for i in range(n)]
     group_of = []
@@ -56,33 +53,32 @@ def test_every_seen_position_is_read_once_and_records_have_one_writer(case):
     read = {}
     writer = {}
     alone = set()
-    for kind, items in enumerate(kinds):
-        for tok0, ntok, kvh, seq, k0, k1, pos0, rec in items.tolist():
-            assert 1 <= ntok * G <= 32 << kind and 0 <= kvh < nkv and 0 <= k0 < k1
-            for i in range(ntok):
-                t = tok0 + i
-                end = min(k1, pos0 + i + 1)
-                if pos0 == ALL:                             # shared positions, through another sequence's table
-                    g, shared = group_of[seqs[t]]
-                    assert group_of[seq] == (g, shared) and k1 <= shared and q_lens[seq] > 0 and k1 <= pos[t] + 1
-                    end = k1
-                else:
-                    assert seq == seqs[t] and pos0 + i == pos[t] and k1 <= max(kv_lens[seq], 1)
-                if end > k0:
-                    read.setdefault((t, kvh), []).append((k0, end))
-                base, parts, tile, at = toks[t].reshape(4, 2)
-                which = 0 if pos0 == ALL else 1
-                if rec < 0:
-                    assert parts[which] == -1 and parts[1 - which] == 0 and (t, kvh) not in alone
-                    alone.add((t, kvh))
-                else:
-                    assert parts[which] >= 1 and tile[which] == ntok and at[which] == i
-                    part = [j for j in range(parts[which])
-                            if (base[which] + (kvh * parts[which] + j) * tile[which] + i) * G == rec + i * G]
-                    assert len(part) == 1
-                    key = rec + i * G
-                    assert key not in writer and key + G <= n_recs
-                    writer[key] = (t, kvh)
+    for tok0, ntok, kvh, seq, k0, k1, pos0, rec, kind, *_ in items.tolist():
+        assert 1 <= ntok * G <= 32 << kind and 0 <= kvh < nkv and 0 <= k0 < k1
+        for i in range(ntok):
+            t = tok0 + i
+            end = min(k1, pos0 + i + 1)
+            if pos0 == ALL:                             # shared positions, through another sequence's table
+                g, shared = group_of[seqs[t]]
+                assert group_of[seq] == (g, shared) and k1 <= shared and q_lens[seq] > 0 and k1 <= pos[t] + 1
+                end = k1
+            else:
+                assert seq == seqs[t] and pos0 + i == pos[t] and k1 <= max(kv_lens[seq], 1)
+            if end > k0:
+                read.setdefault((t, kvh), []).append((k0, end))
+            base, parts, tile, at = toks[t].reshape(4, 2)
+            which = 0 if pos0 == ALL else 1
+            if rec < 0:
+                assert parts[which] == -1 and parts[1 - which] == 0 and (t, kvh) not in alone
+                alone.add((t, kvh))
+            else:
+                assert parts[which] >= 1 and tile[which] == ntok and at[which] == i
+                part = [j for j in range(parts[which])
+                        if (base[which] + (kvh * parts[which] + j) * tile[which] + i) * G == rec + i * G]
+                assert len(part) == 1
+                key = rec + i * G
+                assert key not in writer and key + G <= n_recs
+                writer[key] = (t, kvh)
     for t, p in enumerate(pos):
         for kvh in range(nkv):
             at = 0
@@ -98,8 +94,7 @@ def test_every_seen_position_is_read_once_and_records_have_one_writer(case):
 
 
 def test_shared_positions_are_read_once_for_the_group():
-    kinds, _, _ = plan(12, 2, [1] * 16, [2048 + 100] * 16, [(16, 2048)])
-    items = np.concatenate(kinds)
+    items, _, _ = plan(12, 2, [1] * 16, [2048 + 100] * 16, [(16, 2048)])
     shared = items[items[:, 6] == ALL]
     for h in range(2):
         assert (shared[shared[:, 2] == h][:, 5] - shared[shared[:, 2] == h][:, 4]).sum() == 2048
@@ -117,10 +112,10 @@ def test_records_stay_within_the_workspace():
         q = rng.integers(0, int(rng.choice([2, 10, 120])), n)
         kv = q + rng.integers(0, int(rng.choice([50, 3000, 60000])), n)
         shared = int(kv.min() * rng.choice([0, 0.5, 1]))
-        kinds, toks, recs = plan(nkv * G, nkv, q.tolist(), kv.tolist(), [(n, shared)])
+        items, toks, recs = plan(nkv * G, nkv, q.tolist(), kv.tolist(), [(n, shared)])
         rows = int(q.sum())
-        assert recs <= 2 * rows * nkv * G + 512 * (32 + 64 + 128)
-        assert all(len(x) <= 2 * rows * nkv + 512 for x in kinds)
+        assert recs <= 2 * rows * nkv * G + 2 * 512 * 128
+        assert len(items) <= 2 * rows * nkv + 512
 
 
 def test_bad_lengths_are_refused():
@@ -139,10 +134,11 @@ def test_bad_lengths_are_refused():
     lib = _lib.load()
     q = (ctypes.c_int32 * 1)(-1)
     n = ctypes.c_int32()
-    assert lib.sp_attn_plan_items(2, 1, 1, q, q, 0, None, None, 0, 0, None, ctypes.byref(n), None, None) == _lib.SP_EINVAL
-    assert lib.sp_attn_plan_items(2, 1, 1, None, q, 0, None, None, 0, 0, None, ctypes.byref(n), None, None) == _lib.SP_EINVAL
-    assert lib.sp_attn_plan_items(2, 1, 0, q, q, 0, None, None, 0, 0, None, ctypes.byref(n), None, None) == _lib.SP_EINVAL
     one = (ctypes.c_int32 * 1)(1)
-    assert lib.sp_attn_plan_items(2, 1, 1, one, one, 0, None, None, 3, 0, None, ctypes.byref(n), None, None) == _lib.SP_EINVAL
-    items = (ctypes.c_int32 * 8)()
-    assert lib.sp_attn_plan_items(2, 1, 1, one, one, 0, None, None, 0, 0, items, ctypes.byref(n), None, None) == _lib.SP_ECAPACITY
+    items = (ctypes.c_int32 * 12)()
+    call = lambda a, b, n_seq=1, cap=0, out=None, count=n: lib.sp_attn_plan_items(
+        2, 1, n_seq, a, b, 0, None, None, cap, out, None if count is None else ctypes.byref(count), None, None)
+    assert call(one, one) == _lib.SP_OK and n.value == 1
+    assert call(q, one) == _lib.SP_EINVAL and call(None, one) == _lib.SP_EINVAL and call(one, one, n_seq=0) == _lib.SP_EINVAL
+    assert call(one, one, count=None) == _lib.SP_EINVAL
+    assert call(one, one, out=items) == _lib.SP_ECAPACITY and call(one, one, cap=1, out=items) == _lib.SP_OK
