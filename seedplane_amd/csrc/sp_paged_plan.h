@@ -32,9 +32,11 @@ constexpr int32_t ALL_SEEN = 1 << 30;
 constexpr int KINDS = 3;                                       // row tiles of 32 << kind rows
 constexpr int TILE_ROWS_OF[KINDS] = {32, 64, 128};
 constexpr int KEY_STEP = 64;                                   // parts are whole steps of keys
-// Cost of a step by kind, in units of a 128-row tile's (bound by its matrix products); the others read their keys for few rows
-// and are bound by memory.  And the fewest steps of a part: shorter ones cost more in records and latency than they spread.
-constexpr int STEP_COST[KINDS] = {1, 1, 1};
+// Cost of a step by kind: a tile of many rows is bound by its matrix products, one of few by memory.  With two blocks on every
+// CU a step of head_dim 128 takes 2.6 us (128 rows, 16 bits; e4m3 2.8) against 3.1 us (32 rows, 16 bits) and 1.6 (e4m3); 2 : 3
+// lies between (decode of 32 / 96 requests over 8192 / 16384 shared positions, bf16 / e4m3: 1 : 1 20.0 / 66.8 us, 2 : 3 19.4 / 59.9,
+// 1 : 2 20.6 / 57.1).  And the fewest steps of a part: shorter ones cost more in records and latency than they spread.
+constexpr int STEP_COST[KINDS] = {2, 3, 3};
 constexpr int LEAST_STEPS[KINDS] = {2, 2, 2};
 constexpr int MAX_GROUP = 32;                                  // query heads per K/V head
 
@@ -76,24 +78,35 @@ inline void make_plan(int n_heads, int n_kv, int n_seq, const int32_t *q_len, co
             if (end > k0) segs.push_back({tok0 + t, n, seq, k0, end, which ? pos0 + t : ALL_SEEN, which, kind});
         }
     };
+    // a sequence whose own queries fill their row tiles (an eighth empty at most) gains nothing from rows of others beside
+    // them: it reads the shared positions with its own, in one range, and needs no join
+    const int per_tile = TILE_ROWS_OF[KINDS - 1] / G;
+    auto fills_tiles = [&](int32_t q) { return (int64_t)(q + per_tile - 1) / per_tile * per_tile * 8 <= (int64_t)q * 9; };
     int s0 = 0;
     for (int g = 0; g < n_groups; ++g) {
-        int32_t shared = group_shared[g], tokens = 0, first = -1, members = 0;
-        for (int s = s0; s < s0 + group_size[g]; ++s) {
-            if (q_len[s] == 0) continue;
-            if (first < 0) first = s;
-            ++members;
-            tokens += q_len[s];
-            shared = std::min(shared, std::max(0, kv_len[s] - q_len[s]));
+        const int s1 = s0 + group_size[g];
+        // runs of sequences that share
+        for (int a = s0; a < s1;) {
+            int b = a;
+            int32_t shared = group_shared[g], tokens = 0, first = -1, members = 0;
+            for (; b < s1 && !fills_tiles(q_len[b]); ++b) {
+                if (q_len[b] == 0) continue;
+                if (first < 0) first = b;
+                ++members;
+                tokens += q_len[b];
+                shared = std::min(shared, std::max(0, kv_len[b] - q_len[b]));
+            }
+            if (members < 2) shared = 0;                                     // nothing to share
+            if (b == a) b = a + 1;
+            if (shared > 0) add(n_tok, tokens, first, 0, shared, 0, 0);
+            for (int s = a; s < b; ++s) {
+                if (q_len[s]) add(n_tok, q_len[s], s, shared, kv_len[s], kv_len[s] - q_len[s], 1);
+                out.max_kv = std::max(out.max_kv, q_len[s] ? kv_len[s] : 0);
+                n_tok += q_len[s];
+            }
+            a = b;
         }
-        if (members < 2) shared = 0;                                         // nothing to share
-        if (shared > 0) add(n_tok, tokens, first, 0, shared, 0, 0);
-        for (int s = s0; s < s0 + group_size[g]; ++s) {
-            if (q_len[s]) add(n_tok, q_len[s], s, shared, kv_len[s], kv_len[s] - q_len[s], 1);
-            out.max_kv = std::max(out.max_kv, q_len[s] ? kv_len[s] : 0);
-            n_tok += q_len[s];
-        }
-        s0 += group_size[g];
+        s0 = s1;
     }
     out.toks.assign(n_tok, TokenRecs{});
     auto steps_of = [](const Segment &s) { return (int64_t)(s.k1 - s.k0 + KEY_STEP - 1) / KEY_STEP; };
@@ -102,7 +115,7 @@ inline void make_plan(int n_heads, int n_kv, int n_seq, const int32_t *q_len, co
     const int64_t share = (total + ITEM_TARGET - 1) / ITEM_TARGET;
     auto parts_of = [&](const Segment &s) {
         const int64_t len = std::max<int64_t>(LEAST_STEPS[s.kind], (share + STEP_COST[s.kind] - 1) / STEP_COST[s.kind]);
-        return (steps_of(s) + len - 1) / len;
+        return std::max<int64_t>(1, (steps_of(s) + len / 2) / len);        // (half a part more costs less than a cut)
     };
     for (const Segment &s : segs)
         for (int i = 0; i < s.ntok; ++i) {
