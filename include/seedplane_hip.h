@@ -451,7 +451,7 @@ int sp_attn_plan_set(sp_attn_plan *plan, int32_t n_seq, const int32_t *q_len, co
  * head, sequence, first position, end, position seen by the first token (2^30: all), first record or -1, kind (row tile of
  * 32 << kind rows), three reserved; and per token 8 int32: base, parts, tile and index of its records of the shared and of its own
  * positions (pairs).  items and token_recs may be NULL. */
-int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len,
+int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len,
                        int32_t n_groups, const int32_t *group_size, const int32_t *group_shared, int32_t capacity,
                        int32_t *items, int32_t *n_items, int32_t *token_recs, int64_t *n_records);
 /* Bytes of sp_op_paged_attention's workspace, for every batch within max_rows. */

@@ -120,7 +120,7 @@ SIGNATURES = {
     'sp_attn_plan_create': (c_int, [c_int32, c_int32, c_int32, c_int32, c_int32, ctypes.POINTER(c_void_p)]),
     'sp_attn_plan_destroy': (None, [c_void_p]),
     'sp_attn_plan_set': (c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
-    'sp_attn_plan_items': (c_int, [c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32,
+    'sp_attn_plan_items': (c_int, [c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32,
                                    c_void_p, c_void_p, c_void_p, c_void_p]),
     'sp_attn_plan_workspace': (c_size_t, [c_void_p]),
     'sp_op_paged_attention': (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_int32,

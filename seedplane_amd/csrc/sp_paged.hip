@@ -97,7 +97,7 @@ void check_output(const Span &out) { require(!out.folded, SP_EINVAL, "the output
 // Rows of a block and its threads: about 256 threads a block, whole rows.
 void shape_of(int per_row, int rows, int &per_block, int &threads) {
     per_block = std::max(1, std::min(rows, 256 / per_row));
-    threads = std::min(ROT_MAX_THREADS, (per_block * per_row + 63) / 64 * 64);
+    threads = std::min(ROT_THREADS, (per_block * per_row + 63) / 64 * 64);
 }
 
 template <class F>
@@ -186,15 +186,15 @@ int check_lengths(int n_seq, const int32_t *q_len, const int32_t *kv_len, int n_
     return (int)tokens;
 }
 
-void tables_of(int NH, int NKV, int n_seq, const int32_t *q_len, const int32_t *kv_len, int n_groups, const int32_t *size,
+void tables_of(int NH, int NKV, int HD, int n_seq, const int32_t *q_len, const int32_t *kv_len, int n_groups, const int32_t *size,
                const int32_t *shared, PlanTables &t) {
     std::vector<int32_t> one, none;
     if (n_groups == 0) {                                     // no sharing: every sequence a group of its own
         one.assign(n_seq, 1);
         none.assign(n_seq, 0);
-        make_plan(NH, NKV, n_seq, q_len, kv_len, n_seq, one.data(), none.data(), t);
+        make_plan(NH, NKV, HD, n_seq, q_len, kv_len, n_seq, one.data(), none.data(), t);
     } else {
-        make_plan(NH, NKV, n_seq, q_len, kv_len, n_groups, size, shared, t);
+        make_plan(NH, NKV, HD, n_seq, q_len, kv_len, n_groups, size, shared, t);
     }
 }
 
@@ -365,7 +365,7 @@ int sp_attn_plan_set(sp_attn_plan *p, int32_t n_seq, const int32_t *q_len, const
         const hipStream_t st = (hipStream_t)stream;
         require(!is_capturing(st), SP_ESTATE, "a plan is not set in a stream capture: captured calls read the tables of the last set");
         PlanTables t;
-        tables_of(p->NH, p->NKV, n_seq, q_len, kv_len, n_groups, group_size, group_shared, t);
+        tables_of(p->NH, p->NKV, p->HD, n_seq, q_len, kv_len, n_groups, group_size, group_shared, t);
         const int turn = p->turn;
         if (p->used[turn]) HIPCHK(hipEventSynchronize(p->copied[turn]));
         int32_t *img = p->staging[turn];
@@ -392,15 +392,15 @@ int sp_attn_plan_set(sp_attn_plan *p, int32_t n_seq, const int32_t *q_len, const
     });
 }
 
-int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len,
+int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len,
                        int32_t n_groups, const int32_t *group_size, const int32_t *group_shared, int32_t capacity,
                        int32_t *items, int32_t *n_items, int32_t *token_recs, int64_t *n_records) {
     return guarded([&] {
-        check_shape(n_heads, n_kv_heads, 64, 1, 1);
+        check_shape(n_heads, n_kv_heads, head_dim, 1, 1);
         require(n_items != nullptr, SP_EINVAL, "n_items is NULL");
         check_lengths(n_seq, q_len, kv_len, n_groups, group_size, group_shared, (1 << 27) / n_heads, 65535);
         PlanTables t;
-        tables_of(n_heads, n_kv_heads, n_seq, q_len, kv_len, n_groups, group_size, group_shared, t);
+        tables_of(n_heads, n_kv_heads, head_dim, n_seq, q_len, kv_len, n_groups, group_size, group_shared, t);
         *n_items = (int32_t)t.items.size();
         if (n_records) *n_records = t.records;
         if (items) {

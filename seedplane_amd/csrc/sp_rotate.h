@@ -125,7 +125,7 @@ __device__ __forceinline__ void turn_unit(const Rotation &r, const float2 *cs, f
     }
 }
 
-constexpr int ROT_MAX_THREADS = 512;
+constexpr int ROT_THREADS = 256;
 
 // n / d for n, d < 2^16 by a multiplication: the rounded-up reciprocal is off by less than 2^-32 d, so n times it is off by
 // less than one part of d.
@@ -159,7 +159,7 @@ __device__ __forceinline__ void turn_rows(const Rotation &rot, const int *pos, i
 template <class T> constexpr int dtype_of() { return sizeof(T) == 4 ? SP_DT_F32 : std::is_same<T, f16>::value ? SP_DT_F16 : SP_DT_BF16; }
 
 template <class T, int VEC>
-__global__ void __launch_bounds__(ROT_MAX_THREADS) k_rotate(RotateArgs a) {
+__global__ void __launch_bounds__(ROT_THREADS) k_rotate(RotateArgs a) {
     extern __shared__ __align__(16) unsigned char rot_smem[];
     float2 *cs = (float2 *)rot_smem;
     const int row0 = blockIdx.x * a.per_block, n = min(a.per_block, a.rows - row0), half = a.rot.rot >> 1;
@@ -213,7 +213,7 @@ struct AppendArgs {
 // Units of a row: the rotated parts of the query and key heads, their unrotated rests, the value heads.  A row whose
 // sequence, position or page is out of range writes nothing.
 template <class T, int VEC>
-__global__ void __launch_bounds__(ROT_MAX_THREADS) k_append(AppendArgs a) {
+__global__ void __launch_bounds__(ROT_THREADS) k_append(AppendArgs a) {
     extern __shared__ __align__(16) unsigned char rot_smem[];
     int64_t *dst = (int64_t *)rot_smem;                                // [rows of the block]: element offset in the pools, or -1
     float2 *cs = (float2 *)(dst + a.per_block);                        // [rows of the block][rot / 2]
@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(ROT_MAX_THREADS) k_append(AppendArgs a) {
     };
     int i = threadIdx.x;
     if (i < total) fetch(i);
-    for (int k = threadIdx.x; k < n; k += blockDim.x) {
+    // (the places are looked up by the last threads, the angles formed by the first)
+    for (int k = blockDim.x - 1 - threadIdx.x; k < n; k += blockDim.x) {
         const int s = a.seq[row0 + k], p = a.at[row0 + k];
         int64_t to = -1;
         if (s >= 0 && s < a.n_seq && p >= 0 && p / a.page_size < a.max_pages) {

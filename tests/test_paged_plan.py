@@ -10,14 +10,14 @@ from seedplane_amd import _lib
 ALL = 1 << 30
 
 
-def plan(nh, nkv, q_lens, kv_lens, groups):
+def plan(nh, nkv, q_lens, kv_lens, groups, hd=128):
     lib = _lib.load()
     q, kv = np.array(q_lens, np.int32), np.array(kv_lens, np.int32)
     g = np.array(groups if groups is not None else [], np.int32).reshape(-1, 2)
     size, shared = np.ascontiguousarray(g[:, 0]), np.ascontiguousarray(g[:, 1])
     toks = np.zeros((int(q.sum()), 8), np.int32)
     recs, n = ctypes.c_int64(), ctypes.c_int32()
-    args = (nh, nkv, len(q), q.ctypes.data, kv.ctypes.data, len(g), size.ctypes.data, shared.ctypes.data)
+    args = (nh, nkv, hd, len(q), q.ctypes.data, kv.ctypes.data, len(g), size.ctypes.data, shared.ctypes.data)
     _lib.check(lib.sp_attn_plan_items(*args, 0, None, ctypes.byref(n), None, ctypes.byref(recs)))
     items = np.zeros((n.value, 12), np.int32)
     _lib.check(lib.sp_attn_plan_items(*args, n.value, items.ctypes.data, ctypes.byref(n), toks.ctypes.data, None))
@@ -40,11 +40,12 @@ CASES = [
 ]
 
 
+@pytest.mark.parametrize('hd', [64, 128])
 @pytest.mark.parametrize('case', range(len(CASES)))
-def test_every_seen_position_is_read_once_and_records_have_one_writer(case):
+def test_every_seen_position_is_read_once_and_records_have_one_writer(case, hd):
     nh, nkv, q_lens, kv_lens, groups = CASES[case]
     G = nh // nkv
-    items, toks, n_recs = plan(nh, nkv, q_lens, kv_lens, groups)
+    items, toks, n_recs = plan(nh, nkv, q_lens, kv_lens, groups, hd)
     seqs = [s for s, n in enumerate(q_lens) for _ in range(n)]
     pos = [kv_lens[s] - q_lens[s] + i for s, n in enumerate(q_lens) for i in range(n)]
     group_of = []
@@ -137,7 +138,7 @@ def test_bad_lengths_are_refused():
     one = (ctypes.c_int32 * 1)(1)
     items = (ctypes.c_int32 * 12)()
     call = lambda a, b, n_seq=1, cap=0, out=None, count=n: lib.sp_attn_plan_items(
-        2, 1, n_seq, a, b, 0, None, None, cap, out, None if count is None else ctypes.byref(count), None, None)
+        2, 1, 64, n_seq, a, b, 0, None, None, cap, out, None if count is None else ctypes.byref(count), None, None)
     assert call(one, one) == _lib.SP_OK and n.value == 1
     assert call(q, one) == _lib.SP_EINVAL and call(None, one) == _lib.SP_EINVAL and call(one, one, n_seq=0) == _lib.SP_EINVAL
     assert call(one, one, count=None) == _lib.SP_EINVAL
