@@ -233,3 +233,336 @@ TYPES = [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, E4M3)]
 def test_attention(gpu_device, dtype, cache, hd, q_lens, kv_lens, groups, nh, nkv, page):
     print(f'attend {dtype} {cache} {hd} {q_lens} {kv_lens} {groups} {nh} {nkv} {page}', flush=True)
     _attend(gpu_device, q_lens, kv_lens, groups, nh, nkv, hd, page, dtype, cache, seed=len(q_lens) + hd)
+
+
+def test_attention_views_pages_apart_scale_and_no_lse(gpu_device):
+    """q and out as views of wider rows, pages further apart than their size, another scale, no lse."""
+    q_lens, kv_lens, groups = [1, 4, 1], [90, 100, 70], [(3, 64)]
+    plan, q, kv, table, want = _attend(gpu_device, q_lens, kv_lens, groups, 12, 2, 128, 16, F16, F16, seed=5, scale=0.2,
+                                       stride=2 * 2 * 16 * 128, rows_behind=0)
+    wide = torch.full((6, 40, 136), 2.0, dtype=F16, device=gpu_device)
+    wide[:, 3:15, :128] = q
+    out = torch.full((6, 13, 160), 4.0, dtype=F16, device=gpu_device)
+    got = plan.run(wide[:, 3:15, :128], kv, table, out=out[:, 1:, 8:136], scale=0.2)
+    assert torch.equal(got, want) and (out[:, 0] == 4).all() and (out[..., :8] == 4).all() and (out[..., 136:] == 4).all()
+    assert torch.equal(plan.run(q, kv, table, scale=0.2), want)
+
+
+@pytest.mark.parametrize('fill', [math.inf, -math.inf, 1e4])
+@pytest.mark.parametrize('cache', [F16, BF16])
+def test_what_the_pool_holds_elsewhere_does_not_matter(gpu_device, fill, cache):
+    _attend(gpu_device, [1, 20, 3], [33, 47, 3], None, 14, 2, 64, 16, cache, cache, seed=9, fill=fill)
+
+
+@pytest.mark.parametrize('dtype,cache', [(F16, F16), (BF16, E4M3)])
+def test_entries_outside_the_pool_hide_their_positions(gpu_device, dtype, cache):
+    """Of a shared prefix, of a sequence's own positions, and all of a sequence's: zeros and lse -inf where nothing is left."""
+    g = torch.Generator().manual_seed(11)
+    q_lens, kv_lens, groups = [1, 1, 20, 2, 1], [300, 280, 290, 20, 16], [(3, 256), (1, 0), (1, 0)]
+    q, k, v, table, scales = paged_batch(g, q_lens, kv_lens, groups, 14, 2, 128, 16, dtype, cache, gpu_device)
+    bad = k.shape[0]
+    table[:3, 5] = bad
+    table[:3, 15] = -1
+    table[1, 17] = 1 << 30
+    table[2, 18] = -(1 << 31)
+    table[3] = -7
+    kv = PagedKV(k, v, *scales)
+    plan = AttentionPlan(14, 2, 128, max_rows=25, max_seqs=5).set(q_lens, kv_lens, groups)
+    lse = torch.zeros(25, 14, device=gpu_device)
+    out = plan.run(q, kv, table, lse=lse)
+    want, wl, bound = attend64(q, k, v, table, q_lens, kv_lens, 128 ** -0.5, *scales)
+    _within(out, want, bound)
+    assert torch.equal(lse.cpu() == -math.inf, wl == -math.inf) and (out[22:24] == 0).all() and (lse[22:24] == -math.inf).all()
+
+
+def test_long_contexts(gpu_device):
+    """Parts of many row tables, more parts than the join's waves hold at once, a prefix of an odd page size."""
+    _attend(gpu_device, [1], [40000], None, 2, 1, 64, 16, F16, F16, seed=1)
+    _attend(gpu_device, [1, 1, 1], [9003, 9100, 9001], [(3, 9000)], 28, 4, 128, 24, BF16, BF16, seed=2)
+    _attend(gpu_device, [1] * 24, [2500 + 3 * i for i in range(24)], [(24, 2450)], 8, 2, 64, 49, BF16, E4M3, seed=3)
+    _attend(gpu_device, [130], [5000], None, 4, 4, 64, 128, F16, F16, seed=4)
+
+
+def test_peaked_and_extreme_scores(gpu_device):
+    """Scores of hundreds (one weight is all), large values next to the type's limit, and a late maximum after many flat ones."""
+    g = torch.Generator().manual_seed(2)
+    q, k, v, table, _ = paged_batch(g, [1, 30], [700, 730], None, 8, 2, 64, 16, F16, F16, gpu_device)
+    q *= 40
+    v *= 3000
+    k[int(table[0, 40])] *= 5
+    kv = PagedKV(k, v)
+    plan = AttentionPlan(8, 2, 64, 31, 2).set([1, 30], [700, 730])
+    _within(plan.run(q, kv, table), *attend64(q, k, v, table, [1, 30], [700, 730], 0.125)[::2])
+
+
+def test_offsets_past_32_bits(gpu_device):
+    """Pages whose elements lie beyond 2^32 of the pool's start: append and attention."""
+    free, _ = torch.cuda.mem_get_info(gpu_device)
+    nkv, hd, page = 2, 128, 16
+    n, stride = 40, 1 << 27                                  # 40 pages, 2^27 elements apart: 10 GiB each for k and v
+    if free < 26 << 30:
+        pytest.skip('needs 26 GiB of free memory')
+    pools = [torch.empty((n, stride), dtype=F16, device=gpu_device)[:, :nkv * page * hd].view(n, nkv, page, hd) for _ in range(2)]
+    kv = PagedKV(*pools)
+    L = 4 * page
+    table = torch.tensor([[39, 33, 36, 38]], dtype=torch.int32, device=gpu_device)
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn((L, 3 * nkv, hd), generator=g).half().to(gpu_device)
+    at = torch.arange(L, dtype=torch.int32, device=gpu_device)
+    kv.append(x[:, :nkv], x[:, nkv:2 * nkv], torch.zeros_like(at), at, table)
+    for i, p in enumerate(table[0].tolist()):
+        assert torch.equal(pools[0][p], x[i * page:(i + 1) * page, :nkv].permute(1, 0, 2))
+        assert torch.equal(pools[1][p], x[i * page:(i + 1) * page, nkv:2 * nkv].permute(1, 0, 2))
+    plan = AttentionPlan(nkv, nkv, hd, L, 1).set([L], [L])
+    q = x[:, 2 * nkv:].contiguous()
+    small = [torch.zeros((40, nkv, page, hd), dtype=F16) for _ in range(2)]
+    for s, p in zip(small, pools):
+        s[table[0].cpu().long()] = p[table[0].long()].cpu()
+    want, _, bound = attend64(q, small[0], small[1], table, [L], [L], hd ** -0.5)
+    _within(plan.run(q, kv, table), want, bound)
+
+
+def test_results_repeat_bit_for_bit_and_do_not_depend_on_the_stream(gpu_device):
+    plan, q, kv, table, out = _attend(gpu_device, [1] * 12, [700 + 31 * i for i in range(12)], [(12, 640)], 28, 4, 128, 16, BF16, BF16)
+    for _ in range(3):
+        assert torch.equal(plan.run(q[:12], kv, table), out[:12])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = plan.run(q[:12], kv, table, workspace=torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=gpu_device))
+        b = Rotary(128).apply(q[:12], torch.arange(12, dtype=torch.int32, device=gpu_device))
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(a, out[:12])
+    assert torch.equal(b, Rotary(128).apply(q[:12], torch.arange(12, dtype=torch.int32, device=gpu_device)))
+
+
+def test_two_plans_on_two_streams(gpu_device):
+    """Plans have workspaces of their own: batches that run side by side do not meet."""
+    runs = []
+    for seed, n in ((0, 9), (1, 5)):
+        runs.append(_attend(gpu_device, [1] * n, [900 + 50 * i for i in range(n)], [(n, 896)], 12, 2, 128, 16, F16, F16, seed=seed, lse=False))
+    streams = [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(10):
+        for i, ((plan, q, kv, table, _), s) in enumerate(zip(runs, streams)):
+            with torch.cuda.stream(s):
+                outs[i].append(plan.run(q, kv, table))
+    torch.cuda.synchronize()
+    for i, (_, q, _, _, want) in enumerate(runs):
+        n = q.shape[0] - 3
+        assert all(torch.equal(o[:n], want[:n]) and (o[n:] == 0).all() for o in outs[i])
+
+
+def test_captured_step_follows_later_lengths(gpu_device):
+    """Append and attention captured once; lengths, tables and positions change between replays, eager work in between."""
+    nh, nkv, hd, page, B, width = 12, 2, 128, 16, 6, 64
+    g = torch.Generator().manual_seed(4)
+    n_pages = B * width
+    kv = PagedKV(*[torch.randn((n_pages, nkv, page, hd), generator=g).half().to(gpu_device) for _ in range(2)])
+    table = torch.randperm(n_pages, generator=g).int().view(B, width).to(gpu_device)
+    table[:, :8] = table[0, :8]                               # 128 common positions
+    r = Rotary(hd, theta=1e6)
+    x = torch.randn((B, nh + 2 * nkv, hd), generator=g).half().to(gpu_device)
+    seq = torch.arange(B, dtype=torch.int32, device=gpu_device)
+    at = torch.zeros(B, dtype=torch.int32, device=gpu_device)
+    qr, out = (torch.zeros((B, nh, hd), dtype=F16, device=gpu_device) for _ in range(2))
+    plan = AttentionPlan(nh, nkv, hd, B, B)
+    lens = [200 + 17 * i for i in range(B)]
+
+    def step():
+        kv.append(x[:, nh:nh + nkv], x[:, nh + nkv:], seq, at, table, rotary=r, q=x[:, :nh], q_out=qr)
+        plan.run(qr, kv, table, out=out)
+
+    def place(groups):
+        at.copy_(torch.tensor(lens, dtype=torch.int32) - 1)
+        plan.set([1] * B, lens, groups)
+    place([(B, 128)])
+    step()                                                    # (warm)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(5):
+        lens = [n + 90 * (i % 3) + 1 for n in lens]
+        place([(B, 128)] if i % 2 == 0 else None)
+        x.copy_(torch.randn(x.shape, generator=g).half())
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        step()
+        assert torch.equal(got, out), i
+        want, _, bound = attend64(qr, kv.k, kv.v, table, [1] * B, lens, hd ** -0.5)
+        _within(got, want, bound)
+
+
+def test_set_is_refused_in_a_capture(gpu_device):
+    from seedplane_amd._lib import SeedPlaneError
+    plan = AttentionPlan(2, 1, 64, 4, 4).set([1], [1])
+    y = torch.zeros(1, device=gpu_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y += 1
+        with pytest.raises(SeedPlaneError):
+            plan.set([1], [2])
+    graph.replay()
+    torch.cuda.synchronize()
+
+
+def test_many_sets_in_flight(gpu_device):
+    """A plan set again and again without waiting: every run sees the lengths set before it."""
+    plan, q, kv, table, _ = _attend(gpu_device, [1] * 4, [1000] * 4, None, 4, 2, 64, 16, F16, F16, rows_behind=0)
+    wants = {}
+    for n in (1000, 3, 517):
+        plan.set([1] * 4, [n] * 4)
+        wants[n] = plan.run(q, kv, table)
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(60):
+        n = (1000, 3, 517)[i % 3]
+        plan.set([1] * 4, [n] * 4)
+        outs.append((n, plan.run(q, kv, table)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, wants[n]) for n, o in outs)
+
+
+@pytest.mark.parametrize('dtype,cache', [(F16, F16), (BF16, BF16), (BF16, E4M3)])
+def test_a_conversation_as_a_server_runs_it(gpu_device, dtype, cache):
+    """One system prompt prefilled once, requests' prompts on top of it, then decode steps and a draft of several tokens:
+    positions, pages and sharing as a server keeps them; every step against attention over the tokens so far."""
+    nh, nkv, hd, page, B, P = 14, 2, 64, 16, 5, 70            # 70 shared tokens: 4 whole pages and 6 positions of each one's own
+    g = torch.Generator().manual_seed(8)
+    e4m3 = cache == E4M3
+    scales = [torch.full((nkv,), 0.01, device=gpu_device) for _ in range(2)] if e4m3 else [None, None]
+    kv = PagedKV.allocate(200, page, nkv, hd, cache, *scales)
+    r = Rotary(hd, theta=1e4, scaling={'rope_type': 'linear', 'factor': 2.0})
+    plan = AttentionPlan(nh, nkv, hd, max_rows=256, max_seqs=B)
+    free = list(range(199, -1, -1))
+    shared = [free.pop() for _ in range(P // page)]
+    table = np.full((B, 20), -1, np.int32)
+    table[:, :len(shared)] = shared
+    lens = [0] * B
+    hist = [[torch.zeros((0, nkv, hd), dtype=torch.float64) for _ in range(2)] for _ in range(B)]
+    head = torch.randn((P, nh + 2 * nkv, hd), generator=g).to(dtype)
+
+    def step(counts, rows, groups):
+        for s, n in enumerate(counts):
+            for p in range(lens[s] // page, -(-(lens[s] + n) // page)):
+                if table[s, p] < 0:
+                    table[s, p] = free.pop()
+        dev = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(gpu_device)
+        seq, at = np.repeat(np.arange(B), counts), np.concatenate([np.arange(lens[s], lens[s] + n) for s, n in enumerate(counts)])
+        x, t = rows.to(gpu_device), dev(table)
+        q = kv.append(x[:, nh:nh + nkv], x[:, nh + nkv:], dev(seq), dev(at), t, rotary=r, q=x[:, :nh])
+        for s, n in enumerate(counts):
+            lens[s] += n
+        kv_lens = [lens[s] if n else 0 for s, n in enumerate(counts)]
+        plan.set(counts, kv_lens, groups)
+        out = plan.run(q, kv, t)
+        want, _, bound = attend64(q, kv.k, kv.v, t, counts, kv_lens, hd ** -0.5, *(scales if e4m3 else ()))
+        _within(out, want, bound)
+        # and against the tokens themselves, rotated in 64 bits and rounded to the cache
+        turned = rotate64(rows[:, :nh + nkv], torch.from_numpy(at.astype(np.int32)), r.inv_freq, r.factor, hd, 'half')
+        i = 0
+        for s, n in enumerate(counts):
+            for j, new in enumerate((turned[i:i + n, nh:], rows[i:i + n, nh + nkv:].double())):
+                if e4m3:
+                    new = (new / 0.01).clamp(-448, 448).float().to(E4M3).double() * 0.01
+                else:
+                    new = new.to(dtype).double()
+                hist[s][j] = torch.cat([hist[s][j], new])
+            for a in range(n):
+                m = lens[s] - n + a + 1
+                k, v = (h[:m].repeat_interleave(nh // nkv, 1) for h in hist[s])
+                w = torch.softmax((turned[i + a, :nh].to(dtype).double()[None] * k).sum(-1) * hd ** -0.5, 0)
+                ref = (w[..., None] * v).sum(0)
+                # roundings of the cache that fall on the other side: a step of the cache's type on single keys
+                assert float((out[i + a].double().cpu() - ref).abs().max()) <= float(bound[i + a].max()) + 4 * HALF[cache]
+            i += n
+
+    # the system prompt goes through sequence 0's table; the others' copies of its last 6 tokens come with their own prompts
+    step([P, 0, 0, 0, 0], head, None)
+    for s in range(1, B):
+        lens[s] = len(shared) * page
+        hist[s] = [h[:lens[s]].clone() for h in hist[0]]
+    counts = [11, 20, 7, 33, 9]
+    rows = torch.cat([torch.cat([head[len(shared) * page:] if s else head[:0], torch.randn((n - (6 if s else 0), nh + 2 * nkv, hd),
+                                                                                          generator=g).to(dtype)]) for s, n in enumerate(counts)])
+    step(counts, rows, [(B, len(shared) * page)])
+    for _ in range(4):
+        step([1] * B, torch.randn((B, nh + 2 * nkv, hd), generator=g).to(dtype), [(B, len(shared) * page)])
+    step([4, 1, 0, 3, 5], torch.randn((13, nh + 2 * nkv, hd), generator=g).to(dtype), [(2, 64), (3, 64)])
+
+
+# ------------------------------------------------------------------------------------------------ refusals of the Python layer
+def test_python_refusals(gpu_device):
+    kv = PagedKV.allocate(4, 16, 2, 64)
+    plan = AttentionPlan(4, 2, 64, 8, 4).set([1, 1], [5, 9])
+    t = torch.zeros((2, 3), dtype=torch.int32, device=gpu_device)
+    q = torch.zeros((2, 4, 64), dtype=F16, device=gpu_device)
+    i = torch.zeros(2, dtype=torch.int32, device=gpu_device)
+    r = Rotary(64)
+    plan.run(q, kv, t)
+
+    def bad(f, kind=ValueError):
+        with pytest.raises(kind):
+            f()
+    bad(lambda: plan.run(q.float(), kv, t))
+    bad(lambda: plan.run(q.bfloat16(), kv, t))                   # not the cache's type
+    bad(lambda: plan.run(q[:1], kv, t))                          # fewer rows than the plan
+    bad(lambda: plan.run(q[:, :2], kv, t))
+    bad(lambda: plan.run(q.cpu(), kv, t))
+    bad(lambda: plan.run(q, kv, t.long()))
+    bad(lambda: plan.run(q, kv, t[:1]))                          # a table of fewer sequences
+    bad(lambda: plan.run(q, kv, t[:, ::2]))
+    bad(lambda: plan.run(q, kv, t, out=q))
+    bad(lambda: plan.run(q, kv, t, out=q.float()))
+    bad(lambda: plan.run(q, kv, t, scale=0.0))
+    bad(lambda: plan.run(q, kv, t, scale=math.nan))
+    bad(lambda: plan.run(q, kv, t, lse=torch.zeros(2, 4, dtype=F16, device=gpu_device)))
+    bad(lambda: plan.run(q, kv, t, workspace=torch.zeros(8, dtype=torch.uint8, device=gpu_device)))
+    bad(lambda: plan.run(q, PagedKV.allocate(4, 16, 4, 64), t))
+    bad(lambda: plan.set([1] * 5, [1] * 5))
+    bad(lambda: plan.set([9], [9]))
+    bad(lambda: plan.set([1, 1], [5]))
+    bad(lambda: plan.set([1, 1], [5, 9], [(1, 5)]))
+    bad(lambda: plan.set([1, 1], [5, 9], []))
+    bad(lambda: plan.set([1, 1], [5, 49]) and plan.run(q, kv, t))        # longer than the table
+    bad(lambda: AttentionPlan(4, 2, 64, 8, 4).run(q, kv, t), RuntimeError)   # no lengths yet
+    bad(lambda: AttentionPlan(4, 2, 80, 8, 4))
+    bad(lambda: AttentionPlan(4, 2, 64, 8, 4, device='cpu'))
+    odd = torch.zeros(2 * 4 * 64 + 1, dtype=F16, device=gpu_device)[1:].view(2, 4, 64)
+    plan.set([1, 1], [5, 9])
+    bad(lambda: plan.run(odd, kv, t))                            # not aligned to 16 bytes
+    bad(lambda: r.apply(q, i.long()))
+    bad(lambda: r.apply(q, i[:1]))
+    bad(lambda: r.apply(q.half()[:, :, :32], i))
+    bad(lambda: r.apply(q, i, out=q[:1]))
+    bad(lambda: r.apply(q, i, out=q.float()))
+    buf = torch.zeros(3, 4, 64, dtype=F16, device=gpu_device)
+    bad(lambda: r.apply(buf[:2], i, out=buf[1:]))
+    bad(lambda: r.apply(q, i, out=buf[:1].expand(2, 4, 64)))
+    bad(lambda: Rotary(64, layout='other'))
+    bad(lambda: Rotary(64, rot_dim=128))
+    k = torch.zeros((2, 2, 64), dtype=F16, device=gpu_device)
+    app = lambda **kw: kv.append(**{**dict(k=k, v=k, seq=i, pos=i, table=t, rotary=r, q=q), **kw})
+    assert app().shape == q.shape
+    bad(lambda: app(v=k.float()))
+    bad(lambda: app(k=k[:, :1]))
+    bad(lambda: app(seq=i[:1]))
+    bad(lambda: app(pos=i.long()))
+    bad(lambda: app(table=t.view(-1)))
+    bad(lambda: app(q=q[:1]))
+    bad(lambda: app(q=None, q_out=q))
+    bad(lambda: app(q_out=q[:1]))
+    bad(lambda: app(q_out=torch.cat([q, q])[1:3], q=torch.cat([q, q])[:2].float()))
+    bad(lambda: app(rotary=Rotary(128)))
+    z = torch.zeros((4, 2, 16, 64), dtype=F16, device=gpu_device)
+    bad(lambda: PagedKV(z, z.float()))
+    bad(lambda: PagedKV(z.float(), z.float()))
+    bad(lambda: PagedKV(z.transpose(1, 2), z.transpose(1, 2)))
+    bad(lambda: PagedKV(z[:1].expand(4, 2, 16, 64), z))
+    bad(lambda: PagedKV(z, z, k_scale=torch.ones(2, device=gpu_device)))
+    bad(lambda: PagedKV(z.to(E4M3), z.to(E4M3)))
+    bad(lambda: PagedKV(z.cpu(), z.cpu()))
+    torch.cuda.synchronize()
