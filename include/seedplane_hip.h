@@ -407,13 +407,14 @@ int sp_op_rotate(const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t
                  int64_t x_row, int64_t x_head, void *out_dev, int64_t out_row, int64_t out_head, const int32_t *pos_dev,
                  void *hip_stream);
 
-/* One layer's paged cache: pages [n_pages] of [n_kv_heads][page_size][head_dim] values, page_stride elements apart (the same
- * for keys and values).  A sequence's position p lies in row p % page_size of page table[seq][p / page_size].  e4m3 caches hold
- * value / scale with a positive fp32 scale per K/V head, for keys and for values. */
+/* One layer's paged cache: row r of head h of page e starts at e * page_stride + h * head_stride + r * row_stride elements, the same
+ * for keys and values ([pages][heads][rows], [pages][rows][heads], one allocation for both, ...: distinct rows must not
+ * overlap).  A sequence's position p lies in row p % page_size of page table[seq][p / page_size].  e4m3 caches hold value / scale
+ * with a positive fp32 scale per K/V head, for keys and for values. */
 typedef struct sp_paged_kv {
     void *k_dev, *v_dev;
     const float *k_scale_dev, *v_scale_dev;   /* device [n_kv_heads], SP_DT_E4M3 only (NULL otherwise) */
-    int64_t page_stride;
+    int64_t page_stride, head_stride, row_stride;
     int32_t dtype;                            /* SP_DT_F16, SP_DT_BF16 or SP_DT_E4M3 */
     int32_t n_pages, page_size, n_kv_heads, head_dim;
     int32_t reserved0;
@@ -463,7 +464,9 @@ size_t sp_attn_plan_workspace(const sp_attn_plan *plan);
  * logarithm of each row's sum of exponentials (-infinity for a row that sees nothing).  table_dev: int32 [n_seq][max_pages];
  * entries of positions at or behind a sequence's length are not read, an entry outside [0, n_pages) hides its positions.  What
  * the pool holds outside the positions read does not matter (NaN included).  scale must be positive.  workspace_dev: see
- * above; calls that overlap (other streams, graphs replayed side by side) need a workspace each. */
+ * above; calls that overlap (other streams, graphs replayed side by side) need a workspace each.  The cache's strides are
+ * multiples of head_dim here.  A captured call keeps its own n_rows, n_seq and max_pages: what a later set has beyond them is not
+ * read or written. */
 int sp_op_paged_attention(const sp_attn_plan *plan, const sp_paged_kv *kv, int32_t dtype, int32_t n_rows, const void *q_dev,
                           int64_t q_row, int64_t q_head, const int32_t *table_dev, int32_t n_seq, int32_t max_pages, float scale,
                           void *out_dev, int64_t out_row, int64_t out_head, float *lse_dev, void *workspace_dev,

@@ -49,6 +49,7 @@ class RotaryDesc(ctypes.Structure):
 
 class PagedKVDesc(ctypes.Structure):
     _fields_ = [('k', c_void_p), ('v', c_void_p), ('k_scale', c_void_p), ('v_scale', c_void_p), ('page_stride', c_int64),
+                ('head_stride', c_int64), ('row_stride', c_int64),
                 ('dtype', c_int32), ('n_pages', c_int32), ('page_size', c_int32), ('n_kv_heads', c_int32), ('head_dim', c_int32),
                 ('reserved0', c_int32)]
 

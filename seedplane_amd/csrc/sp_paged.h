@@ -34,7 +34,7 @@ struct AttnArgs {
     const float *ks, *vs;             // e4m3: scale per K/V head
     const int *table;                 // [n_seq][max_pages]
     int rows, n_seq, max_pages, n_pages, page_size;      // rows of q and out, of the table; its width; the pool
-    uint32_t page_rows;               // page stride in rows of head_dim values
+    uint32_t page_rows, head_rows, slot_rows;     // strides of the pool in rows of head_dim values
     int NH, G;
     float scale;                      // of the scores, times log2(e)
     const Item *items;
@@ -308,7 +308,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
             if (key < w.k1 && w.seq < a.n_seq && page < a.max_pages) {
                 const int e = table[page];
                 ok = e >= 0 && e < a.n_pages;
-                if (ok) r = (uint32_t)e * a.page_rows + (uint32_t)(w.kvh * a.page_size + key - page * a.page_size);
+                if (ok) r = (uint32_t)e * a.page_rows + (uint32_t)w.kvh * a.head_rows + (uint32_t)(key - page * a.page_size) * a.slot_rows;
             }
             sh.rows[j] = r;
             const uint64_t b = __ballot(ok);

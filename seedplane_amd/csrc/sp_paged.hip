@@ -113,8 +113,9 @@ void check_cache(const sp_paged_kv *kv) {
             "the cache's dtype must be SP_DT_F16, SP_DT_BF16 or SP_DT_E4M3");
     require(kv->n_pages >= 1 && kv->page_size >= 1 && kv->n_kv_heads >= 1 && kv->head_dim >= 2, SP_EINVAL,
             "the cache's sizes must be positive");
-    require(kv->page_stride >= (int64_t)kv->n_kv_heads * kv->page_size * kv->head_dim, SP_EINVAL,
-            "page_stride is smaller than a page");
+    require((kv->n_pages == 1 || kv->page_stride >= kv->head_dim) && (kv->n_kv_heads == 1 || kv->head_stride >= kv->head_dim) &&
+                (kv->page_size == 1 || kv->row_stride >= kv->head_dim) && kv->page_stride >= 0 && kv->head_stride >= 0 && kv->row_stride >= 0,
+            SP_EINVAL, "the cache's strides are smaller than a row");
     require((kv->dtype == SP_DT_E4M3) == (kv->k_scale_dev != nullptr) && (kv->dtype == SP_DT_E4M3) == (kv->v_scale_dev != nullptr),
             SP_EINVAL, "an e4m3 cache has k_scale_dev and v_scale_dev, others have none");
 }
@@ -300,10 +301,11 @@ int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t d
         a.pos = pos_dev; a.seq = seq_dev; a.at = at_dev; a.table = table_dev;
         a.rows = n_rows; a.nq = nq; a.nkv = kv->n_kv_heads; a.hd = hd; a.qo_dt = q_out_dtype; a.kv_dt = kv->dtype;
         a.n_seq = n_seq; a.max_pages = max_pages; a.n_pages = kv->n_pages; a.page_size = kv->page_size;
-        a.page_stride = kv->page_stride;
+        a.page_stride = kv->page_stride; a.head_stride = kv->head_stride; a.row_stride = kv->row_stride;
         const bool wide = (!q_dev || (wide_ok(q_dev, dtype, q_row, q_head) && wide_ok(q_out_dev, q_out_dtype, q_out_row, q_out_head))) &&
                           wide_ok(k_dev, dtype, k_row, k_head) && wide_ok(v_dev, dtype, v_row, v_head) &&
-                          wide_ok(kv->k_dev, kv->dtype, kv->page_stride, 0) && wide_ok(kv->v_dev, kv->dtype, kv->page_stride, 0) &&
+                          wide_ok(kv->k_dev, kv->dtype, kv->page_stride, kv->head_stride) &&
+                          wide_ok(kv->v_dev, kv->dtype, kv->row_stride, 0) &&
                           rot.rot % 16 == 0 && hd % 8 == 0;
         const int vec = wide ? 8 : 1;
         a.units = rot.rot / 2 / vec;
@@ -430,8 +432,14 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         require(n_rows >= p->n_tok, SP_EINVAL, "the queries have fewer rows than the plan");
         require(n_seq >= p->n_seq && max_pages >= 1, SP_EINVAL, "the page table has fewer sequences than the plan");
         require((int64_t)max_pages * kv->page_size >= p->max_kv, SP_EINVAL, "the page table is too short for the plan's lengths");
-        require(kv->page_stride % kv->head_dim == 0 && (int64_t)kv->n_pages * (kv->page_stride / kv->head_dim) < ((int64_t)1 << 32),
-                SP_EINVAL, "page_stride must be a multiple of head_dim and the pool below 2^32 rows");
+        const int64_t hd = kv->head_dim;
+        require(kv->page_stride % hd == 0 && kv->head_stride % hd == 0 && kv->row_stride % hd == 0, SP_EINVAL,
+                "the cache's strides must be multiples of head_dim");
+        constexpr int64_t MOST = (int64_t)1 << 32;
+        require(kv->page_stride / hd < MOST && kv->head_stride / hd < MOST && kv->row_stride / hd < MOST &&
+                    (double)(kv->n_pages - 1) * (kv->page_stride / hd) + (double)(kv->n_kv_heads - 1) * (kv->head_stride / hd) +
+                            (double)(kv->page_size - 1) * (kv->row_stride / hd) < (double)MOST,
+                SP_EINVAL, "the pool must be below 2^32 rows");
         int dev = 0;
         HIPCHK(hipGetDevice(&dev));
         require(dev == p->device, SP_EINVAL, "the plan belongs to another device than the current one");
@@ -444,8 +452,7 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
             require(!may_overlap(to, q_dev, dtype, n_rows, p->NH, p->HD, q_row, q_head), SP_EINVAL, "the output overlaps the queries");
         }
         require(aligned(out_dev, 8) && out_row % 4 == 0 && out_head % 4 == 0, SP_EINVAL, "outputs must be aligned to 8 bytes");
-        require(aligned(kv->k_dev, 16) && aligned(kv->v_dev, 16) && kv->page_stride * bytes_of(kv->dtype) % 16 == 0 &&
-                    kv->head_dim * bytes_of(kv->dtype) % 16 == 0,
+        require(aligned(kv->k_dev, 16) && aligned(kv->v_dev, 16) && kv->head_dim * bytes_of(kv->dtype) % 16 == 0,
                 SP_EINVAL, "the cache's pages must be aligned to 16 bytes");
         require(aligned(workspace_dev, 16), SP_EINVAL, "the workspace must be aligned to 16 bytes");
         const hipStream_t st = (hipStream_t)stream;
@@ -456,7 +463,8 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         a.k = (const uint8_t *)kv->k_dev; a.v = (const uint8_t *)kv->v_dev; a.ks = kv->k_scale_dev; a.vs = kv->v_scale_dev;
         a.rows = n_rows; a.n_seq = n_seq;
         a.table = table_dev; a.max_pages = max_pages; a.n_pages = kv->n_pages; a.page_size = kv->page_size;
-        a.page_rows = (uint32_t)(kv->page_stride / kv->head_dim);
+        a.page_rows = (uint32_t)(kv->page_stride / hd); a.head_rows = (uint32_t)(kv->head_stride / hd);
+        a.slot_rows = (uint32_t)(kv->row_stride / hd);
         a.NH = p->NH; a.G = p->NH / p->NKV;
         a.scale = scale * LOG2E;
         const size_t recs = (size_t)records_bound(p->max_rows, p->NH);

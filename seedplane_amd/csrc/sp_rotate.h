@@ -204,7 +204,7 @@ struct AppendArgs {
     const int *pos, *seq, *at, *table;           // rotation position, sequence, cached position of a row; [n_seq][max_pages]
     int rows, nq, nkv, hd, qo_dt, kv_dt, per_block;
     int n_seq, max_pages, n_pages, page_size;
-    int64_t page_stride;
+    int64_t page_stride, head_stride, row_stride;
     int units, tail, vecs;                       // of a head: rotated units, vectors of the rest, vectors of a value
     int turned, rest, per_row;                   // units of a row: rotated, unrotated rests of queries and keys, all
     Divisor by_row, by_units, by_tail, by_vecs, by_half;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(ROT_THREADS) k_append(AppendArgs a) {
         int64_t to = -1;
         if (s >= 0 && s < a.n_seq && p >= 0 && p / a.page_size < a.max_pages) {
             const int e = a.table[(int64_t)s * a.max_pages + p / a.page_size];
-            if (e >= 0 && e < a.n_pages) to = e * a.page_stride + (int64_t)(p % a.page_size) * a.hd;
+            if (e >= 0 && e < a.n_pages) to = e * a.page_stride + (p % a.page_size) * a.row_stride;
         }
         dst[k] = to;
     }
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(ROT_THREADS) k_append(AppendArgs a) {
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) { v1[j] /= scale; v2[j] /= scale; }
                 }
-                const int64_t o = to + (int64_t)h * a.page_size * a.hd;
+                const int64_t o = to + h * a.head_stride;
                 store_values<VEC>(key ? a.kc : a.vc, o + at1, a.kv_dt, v1);
                 if (two) store_values<VEC>(key ? a.kc : a.vc, o + at2, a.kv_dt, v2);
             }

@@ -172,8 +172,10 @@ class Rotary:
 
 
 class PagedKV:
-    """One layer's pages: `k` and `v` [n_pages, kv_heads, page_size, head_dim], fp16, bf16 or float8_e4m3fn; pages may lie
-    further apart than their size (the same for both).  An e4m3 cache holds value / scale, with fp32 scales per K/V head."""
+    """One layer's pages: `k` and `v` [n_pages, kv_heads, page_size, head_dim], fp16, bf16 or float8_e4m3fn, or views of that
+    shape (`pool.transpose(1, 2)` of a [n_pages, page_size, kv_heads, head_dim] pool, halves of one allocation, ...) with the
+    same strides for both and the values of a row side by side.  An e4m3 cache holds value / scale, with fp32 scales per K/V
+    head."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
@@ -181,8 +183,8 @@ class PagedKV:
         if k.dtype not in _DTYPES or k.dtype == torch.float32:
             raise ValueError('the cache must be fp16, bf16 or float8_e4m3fn')
         n, nkv, page, hd = k.shape
-        if 0 in k.shape or k.stride()[1:] != (page * hd, hd, 1) or (n > 1 and k.stride(0) < nkv * page * hd):
-            raise ValueError('a page must be contiguous and pages must not overlap')
+        if 0 in k.shape or k.stride(3) != 1 or any(m > 1 and s < hd for m, s in zip(k.shape[:3], k.stride())):
+            raise ValueError('the values of a row must lie side by side and rows must not overlap')
         e4m3 = k.dtype == torch.float8_e4m3fn
         for s in (k_scale, v_scale):
             if (s is not None) != e4m3:
@@ -197,10 +199,13 @@ class PagedKV:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, nkv, page, hd
         self.dtype = k.dtype
-        stride = k.stride(0) if n > 1 else nkv * page * hd
         self.desc = _lib.PagedKVDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if e4m3 else None,
-                                     v_scale.data_ptr() if e4m3 else None, stride, _DTYPES[k.dtype], n, page, nkv, hd, 0)
+                                     v_scale.data_ptr() if e4m3 else None, *self._strides(), _DTYPES[k.dtype], n, page, nkv, hd, 0)
         self._ref = ctypes.addressof(self.desc)
+
+    def _strides(self):
+        """Strides of pages, heads and rows; of a dimension of one entry: any that suits the kernels."""
+        return [s if n > 1 else self.head_dim for n, s in zip(self.k.shape[:3], self.k.stride())]
 
     @classmethod
     def allocate(cls, n_pages, page_size, n_kv_heads, head_dim, dtype=torch.float16, k_scale=None, v_scale=None, device='cuda'):

@@ -344,6 +344,36 @@ class Qwen2Engine:
             return torch.as_tensor(_Pool(), device=self.device)
         return view(k), view(v)
 
+    def paged_kv(self, layer, page_size=None):
+        """Layer `layer`'s pool as a paged cache (paged.PagedKV) that shares the engine's memory: pages of `page_size` ring
+        slots, a divisor of the pool's slots (default: a sequence's whole ring), so that what the engine prefilled can be a
+        shared prefix of paged attention without a copy.  Valid until the pool is reserved or grown again."""
+        from .paged import PagedKV
+        k, v = self._kv_pool(range(self.n_layers)[layer])
+        n, nkv, S, hd = k.shape
+        page = self._page_size(page_size)
+        pages = (n * nkv * S - (nkv - 1) * S) // page           # head 0 of any page, so that every head lies in the pool
+        return PagedKV(*(t.as_strided((pages, nkv, page, hd), (page * hd, S * hd, hd, 1)) for t in (k, v)))
+
+    def page_table(self, caches, page_size=None):
+        """The pages of `caches` in paged_kv(layer, page_size), int32 [len(caches), slots / page_size] on the engine's device: of
+        caches whose ring has not wrapped, position p lies in page p // page_size."""
+        page, S = self._page_size(page_size), self._pool_slots
+        for c in caches:
+            self._check_cache(c)
+            if c.length > S:
+                raise ValueError('the ring of a cache has wrapped: its positions have no pages of their own')
+        first = torch.tensor([c.seq * self.n_kv_heads * S // page for c in caches], dtype=torch.int32).view(-1, 1)
+        return (first + torch.arange(S // page, dtype=torch.int32)).to(self.device)
+
+    def _page_size(self, page_size):
+        if not self._pool_slots:
+            raise ValueError('the KV pool is not reserved')
+        page = self._pool_slots if page_size is None else int(page_size)
+        if page < 1 or self._pool_slots % page:
+            raise ValueError(f'page_size must divide the pool\'s {self._pool_slots} slots')
+        return page
+
     def _kv_copy(self, cache, layer, which):
         """Layer `layer`'s keys ('k') or values ('v') of `cache`, copied out of the HBM ring (see _KVLayers)."""
         self._check_cache(cache)

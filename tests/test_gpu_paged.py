@@ -235,6 +235,32 @@ def test_attention(gpu_device, dtype, cache, hd, q_lens, kv_lens, groups, nh, nk
     _attend(gpu_device, q_lens, kv_lens, groups, nh, nkv, hd, page, dtype, cache, seed=len(q_lens) + hd)
 
 
+def test_layouts_of_the_pool(gpu_device):
+    """Heads before rows, rows before heads, keys and values in one allocation, one page, one head: append and attention."""
+    nkv, hd, page, n, L = 2, 64, 16, 12, 150
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn((L, 4 + 2 * nkv, hd), generator=g).half().to(gpu_device)
+    at = torch.arange(L, dtype=torch.int32, device=gpu_device)
+    table = torch.randperm(n, generator=g).int().view(1, n).to(gpu_device)
+    plan = AttentionPlan(4, nkv, hd, 9, 1).set([9], [L])
+    zeros = lambda *s: torch.zeros(s, dtype=F16, device=gpu_device)
+    nhd, both, apart = zeros(2, n, page, nkv, hd), zeros(n, 2, nkv, page, hd), zeros(2, n, nkv + 1, page + 3, 2 * hd)
+    outs, pools = [], []
+    for kv in (PagedKV.allocate(n, page, nkv, hd), PagedKV(nhd[0].transpose(1, 2), nhd[1].transpose(1, 2)), PagedKV(both[:, 0], both[:, 1]),
+               PagedKV(apart[0, :, :nkv, :page, :hd], apart[1, :, :nkv, :page, :hd])):
+        kv.append(x[:, 4:4 + nkv], x[:, 4 + nkv:], torch.zeros_like(at), at, table)
+        outs.append(plan.run(x[-9:, :4], kv, table))
+        pools.append((kv.k.clone(), kv.v.clone()))
+    assert all(torch.equal(o, outs[0]) for o in outs) and all(torch.equal(a, b) for p in pools for a, b in zip(p, pools[0]))
+    assert (apart[:, :, nkv:] == 0).all() and (apart[:, :, :, page:] == 0).all() and (apart[..., hd:] == 0).all()
+    _within(outs[0], *attend64(x[-9:, :4], *pools[0], table, [9], [L], 0.125)[::2])
+    one = PagedKV(zeros(1, 1, 200, hd), zeros(1, 1, 200, hd))
+    t1 = torch.zeros((1, 1), dtype=torch.int32, device=gpu_device)
+    one.append(x[:, 4:5], x[:, 6:7], torch.zeros_like(at), at, t1)
+    got = AttentionPlan(2, 1, hd, 9, 1).set([9], [L]).run(x[-9:, :2], one, t1)
+    _within(got, *attend64(x[-9:, :2], one.k, one.v, t1, [9], [L], 0.125)[::2])
+
+
 def test_attention_views_pages_apart_scale_and_no_lse(gpu_device):
     """q and out as views of wider rows, pages further apart than their size, another scale, no lse."""
     q_lens, kv_lens, groups = [1, 4, 1], [90, 100, 70], [(3, 64)]
@@ -560,7 +586,8 @@ def test_python_refusals(gpu_device):
     z = torch.zeros((4, 2, 16, 64), dtype=F16, device=gpu_device)
     bad(lambda: PagedKV(z, z.float()))
     bad(lambda: PagedKV(z.float(), z.float()))
-    bad(lambda: PagedKV(z.transpose(1, 2), z.transpose(1, 2)))
+    bad(lambda: PagedKV(z.transpose(2, 3), z.transpose(2, 3)))
+    bad(lambda: PagedKV(z, z.transpose(1, 2).contiguous().transpose(1, 2)))
     bad(lambda: PagedKV(z[:1].expand(4, 2, 16, 64), z))
     bad(lambda: PagedKV(z, z, k_scale=torch.ones(2, device=gpu_device)))
     bad(lambda: PagedKV(z.to(E4M3), z.to(E4M3)))

@@ -12,8 +12,8 @@ def rotary(inv=P, rot=64, layout=0):
     return _lib.RotaryDesc(inv, rot, layout, 1.0, 0)
 
 
-def cache(dtype=_lib.SP_DT_F16, k=P, v=2 * P, ks=None, vs=None, stride=4 * 16 * 64, n=8, page=16, nkv=4, hd=64):
-    return _lib.PagedKVDesc(k, v, ks, vs, stride, dtype, n, page, nkv, hd, 0)
+def cache(dtype=_lib.SP_DT_F16, k=P, v=2 * P, ks=None, vs=None, stride=4 * 16 * 64, head=16 * 64, row=64, n=8, page=16, nkv=4, hd=64):
+    return _lib.PagedKVDesc(k, v, ks, vs, stride, head, row, dtype, n, page, nkv, hd, 0)
 
 
 def rotate(r=None, dtype=_lib.SP_DT_F16, rows=4, heads=8, hd=64, x=P, x_row=512, x_head=64, out=4 * P, out_row=512, out_head=64, pos=P):
@@ -50,7 +50,8 @@ def append(kv=None, r=None, dtype=_lib.SP_DT_F16, rows=4, heads=8, q=8 * P, q_ro
 
 @pytest.mark.parametrize('kw', [
     dict(kv=False), dict(kv=cache(k=None)), dict(kv=cache(v=None)), dict(kv=cache(dtype=_lib.SP_DT_F32)), dict(kv=cache(dtype=9)),
-    dict(kv=cache(n=0)), dict(kv=cache(page=0)), dict(kv=cache(nkv=0)), dict(kv=cache(hd=0)), dict(kv=cache(stride=100)),
+    dict(kv=cache(n=0)), dict(kv=cache(page=0)), dict(kv=cache(nkv=0)), dict(kv=cache(hd=0)), dict(kv=cache(stride=63)), dict(kv=cache(head=0)),
+    dict(kv=cache(row=-64)), dict(kv=cache(row=32)),
     dict(kv=cache(ks=P, vs=P)), dict(kv=cache(dtype=_lib.SP_DT_E4M3)), dict(kv=cache(dtype=_lib.SP_DT_E4M3, ks=P)),
     dict(dtype=_lib.SP_DT_E4M3), dict(rows=-1), dict(heads=0), dict(heads=2000), dict(q_out=None), dict(q=None),
     dict(q_dt=_lib.SP_DT_E4M3), dict(n_seq=0), dict(width=0), dict(r=rotary(rot=128)),
