@@ -35,12 +35,16 @@ struct AttnArgs {
     const int *table;                 // [n_seq][max_pages]
     int rows, n_seq, max_pages, n_pages, page_size;      // rows of q and out, of the table; its width; the pool
     uint32_t page_rows, head_rows, slot_rows;     // strides of the pool in rows of head_dim values
-    int NH, G;
+    int NH, G, page_shift;            // page_shift: log2 of page_size, -1 where that is no power of two
+    Divisor by_g;
     float scale;                      // of the scores, times log2(e)
     const Item *items;
     const int *n_items;               // NULL: one block per item
-    float *po;                        // records: [rows][HD] unnormalised outputs
-    float2 *ml;                       // [rows] (m in log2 units, l)
+    // Records: [rows][HD] unnormalised outputs as fp16 shares of the row's largest (half the traffic of fp32; off by 2^-12 of
+    // that largest at most, whatever its size, where the outputs themselves are rounded by 2^-9 or 2^-12 of each), and [rows]
+    // (m in log2 units, l, the largest)
+    f16 *po;
+    f32x4 *ml;
 };
 
 template <class T> struct Mma;
@@ -102,6 +106,7 @@ struct AttnShared {                                                    // beside
     uint32_t rows[TABLE_KEYS];                                         // pool row of each position (0 where there is none)
     uint32_t seen[TABLE_KEYS / 32];                                    // which positions exist
     float2 ml[4][32];
+    float top[4][32];
 };
 
 template <bool KV8, int HD, int WM>
@@ -113,7 +118,8 @@ struct AttnTile {
     static constexpr int TILE = KT * RB;                               // bytes of a tile's keys (and of its values)
     static constexpr int ALL = KT * NCH / 64;                          // copies of a tile's keys, and of its values
     static constexpr int COPIES = ALL < WM ? 1 : ALL / WM;             // ... of a wave (of the first ALL waves, if fewer)
-    static constexpr int JOIN = (WK - 1) * WM * 32 * HD * 4;           // LDS of the join over the key waves
+    static constexpr int QUADS = HD / 8;                               // 4-value pieces of a lane's half of a row
+    static constexpr int JOIN = 4 * 32 * HD * 4;                       // LDS of the join over the key waves
     static_assert(ALL >= 1 && (ALL < WM || ALL % WM == 0), "whole copies");
     static_assert(WK * STAGES * 2 * TILE <= TILE_SMEM && JOIN <= TILE_SMEM, "LDS plan");
     static_assert(TABLE_KEYS % (WK * KT) == 0, "whole rounds of the row table");
@@ -143,23 +149,28 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
         (uint32_t)(size_t)((__attribute__((address_space(3))) unsigned char *)buf0));
 
+    // The chain of an item is its table's entries, their rows of the pool, the copies: the entries are asked for first.
+    const int *table = a.table + (int64_t)w.seq * a.max_pages;
+    auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size; };
+    auto entry_of = [&](int key, int page) { return key < w.k1 && w.seq < a.n_seq && page < a.max_pages ? table[page] : -1; };
+    const int key0 = w.k0 + (int)threadIdx.x, page0 = page_of(key0), entry0 = entry_of(key0, page0);
+
     const int row = rw * 32 + col;
     // (a captured call may meet tables set later: its own sizes bound every access)
-    const bool live = row < w.ntok * a.G && w.tok0 + row / a.G < a.rows;
-    const int tok = live ? row / a.G : 0, hh = live ? row - tok * a.G : 0;
+    const int rt = row / a.by_g;
+    const bool live = row < w.ntok * a.G && w.tok0 + rt < a.rows;
+    const int tok = live ? rt : 0, hh = live ? row - rt * a.G : 0;
     frag qf[NS];
     {
         const T *q = (const T *)a.q + (int64_t)min(w.tok0 + tok, a.rows - 1) * a.q_row + (int64_t)(w.kvh * a.G + hh) * a.q_head + 8 * h;
 #pragma unroll
         for (int s = 0; s < NS; ++s) qf[s] = *(const frag *)(q + 16 * s);
     }
-    // the row sees positions < lim; rows behind the tile's last compute along and are never stored
+    // the row sees positions < lim; rows behind the tile's last compute along and are never stored.  lo and hi: the least and
+    // the greatest of the wave's rows (its first and last token)
     const int lim = live ? min(w.k1, w.pos0 + tok + 1) : w.k1;
-    int lo = lim, hi = live ? lim : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o)); hi = max(hi, __shfl_xor(hi, o)); }
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    hi = __builtin_amdgcn_readfirstlane(hi);
+    const int lo = min(w.k1, w.pos0 + (rw * 32) / a.by_g + 1);
+    const int hi = rw * 32 < w.ntok * a.G ? min(w.k1, w.pos0 + min(w.ntok - 1, (rw * 32 + 31) / a.by_g) + 1) : 0;
     const float sc = KV8 ? a.scale * a.ks[w.kvh] : a.scale;
 
     const int swz = piece_swap<NCH>(col);
@@ -245,20 +256,25 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
 #pragma unroll
         for (int p = 0; p < NS; ++p) s = M::run(kf[p], qf[p], s);
     };
-    // masks the scores of positions t0 .. t0 + 31 and brings the running maximum up to date; returns the exponent's base
-    auto maxima = [&](f32x16 &s, int t0, uint32_t seen) -> float {
-        if (t0 + 32 > lo || seen != ~0u) {
-            const uint32_t mine = seen >> (4 * h);
-            const int left = lim - t0 - 4 * h;
+    // masks a tile's scores, positions from t0, and brings the running maximum up to date; returns the exponent's base
+    auto maxima = [&](f32x16 (&s)[SUB], int t0, const uint32_t (&seen)[SUB]) -> float {
+        if (t0 + KT > lo || (seen[0] & seen[SUB - 1]) != ~0u) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int kk = 8 * (j / 4) + j % 4;
-                s[j] = kk < left && ((mine >> kk) & 1) ? s[j] : -INFINITY;
+            for (int u = 0; u < SUB; ++u) {
+                const uint32_t mine = seen[u] >> (4 * h);
+                const int left = lim - t0 - u * 32 - 4 * h;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int kk = 8 * (j / 4) + j % 4;
+                    s[u][j] = kk < left && ((mine >> kk) & 1) ? s[u][j] : -INFINITY;
+                }
             }
         }
-        float mx = s[0];
+        float mx = s[0][0];
 #pragma unroll
-        for (int j = 1; j < 16; ++j) mx = fmaxf(mx, s[j]);
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[u][j]);
         mx = fmaxf(m, half_max(mx) * sc);
         // weights are taken from the base m, which follows the maximum only when that has grown by more than 2^8: up to there
         // they fit every type, and the outputs need no rescaling.  (A row that has seen nothing stays empty.)
@@ -273,8 +289,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         }
         return m == -INFINITY ? 0.f : m;
     };
-    frag pf[2];
-    auto weights = [&](const f32x16 &s, float base) {
+    auto weights = [&](const f32x16 &s, float base, frag (&pf)[2]) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const float p = __builtin_amdgcn_exp2f(s[j] * sc - base);
@@ -282,7 +297,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
             pf[j / 8][j % 8] = (T)p;
         }
     };
-    auto outputs = [&](const unsigned char *vb) {
+    auto outputs = [&](const unsigned char *vb, const frag (&pf)[2]) {
         frag vf[2][ND];
 #pragma unroll
         for (int y = 0; y < 2; ++y)
@@ -294,23 +309,40 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] = M::run(vf[y][d], pf[y], o[d]);
     };
+    // the tile's weights and outputs: the second half's exponentials stand between the first half's matrix products
+    auto tile_outputs = [&](const unsigned char *vb, const f32x16 (&s)[SUB], float base) {
+        frag pf[SUB][2];
+        weights(s[0], base, pf[0]);
+        if constexpr (SUB == 2) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] = M::run(value_frag(vb, y, d), pf[0][y], o[d]);
+            weights(s[1], base, pf[1]);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);                 // LDS reads ahead
+#pragma unroll
+            for (int i = 0; i < 2 * ND; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // a matrix product
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 64 / (2 * ND), 0); // exponentials, sums, roundings
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        outputs(vb + (SUB - 1) * 32 * RB, pf[SUB - 1]);
+    };
 
-    const int *table = a.table + (int64_t)w.seq * a.max_pages;
     for (int c0 = w.k0; c0 < w.k1; c0 += TABLE_KEYS) {
-        // the pool rows of the next positions, NO_ROW where there is none
-        if (c0 != w.k0) lds_barrier();
+        // the pool rows of the next positions (row 0 where there is none), and which exist
+        const bool first = c0 == w.k0;
+        if (!first) lds_barrier();
         const int tid = opaque(threadIdx.x);
 #pragma unroll 1
         for (int j = tid; j < TABLE_KEYS && c0 + j - tid < w.k1 + 64; j += 256) {  // (a tile past the end reads up to 63 rows past it)
-            const int key = c0 + j, page = key / a.page_size;
-            uint32_t r = 0;
-            bool ok = false;
-            if (key < w.k1 && w.seq < a.n_seq && page < a.max_pages) {
-                const int e = table[page];
-                ok = e >= 0 && e < a.n_pages;
-                if (ok) r = (uint32_t)e * a.page_rows + (uint32_t)w.kvh * a.head_rows + (uint32_t)(key - page * a.page_size) * a.slot_rows;
-            }
-            sh.rows[j] = r;
+            const int key = c0 + j, page = first && j == tid ? page0 : page_of(key);
+            const int e = first && j == tid ? entry0 : entry_of(key, page);
+            const bool ok = e >= 0 && e < a.n_pages;
+            sh.rows[j] = ok ? (uint32_t)e * a.page_rows + (uint32_t)w.kvh * a.head_rows + (uint32_t)(key - page * a.page_size) * a.slot_rows : 0u;
             const uint64_t b = __ballot(ok);
             if ((tid & 63) == 0) *(uint64_t *)&sh.seen[j / 32] = b;
         }
@@ -330,23 +362,20 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
             }
             for (int t = kw; t < n; t += WK) {
                 const bool more = t + WK < n;
-                copies_wait<TL::COPIES>();
+                uint32_t seen[SUB];
 #pragma unroll
-                for (int u = 0; u < SUB; ++u) {
-                    f32x16 s;
-                    scores(kb + u * 32 * RB, s);
-                    if (u == SUB - 1) {
-                        lds_wait();
-                        if (more) copy_tile(a.k, t + WK, lds0);
-                    }
-                    weights(s, maxima(s, c0 + t * KT + u * 32, seen_of(t * SUB + u)));
-                    if (u == 0) {
-                        if (more && SUB == 1) copies_wait<TL::COPIES>();
-                        else copies_wait<0>();
-                        clear_values(vb, t, SUB == 1 ? seen_of(t) : seen_of(t * SUB) & seen_of(t * SUB + SUB - 1));
-                    }
-                    outputs(vb + u * 32 * RB);
-                }
+                for (int u = 0; u < SUB; ++u) seen[u] = seen_of(t * SUB + u);
+                copies_wait<TL::COPIES>();
+                f32x16 s[SUB];
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) scores(kb + u * 32 * RB, s[u]);
+                lds_wait();
+                if (more) copy_tile(a.k, t + WK, lds0);
+                const float base = maxima(s, c0 + t * KT, seen);
+                if (more) copies_wait<TL::COPIES>();
+                else copies_wait<0>();
+                clear_values(vb, t, seen[0] & seen[SUB - 1]);
+                tile_outputs(vb, s, base);
                 lds_wait();
                 if (more) copy_tile(a.v, t + WK, lds0 + TL::TILE);
             }
@@ -396,11 +425,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                     scores(kb + u * 32 * RB, s[u]);
                     copies(u);
                 }
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) {
-                    weights(s[u], maxima(s[u], c0 + t * KT + u * 32, seen[u]));
-                    outputs(vb + u * 32 * RB);
-                }
+                tile_outputs(vb, s, maxima(s, c0 + t * KT, seen));
             };
             for (int i = 0; i < rounds; i += 2) {
                 step(i, std::integral_constant<int, 0>{});
@@ -410,76 +435,84 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     }
     l = half_sum(l);
 
+    // The key waves of a row group joined in LDS: each takes a share of the values (4-value pieces q0 ..) of all of them
+    constexpr int SHARE = TL::QUADS / WK;
+    const int q0 = WK > 1 ? kw * SHARE : 0;
+    f32x4 out[SHARE];
     if constexpr (WK > 1) {
-        // the key waves of a row group joined in LDS: waves kw > 0 leave theirs, wave kw = 0 adds them in order
         lds_barrier();
-        f32x4 *const area = (f32x4 *)smem;
+        f32x4 *const area = (f32x4 *)smem;                             // [key wave][piece][row wave][lane]
         if (h == 0) sh.ml[wv][col] = make_float2(m, l);
-        if (kw > 0) {
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    area[(((kw - 1) * WM + rw) * (4 * ND) + d * 4 + j) * 64 + lane] =
-                        (f32x4){o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
-        }
+            for (int j = 0; j < 4; ++j)
+                area[((kw * TL::QUADS + d * 4 + j) * WM + rw) * 64 + lane] =
+                    (f32x4){o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
         lds_barrier();
-        if (kw == 0) {
-            float mm = m;
+        float mm = -INFINITY, f[WK];
 #pragma unroll
-            for (int k = 1; k < WK; ++k) mm = fmaxf(mm, sh.ml[k * WM + rw][col].x);
-            const float base = mm == -INFINITY ? 0.f : mm;
-            float f = __builtin_amdgcn_exp2f(m - base);
-            l *= f;
+        for (int k = 0; k < WK; ++k) mm = fmaxf(mm, sh.ml[k * WM + rw][col].x);
+        const float base = mm == -INFINITY ? 0.f : mm;
+        l = 0.f;
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+        for (int k = 0; k < WK; ++k) {
+            const float2 x = sh.ml[k * WM + rw][col];
+            f[k] = __builtin_amdgcn_exp2f(x.x - base);
+            l += x.y * f[k];
+        }
+        m = mm;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[d][j] *= f;
+        for (int i = 0; i < SHARE; ++i) {
+            out[i] = area[((q0 + i) * WM + rw) * 64 + lane] * f[0];
 #pragma unroll
-            for (int k = 1; k < WK; ++k) {
-                const float2 x = sh.ml[k * WM + rw][col];
-                f = __builtin_amdgcn_exp2f(x.x - base);
-                l += x.y * f;
+            for (int k = 1; k < WK; ++k) out[i] += area[((k * TL::QUADS + q0 + i) * WM + rw) * 64 + lane] * f[k];
+        }
+    } else {
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
+        for (int i = 0; i < SHARE; ++i)
+            out[i] = (f32x4){o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+    }
+    // the row's largest value: over the lane's values, its other half, the key waves' shares
+    float top = 0.f;
+    if (w.rec >= 0) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const f32x4 y = area[(((k - 1) * WM + rw) * (4 * ND) + d * 4 + j) * 64 + lane];
+        for (int i = 0; i < SHARE; ++i)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) o[d][4 * j + c] += y[c] * f;
-                    }
-            }
-            m = mm;
+            for (int c = 0; c < 4; ++c) top = fmaxf(top, fabsf(out[i][c]));
+        top = half_max(top);
+        if constexpr (WK > 1) {
+            if (h == 0) sh.top[wv][col] = top;
+            lds_barrier();
+#pragma unroll
+            for (int k = 0; k < WK; ++k) top = fmaxf(top, sh.top[k * WM + rw][col]);
         }
     }
-    const int row2 = rw * 32 + (opaque(lane) & 31), tok2 = row2 / a.G;
-    if (kw == 0 && row2 < w.ntok * a.G && w.tok0 + tok2 < a.rows) {
-        const int row = row2, tok = tok2, hh = row2 - tok2 * a.G;
+    const int row2 = rw * 32 + (opaque(lane) & 31), tok2 = row2 / a.by_g;
+    if (row2 < w.ntok * a.G && w.tok0 + tok2 < a.rows) {
+        const int hh2 = row2 - tok2 * a.G;
         const float vs = KV8 ? a.vs[w.kvh] : 1.f;
         if (w.rec < 0) {
             const float il = l > 0.f ? vs / l : 0.f;                   // a row that sees nothing: zeros
-            const int64_t head = w.kvh * a.G + hh;
-            T *d0 = (T *)a.out + (int64_t)(w.tok0 + tok) * a.out_row + head * a.out_head + 4 * h;
+            const int64_t head = w.kvh * a.G + hh2;
+            T *d0 = (T *)a.out + (int64_t)(w.tok0 + tok2) * a.out_row + head * a.out_head + 4 * h + 8 * q0;
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    typedef T T4 __attribute__((ext_vector_type(4)));
-                    *(T4 *)(d0 + d * 32 + 8 * j) = (T4){(T)(o[d][4 * j] * il), (T)(o[d][4 * j + 1] * il),
-                                                        (T)(o[d][4 * j + 2] * il), (T)(o[d][4 * j + 3] * il)};
-                }
-            if (a.lse && h == 0)
-                a.lse[(int64_t)(w.tok0 + tok) * a.NH + head] = l > 0.f ? LN2 * (m + log2f(l)) : -INFINITY;
+            for (int i = 0; i < SHARE; ++i) {
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                *(T4 *)(d0 + 8 * i) = (T4){(T)(out[i][0] * il), (T)(out[i][1] * il), (T)(out[i][2] * il), (T)(out[i][3] * il)};
+            }
+            if (a.lse && h == 0 && kw == 0)
+                a.lse[(int64_t)(w.tok0 + tok2) * a.NH + head] = l > 0.f ? LN2 * (m + log2f(l)) : -INFINITY;
         } else {
-            const int64_t rec = w.rec + row;
-            float *d0 = a.po + rec * HD + 4 * h;
+            const int64_t rec = w.rec + row2;
+            const float share = top > 0.f ? 1.f / top : 0.f;
+            f16 *d0 = a.po + rec * HD + 4 * h + 8 * q0;
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    *(f32x4 *)(d0 + d * 32 + 8 * j) = (f32x4){o[d][4 * j] * vs, o[d][4 * j + 1] * vs, o[d][4 * j + 2] * vs,
-                                                              o[d][4 * j + 3] * vs};
-            if (h == 0) a.ml[rec] = make_float2(m, l);
+            for (int i = 0; i < SHARE; ++i) {
+                typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+                *(f16x4 *)(d0 + 8 * i) = (f16x4){(f16)(out[i][0] * share), (f16)(out[i][1] * share), (f16)(out[i][2] * share), (f16)(out[i][3] * share)};
+            }
+            if (h == 0 && kw == 0) a.ml[rec] = (f32x4){m, l, top * vs, 0.f};
         }
     }
 }
@@ -499,22 +532,25 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(AttnArgs a) {
 }
 
 // The records of a token joined.  Tokens whose item wrote the output itself are left alone; a token without any key gets zeros
-// (and lse -inf).  WAVES waves of a block share a (token, query head): each takes every WAVES-th batch of records, two
-// (HD 128) or four (64) records per load and UNROLL loads in flight, and wave 0 adds the waves' sums in order.
+// (and lse -inf).  WAVES waves of a block share a (token, query head): each takes every WAVES-th batch of records, four
+// (HD 128) or eight (64) records per load and UNROLL loads in flight, and wave 0 adds the waves' sums in order.
 struct JoinArgs {
     const TokenRecs *toks;
     const int *n_toks;
-    const float *po;
-    const float2 *ml;
+    const f16 *po;
+    const f32x4 *ml;
     void *out;
     float *lse;
     int64_t out_row, out_head;
     int rows, NH, G;
 };
+constexpr int JOIN_UNROLL = 4;
+template <int HD> constexpr int JOIN_BATCH = 64 / (HD / 8) * JOIN_UNROLL;      // records that a wave has in flight
 template <class T, int HD, int WAVES>
 __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
-    constexpr int LPR = HD / 4, RPL = 64 / LPR, UNROLL = 4;            // lanes per record, records per load
-    __shared__ f32x4 sum_s[4][LPR];
+    constexpr int LPR = HD / 8, RPL = 64 / LPR, UNROLL = JOIN_UNROLL;  // lanes per record, records per load
+    typedef float f32x8 __attribute__((ext_vector_type(8)));
+    __shared__ f32x8 sum_s[4][LPR];
     const int tok = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int head = blockIdx.y * (4 / WAVES) + wv / WAVES, part = wv % WAVES;
     if (tok >= min(*a.n_toks, a.rows)) return;
@@ -528,32 +564,35 @@ __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
     };
     const int sub = lane / LPR, li = lane % LPR;
     float M = -INFINITY, L = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    f32x8 acc = {};
     for (int j0 = 0; j0 < n; j0 += 64) {
         const int cnt = min(64, n - j0);
-        f32x4 v[UNROLL];
+        f16x8 v[UNROLL];
         auto fetch = [&](int b) {
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 const int j = (b + u * WAVES) * RPL + sub;             // (records past the last read the last again, weight 0)
-                v[u] = *(const f32x4 *)(a.po + rec_of(j0 + min(j, cnt - 1)) * HD + li * 4);
+                v[u] = *(const f16x8 *)(a.po + rec_of(j0 + min(j, cnt - 1)) * HD + li * 8);
             }
         };
         fetch(part);
-        const float2 x = lane < cnt ? a.ml[rec_of(j0 + lane)] : make_float2(-INFINITY, 0.f);
+        const f32x4 x = lane < cnt ? a.ml[rec_of(j0 + lane)] : (f32x4){-INFINITY, 0.f, 0.f, 0.f};
         const float top = fmaxf(M, wave_max_dpp(x.x));
         const float base = top == -INFINITY ? 0.f : top;
         const float keep = __builtin_amdgcn_exp2f(M - base), f = __builtin_amdgcn_exp2f(x.x - base);
         L = L * keep + wave_sum_dpp(x.y * f);
         acc *= keep;
         M = top;
+        const float share = lane < cnt ? x.z * f : 0.f;
         for (int b = part; b * RPL < cnt; b += UNROLL * WAVES) {
             if (b != part) fetch(b);
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 const int j = (b + u * WAVES) * RPL + sub;
-                const float fj = __shfl(f, min(j, 63));
-                acc += v[u] * (j < cnt ? fj : 0.f);
+                const float fj = __shfl(share, min(j, 63));
+                const float w = j < cnt ? fj : 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) acc[c] += (float)v[u][c] * w;
             }
         }
     }
@@ -561,7 +600,7 @@ __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
 #pragma unroll
     for (int o = LPR; o < 64; o <<= 1)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[c] += __shfl_xor(acc[c], o);
+        for (int c = 0; c < 8; ++c) acc[c] += __shfl_xor(acc[c], o);
     if constexpr (WAVES > 1) {
         if (sub == 0) sum_s[wv][li] = acc;
         __syncthreads();
@@ -572,8 +611,9 @@ __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
     if (!live || sub != 0) return;
     const float il = L > 0.f ? 1.f / L : 0.f;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    *(T4 *)((T *)a.out + (int64_t)tok * a.out_row + (int64_t)head * a.out_head + li * 4) =
-        (T4){(T)(acc[0] * il), (T)(acc[1] * il), (T)(acc[2] * il), (T)(acc[3] * il)};
+    T *o = (T *)a.out + (int64_t)tok * a.out_row + (int64_t)head * a.out_head + li * 8;
+    *(T4 *)o = (T4){(T)(acc[0] * il), (T)(acc[1] * il), (T)(acc[2] * il), (T)(acc[3] * il)};
+    *(T4 *)(o + 4) = (T4){(T)(acc[4] * il), (T)(acc[5] * il), (T)(acc[6] * il), (T)(acc[7] * il)};
     if (a.lse && lane == 0) a.lse[(int64_t)tok * a.NH + head] = L > 0.f ? LN2 * (M + log2f(L)) : -INFINITY;
 }
 
