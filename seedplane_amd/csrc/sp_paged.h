@@ -40,16 +40,19 @@ struct AttnArgs {
     float scale;                      // of the scores, times log2(e)
     const Item *items;
     const int *n_items;               // NULL: one block per item
-    // Records: [rows][HD] unnormalised outputs as fp16 shares of the row's largest (half the traffic of fp32; off by 2^-12 of
-    // that largest at most, whatever its size, where the outputs themselves are rounded by 2^-9 or 2^-12 of each), and [rows]
-    // (m in log2 units, l, the largest)
-    f16 *po;
+    // Records: [rows][HD] unnormalised outputs, and [rows] (m in log2 units, l, a factor of the outputs).  For bf16 outputs, which
+    // round by 2^-9 of themselves, they are fp16 shares of the row's largest finite one (half the traffic; off by 2^-12 of the
+    // largest at most); for fp16 outputs fp32, since 11 bits twice would be seen (3.3e-4 from the 64-bit result, 2.4e-4 so)
+    void *po;
     f32x4 *ml;
 };
 
 template <class T> struct Mma;
 template <> struct Mma<f16> {
     typedef f16x8 frag;
+    typedef float share;
+    static constexpr uint32_t INF = 0x7c00;                            // bits of infinity
+    static constexpr float LAZY = 0.f;
     static __device__ __forceinline__ f32x16 run(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ uint32_t pair(uint32_t codes, bool hi) {          // two e4m3 codes of a dword's half
         return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, true))
@@ -58,6 +61,9 @@ template <> struct Mma<f16> {
 };
 template <> struct Mma<bf16> {
     typedef bf16x8 frag;
+    typedef f16 share;
+    static constexpr uint32_t INF = 0x7f80;
+    static constexpr float LAZY = 8.f;
     static __device__ __forceinline__ f32x16 run(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ uint32_t pair(uint32_t codes, bool hi) {
         return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true))
@@ -99,12 +105,12 @@ __device__ __forceinline__ float half_sum(float v) {
 
 // LDS of a block: tiles (64 KiB), which the join over key waves reuses, the pool rows of the next TABLE_KEYS positions, the
 // key waves' (m, l).  Two blocks share a CU (8 waves: one block's loads and exponentials beside the other's matrix products).
-constexpr float LAZY = 8.f;
 constexpr int TABLE_KEYS = 2048;
 constexpr int TILE_SMEM = 65536;
 struct AttnShared {                                                    // beside the tiles
     uint32_t rows[TABLE_KEYS];                                         // pool row of each position (0 where there is none)
     uint32_t seen[TABLE_KEYS / 32];                                    // which positions exist
+    int nonfinite;                                                     // values cleared at the border
     float2 ml[4][32];
     float top[4][32];
 };
@@ -153,6 +159,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     const int *table = a.table + (int64_t)w.seq * a.max_pages;
     auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size; };
     auto entry_of = [&](int key, int page) { return key < w.k1 && w.seq < a.n_seq && page < a.max_pages ? table[page] : -1; };
+    if (threadIdx.x == 0) sh.nonfinite = 0;
     const int key0 = w.k0 + (int)threadIdx.x, page0 = page_of(key0), entry0 = entry_of(key0, page0);
 
     const int row = rw * 32 + col;
@@ -205,14 +212,33 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     };
     // which of 32 positions exist (block b of the row table)
     auto seen_of = [&](int b) -> uint32_t { return __builtin_amdgcn_readfirstlane(sh.seen[b]); };
-    // values without a position are row 0 of the pool: zeros instead, so that a weight of 0 stays 0 (each wave its own copies)
-    auto clear_values = [&](unsigned char *vb, int t, uint32_t all) {
-        if (all == ~0u || (TL::ALL < WM && rw >= TL::ALL)) return;
+    // Values that a weight of 0 may meet must be finite (each wave its own copies): those without a position, which are row 0 of
+    // the pool, become zeros; so do infinities and NaNs of the border's tiles, which hold keys that some rows see and some
+    // do not, and the rows that see them get them at the end.
+    const int border = w.ntok > 1 ? w.k0 + max(min(w.k1, w.pos0 + 1) - w.k0, 0) / KT * KT : w.k1;
+    auto clear_values = [&](unsigned char *vb, int t, int t0, uint32_t all) {
+        if ((all == ~0u && t0 < border) || (TL::ALL < WM && rw >= TL::ALL)) return;
         const int ln = opaque(lane);
 #pragma unroll 1
         for (int c = 0; c < TL::COPIES; ++c) {
             const int n = rw * TL::COPIES + c, kr = n * RPC + ln / NCH;
-            if (!((sh.seen[t * SUB + kr / 32] >> (kr & 31)) & 1)) *(u32x4 *)(vb + n * 1024 + ln * 16) = (u32x4){0, 0, 0, 0};
+            u32x4 *const at = (u32x4 *)(vb + n * 1024 + ln * 16);
+            u32x4 v = {0, 0, 0, 0};
+            if ((sh.seen[t * SUB + kr / 32] >> (kr & 31)) & 1) {
+                if (t0 < border) continue;
+                v = *at;
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t big = KV8 ? ((v[i] & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u
+                                             : ((v[i] & 0x7fff7fffu) + (0x8000u - M::INF) * 0x10001u) >> 15 & 0x00010001u;
+                    v[i] &= ~(big * (KV8 ? 0xffu : 0xffffu));
+                    any |= big != 0;
+                }
+                if (!any) continue;
+                sh.nonfinite = 1;
+            }
+            *at = v;
         }
         lds_wait();
     };
@@ -276,9 +302,10 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
 #pragma unroll
             for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[u][j]);
         mx = fmaxf(m, half_max(mx) * sc);
-        // weights are taken from the base m, which follows the maximum only when that has grown by more than 2^8: up to there
-        // they fit every type, and the outputs need no rescaling.  (A row that has seen nothing stays empty.)
-        if (__any(mx > m + LAZY)) {
+        // weights are taken from the base m.  With bf16 weights it follows the maximum only when that has grown by more than
+        // 2^8, and the outputs need no rescaling up to there; with fp16 weights it is the maximum, whose weight is then
+        // exactly 1 (outputs 2.4e-4 from the 64-bit result, 3.3e-4 by the other rule).  (A row that has seen nothing stays empty.)
+        if (__any(mx > m + M::LAZY)) {
             const float keep = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mx);
             l *= keep;
 #pragma unroll
@@ -374,7 +401,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 const float base = maxima(s, c0 + t * KT, seen);
                 if (more) copies_wait<TL::COPIES>();
                 else copies_wait<0>();
-                clear_values(vb, t, seen[0] & seen[SUB - 1]);
+                clear_values(vb, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
                 tile_outputs(vb, s, base);
                 lds_wait();
                 if (more) copy_tile(a.v, t + WK, lds0 + TL::TILE);
@@ -402,7 +429,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                     for (int u = 0; u < SUB; ++u) seen_next[u] = seen_of((t + WK) * SUB + u);
                 }
                 copies_wait<0>();
-                clear_values(vb, t, seen[0] & seen[SUB - 1]);
+                clear_values(vb, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
                 lds_barrier();
                 // the next tile's copies are issued behind matrix products: a CU takes one in 16 cycles, and four waves that
                 // issue theirs together wait for each other
@@ -434,6 +461,8 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         }
     }
     l = half_sum(l);
+    if (w.ntok > 1) lds_barrier();
+    const bool nonfinite = w.ntok > 1 && __builtin_amdgcn_readfirstlane(sh.nonfinite);
 
     // The key waves of a row group joined in LDS: each takes a share of the values (4-value pieces q0 ..) of all of them
     constexpr int SHARE = TL::QUADS / WK;
@@ -473,13 +502,35 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         for (int i = 0; i < SHARE; ++i)
             out[i] = (f32x4){o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
     }
-    // the row's largest value: over the lane's values, its other half, the key waves' shares
-    float top = 0.f;
-    if (w.rec >= 0) {
+    if (nonfinite) {
+#pragma unroll 1
+        for (int key = border; key < w.k1; ++key) {
+            const int page = page_of(key), e = entry_of(key, page);
+            if (e < 0 || e >= a.n_pages || key >= lim) continue;
+            const uint8_t *v = a.v + (uint64_t)((uint32_t)e * a.page_rows + (uint32_t)w.kvh * a.head_rows + (uint32_t)(key - page * a.page_size) * a.slot_rows) * RB +
+                               (4 * h + 8 * q0) * (KV8 ? 1 : 2);
+#pragma unroll
+            for (int i = 0; i < SHARE; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if constexpr (KV8) {
+                        if ((v[8 * i + c] & 0x7f) == 0x7f) out[i][c] = NAN;
+                    } else {
+                        const float x = (float)((const T *)v)[8 * i + c];
+                        if (!(fabsf(x) < INFINITY)) out[i][c] += x;
+                    }
+                }
+        }
+    }
+    // the row's largest finite value: over the lane's values, its other half, the key waves' shares.  (No less than 2^-126, whose
+    // reciprocal is finite.)
+    constexpr bool SHARES = sizeof(typename M::share) == 2;
+    float top = SHARES ? 0x1p-126f : 1.f;
+    if (SHARES && w.rec >= 0) {
 #pragma unroll
         for (int i = 0; i < SHARE; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) top = fmaxf(top, fabsf(out[i][c]));
+            for (int c = 0; c < 4; ++c) top = fabsf(out[i][c]) < INFINITY ? fmaxf(top, fabsf(out[i][c])) : top;
         top = half_max(top);
         if constexpr (WK > 1) {
             if (h == 0) sh.top[wv][col] = top;
@@ -505,13 +556,13 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 a.lse[(int64_t)(w.tok0 + tok2) * a.NH + head] = l > 0.f ? LN2 * (m + log2f(l)) : -INFINITY;
         } else {
             const int64_t rec = w.rec + row2;
-            const float share = top > 0.f ? 1.f / top : 0.f;
-            f16 *d0 = a.po + rec * HD + 4 * h + 8 * q0;
+            const float share = SHARES ? 1.f / top : 1.f;
+            typedef typename M::share S;
+            typedef S S4 __attribute__((ext_vector_type(4)));
+            S *d0 = (S *)a.po + rec * HD + 4 * h + 8 * q0;
 #pragma unroll
-            for (int i = 0; i < SHARE; ++i) {
-                typedef f16 f16x4 __attribute__((ext_vector_type(4)));
-                *(f16x4 *)(d0 + 8 * i) = (f16x4){(f16)(out[i][0] * share), (f16)(out[i][1] * share), (f16)(out[i][2] * share), (f16)(out[i][3] * share)};
-            }
+            for (int i = 0; i < SHARE; ++i)
+                *(S4 *)(d0 + 8 * i) = (S4){(S)(out[i][0] * share), (S)(out[i][1] * share), (S)(out[i][2] * share), (S)(out[i][3] * share)};
             if (h == 0 && kw == 0) a.ml[rec] = (f32x4){m, l, top * vs, 0.f};
         }
     }
@@ -537,7 +588,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(AttnArgs a) {
 struct JoinArgs {
     const TokenRecs *toks;
     const int *n_toks;
-    const f16 *po;
+    const void *po;
     const f32x4 *ml;
     void *out;
     float *lse;
@@ -550,6 +601,8 @@ template <class T, int HD, int WAVES>
 __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
     constexpr int LPR = HD / 8, RPL = 64 / LPR, UNROLL = JOIN_UNROLL;  // lanes per record, records per load
     typedef float f32x8 __attribute__((ext_vector_type(8)));
+    typedef typename Mma<T>::share S;
+    typedef S S8 __attribute__((ext_vector_type(8)));
     __shared__ f32x8 sum_s[4][LPR];
     const int tok = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int head = blockIdx.y * (4 / WAVES) + wv / WAVES, part = wv % WAVES;
@@ -567,12 +620,12 @@ __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
     f32x8 acc = {};
     for (int j0 = 0; j0 < n; j0 += 64) {
         const int cnt = min(64, n - j0);
-        f16x8 v[UNROLL];
+        S8 v[UNROLL];
         auto fetch = [&](int b) {
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
-                const int j = (b + u * WAVES) * RPL + sub;             // (records past the last read the last again, weight 0)
-                v[u] = *(const f16x8 *)(a.po + rec_of(j0 + min(j, cnt - 1)) * HD + li * 8);
+                const int j = (b + u * WAVES) * RPL + sub;             // (past the last record: the last again, unused)
+                v[u] = *(const S8 *)((const S *)a.po + rec_of(j0 + min(j, cnt - 1)) * HD + li * 8);
             }
         };
         fetch(part);
@@ -590,9 +643,9 @@ __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
             for (int u = 0; u < UNROLL; ++u) {
                 const int j = (b + u * WAVES) * RPL + sub;
                 const float fj = __shfl(share, min(j, 63));
-                const float w = j < cnt ? fj : 0.f;
+                const S8 x = j < cnt ? v[u] : (S8){};
 #pragma unroll
-                for (int c = 0; c < 8; ++c) acc[c] += (float)v[u][c] * w;
+                for (int c = 0; c < 8; ++c) acc[c] += (float)x[c] * fj;
             }
         }
     }

@@ -416,7 +416,7 @@ int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, in
 
 size_t sp_attn_plan_workspace(const sp_attn_plan *p) {
     if (!p) return 0;
-    return (size_t)records_bound(p->max_rows, p->NH) * ((size_t)p->HD * sizeof(f16) + sizeof(f32x4));
+    return (size_t)records_bound(p->max_rows, p->NH) * ((size_t)p->HD * sizeof(float) + sizeof(f32x4));
 }
 
 int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t dtype, int32_t n_rows, const void *q_dev, int64_t q_row,
@@ -471,8 +471,8 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         a.page_shift = (kv->page_size & (kv->page_size - 1)) == 0 ? __builtin_ctz(kv->page_size) : -1;
         a.scale = scale * LOG2E;
         const size_t recs = (size_t)records_bound(p->max_rows, p->NH);
-        a.po = (f16 *)workspace_dev;
-        a.ml = (f32x4 *)(a.po + recs * p->HD);
+        a.ml = (f32x4 *)workspace_dev;
+        a.po = a.ml + recs;
         const bool kv8 = kv->dtype == SP_DT_E4M3;
         a.items = (const Item *)(p->dev + p->item_at);
         a.n_items = capturing ? p->dev : nullptr;

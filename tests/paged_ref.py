@@ -36,8 +36,8 @@ def attend64(q, k, v, table, q_lens, kv_lens, scale, k_scale=None, v_scale=None)
     bound, per output value, of a kernel with 32-bit sums whose weights are rounded to q's type before their product with
     V: scores carry (hd + 4) roundings of their absolute sum and the exponent's argument and exp2 a few of their own, so a
     weight is off by e^d - 1 <= 2 d of itself (the weights' sum likewise); rounding a weight costs half a step, or the
-    type's smallest half step where it is subnormal; the sum over n keys n 2^-24; the output half a step.  Where a row's keys
-    are read in parts, a part's outputs are kept as fp16 shares of its largest: a share of at most 1 is off by 2^-12, its
+    type's smallest half step where it is subnormal; the sum over n keys n 2^-24; the output half a step.  Where a bf16 row's
+    keys are read in parts, a part's outputs are kept as fp16 shares of its largest: a share of at most 1 is off by 2^-12, its
     scaling there and back by a few 2^-24, and the parts' largest, joined by their weights, are at most the row's largest sum of
     weighted magnitudes."""
     n_pages, nkv, page, hd = k.shape
@@ -72,7 +72,8 @@ def attend64(q, k, v, table, q_lens, kv_lens, scale, k_scale=None, v_scale=None)
                 # a weight relative to the largest of its part (1); the sum of a part's weights is at least 1
                 small = see * TINY[q.dtype] * vv.abs().amax(0)
                 bound[r0 + i] = A * (4 * d[:, None] + half + see * 2.0 ** -24 + 2.0 ** -22) + small + \
-                    (out[r0 + i].abs() + A * half) * half + TINY[q.dtype] + A.amax(-1, keepdim=True) * (2.0 ** -12 + 2.0 ** -20)
+                    (out[r0 + i].abs() + A * half) * half + TINY[q.dtype] + \
+                    (A.amax(-1, keepdim=True) * (2.0 ** -12 + 2.0 ** -20) if q.dtype == torch.bfloat16 else 0)
         r0 += nq
     return out, lse, bound
 

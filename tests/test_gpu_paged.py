@@ -321,6 +321,56 @@ def test_peaked_and_extreme_scores(gpu_device):
     _within(plan.run(q, kv, table), *attend64(q, k, v, table, [1, 30], [700, 730], 0.125)[::2])
 
 
+@pytest.mark.parametrize('dtype,cache', TYPES)
+@pytest.mark.parametrize('q_lens,kv_lens,groups,nh,nkv,hd', [
+    ([1, 3, 5], [40, 300, 2900], None, 12, 2, 128),
+    ([40, 9], [140, 4109], None, 8, 2, 64),
+    ([130, 20], [130, 700], None, 28, 4, 128),
+    ([6, 6], [518, 530], [(2, 512)], 14, 2, 64),
+])
+def test_infinities_and_nans_reach_only_the_rows_and_columns_that_see_them(gpu_device, dtype, cache, q_lens, kv_lens, groups, nh, nkv, hd):
+    """A later token's values may be anything: earlier rows do not see them, other columns do not meet them."""
+    g = torch.Generator().manual_seed(9)
+    q, k, v, table, scales = paged_batch(g, q_lens, kv_lens, groups, nh, nkv, hd, 16, dtype, cache, gpu_device)
+    scale = hd ** -0.5
+    want, _, bound = attend64(q, k, v, table, q_lens, kv_lens, scale, *scales)
+    plan = AttentionPlan(nh, nkv, hd, sum(q_lens), len(q_lens)).set(q_lens, kv_lens, groups)
+    inf = math.inf if cache != E4M3 else math.nan
+    r0 = 0
+    for s, (nq, n) in enumerate(zip(q_lens, kv_lens)):
+        back, last = max(0, nq // 2), r0 + nq - 1                # the token seen from row last - back on, and the newest
+        mid, end = n - 1 - back, n - 1
+        page, slot = int(table[s, mid // 16]), mid % 16
+        v[page, :, slot, 3] = inf
+        v[page, :, slot, 7] = math.nan
+        v[page, :, slot, 9] = inf
+        want[last - back:last + 1, :, 3] = inf
+        want[last - back:last + 1, :, 7] = math.nan
+        want[last - back:last + 1, :, 9] = inf
+        if back:
+            v[int(table[s, end // 16]), :, end % 16, 9] = -inf
+            want[last, :, 9] = math.nan
+            v[int(table[s, end // 16]), :, end % 16, hd - 1] = -inf
+            want[last, :, hd - 1] = -inf
+        r0 += nq
+    out = plan.run(q, PagedKV(k, v, *scales), table).double().cpu()
+    assert torch.equal(out.isnan(), want.isnan())
+    whole = want.isfinite()
+    assert torch.equal(out[~whole & ~want.isnan()], want[~whole & ~want.isnan()])
+    assert ((out - want).abs() <= bound)[whole].all()
+
+
+def test_values_near_the_least_and_the_greatest(gpu_device):
+    """Contexts read in parts whose values are all subnormal, all zero, or large."""
+    g = torch.Generator().manual_seed(11)
+    q, k, v, table, _ = paged_batch(g, [1, 1, 1], [9000, 9000, 9000], None, 4, 2, 64, 16, BF16, BF16, gpu_device)
+    for s, size in enumerate((2.0 ** -128, 0.0, 2.0 ** 90)):
+        pages = table[s, :-(-9000 // 16)].long()
+        v[pages] = (v[pages].float() * size).to(BF16)
+    plan = AttentionPlan(4, 2, 64, 3, 3).set([1] * 3, [9000] * 3)
+    _within(plan.run(q, PagedKV(k, v), table), *attend64(q, k, v, table, [1] * 3, [9000] * 3, 0.125)[::2])
+
+
 def test_offsets_past_32_bits(gpu_device):
     """Pages whose elements lie beyond 2^32 of the pool's start: append and attention."""
     free, _ = torch.cuda.mem_get_info(gpu_device)
