@@ -407,10 +407,10 @@ int sp_op_rotate(const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t
                  int64_t x_row, int64_t x_head, void *out_dev, int64_t out_row, int64_t out_head, const int32_t *pos_dev,
                  void *hip_stream);
 
-/* One layer's paged cache: row r of head h of page e starts at e * page_stride + h * head_stride + r * row_stride elements, the same
- * for keys and values ([pages][heads][rows], [pages][rows][heads], one allocation for both, ...: distinct rows must not
- * overlap).  A sequence's position p lies in row p % page_size of page table[seq][p / page_size].  e4m3 caches hold value / scale
- * with a positive fp32 scale per K/V head, for keys and for values. */
+/* One layer's paged cache: row r of head h of page e starts at e * page_stride + h * head_stride + r * row_stride elements, the
+ * same for keys and values ([pages][heads][rows], [pages][rows][heads], one allocation for both, ...; rows that tables name
+ * must not lie on top of each other).  A sequence's position p lies in row p % page_size of page table[seq][p / page_size].
+ * e4m3 caches hold value / scale with a positive fp32 scale per K/V head, for keys and for values. */
 typedef struct sp_paged_kv {
     void *k_dev, *v_dev;
     const float *k_scale_dev, *v_scale_dev;   /* device [n_kv_heads], SP_DT_E4M3 only (NULL otherwise) */
@@ -422,9 +422,11 @@ typedef struct sp_paged_kv {
 
 /* Appends n_rows new tokens: row r's keys (rotated at pos_dev[r] unless rotary is NULL) and values go to position at_dev[r] of
  * sequence seq_dev[r], and with q_dev its n_heads query heads are rotated into q_out_dev (dtype q_out_dtype; q_dev itself
- * with the same type and strides, or memory apart from the inputs).  table_dev is int32 [n_seq][max_pages].  A row whose seq, position or page entry is out of range (e.g. seq -1:
- * padding) writes nothing, not its queries either.  dtype: of q, k and v (F32, F16 or BF16).  Values too large for an e4m3
- * cache saturate at 448 scales, NaN stays NaN.  Two rows of one call must not name the same position of a sequence. */
+ * with the same type and strides, or memory apart from the inputs; nothing of the cache's range of memory).  table_dev is int32
+ * [n_seq][max_pages].  A row whose seq, position or page entry is out of range (e.g. seq -1: padding) writes nothing, not its
+ * queries either.  dtype: of q, k and v (F32, F16 or BF16).  Values too large for an e4m3 cache saturate at 448 scales, NaN
+ * stays NaN.  Two rows of one call must not name the same place (nor two positions share a page that the call writes): whose
+ * values it then holds is not defined. */
 int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t n_heads,
                        const void *q_dev, int64_t q_row, int64_t q_head, const void *k_dev, int64_t k_row, int64_t k_head,
                        const void *v_dev, int64_t v_row, int64_t v_head, const int32_t *pos_dev, const int32_t *seq_dev,
@@ -463,7 +465,8 @@ size_t sp_attn_plan_workspace(const sp_attn_plan *plan);
  * and heads; rows behind the plan's last are left as they are.  lse_dev (may be NULL): fp32 [n_rows][n_heads], the natural
  * logarithm of each row's sum of exponentials (-infinity for a row that sees nothing).  table_dev: int32 [n_seq][max_pages];
  * entries of positions at or behind a sequence's length are not read, an entry outside [0, n_pages) hides its positions.  What
- * the pool holds outside the positions read does not matter (NaN included).  scale must be positive.  workspace_dev: see
+ * the pool holds outside the positions read does not matter (NaN included), and an infinite or NaN value of a position reaches
+ * only the rows that see it and its own place in them.  Weighted sums of values are held in fp32.  scale must be positive.  workspace_dev: see
  * above; calls that overlap (other streams, graphs replayed side by side) need a workspace each.  The cache's strides are
  * multiples of head_dim here.  A captured call keeps its own n_rows, n_seq and max_pages: what a later set has beyond them is not
  * read or written. */

@@ -92,6 +92,14 @@ bool may_overlap(const Span &out, const void *p, int dt, int64_t rows, int64_t h
     const intptr_t hi = (intptr_t)p + (std::max<int64_t>(r, 0) + std::max<int64_t>(h, 0) + hd) * b;
     return lo < (intptr_t)out.hi && (intptr_t)out.lo < hi;
 }
+// A cache's keys or values, from the first byte to the last.
+Span pool_of(const sp_paged_kv *kv, const void *p) {
+    Span s;
+    s.lo = (uintptr_t)p;
+    s.hi = s.lo + (uintptr_t)((kv->n_pages - 1) * kv->page_stride + (kv->n_kv_heads - 1) * kv->head_stride +
+                              (kv->page_size - 1) * kv->row_stride + kv->head_dim) * bytes_of(kv->dtype);
+    return s;
+}
 void check_output(const Span &out) { require(!out.folded, SP_EINVAL, "the output's rows or heads lie on top of each other"); }
 
 // Rows of a block and its threads: about 256 threads a block, whole rows.
@@ -116,6 +124,11 @@ void check_cache(const sp_paged_kv *kv) {
     require((kv->n_pages == 1 || kv->page_stride >= kv->head_dim) && (kv->n_kv_heads == 1 || kv->head_stride >= kv->head_dim) &&
                 (kv->page_size == 1 || kv->row_stride >= kv->head_dim) && kv->page_stride >= 0 && kv->head_stride >= 0 && kv->row_stride >= 0,
             SP_EINVAL, "the cache's strides are smaller than a row");
+    int64_t reach = kv->head_dim, more = 0;
+    const int64_t dims[3][2] = {{kv->n_pages, kv->page_stride}, {kv->n_kv_heads, kv->head_stride}, {kv->page_size, kv->row_stride}};
+    for (const auto &d : dims)
+        require(!__builtin_mul_overflow(d[0] - 1, d[1], &more) && more < ((int64_t)1 << 60) && (reach += more) < ((int64_t)1 << 60),
+                SP_EINVAL, "the cache is too large");
     require((kv->dtype == SP_DT_E4M3) == (kv->k_scale_dev != nullptr) && (kv->dtype == SP_DT_E4M3) == (kv->v_scale_dev != nullptr),
             SP_EINVAL, "an e4m3 cache has k_scale_dev and v_scale_dev, others have none");
 }
@@ -283,6 +296,15 @@ int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t d
         const Rotation rot = rotation_of(rotary, hd);
         if (n_rows == 0) return;
         require(k_dev && v_dev && seq_dev && at_dev && table_dev && (!rotary || pos_dev), SP_EINVAL, "NULL pointer");
+        require(kv->k_dev != kv->v_dev, SP_EINVAL, "keys and values need memory of their own");
+        for (const void *p : {kv->k_dev, kv->v_dev}) {
+            const Span pool = pool_of(kv, p);
+            require(!may_overlap(pool, k_dev, dtype, n_rows, kv->n_kv_heads, hd, k_row, k_head) &&
+                        !may_overlap(pool, v_dev, dtype, n_rows, kv->n_kv_heads, hd, v_row, v_head) &&
+                        (!q_dev || (!may_overlap(pool, q_dev, dtype, n_rows, nq, hd, q_row, q_head) &&
+                                    !may_overlap(pool, q_out_dev, q_out_dtype, n_rows, nq, hd, q_out_row, q_out_head))),
+                    SP_EINVAL, "the queries, keys or values overlap the cache");
+        }
         if (q_dev) {
             const bool in_place = q_dev == q_out_dev && q_out_dtype == dtype && q_row == q_out_row && q_head == q_out_head;
             const Span to = span_of(q_out_dev, q_out_dtype, n_rows, nq, hd, q_out_row, q_out_head);
@@ -444,20 +466,21 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         int dev = 0;
         HIPCHK(hipGetDevice(&dev));
         require(dev == p->device, SP_EINVAL, "the plan belongs to another device than the current one");
-        if (p->n_tok == 0) return;
+        const hipStream_t st = (hipStream_t)stream;
+        const bool capturing = is_capturing(st);
+        if (capturing ? n_rows == 0 : p->n_tok == 0) return;           // (a captured call serves later sets too)
         require(q_dev && out_dev && table_dev && workspace_dev, SP_EINVAL, "NULL pointer");
         require(aligned(q_dev, 16) && q_row % 8 == 0 && q_head % 8 == 0, SP_EINVAL, "queries must be aligned to 16 bytes");
         {
             const Span to = span_of(out_dev, dtype, n_rows, p->NH, p->HD, out_row, out_head);
             check_output(to);
             require(!may_overlap(to, q_dev, dtype, n_rows, p->NH, p->HD, q_row, q_head), SP_EINVAL, "the output overlaps the queries");
+            require(!overlap(to, pool_of(kv, kv->k_dev)) && !overlap(to, pool_of(kv, kv->v_dev)), SP_EINVAL, "the output overlaps the cache");
         }
         require(aligned(out_dev, 8) && out_row % 4 == 0 && out_head % 4 == 0, SP_EINVAL, "outputs must be aligned to 8 bytes");
         require(aligned(kv->k_dev, 16) && aligned(kv->v_dev, 16) && kv->head_dim * bytes_of(kv->dtype) % 16 == 0,
                 SP_EINVAL, "the cache's pages must be aligned to 16 bytes");
         require(aligned(workspace_dev, 16), SP_EINVAL, "the workspace must be aligned to 16 bytes");
-        const hipStream_t st = (hipStream_t)stream;
-        const bool capturing = is_capturing(st);
         AttnArgs a{};
         a.q = q_dev; a.out = out_dev; a.lse = lse_dev;
         a.q_row = q_row; a.q_head = q_head; a.out_row = out_row; a.out_head = out_head;

@@ -126,6 +126,16 @@ def _table(x, device):
     return x.data_ptr()
 
 
+def _lengths(x, name):
+    """Host integers as int32."""
+    a = np.asarray(x)
+    if a.size == 0:
+        a = a.astype(np.int32)
+    if a.dtype.kind not in 'iu' or (a.size and (a.min() < 0 or a.max() >= 1 << 30)):
+        raise ValueError(f'{name} must be integers in [0, 2^30)')
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
 class Rotary:
     """A rotary position table on a device: `layout` 'half' (pairs j, j + rot_dim/2) or 'interleaved' (2j, 2j + 1), over the
     first `rot_dim` values of a head (default: all)."""
@@ -275,14 +285,13 @@ class AttentionPlan:
         """The next batch (host integers): sequence s has q_lens[s] query tokens, the last of its kv_lens[s] cached positions.
         groups: (sequences, shared positions) of each run of sequences whose tables name the same pages for their first positions;
         None: nothing is shared."""
-        q = np.ascontiguousarray(q_lens, dtype=np.int32)
-        kv = np.ascontiguousarray(kv_lens, dtype=np.int32)
+        q, kv = _lengths(q_lens, 'q_lens'), _lengths(kv_lens, 'kv_lens')
         if q.ndim != 1 or q.shape != kv.shape:
             raise ValueError('q_lens and kv_lens must have one entry per sequence')
         size = shared = None
         n = 0
         if groups is not None:
-            g = np.ascontiguousarray(groups, dtype=np.int32).reshape(-1, 2)
+            g = _lengths(groups, 'groups').reshape(-1, 2)
             size, shared, n = np.ascontiguousarray(g[:, 0]), np.ascontiguousarray(g[:, 1]), len(g)
             if n == 0 and len(q):
                 raise ValueError('the groups do not cover the sequences')

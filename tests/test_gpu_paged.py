@@ -472,6 +472,30 @@ def test_captured_step_follows_later_lengths(gpu_device):
         _within(got, want, bound)
 
 
+def test_a_step_captured_before_any_request(gpu_device):
+    """A call captured while the plan holds no queries serves the batches set later."""
+    g = torch.Generator().manual_seed(8)
+    q, k, v, table, _ = paged_batch(g, [1, 2], [700, 90], None, 8, 2, 64, 16, BF16, BF16, gpu_device, rows_behind=1)
+    kv = PagedKV(k, v)
+    plan = AttentionPlan(8, 2, 64, 4, 2).set([0, 0], [0, 0])
+    out = torch.full_like(q, 3.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.run(q, kv, table, out=out)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (out == 3).all()
+    for lens in ([1, 2], [1, 0], [0, 2]):
+        out.fill_(3.0)
+        plan.set(lens, [700, 90])
+        graph.replay()
+        got, n = out.clone(), sum(lens)
+        want, _, bound = attend64(q[:n], k, v, table, lens, [700, 90], 0.125)
+        _within(got[:n], want, bound)
+        assert (got[n:] == 3).all()
+
+
 def test_set_is_refused_in_a_capture(gpu_device):
     from seedplane_amd._lib import SeedPlaneError
     plan = AttentionPlan(2, 1, 64, 4, 4).set([1], [1])

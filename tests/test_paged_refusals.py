@@ -57,6 +57,8 @@ def append(kv=None, r=None, dtype=_lib.SP_DT_F16, rows=4, heads=8, q=8 * P, q_ro
     dict(q_dt=_lib.SP_DT_E4M3), dict(n_seq=0), dict(width=0), dict(r=rotary(rot=128)),
     dict(k=None), dict(v=None), dict(seq=None), dict(at=None), dict(table=None), dict(pos=None),
     dict(q_out=8 * P, qo_row=1024, q_dt=_lib.SP_DT_F32),        # in place with another type
+    dict(kv=cache(k=P, v=P)), dict(kv=cache(stride=1 << 62)), dict(kv=cache(row=1 << 57)),
+    dict(k=P + 1024), dict(v=2 * P), dict(q=P), dict(q_out=2 * P + 4096), dict(k=P - 128),
     dict(q_out=9 * P), dict(q_out=10 * P + 64), dict(q_out=8 * P + 64), dict(qo_row=0), dict(qo_head=0),
 ])
 def test_append_refusals(kw):
@@ -94,3 +96,13 @@ def test_struct_layouts_match_c(tmp_path):
     got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     R, K = _lib.RotaryDesc, _lib.PagedKVDesc
     assert got == [ctypes.sizeof(R), R.factor.offset, ctypes.sizeof(K), K.page_stride.offset, K.dtype.offset, K.head_dim.offset]
+
+
+def test_lengths_are_integers_in_range():
+    import numpy as np
+    from seedplane_amd.paged import _lengths
+    assert _lengths([], 'x').tolist() == [] and _lengths([3, 0], 'x').dtype == np.int32
+    assert _lengths(np.array([1 << 20], np.int64), 'x').tolist() == [1 << 20]
+    for bad in ([1.5], [-1], [1 << 30], np.array([(1 << 32) + 5]), ['1'], [True]):
+        with pytest.raises(ValueError):
+            _lengths(bad, 'x')
