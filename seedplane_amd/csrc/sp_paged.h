@@ -257,30 +257,36 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
             va[1][d] = (key + 8) * RB + ((c ^ piece_swap<NCH>(key + 8)) << 4) + ((ti & 1) << 3);
         }
     }
-    auto key_frag = [&](const unsigned char *kb, int p) -> frag {
-        if constexpr (KV8) return from_e4m3<T>(*(const u32x2 *)(kb + ka[p]));
-        else return *(const frag *)(kb + ka[p]);
+    // operands as LDS gives them, and as the products take them: e4m3 is converted when it is used, after the wait for it
+    typedef std::conditional_t<KV8, u32x2, u32x4> raw;
+    auto cooked = [&](raw x) -> frag {
+        if constexpr (KV8) return from_e4m3<T>(x);
+        else return __builtin_bit_cast(frag, x);
     };
-    auto value_frag = [&](const unsigned char *vb, int y, int d) -> frag {         // keys 16 y .. + 15
+    auto value_raw = [&](const unsigned char *vb, int y, int d) -> raw {           // keys 16 y .. + 15
         if constexpr (KV8) {
-            return from_e4m3<T>(__builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                (__attribute__((address_space(3))) i32x2 *)(vb + 16 * y * RB + va[0][d]))));
+            return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (__attribute__((address_space(3))) i32x2 *)(vb + 16 * y * RB + va[0][d])));
         } else {
             const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vb + 16 * y * RB + va[0][d]));
             const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vb + 16 * y * RB + va[1][d]));
             const u32x2 xx = __builtin_bit_cast(u32x2, x), zz = __builtin_bit_cast(u32x2, z);
-            return __builtin_bit_cast(frag, (u32x4){xx.x, xx.y, zz.x, zz.y});
+            return (u32x4){xx.x, xx.y, zz.x, zz.y};
         }
     };
-    auto scores = [&](const unsigned char *kb, f32x16 &s) {
+    auto read_keys = [&](const unsigned char *kb, raw (&k)[NS]) {
+#pragma unroll
+        for (int p = 0; p < NS; ++p) k[p] = *(const raw *)(kb + ka[p]);
+    };
+    auto read_values = [&](const unsigned char *vb, int y, raw (&v)[ND]) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d) v[d] = value_raw(vb, y, d);
+    };
+    auto scores = [&](const raw (&k)[NS], f32x16 &s) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[j] = 0.f;
-        frag kf[NS];
 #pragma unroll
-        for (int p = 0; p < NS; ++p) kf[p] = key_frag(kb, p);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int p = 0; p < NS; ++p) s = M::run(kf[p], qf[p], s);
+        for (int p = 0; p < NS; ++p) s = M::run(cooked(k[p]), qf[p], s);
     };
     // masks a tile's scores, positions from t0, and brings the running maximum up to date; returns the exponent's base
     auto maxima = [&](f32x16 (&s)[SUB], int t0, const uint32_t (&seen)[SUB]) -> float {
@@ -316,47 +322,41 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         }
         return m == -INFINITY ? 0.f : m;
     };
-    auto weights = [&](const f32x16 &s, float base, frag (&pf)[2]) {
+    auto weights = [&](const f32x16 &s, float base, frag (&pf)[2], int j0, int n) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = j0; j < j0 + n; ++j) {
             const float p = __builtin_amdgcn_exp2f(s[j] * sc - base);
             l += p;
             pf[j / 8][j % 8] = (T)p;
         }
     };
-    auto outputs = [&](const unsigned char *vb, const frag (&pf)[2]) {
-        frag vf[2][ND];
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) vf[y][d] = value_frag(vb, y, d);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) o[d] = M::run(vf[y][d], pf[y], o[d]);
-    };
-    // the tile's weights and outputs: the second half's exponentials stand between the first half's matrix products
-    auto tile_outputs = [&](const unsigned char *vb, const f32x16 (&s)[SUB], float base) {
+    // The tile's weights and outputs; v0: the values of its first 16 keys.  Operands are read a group of products ahead, and the
+    // second half's exponentials stand between the first half's products: left to itself the compiler reads each product's
+    // operands right before it and waits for them.
+    auto tile_outputs = [&](const unsigned char *vb, raw (&v0)[ND], const f32x16 (&s)[SUB], float base) {
+        raw v1[ND];
         frag pf[SUB][2];
-        weights(s[0], base, pf[0]);
+        read_values(vb, 1, v1);
+        __builtin_amdgcn_sched_barrier(0);
+        weights(s[0], base, pf[0], 0, 16);
+        __builtin_amdgcn_sched_barrier(0);
         if constexpr (SUB == 2) {
-            __builtin_amdgcn_sched_barrier(0);
+            constexpr int PER = 16 / (2 * ND);
 #pragma unroll
             for (int y = 0; y < 2; ++y)
 #pragma unroll
-                for (int d = 0; d < ND; ++d) o[d] = M::run(value_frag(vb, y, d), pf[0][y], o[d]);
-            weights(s[1], base, pf[1]);
-            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);                 // LDS reads ahead
-#pragma unroll
-            for (int i = 0; i < 2 * ND; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // a matrix product
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 64 / (2 * ND), 0); // exponentials, sums, roundings
-            }
-            __builtin_amdgcn_sched_barrier(0);
+                for (int d = 0; d < ND; ++d) {
+                    raw &v = y ? v1[d] : v0[d];
+                    o[d] = M::run(cooked(v), pf[0][y], o[d]);
+                    v = value_raw(vb + 32 * RB, y, d);
+                    weights(s[1], base, pf[1], (y * ND + d) * PER, PER);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
         }
-        outputs(vb + (SUB - 1) * 32 * RB, pf[SUB - 1]);
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[d] = M::run(cooked(y ? v1[d] : v0[d]), pf[SUB - 1][y], o[d]);
     };
 
     for (int c0 = w.k0; c0 < w.k1; c0 += TABLE_KEYS) {
@@ -394,15 +394,20 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 for (int u = 0; u < SUB; ++u) seen[u] = seen_of(t * SUB + u);
                 copies_wait<TL::COPIES>();
                 f32x16 s[SUB];
+                raw k[SUB][NS], v0[ND];
 #pragma unroll
-                for (int u = 0; u < SUB; ++u) scores(kb + u * 32 * RB, s[u]);
+                for (int u = 0; u < SUB; ++u) read_keys(kb + u * 32 * RB, k[u]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) scores(k[u], s[u]);
                 lds_wait();
                 if (more) copy_tile(a.k, t + WK, lds0);
                 const float base = maxima(s, c0 + t * KT, seen);
                 if (more) copies_wait<TL::COPIES>();
                 else copies_wait<0>();
                 clear_values(vb, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
-                tile_outputs(vb, s, base);
+                read_values(vb, 0, v0);
+                tile_outputs(vb, v0, s, base);
                 lds_wait();
                 if (more) copy_tile(a.v, t + WK, lds0 + TL::TILE);
             }
@@ -447,12 +452,17 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                     return;
                 }
                 f32x16 s[SUB];
+                raw k[SUB][NS], v0[ND];
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) read_keys(kb + u * 32 * RB, k[u]);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) {
-                    scores(kb + u * 32 * RB, s[u]);
+                    scores(k[u], s[u]);
                     copies(u);
                 }
-                tile_outputs(vb, s, maxima(s, c0 + t * KT, seen));
+                read_values(vb, 0, v0);
+                tile_outputs(vb, v0, s, maxima(s, c0 + t * KT, seen));
             };
             for (int i = 0; i < rounds; i += 2) {
                 step(i, std::integral_constant<int, 0>{});
