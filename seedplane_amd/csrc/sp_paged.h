@@ -199,16 +199,19 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
 #pragma unroll
         for (int c = 0; c < TL::COPIES; ++c) r[c] = rows[c * RPC];
     };
-    auto copy_row = [&](const uint8_t *pool, const uint32_t *r, uint32_t to, int c) {
+    auto offset_of = [&](uint32_t r, int c) -> uint64_t {                // (keys and values at the same place; rows of 2^n bytes)
+        const uint32_t low = r * RB + ((uint32_t)opaque(piece0) ^ (uint32_t)(piece_swap<NCH>(c * RPC) << 4));
+        return (uint64_t)(r >> (32 - __builtin_ctz(RB))) << 32 | low;
+    };
+    auto copy_row = [&](const uint8_t *pool, uint64_t offset, uint32_t to, int c) {
         if (TL::ALL < WM && rw >= TL::ALL) return;
-        const uint32_t piece = opaque(piece0);
-        copy_to_lds(pool + ((uint64_t)r[c] * RB + (piece ^ (uint32_t)(piece_swap<NCH>(c * RPC) << 4))), to + (rw * TL::COPIES + c) * 1024);
+        copy_to_lds(pool + offset, to + (rw * TL::COPIES + c) * 1024);
     };
     auto copy_tile = [&](const uint8_t *pool, int t, uint32_t to) {
         uint32_t r[TL::COPIES];
         rows_of(t, r);
 #pragma unroll
-        for (int c = 0; c < TL::COPIES; ++c) copy_row(pool, r, to, c);
+        for (int c = 0; c < TL::COPIES; ++c) copy_row(pool, offset_of(r[c], c), to, c);
     };
     // which of 32 positions exist (block b of the row table)
     auto seen_of = [&](int b) -> uint32_t { return __builtin_amdgcn_readfirstlane(sh.seen[b]); };
@@ -442,8 +445,9 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                     if (!more) return;
 #pragma unroll
                     for (int c = part; c < TL::COPIES; c += SUB) {
-                        copy_row(a.k, r, to, c);
-                        copy_row(a.v, r, to + TL::TILE, c);
+                        const uint64_t at = offset_of(r[c], c);
+                        copy_row(a.k, at, to, c);
+                        copy_row(a.v, at, to + TL::TILE, c);
                     }
                 };
                 if (c0 + t * KT >= hi) {
