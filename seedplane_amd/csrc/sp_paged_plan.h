@@ -32,18 +32,19 @@ constexpr int32_t ALL_SEEN = 1 << 30;
 constexpr int KINDS = 3;                                       // row tiles of 32 << kind rows
 constexpr int TILE_ROWS_OF[KINDS] = {32, 64, 128};
 constexpr int KEY_STEP = 64;                                   // parts are whole steps of keys
-// Cost of a step by kind: a tile of many rows is bound by its matrix products, one of few by memory.  With two blocks on every
-// CU a step of head_dim 128 takes 2.6 us (128 rows, 16 bits; e4m3 2.8) against 3.1 us (32 rows, 16 bits) and 1.6 (e4m3); 2 : 3
-// lies between (decode of 32 / 96 requests over 8192 / 16384 shared positions, bf16 / e4m3: 1 : 1 20.0 / 66.8 us, 2 : 3 19.4 / 59.9,
-// 1 : 2 20.6 / 57.1).  And the fewest steps of a part: shorter ones cost more in records and latency than they spread.
-constexpr int STEP_COST[KINDS] = {2, 3, 3};
+// Cost of a step by kind: a tile of many rows is bound by its products and exponentials, one of few by memory, and how much
+// they take of each other depends on the batch.  Decode of 32 / 96 requests over 8192 / 16384 shared positions, bf16 / e4m3, costs of
+// 32 rows : more: 1 : 1 23.0 / 68.0 us, 2 : 3 23.4 / 62, 1 : 2 23.1 / 59.5, 2 : 5 24.5 / 60.4, 1 : 3 24.1 / 62.6.  And the fewest
+// steps of a part: shorter ones cost more in records and latency than they spread (9 drafted tokens of 12 sequences over 1531
+// positions: 16.3 us, with single steps 18.6).
+constexpr int STEP_COST[KINDS] = {1, 2, 2};
 constexpr int LEAST_STEPS[KINDS] = {2, 2, 2};
 constexpr int MAX_GROUP = 32;                                  // query heads per K/V head
 
 // Tiles without shared positions up to this many values a row (positions x head_dim) are not cut: their items write the outputs, and
-// the join's launch is saved (a pass over 256 / 448 / 512 positions, head_dim 128, 1 to 16 sequences: 7.7 / 9.3 / 10.0 us uncut,
-// 9.6 / 9.6 / 9.6 cut and joined; head_dim 64, 512 / 1024: 7.2 / 10.0 against 9.6).
-constexpr int64_t UNCUT_VALUES = 896 * 64;
+// the join's launch is saved (a pass over 1 to 16 sequences of head_dim 128, 256 / 512 / 640 / 768 positions: 7.2 / 9.1 / 10.2 / 11.6 us
+// uncut, 10.7 cut and joined; head_dim 64, 512 / 1024: 7.3 / 9.3 against 10.6).
+constexpr int64_t UNCUT_VALUES = 640 * 128;
 struct Segment {
     int32_t tok0, ntok, seq, k0, k1, pos0, which, kind;        // which: 0 shared, 1 own
 };
@@ -57,7 +58,8 @@ struct PlanTables {
     int32_t max_kv = 0;
 };
 
-// A part has the ITEM_TARGET-th of the whole cost: two blocks on each of 256 CUs get about the same; shorter tiles fill in.
+// A part has the ITEM_TARGET-th of the whole cost: two blocks on each of 256 CUs get about the same; shorter tiles fill in (the
+// two batches above: 512 23.1 / 59.5 us, 576 26.9 / 62.8, 1024 33.4 / 65.4).
 constexpr int ITEM_TARGET = 512;
 // Most rows of records: a tile that is not cut leaves one record per row and range; the parts of those that are, each of more
 // than one part's cost, are fewer than 2 ITEM_TARGET.

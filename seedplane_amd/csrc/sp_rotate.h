@@ -7,7 +7,9 @@
 // The angle is formed and reduced to one turn in 64 bits: at position 1e6 a 32-bit product is off by 0.03 rad.  Its cosine
 // and sine come from sincospif of the reduced turn (32 bits), the rotation runs in 32 bits and rounds once, on the store.
 //
-// Both kernels are bound by memory for long inputs and by the chain position -> angle -> store for short ones.  A block
+// Both kernels are bound by memory for long inputs and by the chain position -> angle -> store for short ones: 2048 rows x 32
+// heads of 128 in bf16 rotate in 8.3 us (33.6 MB, 4.0 TB/s), 2048 rows of 28 + 4 + 4 heads are appended in 11.0 us (37.7 MB, 3.4 TB/s),
+// and steps of 16 rows take 2.7 and 3.9 us, where an empty launch takes 2.3 (a copy of 1 GiB: 5.1 TB/s).  A block
 // takes whole rows: its threads load their values, then form the rows' (cos, sin) table in LDS, each pair once for all heads
 // (a thread per pair and head would spend more on angles than on memory), then rotate and store.
 #pragma once
@@ -166,7 +168,8 @@ __global__ void __launch_bounds__(ROT_THREADS) k_rotate(RotateArgs a) {
     const int total = n * a.per_row;
     float v1[VEC], v2[VEC];
     int at1 = 0, at2 = 0, r = 0, head = 0, u = 0;
-    // (the unrotated rest has one vector: v2 repeats it and is not stored)
+    // (the unrotated rest has one vector: v2 repeats it and is not stored; a load under a condition would put the vectors into
+    // scratch memory: 20.1 us instead of 8.3 for 2048 rows x 32 heads)
     auto fetch = [&](int i) {
         r = i / a.by_row;
         const int k = i - r * a.per_row;
