@@ -17,8 +17,8 @@
 // What bounds it.  Few rows: memory; 64 sequences x 4096 positions, 28 / 4 heads of 128 in bf16, 537 MB: 101 us, 5.3 TB/s, the rate of
 // a large copy (e4m3 50 us).  Many rows: the products and the other vector instructions, which two waves of a SIMD hardly
 // overlap; 128 tiles of 126 rows x 4 heads on the same 4096 positions: 178 us, 760 TFLOP/s, 53 % of a large library product, the matrix
-// cores 48 % and the rest of the vector unit 55 % of the waves' time, either busy 90 %.  (One exponential, scaling, sum
-// and half a rounding per score against a product's 4 HD operations; LDS is used 21 % of the time, without conflicts.  Tried: four tiles
+// cores 49 % and the rest of the vector unit 52 % of the waves' time, either busy 88 %.  (One exponential, scaling, sum
+// and half a rounding per score against a product's 4 HD operations; LDS is used 24 % of the time, without conflicts.  Tried: four tiles
 // deep with 32 keys, sums of rounded weights by dot products, priorities, and blocks of 8 waves whose halves take turns
 // multiplying and weighing: 188 us.)
 #pragma once
