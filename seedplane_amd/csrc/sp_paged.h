@@ -575,7 +575,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 *(T4 *)(d0 + 8 * i) = (T4){(T)(out[i][0] * il), (T)(out[i][1] * il), (T)(out[i][2] * il), (T)(out[i][3] * il)};
             }
             if (a.lse && h == 0 && kw == 0)
-                a.lse[(int64_t)(w.tok0 + tok2) * a.NH + head] = l > 0.f ? LN2 * (m + log2f(l)) : -INFINITY;
+                a.lse[(int64_t)(w.tok0 + tok2) * a.NH + head] = l == 0.f ? -INFINITY : LN2 * (m + log2f(l));
         } else {
             const int64_t rec = w.rec + row2;
             const float share = SHARES ? 1.f / top : 1.f;
@@ -689,7 +689,7 @@ __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
     T *o = (T *)a.out + (int64_t)tok * a.out_row + (int64_t)head * a.out_head + li * 8;
     *(T4 *)o = (T4){(T)(acc[0] * il), (T)(acc[1] * il), (T)(acc[2] * il), (T)(acc[3] * il)};
     *(T4 *)(o + 4) = (T4){(T)(acc[4] * il), (T)(acc[5] * il), (T)(acc[6] * il), (T)(acc[7] * il)};
-    if (a.lse && lane == 0) a.lse[(int64_t)tok * a.NH + head] = L > 0.f ? LN2 * (M + log2f(L)) : -INFINITY;
+    if (a.lse && lane == 0) a.lse[(int64_t)tok * a.NH + head] = L == 0.f ? -INFINITY : LN2 * (M + log2f(L));
 }
 
 }  // namespace paged

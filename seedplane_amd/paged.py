@@ -151,9 +151,15 @@ class Rotary:
         self.lib = _lib.load()
         self.device = _device(device)
         self._inv = self.inv_freq.to(self.device)
+        self._stream = _raw_stream(self.device.index)
         self.desc = _lib.RotaryDesc(self._inv.data_ptr(), self.rot_dim,
                                     _lib.SP_ROPE_HALF if layout == 'half' else _lib.SP_ROPE_INTERLEAVED, self.factor, 0)
         self._ref = ctypes.addressof(self.desc)
+
+    def _used(self):
+        """The table's memory is given back only after the calls on this stream."""
+        if _raw_stream(self.device.index) != self._stream:
+            self._inv.record_stream(torch.cuda.current_stream(self.device))
 
     @classmethod
     def from_config(cls, config, layout='half', length=None, device='cuda'):
@@ -178,6 +184,7 @@ class Rotary:
         _, _, o_row, o_head, o_addr = _heads(out, 'out', self.device, None, self.head_dim)
         _call(self.lib.sp_op_rotate, self.device, self._ref, dt, rows, x.shape[1], self.head_dim, addr, row, head, o_addr, o_row,
               o_head, pos)
+        self._used()
         return out
 
 
@@ -253,6 +260,8 @@ class PagedKV:
         if rows:
             _call(self.lib.sp_op_paged_append, dev, self._ref, None if rotary is None else rotary._ref, dt, rows, nh, *queries,
                   k_addr, k_row, k_head, v_addr, v_row, v_head, turn, s, p, t, table.shape[0], table.shape[1], *turned)
+            if rotary is not None:
+                rotary._used()
         return q_out
 
 

@@ -360,6 +360,43 @@ def test_infinities_and_nans_reach_only_the_rows_and_columns_that_see_them(gpu_d
     assert ((out - want).abs() <= bound)[whole].all()
 
 
+def test_a_nan_key_reaches_the_rows_that_see_it(gpu_device):
+    """Outputs and lse of the rows that see it, in one item and in parts."""
+    g = torch.Generator().manual_seed(10)
+    q_lens, kv_lens = [1, 4, 2], [60, 300, 5000]
+    q, k, v, table, _ = paged_batch(g, q_lens, kv_lens, None, 8, 2, 64, 16, F16, F16, gpu_device)
+    for s, n in enumerate(kv_lens):
+        k[int(table[s, (n - 1) // 16]), :, (n - 1) % 16] = math.nan
+    plan = AttentionPlan(8, 2, 64, 7, 3).set(q_lens, kv_lens)
+    lse = torch.zeros(q.shape[:2], device=gpu_device)
+    out = plan.run(q, PagedKV(k, v), table, lse=lse)
+    seen = torch.tensor([1, 0, 0, 0, 1, 0, 1], dtype=torch.bool)
+    assert torch.equal(out.isnan().all(-1).all(-1).cpu(), seen) and torch.equal(out.isnan().any(-1).any(-1).cpu(), seen)
+    assert torch.equal(lse.isnan().all(-1).cpu(), seen) and torch.equal(lse.isnan().any(-1).cpu(), seen)
+
+
+def test_a_table_dropped_after_its_call_on_another_stream(gpu_device):
+    """Memory of a rotary table that goes out of use while another stream still reads it is not given out again."""
+    x = torch.randn((2048, 32, 128), device=gpu_device)
+    pos = torch.arange(2048, dtype=torch.int32, device=gpu_device)
+    want = Rotary(128, theta=1e6).apply(x, pos)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = x
+        for _ in range(20):
+            y = y * 1.0                                        # work ahead of the call
+    r = Rotary(128, theta=1e6)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = r.apply(y, pos)
+    del r
+    for _ in range(50):
+        torch.full((64,), math.nan, dtype=torch.float64, device=gpu_device)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_values_near_the_least_and_the_greatest(gpu_device):
     """Contexts read in parts whose values are all subnormal, all zero, or large."""
     g = torch.Generator().manual_seed(11)
