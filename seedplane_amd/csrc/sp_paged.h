@@ -149,6 +149,11 @@ template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+template <class V>
+__device__ __forceinline__ __attribute__((address_space(3))) V *lds_at(uint32_t address) {
+    return (__attribute__((address_space(3))) V *)(size_t)address;
+}
+
 template <class T, bool KV8, int HD, int WM>
 __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsigned char *smem, AttnShared &sh) {
     typedef AttnTile<KV8, HD, WM> TL;
@@ -227,13 +232,13 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     // the pool, become zeros; so do infinities and NaNs of the border's tiles, which hold keys that some rows see and some
     // do not, and the rows that see them get them at the end.
     const int border = w.ntok > 1 ? w.k0 + max(min(w.k1, w.pos0 + 1) - w.k0, 0) / KT * KT : w.k1;
-    auto clear_values = [&](unsigned char *vb, int t, int t0, uint32_t all) {
+    auto clear_values = [&](int vb, int t, int t0, uint32_t all) {
         if ((all == ~0u && t0 < border) || (TL::ALL < WM && rw >= TL::ALL)) return;
         const int ln = opaque(lane);
 #pragma unroll 1
         for (int c = 0; c < TL::COPIES; ++c) {
             const int n = rw * TL::COPIES + c, kr = n * RPC + ln / NCH;
-            u32x4 *const at = (u32x4 *)(vb + n * 1024 + ln * 16);
+            u32x4 *const at = (u32x4 *)(buf0 + vb + n * 1024 + ln * 16);
             u32x4 v = {0, 0, 0, 0};
             if ((sh.seen[t * SUB + kr / 32] >> (kr & 31)) & 1) {
                 if (t0 < border) continue;
@@ -253,43 +258,49 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         }
         lds_wait();
     };
-    // 32 keys at a time: scores (kb: their rows), then maxima, weights, outputs (vb: their rows)
-    int ka[NS], va[2][ND];                                             // LDS offsets of the lane's operands
+    // 32 keys at a time: scores (kb: their rows), then maxima, weights, outputs (vb: their rows).  The lane's operands: LDS addresses in
+    // the wave's first tile, kb and vb constants beside them, so that reads need no address of their own
+    uint32_t ka[NS], va[2][ND];
 #pragma unroll
-    for (int p = 0; p < NS; ++p) ka[p] = KV8 ? col * RB + (((swz ^ p) << 4) | (h << 3)) : col * RB + ((h ^ swz ^ (2 * p)) << 4);
+    for (int p = 0; p < NS; ++p) ka[p] = lds0 + (KV8 ? col * RB + (((swz ^ p) << 4) | (h << 3)) : col * RB + ((h ^ swz ^ (2 * p)) << 4));
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
         if constexpr (KV8) {
             const int rr = ti >> 1, key = 8 * (rr >> 2) + 4 * h + (rr & 3);
-            va[0][d] = va[1][d] = key * RB + (((2 * d + tg) ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
+            va[0][d] = va[1][d] = lds0 + key * RB + (((2 * d + tg) ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
         } else {
             const int key = 4 * h + (ti >> 2), c = 4 * d + 2 * tg + ((ti >> 1) & 1);
-            va[0][d] = key * RB + ((c ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
-            va[1][d] = (key + 8) * RB + ((c ^ piece_swap<NCH>(key + 8)) << 4) + ((ti & 1) << 3);
+            va[0][d] = lds0 + key * RB + ((c ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
+            va[1][d] = lds0 + (key + 8) * RB + ((c ^ piece_swap<NCH>(key + 8)) << 4) + ((ti & 1) << 3);
         }
     }
+    // (sums for good: the compiler would add the wave's part again at every read)
+#pragma unroll
+    for (int p = 0; p < NS; ++p) asm volatile("" : "+v"(ka[p]));
+#pragma unroll
+    for (int d = 0; d < ND; ++d) asm volatile("" : "+v"(va[0][d]), "+v"(va[1][d]));
     // operands as LDS gives them, and as the products take them: e4m3 is converted when it is used, after the wait for it
     typedef std::conditional_t<KV8, u32x2, u32x4> raw;
     auto cooked = [&](raw x) -> frag {
         if constexpr (KV8) return from_e4m3<T>(x);
         else return __builtin_bit_cast(frag, x);
     };
-    auto value_raw = [&](const unsigned char *vb, int y, int d) -> raw {           // keys 16 y .. + 15
+    auto value_raw = [&](int vb, int y, int d) -> raw {           // keys 16 y .. + 15
         if constexpr (KV8) {
             return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                (__attribute__((address_space(3))) i32x2 *)(vb + 16 * y * RB + va[0][d])));
+                lds_at<i32x2>(va[0][d] + vb + 16 * y * RB)));
         } else {
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vb + 16 * y * RB + va[0][d]));
-            const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(vb + 16 * y * RB + va[1][d]));
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(va[0][d] + vb + 16 * y * RB));
+            const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(va[1][d] + vb + 16 * y * RB));
             const u32x2 xx = __builtin_bit_cast(u32x2, x), zz = __builtin_bit_cast(u32x2, z);
             return (u32x4){xx.x, xx.y, zz.x, zz.y};
         }
     };
-    auto read_keys = [&](const unsigned char *kb, raw (&k)[NS]) {
+    auto read_keys = [&](int kb, raw (&k)[NS]) {
 #pragma unroll
-        for (int p = 0; p < NS; ++p) k[p] = *(const raw *)(kb + ka[p]);
+        for (int p = 0; p < NS; ++p) k[p] = *lds_at<raw>(ka[p] + kb);
     };
-    auto read_values = [&](const unsigned char *vb, int y, raw (&v)[ND]) {
+    auto read_values = [&](int vb, int y, raw (&v)[ND]) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) v[d] = value_raw(vb, y, d);
     };
@@ -344,7 +355,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     // The tile's weights and outputs; v0: the values of its first 16 keys.  Operands are read a group of products ahead, and the
     // second half's exponentials stand between the first half's products: left to itself the compiler reads each product's
     // operands right before it and waits for them.
-    auto tile_outputs = [&](const unsigned char *vb, raw (&v0)[ND], const f32x16 (&s)[SUB], float base) {
+    auto tile_outputs = [&](int vb, raw (&v0)[ND], const f32x16 (&s)[SUB], float base) {
         raw v1[ND];
         frag pf[SUB][2];
         read_values(vb, 1, v1);
@@ -392,7 +403,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         if constexpr (WM == 1) {
             // a wave of its own: one tile, keys and values copied apart, so that the next keys are on their way while the
             // values are awaited and used
-            unsigned char *const kb = buf0, *const vb = buf0 + TL::TILE;
+            constexpr int kb = 0, vb = TL::TILE;
             const int n = min(nt, (max(hi - c0, 0) + KT - 1) / KT);    // tiles behind the last seen position are skipped
             if (kw < n) {
                 copy_tile(a.k, kw, lds0);
@@ -434,7 +445,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 constexpr int ST = decltype(stage_of)::value * 2 * TL::TILE;
                 const int t = i * WK + kw;
                 const bool more = i + 1 < rounds;
-                unsigned char *const kb = buf0 + ST, *const vb = kb + TL::TILE;
+                constexpr int kb = ST, vb = ST + TL::TILE;
                 const uint32_t to = lds0 + (2 * TL::TILE - ST);
                 uint32_t seen[SUB], r[TL::COPIES];
 #pragma unroll
