@@ -131,10 +131,10 @@ struct AttnTile {
     static constexpr int STAGES = WM == 1 ? 1 : 2;
     static constexpr int TILE = KT * RB;                               // bytes of a tile's keys (and of its values)
     static constexpr int ALL = KT * NCH / 64;                          // copies of a tile's keys, and of its values
-    static constexpr int COPIES = ALL < WM ? 1 : ALL / WM;             // ... of a wave (of the first ALL waves, if fewer)
+    static constexpr int COPIES = ALL / WM;                            // ... of a wave
     static constexpr int QUADS = HD / 8;                               // 4-value pieces of a lane's half of a row
     static constexpr int JOIN = 4 * 32 * HD * 4;                       // LDS of the join over the key waves
-    static_assert(ALL >= 1 && (ALL < WM || ALL % WM == 0), "whole copies");
+    static_assert(ALL >= WM && ALL % WM == 0, "whole copies");
     static_assert(WK * STAGES * 2 * TILE <= TILE_SMEM && JOIN <= TILE_SMEM, "LDS plan");
     static_assert(TABLE_KEYS % (WK * KT) == 0, "whole rounds of the row table");
 };
@@ -217,7 +217,6 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         return (uint64_t)(r >> (32 - __builtin_ctz(RB))) << 32 | low;
     };
     auto copy_row = [&](const uint8_t *pool, uint64_t offset, uint32_t to, int c) {
-        if (TL::ALL < WM && rw >= TL::ALL) return;
         copy_to_lds(pool + offset, to + (rw * TL::COPIES + c) * 1024);
     };
     auto copy_tile = [&](const uint8_t *pool, int t, uint32_t to) {
@@ -233,7 +232,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     // do not, and the rows that see them get them at the end.
     const int border = w.ntok > 1 ? w.k0 + max(min(w.k1, w.pos0 + 1) - w.k0, 0) / KT * KT : w.k1;
     auto clear_values = [&](int vb, int t, int t0, uint32_t all) {
-        if ((all == ~0u && t0 < border) || (TL::ALL < WM && rw >= TL::ALL)) return;
+        if (all == ~0u && t0 < border) return;
         const int ln = opaque(lane);
 #pragma unroll 1
         for (int c = 0; c < TL::COPIES; ++c) {
