@@ -29,6 +29,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.SP_DT_F32, torch.float16: _lib.SP_DT_F16, torch.bfloat16: _lib.SP_DT_BF16,
            torch.float8_e4m3fn: _lib.SP_DT_E4M3}
+_INT32 = torch.int32
 _FLOATS = {t: code for t, code in _DTYPES.items() if t != torch.float8_e4m3fn}
 
 
@@ -115,7 +116,7 @@ def _heads(x, name, device, heads, hd):
 
 def _ints(x, name, device, n):
     """The address of a contiguous int32 GPU tensor of n entries."""
-    if x.dtype != torch.int32 or x.device != device or x.shape != (n,) or (n > 1 and x.stride(0) != 1):
+    if x.dtype is not _INT32 or x.device != device or x.dim() != 1 or x.numel() != n or not x.is_contiguous():
         raise ValueError(f'{name} must be a contiguous int32 tensor on {device} with one entry per row')
     return x.data_ptr()
 
@@ -179,9 +180,12 @@ class Rotary:
         pos = _ints(positions, 'positions', self.device, rows)
         if out is None:
             out = torch.empty_like(x)
+            o_row, o_head, _ = out.stride()
+            o_addr = out.data_ptr()
         elif out.shape != x.shape or out.dtype != x.dtype:
             raise ValueError('out must have the shape and type of x')
-        _, _, o_row, o_head, o_addr = _heads(out, 'out', self.device, None, self.head_dim)
+        else:
+            _, _, o_row, o_head, o_addr = _heads(out, 'out', self.device, None, self.head_dim)
         _call(self.lib.sp_op_rotate, self.device, self._ref, dt, rows, x.shape[1], self.head_dim, addr, row, head, o_addr, o_row,
               o_head, pos)
         self._used()
@@ -319,9 +323,12 @@ class AttentionPlan:
         t = _table(table, dev)
         if out is None:
             out = torch.empty_like(q) if rows == self.rows else torch.zeros_like(q)
+            o_row, o_head, _ = out.stride()
+            o_addr = out.data_ptr()
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError('out must have the shape and type of q')
-        _, _, o_row, o_head, o_addr = _heads(out, 'out', dev, self.n_heads, self.head_dim)
+        else:
+            _, _, o_row, o_head, o_addr = _heads(out, 'out', dev, self.n_heads, self.head_dim)
         if lse is not None and (lse.shape != q.shape[:2] or lse.dtype != torch.float32 or lse.device != dev
                                 or not lse.is_contiguous()):
             raise ValueError('lse must be a contiguous fp32 [rows, heads] tensor')
