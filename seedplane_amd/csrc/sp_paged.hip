@@ -169,8 +169,8 @@ void lay_out(sp_attn_plan &p) {
 }
 
 void check_shape(int NH, int NKV, int HD, int max_rows, int max_seqs) {
-    require(NH >= 1 && NKV >= 1 && NH % NKV == 0 && NH / NKV <= MAX_GROUP, SP_EINVAL,
-            "n_heads must be a multiple of n_kv_heads with at most 32 query heads per kv head");
+    require(NH >= 1 && NH <= 65535 && NKV >= 1 && NH % NKV == 0 && NH / NKV <= MAX_GROUP, SP_EINVAL,
+            "n_heads must be at most 65535 and a multiple of n_kv_heads with at most 32 query heads per kv head");
     require(HD == 64 || HD == 128, SP_EINVAL, "head_dim must be 64 or 128");
     require(max_rows >= 1 && max_seqs >= 1 && max_seqs <= 65535 && (int64_t)max_rows * NH <= (1 << 27), SP_EINVAL,
             "max_rows and max_seqs must be positive, max_seqs at most 65535 and max_rows * n_heads at most 2^27");

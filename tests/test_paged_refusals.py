@@ -70,7 +70,7 @@ def test_plan_refusals():
     lib = _lib.load()
     h = ctypes.c_void_p()
     ok = (12, 2, 128, 16, 16)
-    for i, bad in [(0, 0), (0, 13), (1, 0), (2, 96), (2, 0), (3, 0), (4, 0), (4, 65536), (3, 1 << 24), (0, 66)]:
+    for i, bad in [(0, 0), (0, 13), (1, 0), (2, 96), (2, 0), (3, 0), (4, 0), (4, 65536), (3, 1 << 24), (0, 66), (0, 131072)]:
         a = list(ok)
         a[i] = bad
         assert lib.sp_attn_plan_create(*a, ctypes.byref(h)) == _lib.SP_EINVAL and not h.value, (i, bad)
