@@ -235,6 +235,26 @@ def test_attention(gpu_device, dtype, cache, hd, q_lens, kv_lens, groups, nh, nk
     _attend(gpu_device, q_lens, kv_lens, groups, nh, nkv, hd, page, dtype, cache, seed=len(q_lens) + hd)
 
 
+@pytest.mark.parametrize('seed', range(24))
+def test_random_batches(gpu_device, seed):
+    """Head counts, page sizes, groups (of sequences without queries too), drafts, prompts and lone tokens drawn together."""
+    rng = np.random.default_rng(1000 + seed)
+    nkv = int(rng.choice([1, 2, 3, 4]))
+    nh = nkv * int(rng.choice([1, 2, 5, 6, 7, 16, 32]))
+    hd, page = int(rng.choice([64, 128])), int(rng.choice([1, 8, 16, 20, 64]))
+    dtype, cache = TYPES[seed % 4]
+    q_lens, kv_lens, groups = [], [], []
+    for _ in range(rng.integers(1, 4)):
+        size, shared = int(rng.integers(1, 7)), int(rng.integers(0, 700)) // page * page
+        for _ in range(size):
+            q = int(rng.choice([0, 1, 1, 1, 2, 5, 9, 33, 70]))
+            q_lens.append(q)
+            kv_lens.append(shared + int(rng.integers(0, 260)))     # (a draft may begin within the shared positions, or before any)
+        groups.append((size, shared))
+    print(f'random {seed}: {nh}/{nkv} heads of {hd}, pages of {page}, {dtype} {cache}, {q_lens} {kv_lens} {groups}', flush=True)
+    _attend(gpu_device, q_lens, kv_lens, groups, nh, nkv, hd, page, dtype, cache, seed=seed)
+
+
 def test_layouts_of_the_pool(gpu_device):
     """Heads before rows, rows before heads, keys and values in one allocation, one page, one head: append and attention."""
     nkv, hd, page, n, L = 2, 64, 16, 12, 150
