@@ -198,6 +198,8 @@ class PagedKV:
     same strides for both and the values of a row side by side.  An e4m3 cache holds value / scale, with fp32 scales per K/V
     head."""
 
+    _lease = None                 # of an engine's pool (Qwen2Engine.paged_kv): what holds and dates its memory
+
     def __init__(self, k, v, k_scale=None, v_scale=None):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
             raise ValueError('k and v must be [n_pages, kv_heads, page_size, head_dim] of one shape, type, device and layout')
@@ -228,6 +230,13 @@ class PagedKV:
         """Strides of pages, heads and rows; of a dimension of one entry: any that suits the kernels."""
         return [s if n > 1 else self.head_dim for n, s in zip(self.k.shape[:3], self.k.stride())]
 
+    def _check_lease(self, table):
+        """An engine's pool is where it was when this cache was made, and a table that Qwen2Engine.page_table gave is of it."""
+        self._lease.check()
+        made_for = getattr(table, '_lease', None)
+        if made_for is not None and made_for != self._lease.key:
+            raise ValueError('the page table is of an older pool, another engine or other pages: call page_table() again')
+
     @classmethod
     def allocate(cls, n_pages, page_size, n_kv_heads, head_dim, dtype=torch.float16, k_scale=None, v_scale=None, device='cuda'):
         shape, device = (n_pages, n_kv_heads, page_size, head_dim), _device(device)
@@ -238,6 +247,8 @@ class PagedKV:
         seq[r] (int32 [rows]; a row with seq -1, or whose position has no page, writes nothing).  With `rotary` the keys turn by
         rotary_pos (default: pos) on the way, and the queries q [rows, heads, head_dim] into q_out (default: a new tensor of q's
         type; may be q itself), which is returned."""
+        if self._lease is not None:
+            self._check_lease(table)
         dev, nkv, hd = self.device, self.n_kv_heads, self.head_dim
         dt, rows, k_row, k_head, k_addr = _heads(k, 'k', dev, nkv, hd)
         v_dt, v_rows, v_row, v_head, v_addr = _heads(v, 'v', dev, nkv, hd)
@@ -316,6 +327,8 @@ class AttentionPlan:
     def run(self, q, kv, table, out=None, lse=None, scale=None, workspace=None):
         """Attention of q [rows, heads, head_dim] (fp16 or bf16) over the pages of `kv`; returns `out` (default: a new tensor,
         zeros behind the plan's rows).  lse: fp32 [rows, heads], filled with the logarithm of each row's sum of exponentials."""
+        if kv._lease is not None:
+            kv._check_lease(table)
         dev = self.device
         dt, rows, q_row, q_head, q_addr = _heads(q, 'q', dev, self.n_heads, self.head_dim)
         if kv.device != dev:

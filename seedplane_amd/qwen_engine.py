@@ -17,6 +17,7 @@ Quantized bundles (`quantization_config.quant_method == 'seedplane'`) carry int8
 (`<name>.qweight/.scales/.qzeros`); float bundles are run with fp16 weights.
 """
 import ctypes
+import itertools
 import json
 import weakref
 from dataclasses import dataclass, field
@@ -30,6 +31,7 @@ from . import native_bundle
 
 GROUP = 32
 WIDE_COLS = 2048          # most columns of one sp_engine_prefill call
+_POOLS = itertools.count(1)
 
 
 class _KVLayers:
@@ -99,6 +101,18 @@ def _id_array(ids):
     return torch.as_tensor(ids, dtype=torch.long).flatten().cpu().numpy()
 
 
+class _PoolLease:
+    """One pool of an engine seen as pages: holds the engine, and tells whether the pool is still that one."""
+
+    def __init__(self, engine, page):
+        self.engine = engine
+        self.key = (engine._pool_generation, page)
+
+    def check(self):
+        if self.engine._pool_generation != self.key[0]:
+            raise ValueError("the engine's KV pool has been reserved or grown again since: call paged_kv() again")
+
+
 class Qwen2Engine:
     """Inference-only Qwen2/Qwen2.5 runtime with a persistent HBM KV cache (reference: qwen_engine.py:32-166)."""
 
@@ -166,6 +180,7 @@ class Qwen2Engine:
         self._pool_n = 0
         self._pool_slots = 0
         self._epoch = 0
+        self._pool_generation = 0                      # which of all engines' pools: each has memory of its own
         self._free = []
         self._live = weakref.WeakValueDictionary()     # sequence index -> its live cache
         self._logits_buf = None
@@ -285,6 +300,7 @@ class Qwen2Engine:
     # ------------------------------------------------------------------------------------------ KV pool
     def reserve(self, n_seq, n_slots):
         """(Re)allocate the HBM KV pool for n_seq sequences x n_slots ring slots; invalidates existing caches."""
+        self._pool_generation = next(_POOLS)           # (before the call, which frees the old pool even where it then fails)
         _lib.check(self.lib.sp_engine_kv_reserve(self.h, int(n_seq), int(n_slots)), self.h)
         self._pool_n, self._pool_slots = int(n_seq), int(n_slots)
         self._epoch += 1
@@ -304,6 +320,7 @@ class Qwen2Engine:
         live = [(s, c) for s, c in list(self._live.items()) if c.epoch == self._epoch]
         seqs = np.array([s for s, _ in live], dtype=np.int32)
         lens = np.array([c.length for _, c in live], dtype=np.int32)
+        self._pool_generation = next(_POOLS)
         _lib.check(self.lib.sp_engine_kv_grow(self.h, n_seq, n_slots, len(live), _ptr(seqs), _ptr(lens)), self.h)
         self._free = list(range(n_seq - 1, self._pool_n - 1, -1)) + self._free
         self._pool_n, self._pool_slots = n_seq, n_slots
@@ -347,24 +364,33 @@ class Qwen2Engine:
     def paged_kv(self, layer, page_size=None):
         """Layer `layer`'s pool as a paged cache (paged.PagedKV) that shares the engine's memory: pages of `page_size` ring
         slots, a divisor of the pool's slots (default: a sequence's whole ring), so that what the engine prefilled can be a
-        shared prefix of paged attention without a copy.  Valid until the pool is reserved or grown again."""
+        shared prefix of paged attention without a copy.  It keeps the engine alive.  When the pool is reserved or grown again
+        (which new_cache and generate_batch do by themselves where it is too small) its memory moves: append() and run()
+        refuse the older PagedKV from then on, with a ValueError, and a program calls paged_kv() and page_table() again.  Its
+        `k` and `v`, and graphs that were captured over it, must not be used any more then."""
         from .paged import PagedKV
         k, v = self._kv_pool(range(self.n_layers)[layer])
         n, nkv, S, hd = k.shape
         page = self._page_size(page_size)
         pages = (n * nkv * S - (nkv - 1) * S) // page           # head 0 of any page, so that every head lies in the pool
-        return PagedKV(*(t.as_strided((pages, nkv, page, hd), (page * hd, S * hd, hd, 1)) for t in (k, v)))
+        kv = PagedKV(*(t.as_strided((pages, nkv, page, hd), (page * hd, S * hd, hd, 1)) for t in (k, v)))
+        kv._lease = _PoolLease(self, page)
+        return kv
 
     def page_table(self, caches, page_size=None):
         """The pages of `caches` in paged_kv(layer, page_size), int32 [len(caches), slots / page_size] on the engine's device: of
-        caches whose ring has not wrapped, position p lies in page p // page_size."""
+        caches whose ring has not wrapped, position p lies in page p // page_size.  Numbers of the present pool: once it is
+        reserved or grown again the table itself is refused beside a PagedKV of the new pool, but what a program has cut or
+        copied out of it is not and must be made anew.  The pages of a cache that goes out of use are another's."""
         page, S = self._page_size(page_size), self._pool_slots
         for c in caches:
             self._check_cache(c)
             if c.length > S:
                 raise ValueError('the ring of a cache has wrapped: its positions have no pages of their own')
         first = torch.tensor([c.seq * self.n_kv_heads * S // page for c in caches], dtype=torch.int32).view(-1, 1)
-        return (first + torch.arange(S // page, dtype=torch.int32)).to(self.device)
+        table = (first + torch.arange(S // page, dtype=torch.int32)).to(self.device)
+        table._lease = _PoolLease(self, page).key
+        return table
 
     def _page_size(self, page_size):
         if not self._pool_slots:

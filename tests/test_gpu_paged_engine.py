@@ -59,3 +59,29 @@ def test_whole_rings_as_pages_and_refusals(gpu_device, engine):
     wrapped.length = 193
     with pytest.raises(ValueError):
         engine.page_table([wrapped])
+
+
+def test_a_pool_that_grows_or_whose_engine_is_let_go(gpu_device):
+    """After the pool has grown by itself the older pages are refused and new ones read the same positions; the pages outlive the
+    program's own reference to the engine."""
+    cfg, w = make_weights(small_cfg(), 'q8', seed=3)
+    eng = Qwen2Engine(config=cfg, tensors=w, max_tokens=16)
+    eng.reserve(1, 64)
+    doc = eng.new_cache(64)
+    eng.prefill([[7, 8, 9, 10, 11] * 6], [doc])
+    nh, nkv, hd = eng.n_heads, eng.n_kv_heads, eng.head_dim
+    plan = AttentionPlan(nh, nkv, hd, 2, 1).set([2], [30])
+    q = torch.randn((2, nh, hd), generator=torch.Generator().manual_seed(1)).half().to(gpu_device)
+    old, old_table = eng.paged_kv(1, 16), eng.page_table([doc], 16)
+    want = plan.run(q, old, old_table)
+    other = eng.new_cache(128)                                 # more slots and more sequences than the pool has
+    new = torch.zeros((1, nkv, hd), dtype=torch.float16, device=gpu_device)
+    at = torch.zeros(1, dtype=torch.int32, device=gpu_device)
+    kv, table = eng.paged_kv(1, 16), eng.page_table([doc], 16)
+    for bad in (lambda: plan.run(q, old, old_table), lambda: plan.run(q, old, table), lambda: plan.run(q, kv, old_table),
+                lambda: old.append(new, new, at, at, old_table)):
+        with pytest.raises(ValueError):
+            bad()
+    assert torch.equal(plan.run(q, kv, table), want)
+    del eng, other, doc
+    assert torch.equal(plan.run(q, kv, table), want)
