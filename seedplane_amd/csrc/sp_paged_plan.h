@@ -87,7 +87,7 @@ inline void make_plan(int n_heads, int n_kv, int head_dim, int n_seq, const int3
     // a sequence whose own queries fill their row tiles (an eighth empty at most) gains nothing from rows of others beside
     // them: it reads the shared positions with its own, in one range, and needs no join
     const int per_tile = TILE_ROWS_OF[KINDS - 1] / G;
-    auto fills_tiles = [&](int32_t q) { return (int64_t)(q + per_tile - 1) / per_tile * per_tile * 8 <= (int64_t)q * 9; };
+    auto fills_tiles = [&](int32_t q) { return q > 0 && (int64_t)(q + per_tile - 1) / per_tile * per_tile * 8 <= (int64_t)q * 9; };
     int s0 = 0;
     for (int g = 0; g < n_groups; ++g) {
         const int s1 = s0 + group_size[g];
@@ -96,14 +96,14 @@ inline void make_plan(int n_heads, int n_kv, int head_dim, int n_seq, const int3
             int b = a;
             int32_t shared = group_shared[g], tokens = 0, first = -1, members = 0;
             for (; b < s1 && !fills_tiles(q_len[b]); ++b) {
-                if (q_len[b] == 0) continue;
+                if (q_len[b] == 0) continue;                                 // idle: no rows, and no length to heed
                 if (first < 0) first = b;
                 ++members;
                 tokens += q_len[b];
                 shared = std::min(shared, std::max(0, kv_len[b] - q_len[b]));
             }
             if (members < 2) shared = 0;                                     // nothing to share
-            if (b == a) b = a + 1;
+            if (b == a) b = a + 1;                                           // (one that fills its tiles)
             if (shared > 0) add(n_tok, tokens, first, 0, shared, 0, 0);
             for (int s = a; s < b; ++s) {
                 if (q_len[s]) add(n_tok, q_len[s], s, shared, kv_len[s], kv_len[s] - q_len[s], 1);
