@@ -444,15 +444,19 @@ void sp_attn_plan_destroy(sp_attn_plan *plan);
 /* Lengths of the next batch (host arrays): sequence s has q_len[s] query rows, the last of its kv_len[s] cached positions:
  * its query i sees positions 0 .. kv_len[s] - q_len[s] + i (none where that is negative: the output row is zeros).  Sequences
  * in order; their query rows lie one after the other.  Groups (n_groups 0: none) are runs of group_size sequences whose page
- * tables name the same rows for positions 0 .. group_shared - 1, which are then read once for the group (through the table of
- * its first sequence with queries); of a group whose first query stands earlier, only the positions before that query.  The
- * tables are copied to the device on hip_stream: later sp_op_paged_attention calls must follow on it.  SP_ESTATE in a stream
- * capture; a captured sp_op_paged_attention reads the tables of the last set before each replay. */
+ * tables name the same rows for positions 0 .. group_shared - 1.  Those are read once (per tile of 128 rows, i.e. query heads
+ * of a K/V head over tokens) for all of the group's sequences whose queries do not fill such tiles by themselves, through the
+ * table of the first of these, as far as the earliest of their queries stands behind them; a sequence that fills its tiles (an
+ * eighth empty at most) reads them with its own positions.  The order of a group's sequences does not matter, and sequences
+ * without queries change nothing.  The tables are copied to the device on hip_stream: later sp_op_paged_attention calls must
+ * follow on it.  SP_ESTATE in a stream capture; a captured sp_op_paged_attention reads the tables of the last set before each
+ * replay. */
 int sp_attn_plan_set(sp_attn_plan *plan, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len, int32_t n_groups,
                      const int32_t *group_size, const int32_t *group_shared, void *hip_stream);
 /* Host only, for inspection: the items that sp_attn_plan_set makes of these lengths, as 12 int32 each: first token, tokens, K/V
  * head, sequence, first position, end, position seen by the first token (2^30: all), first record or -1, kind (row tile of
- * 32 << kind rows), three reserved; and per token 8 int32: base, parts, tile and index of its records of the shared and of its own
+ * 32 << kind rows), -1 or (shared positions of tokens that are no range: from the first on those with records of shared
+ * positions) a place in the plan's list, two reserved; and per token 8 int32: base, parts, tile and index of its records of the shared and of its own
  * positions (pairs).  items and token_recs may be NULL. */
 int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len,
                        int32_t n_groups, const int32_t *group_size, const int32_t *group_shared, int32_t capacity,

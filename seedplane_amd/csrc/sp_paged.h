@@ -33,6 +33,20 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+// key / d for keys below 2^30: m = ceil(2^(30 + l) / d) with 2^l >= d exceeds 2^(30 + l) / d by less than 2^l / d, so
+// key m / 2^(30 + l) exceeds key / d by less than 1 / d; m is at most 2^31 as 2^(l - 1) < d.  (Straight code: a launch fetches its
+// instructions anew, and a branch over a division cost a lone token's call over 733 positions 0.17 us of 8.95.)
+struct PageDivisor {
+    uint32_t m;
+    int l;
+    PageDivisor() = default;
+    explicit PageDivisor(uint32_t d) : l(0) {
+        while (((uint64_t)1 << l) < d) ++l;
+        m = (uint32_t)((((uint64_t)1 << (30 + l)) + d - 1) / d);
+    }
+};
+__device__ __forceinline__ int operator/(int key, PageDivisor d) { return (int)(__umulhi((uint32_t)key << 2, d.m) >> d.l); }
+
 struct AttnArgs {
     const void *q;
     void *out;
@@ -43,10 +57,12 @@ struct AttnArgs {
     const int *table;                 // [n_seq][max_pages]
     int rows, n_seq, max_pages, n_pages, page_size;      // rows of q and out, of the table; its width; the pool
     uint32_t page_rows, head_rows, slot_rows;     // strides of the pool in rows of head_dim values
-    int NH, G, page_shift;            // page_shift: log2 of page_size, -1 where that is no power of two
+    int NH, G;
     Divisor by_g;
+    PageDivisor by_page;
     float scale;                      // of the scores, times log2(e)
     const Item *items;
+    const int *list;                  // tokens of the items that name theirs
     const int *n_items;               // NULL: one block per item
     // Records: [rows][HD] unnormalised outputs, and [rows] (m in log2 units, l, a factor of the outputs).  For bf16 outputs, which
     // round by 2^-9 of themselves, they are fp16 shares of the row's largest finite one (half the traffic; off by 2^-12 of the
@@ -170,7 +186,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
 
     // The chain of an item is its table's entries, their rows of the pool, the copies: the entries are asked for first.
     const int *table = a.table + (int64_t)w.seq * a.max_pages;
-    auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size; };
+    auto page_of = [&](int key) { return key / a.by_page; };           // (of no meaning behind the last key, where it is not used)
     auto entry_of = [&](int key, int page) { return key < w.k1 && w.seq < a.n_seq && page < a.max_pages ? table[page] : -1; };
     if (threadIdx.x == 0) sh.nonfinite = 0;
     const int key0 = w.k0 + (int)threadIdx.x, page0 = page_of(key0), entry0 = entry_of(key0, page0);
@@ -178,11 +194,16 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     const int row = rw * 32 + col;
     // (a captured call may meet tables set later: its own sizes bound every access)
     const int rt = row / a.by_g;
-    const bool live = row < w.ntok * a.G && w.tok0 + rt < a.rows;
+    int at = w.tok0 + rt;
+    if (__builtin_expect(w.list >= 0, 0)) {
+        at = a.list[w.list + min(rt, w.ntok - 1)];
+        asm volatile("" : "+v"(at));                                   // (awaited here: behind the branch every item would wait for its entries)
+    }
+    const bool live = row < w.ntok * a.G && at < a.rows;
     const int tok = live ? rt : 0, hh = live ? row - rt * a.G : 0;
     frag qf[NS];
     {
-        const T *q = (const T *)a.q + (int64_t)min(w.tok0 + tok, a.rows - 1) * a.q_row + (int64_t)(w.kvh * a.G + hh) * a.q_head + 8 * h;
+        const T *q = (const T *)a.q + (int64_t)(live ? at : min(w.tok0, a.rows - 1)) * a.q_row + (int64_t)(w.kvh * a.G + hh) * a.q_head + 8 * h;
 #pragma unroll
         for (int s = 0; s < NS; ++s) qf[s] = *(const frag *)(q + 16 * s);
     }
@@ -572,7 +593,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         }
     }
     const int row2 = rw * 32 + (opaque(lane) & 31), tok2 = row2 / a.by_g;
-    if (row2 < w.ntok * a.G && w.tok0 + tok2 < a.rows) {
+    if (row2 < w.ntok * a.G && (w.rec >= 0 || w.tok0 + tok2 < a.rows)) {       // (records have room for every row of the plan)
         const int hh2 = row2 - tok2 * a.G;
         const float vs = KV8 ? a.vs[w.kvh] : 1.f;
         if (w.rec < 0) {

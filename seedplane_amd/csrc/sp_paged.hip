@@ -137,9 +137,9 @@ void check_cache(const sp_paged_kv *kv) {
 
 struct sp_attn_plan {
     int NH = 0, NKV = 0, HD = 0, max_rows = 0, max_seqs = 0, device = 0;
-    // device block: header [16] (items, tokens), items, and token records, at fixed places
+    // device block: header [16] (items, tokens), token records, items and token list, at fixed places
     int32_t *dev = nullptr;
-    size_t tok_at = 0, item_at = 0, words = 0;
+    size_t tok_at = 0, item_at = 0, list_at = 0, words = 0;
     int32_t *staging[2] = {};            // pinned images of the block, used in turn
     hipEvent_t copied[2] = {};
     bool used[2] = {};
@@ -165,7 +165,8 @@ constexpr size_t HEADER = 16;
 void lay_out(sp_attn_plan &p) {
     p.tok_at = HEADER;
     p.item_at = p.tok_at + (size_t)p.max_rows * (sizeof(TokenRecs) / 4);
-    p.words = p.item_at + (size_t)items_bound(p.max_rows, p.NKV) * (sizeof(Item) / 4);
+    p.list_at = p.item_at + (size_t)items_bound(p.max_rows, p.NKV) * (sizeof(Item) / 4);
+    p.words = p.list_at + (size_t)p.max_rows;
 }
 
 void check_shape(int NH, int NKV, int HD, int max_rows, int max_seqs) {
@@ -398,12 +399,15 @@ int sp_attn_plan_set(sp_attn_plan *p, int32_t n_seq, const int32_t *q_len, const
         img[0] = (int32_t)t.items.size();
         img[1] = (int32_t)t.toks.size();
         p->set = false;                                  // until the tables are on their way
-        // header and token records lie side by side: one copy; then the items
+        // header and token records lie side by side: one copy; then the items, and the list where there is one
         std::memcpy(img + p->tok_at, t.toks.data(), t.toks.size() * sizeof(TokenRecs));
         std::memcpy(img + p->item_at, t.items.data(), t.items.size() * sizeof(Item));
+        std::copy(t.list.begin(), t.list.end(), img + p->list_at);
         HIPCHK(hipMemcpyAsync(p->dev, img, (HEADER + t.toks.size() * (sizeof(TokenRecs) / 4)) * 4, hipMemcpyHostToDevice, st));
         if (!t.items.empty())
             HIPCHK(hipMemcpyAsync(p->dev + p->item_at, img + p->item_at, t.items.size() * sizeof(Item), hipMemcpyHostToDevice, st));
+        if (!t.list.empty())
+            HIPCHK(hipMemcpyAsync(p->dev + p->list_at, img + p->list_at, t.list.size() * 4, hipMemcpyHostToDevice, st));
         HIPCHK(hipEventRecord(p->copied[turn], st));
         p->used[turn] = true;
         p->turn = turn ^ 1;
@@ -491,13 +495,14 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         a.slot_rows = (uint32_t)(kv->row_stride / hd);
         a.NH = p->NH; a.G = p->NH / p->NKV;
         a.by_g = Divisor(a.G);
-        a.page_shift = (kv->page_size & (kv->page_size - 1)) == 0 ? __builtin_ctz(kv->page_size) : -1;
+        a.by_page = PageDivisor(kv->page_size);
         a.scale = scale * LOG2E;
         const size_t recs = (size_t)records_bound(p->max_rows, p->NH);
         a.ml = (f32x4 *)workspace_dev;
         a.po = a.ml + recs;
         const bool kv8 = kv->dtype == SP_DT_E4M3;
         a.items = (const Item *)(p->dev + p->item_at);
+        a.list = p->dev + p->list_at;
         a.n_items = capturing ? p->dev : nullptr;
         const int grid = capturing ? CAPTURED_GRID : p->n_items;
         if (grid) {

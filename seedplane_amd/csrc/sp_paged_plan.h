@@ -2,8 +2,9 @@
 //
 // Query rows of a K/V head: row r of a range of tokens is (token r / G, query head r % G of the head's group).  A segment is a
 // range of tokens, the sequence whose page table gives the keys, and a range of its positions:
-//   - the shared positions of a group of sequences, for all tokens of the group (every token sees all of them: a group's
-//     shared range ends at the earliest query of its sequences at the latest, so that no mask is needed);
+//   - the shared positions of a group of sequences, for all tokens of the group but those of sequences that fill row tiles by
+//     themselves (every token sees all of them: a group's shared range ends at the earliest of these queries at the latest, so
+//     that no mask is needed).  Where filling sequences stand between them the tokens are no range, and a list names them;
 //   - a sequence's remaining positions, for its own tokens (causal).
 // Segments are cut into row tiles of whole tokens: 32, 64 or 128 rows (1, 2 or 4 of a block's four waves side by side over
 // the rows, the others over the keys).  Where the tiles of one size are too few to fill the chip, their keys are cut
@@ -23,7 +24,8 @@ struct Item {                        // one block's work
     int32_t pos0;                    // token tok0 + i sees positions <= pos0 + i (ALL_SEEN: every one)
     int32_t rec;                     // first record (row r of the tile leaves record rec + r), -1: the output itself
     int32_t kind;                    // row tile of 32 << kind rows
-    int32_t reserved[3];
+    int32_t list;                    // the tokens are list[list ..] (tok0 the first), -1: tok0 ..
+    int32_t reserved[2];
 };
 struct TokenRecs {                   // the records of a token: record (kvh * parts + j) * tile + i, times G, from base
     int32_t base[2], parts[2], tile[2], i[2];     // of the shared positions, of its own
@@ -46,12 +48,13 @@ constexpr int MAX_GROUP = 32;                                  // query heads pe
 // uncut, 10.7 cut and joined; head_dim 64, 512 / 1024: 7.3 / 9.3 against 10.6).
 constexpr int64_t UNCUT_VALUES = 640 * 128;
 struct Segment {
-    int32_t tok0, ntok, seq, k0, k1, pos0, which, kind;        // which: 0 shared, 1 own
+    int32_t tok0, ntok, seq, k0, k1, pos0, which, kind, list;  // which: 0 shared, 1 own; list: as an item's
 };
 
 struct PlanTables {
     std::vector<Item> items;         // the costliest first
     std::vector<TokenRecs> toks;
+    std::vector<int32_t> list;       // tokens of shared items whose tokens are no range, each at most once
     bool joined = false;             // some token needs the join
     int32_t most_parts = 0;          // most records of a token that does
     int64_t records = 0;             // rows of records
@@ -74,46 +77,55 @@ inline void make_plan(int n_heads, int n_kv, int head_dim, int n_seq, const int3
                       const int32_t *group_size, const int32_t *group_shared, PlanTables &out) {
     const int G = n_heads / n_kv;
     std::vector<Segment> segs;
+    std::vector<int32_t> sharing;                                            // the tokens that share, of a group
     int32_t n_tok = 0;
     out = PlanTables{};
-    auto add = [&](int32_t tok0, int32_t ntok, int32_t seq, int32_t k0, int32_t k1, int32_t pos0, int which) {
-        const int kind = kind_of((int64_t)ntok * G), per = TILE_ROWS_OF[kind] / G;
-        for (int32_t t = 0; t < ntok; t += per) {
-            const int32_t n = std::min(per, ntok - t);
-            const int32_t end = which ? std::min(k1, pos0 + t + n) : k1;     // the tile's last token sees positions < end
-            if (end > k0) segs.push_back({tok0 + t, n, seq, k0, end, which ? pos0 + t : ALL_SEEN, which, kind});
-        }
-    };
     // a sequence whose own queries fill their row tiles (an eighth empty at most) gains nothing from rows of others beside
     // them: it reads the shared positions with its own, in one range, and needs no join
     const int per_tile = TILE_ROWS_OF[KINDS - 1] / G;
-    auto fills_tiles = [&](int32_t q) { return q > 0 && (int64_t)(q + per_tile - 1) / per_tile * per_tile * 8 <= (int64_t)q * 9; };
+    auto fills_tiles = [&](int32_t q) { return (int64_t)(q + per_tile - 1) / per_tile * per_tile * 8 <= (int64_t)q * 9; };
+    auto shares = [&](int s) { return q_len[s] > 0 && !fills_tiles(q_len[s]); };
+    auto tiles_of = [&](int32_t ntok, auto &&tile) {
+        const int kind = kind_of((int64_t)ntok * G), per = TILE_ROWS_OF[kind] / G;
+        for (int32_t t = 0; t < ntok; t += per) tile(t, std::min(per, ntok - t), kind);
+    };
     int s0 = 0;
     for (int g = 0; g < n_groups; ++g) {
         const int s1 = s0 + group_size[g];
-        // runs of sequences that share
-        for (int a = s0; a < s1;) {
-            int b = a;
-            int32_t shared = group_shared[g], tokens = 0, first = -1, members = 0;
-            for (; b < s1 && !fills_tiles(q_len[b]); ++b) {
-                if (q_len[b] == 0) continue;                                 // idle: no rows, and no length to heed
-                if (first < 0) first = b;
+        int32_t shared = group_shared[g], first = -1, members = 0, at = n_tok;
+        sharing.clear();
+        for (int s = s0; s < s1; ++s) {
+            if (shares(s)) {
+                if (first < 0) first = s;
                 ++members;
-                tokens += q_len[b];
-                shared = std::min(shared, std::max(0, kv_len[b] - q_len[b]));
+                shared = std::min(shared, std::max(0, kv_len[s] - q_len[s]));
+                for (int32_t i = 0; i < q_len[s]; ++i) sharing.push_back(at + i);
             }
-            if (members < 2) shared = 0;                                     // nothing to share
-            if (b == a) b = a + 1;                                           // (one that fills its tiles)
-            if (shared > 0) add(n_tok, tokens, first, 0, shared, 0, 0);
-            for (int s = a; s < b; ++s) {
-                if (q_len[s]) add(n_tok, q_len[s], s, shared, kv_len[s], kv_len[s] - q_len[s], 1);
-                out.max_kv = std::max(out.max_kv, q_len[s] ? kv_len[s] : 0);
-                n_tok += q_len[s];
-            }
-            a = b;
+            at += q_len[s];
+        }
+        if (members < 2) shared = 0;                                         // nothing to share
+        if (shared > 0) {
+            const int32_t n = (int32_t)sharing.size();
+            const bool range = sharing[n - 1] - sharing[0] == n - 1;
+            const int32_t base = (int32_t)out.list.size();
+            if (!range) out.list.insert(out.list.end(), sharing.begin(), sharing.end());
+            tiles_of(n, [&](int32_t t, int32_t len, int kind) {
+                const bool run = sharing[t + len - 1] - sharing[t] == len - 1;
+                segs.push_back({sharing[t], len, first, 0, shared, ALL_SEEN, 0, kind, run ? -1 : base + t});
+            });
+        }
+        for (int s = s0; s < s1; ++s) {
+            const int32_t k0 = shares(s) ? shared : 0, pos0 = kv_len[s] - q_len[s];
+            tiles_of(q_len[s], [&](int32_t t, int32_t len, int kind) {
+                const int32_t end = std::min(kv_len[s], pos0 + t + len);     // the tile's last token sees positions < end
+                if (end > k0) segs.push_back({n_tok + t, len, s, k0, end, pos0 + t, 1, kind, -1});
+            });
+            if (q_len[s]) out.max_kv = std::max(out.max_kv, kv_len[s]);
+            n_tok += q_len[s];
         }
         s0 = s1;
     }
+    auto token = [&](const Segment &s, int i) { return s.list < 0 ? s.tok0 + i : out.list[s.list + i]; };
     out.toks.assign(n_tok, TokenRecs{});
     auto steps_of = [](const Segment &s) { return (int64_t)(s.k1 - s.k0 + KEY_STEP - 1) / KEY_STEP; };
     int64_t total = 0;
@@ -128,7 +140,7 @@ inline void make_plan(int n_heads, int n_kv, int head_dim, int n_seq, const int3
     };
     for (const Segment &s : segs)
         for (int i = 0; i < s.ntok; ++i) {
-            TokenRecs &t = out.toks[s.tok0 + i];
+            TokenRecs &t = out.toks[token(s, i)];
             t.parts[s.which] = (int32_t)parts_of(s);
             t.tile[s.which] = s.ntok;
             t.i[s.which] = i;
@@ -137,10 +149,10 @@ inline void make_plan(int n_heads, int n_kv, int head_dim, int n_seq, const int3
     for (const Segment &s : segs) {
         const int32_t parts = out.toks[s.tok0].parts[s.which];
         bool alone = parts == 1;
-        for (int i = 0; i < s.ntok && alone; ++i) alone = out.toks[s.tok0 + i].parts[1 - s.which] == 0;
+        for (int i = 0; i < s.ntok && alone; ++i) alone = out.toks[token(s, i)].parts[1 - s.which] == 0;
         const int64_t base = out.records;
         for (int i = 0; i < s.ntok; ++i) {
-            TokenRecs &t = out.toks[s.tok0 + i];
+            TokenRecs &t = out.toks[token(s, i)];
             if (alone) t.parts[s.which] = -1;                                // written by its item
             else t.base[s.which] = (int32_t)(base / G);
         }
@@ -151,7 +163,7 @@ inline void make_plan(int n_heads, int n_kv, int head_dim, int n_seq, const int3
                 const int32_t a = s.k0 + (int32_t)(steps * j / parts) * KEY_STEP;
                 const int32_t b = j + 1 == parts ? s.k1 : s.k0 + (int32_t)(steps * (j + 1) / parts) * KEY_STEP;
                 out.items.push_back({s.tok0, s.ntok, h, s.seq, a, b, s.pos0,
-                                     alone ? -1 : (int32_t)(base + ((int64_t)h * parts + j) * s.ntok * G), s.kind, {0, 0, 0}});
+                                     alone ? -1 : (int32_t)(base + ((int64_t)h * parts + j) * s.ntok * G), s.kind, s.list, {0, 0}});
             }
     }
     std::stable_sort(out.items.begin(), out.items.end(), [](const Item &x, const Item &y) {

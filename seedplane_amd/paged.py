@@ -307,8 +307,8 @@ class AttentionPlan:
 
     def set(self, q_lens, kv_lens, groups=None):
         """The next batch (host integers): sequence s has q_lens[s] query tokens, the last of its kv_lens[s] cached positions.
-        groups: (sequences, shared positions) of each run of sequences whose tables name the same pages for their first positions;
-        None: nothing is shared."""
+        groups: (sequences, shared positions) of each run of sequences whose tables name the same pages for their first positions,
+        in any order and with idle ones (q_lens 0) among them; None: nothing is shared."""
         q, kv = _lengths(q_lens, 'q_lens'), _lengths(kv_lens, 'kv_lens')
         if q.ndim != 1 or q.shape != kv.shape:
             raise ValueError('q_lens and kv_lens must have one entry per sequence')
