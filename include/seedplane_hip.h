@@ -473,7 +473,7 @@ size_t sp_attn_plan_workspace(const sp_attn_plan *plan);
  * only the rows that see it and its own place in them.  Weighted sums of values are held in fp32.  scale must be positive.  workspace_dev: see
  * above; calls that overlap (other streams, graphs replayed side by side) need a workspace each.  The cache's strides are
  * multiples of head_dim here.  A captured call keeps its own n_rows, n_seq and max_pages: what a later set has beyond them is not
- * read or written. */
+ * read or written; within them its outputs have the bits of an uncaptured call with the same lengths. */
 int sp_op_paged_attention(const sp_attn_plan *plan, const sp_paged_kv *kv, int32_t dtype, int32_t n_rows, const void *q_dev,
                           int64_t q_row, int64_t q_head, const int32_t *table_dev, int32_t n_seq, int32_t max_pages, float scale,
                           void *out_dev, int64_t out_row, int64_t out_head, float *lse_dev, void *workspace_dev,

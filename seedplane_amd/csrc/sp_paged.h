@@ -640,7 +640,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(AttnArgs a) {
 // (HD 128) or eight (64) records per load and UNROLL loads in flight, and wave 0 adds the waves' sums in order.
 struct JoinArgs {
     const TokenRecs *toks;
-    const int *n_toks;
+    const int *n_toks;                // and behind it the most records of a token
     const void *po;
     const f32x4 *ml;
     void *out;
@@ -651,7 +651,7 @@ struct JoinArgs {
 constexpr int JOIN_UNROLL = 4;
 template <int HD> constexpr int JOIN_BATCH = 64 / (HD / 8) * JOIN_UNROLL;      // records that a wave has in flight
 template <class T, int HD, int WAVES>
-__global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
+__device__ __forceinline__ void join_heads(const JoinArgs &a) {
     constexpr int LPR = HD / 8, RPL = 64 / LPR, UNROLL = JOIN_UNROLL;  // lanes per record, records per load
     typedef float f32x8 __attribute__((ext_vector_type(8)));
     typedef typename Mma<T>::share S;
@@ -721,6 +721,18 @@ __global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
     *(T4 *)o = (T4){(T)(acc[0] * il), (T)(acc[1] * il), (T)(acc[2] * il), (T)(acc[3] * il)};
     *(T4 *)(o + 4) = (T4){(T)(acc[4] * il), (T)(acc[5] * il), (T)(acc[6] * il), (T)(acc[7] * il)};
     if (a.lse && lane == 0) a.lse[(int64_t)tok * a.NH + head] = L == 0.f ? -INFINITY : LN2 * (M + log2f(L));
+}
+// WAVES 0: a captured launch, a block per (token, query head), which takes the form that the tables of each replay ask for, so that
+// its sums have the eager call's order; the blocks that the one-wave form has too many end at once.
+template <class T, int HD, int WAVES>
+__global__ void __launch_bounds__(256) k_paged_join(JoinArgs a) {
+    if constexpr (WAVES > 0) {
+        join_heads<T, HD, WAVES>(a);
+    } else if (a.n_toks[1] > JOIN_BATCH<HD>) {
+        join_heads<T, HD, 4>(a);
+    } else if ((int)blockIdx.y < (a.NH + 3) / 4) {
+        join_heads<T, HD, 1>(a);
+    }
 }
 
 }  // namespace paged

@@ -137,7 +137,7 @@ void check_cache(const sp_paged_kv *kv) {
 
 struct sp_attn_plan {
     int NH = 0, NKV = 0, HD = 0, max_rows = 0, max_seqs = 0, device = 0;
-    // device block: header [16] (items, tokens), token records, items and token list, at fixed places
+    // device block: header [16] (items, tokens, most records of a token), token records, items and token list, at fixed places
     int32_t *dev = nullptr;
     size_t tok_at = 0, item_at = 0, list_at = 0, words = 0;
     int32_t *staging[2] = {};            // pinned images of the block, used in turn
@@ -224,9 +224,11 @@ void launch_typed(bool kv8, int HD, const AttnArgs &a, int grid, hipStream_t st)
 }
 // A wave joins a (token, head) whose records it has in flight at once; more are shared by the block's four waves (15 records of 96
 // tokens x 28 heads: 8.1 us by four, 5.1 by one).
+// (A captured launch leaves the choice to the kernel.)
 template <class T, int HD>
-void launch_join(const JoinArgs &j, int tokens, int most_parts, hipStream_t st) {
-    if (most_parts > JOIN_BATCH<HD>) hipLaunchKernelGGL((k_paged_join<T, HD, 4>), dim3(tokens, j.NH), dim3(256), 0, st, j);
+void launch_join(const JoinArgs &j, int tokens, bool capturing, int most_parts, hipStream_t st) {
+    if (capturing) hipLaunchKernelGGL((k_paged_join<T, HD, 0>), dim3(tokens, j.NH), dim3(256), 0, st, j);
+    else if (most_parts > JOIN_BATCH<HD>) hipLaunchKernelGGL((k_paged_join<T, HD, 4>), dim3(tokens, j.NH), dim3(256), 0, st, j);
     else hipLaunchKernelGGL((k_paged_join<T, HD, 1>), dim3(tokens, (j.NH + 3) / 4), dim3(256), 0, st, j);
 }
 
@@ -398,6 +400,7 @@ int sp_attn_plan_set(sp_attn_plan *p, int32_t n_seq, const int32_t *q_len, const
         std::memset(img, 0, HEADER * sizeof(int32_t));
         img[0] = (int32_t)t.items.size();
         img[1] = (int32_t)t.toks.size();
+        img[2] = t.most_parts;
         p->set = false;                                  // until the tables are on their way
         // header and token records lie side by side: one copy; then the items, and the list where there is one
         std::memcpy(img + p->tok_at, t.toks.data(), t.toks.size() * sizeof(TokenRecs));
@@ -515,11 +518,11 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
                              n_rows, p->NH, a.G};
             const int tokens = capturing ? std::min(n_rows, p->max_rows) : p->n_tok;
             if (dtype == SP_DT_F16) {
-                if (p->HD == 128) launch_join<f16, 128>(j, tokens, p->most_parts, st);
-                else launch_join<f16, 64>(j, tokens, p->most_parts, st);
+                if (p->HD == 128) launch_join<f16, 128>(j, tokens, capturing, p->most_parts, st);
+                else launch_join<f16, 64>(j, tokens, capturing, p->most_parts, st);
             } else {
-                if (p->HD == 128) launch_join<bf16, 128>(j, tokens, p->most_parts, st);
-                else launch_join<bf16, 64>(j, tokens, p->most_parts, st);
+                if (p->HD == 128) launch_join<bf16, 128>(j, tokens, capturing, p->most_parts, st);
+                else launch_join<bf16, 64>(j, tokens, capturing, p->most_parts, st);
             }
             HIPCHK(hipGetLastError());
         }

@@ -50,3 +50,31 @@ def test_a_call_captured_with_fewer_rows(gpu_device, rows):
         n = min(rows, 58)
         _within(out[:n], ref[:n], bound[:n])
         assert (out[n:] == 3).all()
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('hd', [64, 128])
+@pytest.mark.parametrize('captured,later', [(0, 8000), (200, 8000), (8000, 1500), (8000, 300), (200, 700)])
+def test_a_captured_call_has_the_eager_calls_bits(gpu_device, dtype, hd, captured, later):
+    """Whatever lengths the plan held at the capture, empty ones too: few and many parts to join."""
+    B, nh, nkv, page = 5, 14, 2, 16
+    g = torch.Generator().manual_seed(later + hd)
+    lens = [later + 3 * i for i in range(B)]
+    q, k, v, table, _ = paged_batch(g, [1] * B, lens, None, nh, nkv, hd, page, dtype, dtype, gpu_device)
+    wide = torch.full((B, 520), -1, dtype=torch.int32, device=gpu_device)
+    wide[:, :table.shape[1]] = table
+    kv, plan = PagedKV(k, v), AttentionPlan(nh, nkv, hd, B, B)
+    plan.set([1 if captured else 0] * B, [captured] * B)
+    out, lse = torch.zeros_like(q), torch.zeros(B, nh, device=gpu_device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.run(q, kv, wide, out=out, lse=lse)
+    plan.set([1] * B, lens)
+    want_lse = torch.zeros_like(lse)
+    want = plan.run(q, kv, wide, lse=want_lse)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
