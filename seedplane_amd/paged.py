@@ -84,6 +84,7 @@ def rotary_frequencies(rot_dim, theta=10000.0, scaling=None, length=None):
 
 
 _raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_is_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _device(device):
@@ -103,6 +104,14 @@ def _call(fn, device, *args):
             rc = fn(*args, _raw_stream(i))
     if rc:
         _lib.check(rc)
+
+
+def _capturing(device):
+    """Whether the current stream of `device` is being captured."""
+    if _current() == device.index:
+        return _is_capturing()
+    with torch.cuda.device(device):
+        return _is_capturing()
 
 
 def _heads(x, name, device, heads, hd):
@@ -326,7 +335,8 @@ class AttentionPlan:
 
     def run(self, q, kv, table, out=None, lse=None, scale=None, workspace=None):
         """Attention of q [rows, heads, head_dim] (fp16 or bf16) over the pages of `kv`; returns `out` (default: a new tensor,
-        zeros behind the plan's rows).  lse: fp32 [rows, heads], filled with the logarithm of each row's sum of exponentials."""
+        zeros behind the plan's rows; in a capture behind those of each replay).  lse: fp32 [rows, heads], filled with the
+        logarithm of each row's sum of exponentials."""
         if kv._lease is not None:
             kv._check_lease(table)
         dev = self.device
@@ -335,7 +345,8 @@ class AttentionPlan:
             raise ValueError('the cache is on another device')
         t = _table(table, dev)
         if out is None:
-            out = torch.empty_like(q) if rows == self.rows else torch.zeros_like(q)
+            # (a graph's replays may have fewer rows than the capture: they fill the rest anew)
+            out = torch.empty_like(q) if rows == self.rows and not _capturing(dev) else torch.zeros_like(q)
             o_row, o_head, _ = out.stride()
             o_addr = out.data_ptr()
         elif out.shape != q.shape or out.dtype != q.dtype:

@@ -78,3 +78,20 @@ def test_a_captured_call_has_the_eager_calls_bits(gpu_device, dtype, hd, capture
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def test_the_default_output_of_a_captured_call_has_zeros_behind_the_plans_rows(gpu_device):
+    """Replays after the plan has got fewer rows than it had at the capture, and more again."""
+    g = torch.Generator().manual_seed(8)
+    q, k, v, table, _ = paged_batch(g, [1] * 6, [90, 700, 33, 64, 5, 210], None, 8, 2, 64, 16, torch.float16, torch.float16, gpu_device)
+    kv, plan = PagedKV(k, v), AttentionPlan(8, 2, 64, 6, 6).set([1] * 6, [90, 700, 33, 64, 5, 210])
+    want = plan.run(q, kv, table)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = plan.run(q, kv, table)
+    for n in (6, 2, 5, 0, 6):
+        plan.set([1] * n + [0] * (6 - n), [90, 700, 33, 64, 5, 210])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:n], want[:n]) and (out[n:] == 0).all(), n

@@ -65,7 +65,8 @@ def attend(kv, table):
     plan = paged.AttentionPlan.__new__(paged.AttentionPlan)
     plan.device, plan.n_heads, plan.head_dim, plan.rows, plan.h, plan._ws_addr, plan._scale = kv.device, NKV, HD, 3, None, 0, 1.0
     plan.lib, kv._ref = type('', (), {'sp_op_paged_attention': None}), None
-    return plan.run(torch.zeros((3, NKV, HD), dtype=torch.float16), kv, table)
+    q, out = (torch.zeros((3, NKV, HD), dtype=torch.float16) for _ in range(2))
+    return plan.run(q, kv, table, out=out)
 
 
 def test_a_paged_cache_keeps_its_engine_alive(make_engine):
