@@ -470,8 +470,9 @@ size_t sp_attn_plan_workspace(const sp_attn_plan *plan);
  * logarithm of each row's sum of exponentials (-infinity for a row that sees nothing).  table_dev: int32 [n_seq][max_pages];
  * entries of positions at or behind a sequence's length are not read, an entry outside [0, n_pages) hides its positions.  What
  * the pool holds outside the positions read does not matter (NaN included), and an infinite or NaN value of a position reaches
- * only the rows that see it and its own place in them.  Weighted sums of values are held in fp32.  scale must be positive.  workspace_dev: see
- * above; calls that overlap (other streams, graphs replayed side by side) need a workspace each.  The cache's strides are
+ * only the rows that see it and its own place in them.  Scores, weights' sums and weighted sums of values are held in fp32, over
+ * parts of a range too; a weight is rounded to dtype for its product with the values.  scale must be positive.  workspace_dev:
+ * see above; calls that overlap (other streams, graphs replayed side by side) need a workspace each.  The cache's strides are
  * multiples of head_dim here.  A captured call keeps its own n_rows, n_seq and max_pages: what a later set has beyond them is not
  * read or written; within them its outputs have the bits of an uncaptured call with the same lengths. */
 int sp_op_paged_attention(const sp_attn_plan *plan, const sp_paged_kv *kv, int32_t dtype, int32_t n_rows, const void *q_dev,

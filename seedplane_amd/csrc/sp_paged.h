@@ -12,7 +12,8 @@
 // Keys and values go from the pages to LDS by direct copies (16 bytes a lane; no registers), two tiles deep.  A row's 16-byte
 // pieces are stored permuted by its index (the copy fetches them so), which keeps both kinds of reads off each other's banks.
 // Waves stand side by side over rows (WM) and over keys (4 / WM): 1 x 4 for the few rows of a decode step, 4 x 1 for
-// many.  Scores, maxima, sums and outputs are fp32; P is rounded to the queries' type for its product with V.
+// many.  Scores, maxima, sums and outputs are fp32, in the records of parts too; P is rounded to the queries' type, which its
+// product with V takes on the matrix cores (half a step of each weight).
 //
 // What bounds it.  Few rows: memory; 64 sequences x 4096 positions, 28 / 4 heads of 128 in bf16, 537 MB: 101 us, 5.3 TB/s, the rate of
 // a large copy (e4m3 50 us).  Many rows: the products and the other vector instructions, which two waves of a SIMD hardly
@@ -64,17 +65,16 @@ struct AttnArgs {
     const Item *items;
     const int *list;                  // tokens of the items that name theirs
     const int *n_items;               // NULL: one block per item
-    // Records: [rows][HD] unnormalised outputs, and [rows] (m in log2 units, l, a factor of the outputs).  For bf16 outputs, which
-    // round by 2^-9 of themselves, they are fp16 shares of the row's largest finite one (half the traffic; off by 2^-12 of the
-    // largest at most); for fp16 outputs fp32, since 11 bits twice would be seen (3.3e-4 from the 64-bit result, 2.4e-4 so)
-    void *po;
+    // Records: [rows][HD] unnormalised outputs, and [rows] (m in log2 units, l, a factor of the outputs).  Sums stay in fp32: as
+    // fp16 shares of a row's largest one (half the traffic; a decode step of 32 requests on 8192 shared positions 1.1 us of 23.5
+    // less) a column far below the row's largest loses its bits, and all of them below 2^-25 of it
+    float *po;
     f32x4 *ml;
 };
 
 template <class T> struct Mma;
 template <> struct Mma<f16> {
     typedef f16x8 frag;
-    typedef float share;
     static constexpr uint32_t INF = 0x7c00;                            // bits of infinity
     static constexpr float LAZY = 0.f;
     static __device__ __forceinline__ f32x16 run(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -85,7 +85,6 @@ template <> struct Mma<f16> {
 };
 template <> struct Mma<bf16> {
     typedef bf16x8 frag;
-    typedef f16 share;
     static constexpr uint32_t INF = 0x7f80;
     static constexpr float LAZY = 8.f;
     static __device__ __forceinline__ f32x16 run(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -136,7 +135,6 @@ struct AttnShared {                                                    // beside
     uint32_t seen[TABLE_KEYS / 32];                                    // which positions exist
     int nonfinite;                                                     // values cleared at the border
     float2 ml[4][32];
-    float top[4][32];
 };
 
 template <bool KV8, int HD, int WM>
@@ -575,23 +573,6 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 }
         }
     }
-    // the row's largest finite value: over the lane's values, its other half, the key waves' shares.  (No less than 2^-126, whose
-    // reciprocal is finite.)
-    constexpr bool SHARES = sizeof(typename M::share) == 2;
-    float top = SHARES ? 0x1p-126f : 1.f;
-    if (SHARES && w.rec >= 0) {
-#pragma unroll
-        for (int i = 0; i < SHARE; ++i)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) top = fabsf(out[i][c]) < INFINITY ? fmaxf(top, fabsf(out[i][c])) : top;
-        top = half_max(top);
-        if constexpr (WK > 1) {
-            if (h == 0) sh.top[wv][col] = top;
-            lds_barrier();
-#pragma unroll
-            for (int k = 0; k < WK; ++k) top = fmaxf(top, sh.top[k * WM + rw][col]);
-        }
-    }
     const int row2 = rw * 32 + (opaque(lane) & 31), tok2 = row2 / a.by_g;
     if (row2 < w.ntok * a.G && (w.rec >= 0 || w.tok0 + tok2 < a.rows)) {       // (records have room for every row of the plan)
         const int hh2 = row2 - tok2 * a.G;
@@ -609,14 +590,10 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 a.lse[(int64_t)(w.tok0 + tok2) * a.NH + head] = l == 0.f ? -INFINITY : LN2 * (m + log2f(l));
         } else {
             const int64_t rec = w.rec + row2;
-            const float share = SHARES ? 1.f / top : 1.f;
-            typedef typename M::share S;
-            typedef S S4 __attribute__((ext_vector_type(4)));
-            S *d0 = (S *)a.po + rec * HD + 4 * h + 8 * q0;
+            float *d0 = a.po + rec * HD + 4 * h + 8 * q0;
 #pragma unroll
-            for (int i = 0; i < SHARE; ++i)
-                *(S4 *)(d0 + 8 * i) = (S4){(S)(out[i][0] * share), (S)(out[i][1] * share), (S)(out[i][2] * share), (S)(out[i][3] * share)};
-            if (h == 0 && kw == 0) a.ml[rec] = (f32x4){m, l, top * vs, 0.f};
+            for (int i = 0; i < SHARE; ++i) *(f32x4 *)(d0 + 8 * i) = out[i];
+            if (h == 0 && kw == 0) a.ml[rec] = (f32x4){m, l, vs, 0.f};
         }
     }
 }
@@ -641,7 +618,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(AttnArgs a) {
 struct JoinArgs {
     const TokenRecs *toks;
     const int *n_toks;                // and behind it the most records of a token
-    const void *po;
+    const float *po;
     const f32x4 *ml;
     void *out;
     float *lse;
@@ -654,8 +631,6 @@ template <class T, int HD, int WAVES>
 __device__ __forceinline__ void join_heads(const JoinArgs &a) {
     constexpr int LPR = HD / 8, RPL = 64 / LPR, UNROLL = JOIN_UNROLL;  // lanes per record, records per load
     typedef float f32x8 __attribute__((ext_vector_type(8)));
-    typedef typename Mma<T>::share S;
-    typedef S S8 __attribute__((ext_vector_type(8)));
     __shared__ f32x8 sum_s[4][LPR];
     const int tok = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const int head = blockIdx.y * (4 / WAVES) + wv / WAVES, part = wv % WAVES;
@@ -673,12 +648,12 @@ __device__ __forceinline__ void join_heads(const JoinArgs &a) {
     f32x8 acc = {};
     for (int j0 = 0; j0 < n; j0 += 64) {
         const int cnt = min(64, n - j0);
-        S8 v[UNROLL];
+        f32x8 v[UNROLL];
         auto fetch = [&](int b) {
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 const int j = (b + u * WAVES) * RPL + sub;             // (past the last record: the last again, unused)
-                v[u] = *(const S8 *)((const S *)a.po + rec_of(j0 + min(j, cnt - 1)) * HD + li * 8);
+                v[u] = *(const f32x8 *)(a.po + rec_of(j0 + min(j, cnt - 1)) * HD + li * 8);
             }
         };
         fetch(part);
@@ -696,9 +671,9 @@ __device__ __forceinline__ void join_heads(const JoinArgs &a) {
             for (int u = 0; u < UNROLL; ++u) {
                 const int j = (b + u * WAVES) * RPL + sub;
                 const float fj = __shfl(share, min(j, 63));
-                const S8 x = j < cnt ? v[u] : (S8){};
+                const f32x8 x = j < cnt ? v[u] : (f32x8){};
 #pragma unroll
-                for (int c = 0; c < 8; ++c) acc[c] += (float)x[c] * fj;
+                for (int c = 0; c < 8; ++c) acc[c] += x[c] * fj;
             }
         }
     }

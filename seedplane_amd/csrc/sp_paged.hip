@@ -502,7 +502,7 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         a.scale = scale * LOG2E;
         const size_t recs = (size_t)records_bound(p->max_rows, p->NH);
         a.ml = (f32x4 *)workspace_dev;
-        a.po = a.ml + recs;
+        a.po = (float *)(a.ml + recs);
         const bool kv8 = kv->dtype == SP_DT_E4M3;
         a.items = (const Item *)(p->dev + p->item_at);
         a.list = p->dev + p->list_at;
