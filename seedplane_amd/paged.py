@@ -153,7 +153,7 @@ class Rotary:
     def __init__(self, head_dim, theta=10000.0, rot_dim=None, layout='half', scaling=None, length=None, device='cuda'):
         if layout not in ('half', 'interleaved'):
             raise ValueError("layout must be 'half' or 'interleaved'")
-        self.head_dim, self.rot_dim, self.layout = int(head_dim), int(rot_dim or head_dim), layout
+        self.head_dim, self.rot_dim, self.layout = int(head_dim), int(head_dim if rot_dim is None else rot_dim), layout
         if self.rot_dim > self.head_dim:
             raise ValueError('rot_dim exceeds head_dim')
         self.inv_freq, self.factor = rotary_frequencies(self.rot_dim, theta, scaling, length)
@@ -179,7 +179,8 @@ class Rotary:
         scaling = config.get('rope_scaling') or (p if p.get('rope_type', 'default') != 'default' else None)
         if scaling and not scaling.get('original_max_position_embeddings'):
             scaling = dict(scaling, original_max_position_embeddings=config.get('max_position_embeddings'))
-        rot = int(hd * (config.get('partial_rotary_factor') or p.get('partial_rotary_factor') or 1.0))
+        parts = [x for x in (config.get('partial_rotary_factor'), p.get('partial_rotary_factor'), 1.0) if x is not None]
+        rot = int(hd * parts[0])
         return cls(hd, config.get('rope_theta', p.get('rope_theta', 10000.0)), rot, layout, scaling, length, device)
 
     def apply(self, x, positions, out=None):
