@@ -42,8 +42,8 @@ def rotary_frequencies(rot_dim, theta=10000.0, scaling=None, length=None):
     j = torch.arange(0, rot_dim, 2, dtype=torch.float64)
     inv = 1.0 / theta ** (j / rot_dim)
     s = scaling or {}
-    kind = s.get('rope_type', s.get('type', 'default'))
-    if kind in ('default', None):
+    kind = s.get('rope_type') or s.get('type') or 'default'
+    if kind == 'default':
         return inv, 1.0
     if kind not in ('linear', 'dynamic', 'yarn', 'llama3'):
         raise ValueError(f'unknown rope scaling {kind!r}')
