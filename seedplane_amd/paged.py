@@ -47,8 +47,13 @@ def rotary_frequencies(rot_dim, theta=10000.0, scaling=None, length=None):
         return inv, 1.0
     if kind not in ('linear', 'dynamic', 'yarn', 'llama3'):
         raise ValueError(f'unknown rope scaling {kind!r}')
-    factor = float(s['factor'])
-    if factor < 1:
+
+    def value(key):
+        if s.get(key) is None:
+            raise ValueError(f'{kind} scaling needs {key}')
+        return float(s[key])
+    factor = value('factor')
+    if not 1 <= factor < math.inf:
         raise ValueError('the scaling factor must be at least 1')
     if kind == 'linear':
         return inv / factor, 1.0
@@ -63,7 +68,9 @@ def rotary_frequencies(rot_dim, theta=10000.0, scaling=None, length=None):
         return 1.0 / base ** (j / rot_dim), 1.0
     turns = original * inv / (2 * math.pi)                  # turns of each pair over the original length
     if kind == 'llama3':
-        low, high = float(s['low_freq_factor']), float(s['high_freq_factor'])
+        low, high = value('low_freq_factor'), value('high_freq_factor')
+        if not low < high:
+            raise ValueError('low_freq_factor must be less than high_freq_factor')
         keep = ((turns - low) / (high - low)).clamp(0, 1)   # 1: short waves, kept; 0: long ones, slowed by the factor
         return inv * (keep + (1 - keep) / factor), 1.0
     # YaRN: kept above beta_fast turns, slowed below beta_slow, a ramp over the pair's index between
