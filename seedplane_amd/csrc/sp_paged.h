@@ -63,7 +63,6 @@ struct AttnArgs {
     PageDivisor by_page;
     float scale;                      // of the scores, times log2(e)
     const Item *items;
-    const int *list;                  // tokens of the items that name theirs
     const int *n_items;               // NULL: one block per item
     // Records: [rows][HD] unnormalised outputs, and [rows] (m in log2 units, l, a factor of the outputs).  Sums stay in fp32: as
     // fp16 shares of a row's largest one (half the traffic; a decode step of 32 requests on 8192 shared positions 1.1 us of 23.5
@@ -194,7 +193,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     const int rt = row / a.by_g;
     int at = w.tok0 + rt;
     if (__builtin_expect(w.list >= 0, 0)) {
-        at = a.list[w.list + min(rt, w.ntok - 1)];
+        at = ((const int *)a.items)[w.list + min(rt, w.ntok - 1)];     // (the list lies behind the items)
         asm volatile("" : "+v"(at));                                   // (awaited here: behind the branch every item would wait for its entries)
     }
     const bool live = row < w.ntok * a.G && at < a.rows;

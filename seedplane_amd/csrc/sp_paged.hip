@@ -404,8 +404,12 @@ int sp_attn_plan_set(sp_attn_plan *p, int32_t n_seq, const int32_t *q_len, const
         p->set = false;                                  // until the tables are on their way
         // header and token records lie side by side: one copy; then the items, and the list where there is one
         std::memcpy(img + p->tok_at, t.toks.data(), t.toks.size() * sizeof(TokenRecs));
+        if (!t.list.empty()) {                           // (places from the first item on: the kernel has no pointer of its own for them)
+            for (Item &w : t.items)
+                if (w.list >= 0) w.list += (int32_t)(p->list_at - p->item_at);
+            std::copy(t.list.begin(), t.list.end(), img + p->list_at);
+        }
         std::memcpy(img + p->item_at, t.items.data(), t.items.size() * sizeof(Item));
-        std::copy(t.list.begin(), t.list.end(), img + p->list_at);
         HIPCHK(hipMemcpyAsync(p->dev, img, (HEADER + t.toks.size() * (sizeof(TokenRecs) / 4)) * 4, hipMemcpyHostToDevice, st));
         if (!t.items.empty())
             HIPCHK(hipMemcpyAsync(p->dev + p->item_at, img + p->item_at, t.items.size() * sizeof(Item), hipMemcpyHostToDevice, st));
@@ -505,7 +509,6 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         a.po = (float *)(a.ml + recs);
         const bool kv8 = kv->dtype == SP_DT_E4M3;
         a.items = (const Item *)(p->dev + p->item_at);
-        a.list = p->dev + p->list_at;
         a.n_items = capturing ? p->dev : nullptr;
         const int grid = capturing ? CAPTURED_GRID : p->n_items;
         if (grid) {
