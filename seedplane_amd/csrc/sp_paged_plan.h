@@ -36,11 +36,13 @@ constexpr int TILE_ROWS_OF[KINDS] = {32, 64, 128};
 constexpr int KEY_STEP = 64;                                   // parts are whole steps of keys
 // Cost of a step by kind: a tile of many rows is bound by its products and exponentials, one of few by memory, and how much
 // they take of each other depends on the batch.  Decode of 32 / 96 requests over 8192 / 16384 shared positions, bf16 / e4m3, costs of
-// 32 rows : more: 1 : 1 23.0 / 68.0 us, 2 : 3 23.4 / 62, 1 : 2 23.1 / 59.5, 2 : 5 24.5 / 60.4, 1 : 3 24.1 / 62.6.  And the fewest
-// steps of a part: shorter ones cost more in records and latency than they spread (9 drafted tokens of 12 sequences over 1531
-// positions: 16.3 us, with single steps 18.6).
+// 32 rows : more: 1 : 1 24.0 / 68.7 us, 2 : 3 23.7 / 62.2, 1 : 2 24.0 / 59.1, 2 : 5 25.3 / 61.3, 1 : 3 26.2 / 63.8.
 constexpr int STEP_COST[KINDS] = {1, 2, 2};
-constexpr int LEAST_STEPS[KINDS] = {2, 2, 2};
+// The fewest steps of a part: shorter ones cost more in records and latency than they spread.  Two (9 drafted tokens of 12 sequences
+// over 1531 positions: 16.4 us, by one 18.5, by three 17.0); three where two would leave a row more than 32 records and the tile
+// has rows enough for their traffic to count (4, 8, 16 requests of 7 heads on 8192: 12.8, 15.2, 20.1 -> 11.5, 14.1, 18.1 us; 16 on 6000
+// 17.4 -> 16.6, on 4032 15.4 -> 15.3, on 3000 14.4 -> 14.8; a lone token's 7 rows on 8000 9.3 -> 10.3).
+inline int64_t least_steps(int64_t steps, int64_t rows) { return steps > 64 && rows > 16 ? 3 : 2; }
 constexpr int MAX_GROUP = 32;                                  // query heads per K/V head
 
 // Tiles without shared positions up to this many values a row (positions x head_dim) are not cut: their items write the outputs, and
@@ -62,7 +64,7 @@ struct PlanTables {
 };
 
 // A part has the ITEM_TARGET-th of the whole cost: two blocks on each of 256 CUs get about the same; shorter tiles fill in (the
-// two batches above: 512 23.1 / 59.5 us, 576 26.9 / 62.8, 1024 33.4 / 65.4).
+// two batches above: 448 23.9 / 64.8 us, 512 24.0 / 59.1, 576 26.8 / 63.8, 1024 34.8 / 68.0).
 constexpr int ITEM_TARGET = 512;
 // Most rows of records: a tile that is not cut leaves one record per row and range; the parts of those that are, each of more
 // than one part's cost, are fewer than 2 ITEM_TARGET.
@@ -135,7 +137,7 @@ inline void make_plan(int n_heads, int n_kv, int head_dim, int n_seq, const int3
     for (const Segment &s : segs) whole &= s.which == 1 && steps_of(s) * KEY_STEP * head_dim <= UNCUT_VALUES;
     auto parts_of = [&](const Segment &s) {
         if (whole) return (int64_t)1;
-        const int64_t len = std::max<int64_t>(LEAST_STEPS[s.kind], (share + STEP_COST[s.kind] - 1) / STEP_COST[s.kind]);
+        const int64_t len = std::max<int64_t>(least_steps(steps_of(s), (int64_t)s.ntok * G), (share + STEP_COST[s.kind] - 1) / STEP_COST[s.kind]);
         return std::max<int64_t>(1, (steps_of(s) + len / 2) / len);        // (half a part more costs less than a cut)
     };
     for (const Segment &s : segs)
