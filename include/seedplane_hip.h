@@ -448,8 +448,9 @@ void sp_attn_plan_destroy(sp_attn_plan *plan);
  * of a K/V head over tokens) for all of the group's sequences whose queries do not fill such tiles by themselves, through the
  * table of the first of these, as far as the earliest of their queries stands behind them; a sequence that fills its tiles (an
  * eighth empty at most) reads them with its own positions.  The order of a group's sequences does not matter, and sequences
- * without queries change nothing.  The tables are copied to the device on hip_stream: later sp_op_paged_attention calls must
- * follow on it.  SP_ESTATE in a stream capture; a captured sp_op_paged_attention reads the tables of the last set before each
+ * without queries change nothing.  The tables are copied to the device on hip_stream, over those of the set before: later
+ * sp_op_paged_attention calls must follow on it, and calls on other streams that read the tables before it (replays of graphs
+ * too) must have ended.  SP_ESTATE in a stream capture; a captured sp_op_paged_attention reads the tables of the last set before each
  * replay. */
 int sp_attn_plan_set(sp_attn_plan *plan, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len, int32_t n_groups,
                      const int32_t *group_size, const int32_t *group_shared, void *hip_stream);

@@ -15,13 +15,14 @@
 // many.  Scores, maxima, sums and outputs are fp32, in the records of parts too; P is rounded to the queries' type, which its
 // product with V takes on the matrix cores (half a step of each weight).
 //
-// What bounds it.  Few rows: memory; 64 sequences x 4096 positions, 28 / 4 heads of 128 in bf16, 537 MB: 101 us, 5.3 TB/s, the rate of
-// a large copy (e4m3 50 us).  Many rows: the products and the other vector instructions, which two waves of a SIMD hardly
-// overlap; 128 tiles of 126 rows x 4 heads on the same 4096 positions: 178 us, 760 TFLOP/s, 53 % of a large library product, the matrix
-// cores 49 % and the rest of the vector unit 52 % of the waves' time, either busy 88 %.  (One exponential, scaling, sum
-// and half a rounding per score against a product's 4 HD operations; LDS is used 24 % of the time, without conflicts.  Tried: four tiles
-// deep with 32 keys, sums of rounded weights by dot products, priorities, and blocks of 8 waves whose halves take turns
-// multiplying and weighing: 188 us.)
+// What bounds it.  Few rows: memory; 64 sequences x 4096 positions, 28 / 4 heads of 128 in bf16, 537 MB: 102 us, 5.3 TB/s, the rate of
+// a large copy (e4m3 50 us).  Many rows: the products and the other vector instructions, of which little runs at once; 128 tiles of
+// 126 rows x 4 heads on the same 4096 positions: 166 us, 813 TFLOP/s, 57 % of a large library product, the matrix cores busy 49 % and
+// the vector unit's issue 50 % of the waves' time, both at once 12 %.  Part of that is the order within a wave: the first 32 keys'
+// exponentials and the tile's maxima have no product beside them, only the second 32 keys' exponentials do.  (Per score one
+// exponential, scaling, sum, comparison and half a rounding against a product's 4 HD operations; LDS is used 24 % of the time, without
+// conflicts.  Tried, when this batch took 178 us: four tiles deep with 32 keys 243, sums of rounded weights by dot products 181,
+// priorities 172 to 182, blocks of 8 waves whose halves take turns multiplying and weighing 188.)
 #pragma once
 #include "sp_paged_plan.h"
 #include "sp_rotate.h"

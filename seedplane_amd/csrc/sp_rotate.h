@@ -9,7 +9,9 @@
 //
 // Both kernels are bound by memory for long inputs and by the chain position -> angle -> store for short ones: 2048 rows x 32
 // heads of 128 in bf16 rotate in 8.3 us (33.6 MB, 4.0 TB/s), 2048 rows of 28 + 4 + 4 heads are appended in 11.0 us (37.7 MB, 3.4 TB/s),
-// and steps of 16 rows take 2.7 and 3.9 us, where an empty launch takes 2.3 (a copy of 1 GiB: 5.1 TB/s).  A block
+// and steps of 16 rows take 2.7 and 3.9 us, where an empty launch takes 2.3 (a copy of 1 GiB: 5.1 TB/s).  A row of more units than a
+// block has threads (the 320 of 28 + 4 + 4 heads of 128) takes a second round, whose loads are issued behind the first's stores, for
+// few threads' work; blocks of up to 512 threads in equal rounds took 11.9 us a call instead of 11.1.  A block
 // takes whole rows: its threads load their values, then form the rows' (cos, sin) table in LDS, each pair once for all heads
 // (a thread per pair and head would spend more on angles than on memory), then rotate and store.
 #pragma once

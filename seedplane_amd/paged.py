@@ -324,6 +324,7 @@ class AttentionPlan:
 
     def set(self, q_lens, kv_lens, groups=None):
         """The next batch (host integers): sequence s has q_lens[s] query tokens, the last of its kv_lens[s] cached positions.
+        The tables replace those of the set before: runs on other streams that read them must have ended (or be waited for).
         groups: (sequences, shared positions) of each run of sequences whose tables name the same pages for their first positions,
         in any order and with idle ones (q_lens 0) among them; None: nothing is shared."""
         q, kv = _lengths(q_lens, 'q_lens'), _lengths(kv_lens, 'kv_lens')

@@ -367,7 +367,8 @@ class Qwen2Engine:
         shared prefix of paged attention without a copy.  It keeps the engine alive.  When the pool is reserved or grown again
         (which new_cache and generate_batch do by themselves where it is too small) its memory moves: append() and run()
         refuse the older PagedKV from then on, with a ValueError, and a program calls paged_kv() and page_table() again.  Its
-        `k` and `v`, and graphs that were captured over it, must not be used any more then."""
+        `k` and `v`, and graphs that were captured over it, must not be used any more then.  (The new pool has each live cache's
+        `length` positions: tokens that append() put behind them count once the program has set it.)"""
         from .paged import PagedKV
         k, v = self._kv_pool(range(self.n_layers)[layer])
         n, nkv, S, hd = k.shape
