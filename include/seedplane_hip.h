@@ -450,15 +450,15 @@ void sp_attn_plan_destroy(sp_attn_plan *plan);
  * eighth empty at most) reads them with its own positions.  The order of a group's sequences does not matter, and sequences
  * without queries change nothing.  The tables are copied to the device on hip_stream, over those of the set before: later
  * sp_op_paged_attention calls must follow on it, and calls on other streams that read the tables before it (replays of graphs
- * too) must have ended.  SP_ESTATE in a stream capture; a captured sp_op_paged_attention reads the tables of the last set before each
- * replay. */
+ * too) must have ended.  SP_ESTATE in a stream capture; a captured sp_op_paged_attention reads the tables of the last set
+ * before each replay. */
 int sp_attn_plan_set(sp_attn_plan *plan, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len, int32_t n_groups,
                      const int32_t *group_size, const int32_t *group_shared, void *hip_stream);
 /* Host only, for inspection: the items that sp_attn_plan_set makes of these lengths, as 12 int32 each: first token, tokens, K/V
  * head, sequence, first position, end, position seen by the first token (2^30: all), first record or -1, kind (row tile of
  * 32 << kind rows), -1 or (shared positions of tokens that are no range: from the first on those with records of shared
- * positions) a place in the plan's list, two reserved; and per token 8 int32: base, parts, tile and index of its records of the shared and of its own
- * positions (pairs).  items and token_recs may be NULL. */
+ * positions) a place in the plan's list, two reserved; and per token 8 int32: base, parts, tile and index of its records of the
+ * shared and of its own positions (pairs).  items and token_recs may be NULL. */
 int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t n_seq, const int32_t *q_len, const int32_t *kv_len,
                        int32_t n_groups, const int32_t *group_size, const int32_t *group_shared, int32_t capacity,
                        int32_t *items, int32_t *n_items, int32_t *token_recs, int64_t *n_records);

@@ -194,7 +194,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     const int rt = row / a.by_g;
     int at = w.tok0 + rt;
     if (__builtin_expect(w.list >= 0, 0)) {
-        at = ((const int *)a.items)[w.list + min(rt, w.ntok - 1)];     // (the list lies behind the items)
+        at = ((const int *)a.items)[-1 - (w.list + min(rt, w.ntok - 1))];      // (the list lies before the items, backwards)
         asm volatile("" : "+v"(at));                                   // (awaited here: behind the branch every item would wait for its entries)
     }
     const bool live = row < w.ntok * a.G && at < a.rows;

@@ -137,9 +137,10 @@ void check_cache(const sp_paged_kv *kv) {
 
 struct sp_attn_plan {
     int NH = 0, NKV = 0, HD = 0, max_rows = 0, max_seqs = 0, device = 0;
-    // device block: header [16] (items, tokens, most records of a token), token records, items and token list, at fixed places
+    // device block: header [16] (items, tokens, most records of a token) and token records; then, at item_at, the items, and backwards
+    // from there the list of tokens that are no range
     int32_t *dev = nullptr;
-    size_t tok_at = 0, item_at = 0, list_at = 0, words = 0;
+    size_t tok_at = 0, item_at = 0, words = 0;
     int32_t *staging[2] = {};            // pinned images of the block, used in turn
     hipEvent_t copied[2] = {};
     bool used[2] = {};
@@ -164,9 +165,8 @@ constexpr size_t HEADER = 16;
 // The plan's shape and where its tables lie (words).
 void lay_out(sp_attn_plan &p) {
     p.tok_at = HEADER;
-    p.item_at = p.tok_at + (size_t)p.max_rows * (sizeof(TokenRecs) / 4);
-    p.list_at = p.item_at + (size_t)items_bound(p.max_rows, p.NKV) * (sizeof(Item) / 4);
-    p.words = p.list_at + (size_t)p.max_rows;
+    p.item_at = (p.tok_at + (size_t)p.max_rows * (sizeof(TokenRecs) / 4 + 1) + 15) / 16 * 16;
+    p.words = p.item_at + (size_t)items_bound(p.max_rows, p.NKV) * (sizeof(Item) / 4);
 }
 
 void check_shape(int NH, int NKV, int HD, int max_rows, int max_seqs) {
@@ -402,19 +402,16 @@ int sp_attn_plan_set(sp_attn_plan *p, int32_t n_seq, const int32_t *q_len, const
         img[1] = (int32_t)t.toks.size();
         img[2] = t.most_parts;
         p->set = false;                                  // until the tables are on their way
-        // header and token records lie side by side: one copy; then the items, and the list where there is one
+        // header and token records lie side by side: one copy; then the list and the items
         std::memcpy(img + p->tok_at, t.toks.data(), t.toks.size() * sizeof(TokenRecs));
-        if (!t.list.empty()) {                           // (places from the first item on: the kernel has no pointer of its own for them)
-            for (Item &w : t.items)
-                if (w.list >= 0) w.list += (int32_t)(p->list_at - p->item_at);
-            std::copy(t.list.begin(), t.list.end(), img + p->list_at);
-        }
+        // (the list ends where the items begin: the kernel has no pointer of its own for it)
+        const size_t list_at = p->item_at - t.list.size();
+        std::reverse_copy(t.list.begin(), t.list.end(), img + list_at);
         std::memcpy(img + p->item_at, t.items.data(), t.items.size() * sizeof(Item));
         HIPCHK(hipMemcpyAsync(p->dev, img, (HEADER + t.toks.size() * (sizeof(TokenRecs) / 4)) * 4, hipMemcpyHostToDevice, st));
         if (!t.items.empty())
-            HIPCHK(hipMemcpyAsync(p->dev + p->item_at, img + p->item_at, t.items.size() * sizeof(Item), hipMemcpyHostToDevice, st));
-        if (!t.list.empty())
-            HIPCHK(hipMemcpyAsync(p->dev + p->list_at, img + p->list_at, t.list.size() * 4, hipMemcpyHostToDevice, st));
+            HIPCHK(hipMemcpyAsync(p->dev + list_at, img + list_at, t.list.size() * 4 + t.items.size() * sizeof(Item),
+                                  hipMemcpyHostToDevice, st));
         HIPCHK(hipEventRecord(p->copied[turn], st));
         p->used[turn] = true;
         p->turn = turn ^ 1;

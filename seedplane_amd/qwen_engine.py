@@ -349,7 +349,8 @@ class Qwen2Engine:
 
     def _kv_pool(self, layer):
         """Layer `layer`'s K and V pools as fp16 [n_seq, kv_heads, n_slots, head_dim] tensors sharing the engine's
-        memory.  Internal: valid only until the pool is reserved or grown again, so callers drop them at once."""
+        memory.  Internal: valid only until the pool is reserved or grown again, so callers drop them at once or note the
+        pool's number (paged_kv)."""
         k, v = ctypes.c_void_p(), ctypes.c_void_p()
         _lib.check(self.lib.sp_engine_kv_layer(self.h, layer, ctypes.byref(k), ctypes.byref(v)), self.h)
         shape = (self._pool_n, self.n_kv_heads, self._pool_slots, self.head_dim)
