@@ -389,7 +389,7 @@ int sp_op_draft_link(const int32_t *tokens_dev, int32_t n_branches, int32_t leve
  * cache copy (qwen_engine.py:121-125), sp_op_paged_attention its attention (qwen_engine.py:126-135).
  * Strides are in elements of their array.  All calls are asynchronous on hip_stream, allocate nothing, keep no state (the plan
  * is the caller's) and may be captured into a graph. */
-enum { SP_DT_F32 = 0, SP_DT_F16 = 1, SP_DT_BF16 = 2, SP_DT_E4M3 = 3 /* OCP e4m3, no infinities, largest 448 */ };
+enum { SP_DT_F32 = 0, SP_DT_F16 = 1, SP_DT_BF16 = 2, SP_DT_E4M3 = 3 /* OCP e4m3, no infinities, largest 448 */, SP_DT_I8 = 4 };
 enum { SP_ROPE_HALF = 0 /* pairs (j, j + rot_dim/2) */, SP_ROPE_INTERLEAVED = 1 /* pairs (2j, 2j + 1) */ };
 
 typedef struct sp_rotary {
@@ -410,14 +410,16 @@ int sp_op_rotate(const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t
 /* One layer's paged cache: row r of head h of page e starts at e * page_stride + h * head_stride + r * row_stride elements, the
  * same for keys and values ([pages][heads][rows], [pages][rows][heads], one allocation for both, ...; rows that tables name
  * must not lie on top of each other).  A sequence's position p lies in row p % page_size of page table[seq][p / page_size].
- * e4m3 caches hold value / scale with a positive fp32 scale per K/V head, for keys and for values. */
+ * e4m3 caches hold value / scale with a positive fp32 scale per K/V head, for keys and for values; with scale_block they and
+ * int8 caches (whole numbers up to 127) hold value / scale with a scale of each run of scale_block positions of a page and head, which
+ * sp_op_paged_append writes: within 2^-60 .. 2^60 (0, of memory that was cleared and never appended to, counts as 2^-60). */
 typedef struct sp_paged_kv {
     void *k_dev, *v_dev;
-    const float *k_scale_dev, *v_scale_dev;   /* device [n_kv_heads], SP_DT_E4M3 only (NULL otherwise) */
+    float *k_scale_dev, *v_scale_dev;         /* device [n_kv_heads], or [n_pages][n_kv_heads][page_size / scale_block]; NULL for 16 bits */
     int64_t page_stride, head_stride, row_stride;
-    int32_t dtype;                            /* SP_DT_F16, SP_DT_BF16 or SP_DT_E4M3 */
+    int32_t dtype;                            /* SP_DT_F16, SP_DT_BF16, SP_DT_E4M3, or SP_DT_I8 (with scale_block) */
     int32_t n_pages, page_size, n_kv_heads, head_dim;
-    int32_t reserved0;
+    int32_t scale_block;                      /* 0, or a multiple of 16 up to 128 that divides page_size */
 } sp_paged_kv;
 
 /* Appends n_rows new tokens: row r's keys (rotated at pos_dev[r] unless rotary is NULL) and values go to position at_dev[r] of
@@ -426,12 +428,26 @@ typedef struct sp_paged_kv {
  * [n_seq][max_pages].  A row whose seq, position or page entry is out of range (e.g. seq -1: padding) writes nothing, not its
  * queries either.  dtype: of q, k and v (F32, F16 or BF16).  Values too large for an e4m3 cache saturate at 448 scales, NaN
  * stays NaN.  Two rows of one call must not name the same place (nor two positions share a page that the call writes): whose
- * values it then holds is not defined. */
+ * values it then holds is not defined.
+ * With scale_block a block's scale becomes the largest magnitude of a head's new values in it over the largest code (127 or 448), at
+ * least the scale that it has; where it grows, the codes that the call does not write are rounded once more, by old / new scale.  A
+ * block whose first position is among the rows begins anew: its scale is that of the new values alone, and what it held at other
+ * positions is lost.  The rows of a block may stand anywhere in the call; of two rows for the same place the later one
+ * alone counts.
+ * Magnitudes above 2^60 codes saturate; a NaN makes an int8 block's scale NaN until it begins anew, e4m3 keeps it to its place.
+ * Here scale_block * rot_dim is at most 16384 and scale_block * head_dim below 65536. */
 int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t n_heads,
                        const void *q_dev, int64_t q_row, int64_t q_head, const void *k_dev, int64_t k_row, int64_t k_head,
                        const void *v_dev, int64_t v_row, int64_t v_head, const int32_t *pos_dev, const int32_t *seq_dev,
                        const int32_t *at_dev, const int32_t *table_dev, int32_t n_seq, int32_t max_pages, void *q_out_dev,
                        int32_t q_out_dtype, int64_t q_out_row, int64_t q_out_head, void *hip_stream);
+
+/* Positions of a cache of any dtype as dense values: row r of k_out and v_out (dtype F32, F16 or BF16; not over the cache) gets the
+ * keys and values at position at_dev[r] of sequence seq_dev[r] (code * scale in fp32, rounded once), zeros where seq, position or
+ * page entry is out of range.  Rows may repeat. */
+int sp_op_paged_read(const sp_paged_kv *kv, int32_t dtype, int32_t n_rows, const int32_t *seq_dev, const int32_t *at_dev,
+                     const int32_t *table_dev, int32_t n_seq, int32_t max_pages, void *k_out_dev, int64_t k_row, int64_t k_head,
+                     void *v_out_dev, int64_t v_row, int64_t v_head, void *hip_stream);
 
 /* The plan of a batch's attention, kept by the caller over the layers of a step: which block reads which keys for which
  * queries.  max_rows: most query rows (tokens) of a batch, max_seqs: most sequences.  head_dim 64 or 128, at most 32 query
@@ -466,13 +482,14 @@ int sp_attn_plan_items(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, in
 size_t sp_attn_plan_workspace(const sp_attn_plan *plan);
 
 /* out = softmax(scale q k^T) v over the positions each query sees, for the batch of the plan's last set.  q and out: n_rows
- * rows of the plan's n_heads heads, dtype SP_DT_F16 or SP_DT_BF16 (a cache of the same type, or e4m3), 16 / 8 byte aligned rows
+ * rows of the plan's n_heads heads, dtype SP_DT_F16 or SP_DT_BF16 (a cache of the same type, or of 8 bits), 16 / 8 byte aligned rows
  * and heads; rows behind the plan's last are left as they are.  lse_dev (may be NULL): fp32 [n_rows][n_heads], the natural
  * logarithm of each row's sum of exponentials (-infinity for a row that sees nothing).  table_dev: int32 [n_seq][max_pages];
  * entries of positions at or behind a sequence's length are not read, an entry outside [0, n_pages) hides its positions.  What
  * the pool holds outside the positions read does not matter (NaN included), and an infinite or NaN value of a position reaches
  * only the rows that see it and its own place in them.  Scores, weights' sums and weighted sums of values are held in fp32, over
- * parts of a range too; a weight is rounded to dtype for its product with the values.  scale must be positive.  workspace_dev:
+ * parts of a range too; a weight (with scale_block: times its values' scale, over the row's largest such product) is rounded to dtype
+ * for its product with the values.  scale must be positive.  workspace_dev:
  * see above; calls that overlap (other streams, graphs replayed side by side) need a workspace each.  The cache's strides are
  * multiples of head_dim here.  A captured call keeps its own n_rows, n_seq and max_pages: what a later set has beyond them is not
  * read or written; within them its outputs have the bits of an uncaptured call with the same lengths. */

@@ -19,7 +19,7 @@ SP_FMT_F32, SP_FMT_F16, SP_FMT_Q8, SP_FMT_Q4 = range(4)
  SP_T_GATE_UP, SP_T_DOWN) = range(10)
 SP_F_LOGITS, SP_F_ARGMAX, SP_F_GRAPH, SP_F_PERSISTENT, SP_F_UNFUSED, SP_F_FEED, SP_F_CHAIN = 1, 2, 4, 8, 16, 32, 64
 SP_F_DEVCOLS = 128
-SP_DT_F32, SP_DT_F16, SP_DT_BF16, SP_DT_E4M3 = range(4)
+SP_DT_F32, SP_DT_F16, SP_DT_BF16, SP_DT_E4M3, SP_DT_I8 = range(5)
 SP_ROPE_HALF, SP_ROPE_INTERLEAVED = 0, 1
 
 # Every function the header declares, with its ctypes signature.
@@ -51,7 +51,7 @@ class PagedKVDesc(ctypes.Structure):
     _fields_ = [('k', c_void_p), ('v', c_void_p), ('k_scale', c_void_p), ('v_scale', c_void_p), ('page_stride', c_int64),
                 ('head_stride', c_int64), ('row_stride', c_int64),
                 ('dtype', c_int32), ('n_pages', c_int32), ('page_size', c_int32), ('n_kv_heads', c_int32), ('head_dim', c_int32),
-                ('reserved0', c_int32)]
+                ('scale_block', c_int32)]
 
 
 # the same layout as a numpy structured dtype (columns built in bulk)
@@ -118,6 +118,8 @@ SIGNATURES = {
     'sp_op_paged_append': (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int64,
                                    c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
                                    c_void_p, c_int32, c_int64, c_int64, c_void_p]),
+    'sp_op_paged_read': (c_int, [c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_int64,
+                                 c_void_p, c_int64, c_int64, c_void_p]),
     'sp_attn_plan_create': (c_int, [c_int32, c_int32, c_int32, c_int32, c_int32, ctypes.POINTER(c_void_p)]),
     'sp_attn_plan_destroy': (None, [c_void_p]),
     'sp_attn_plan_set': (c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),

@@ -1,0 +1,267 @@
+// A paged cache of 8-bit codes with a scale for each block of positions and K/V head: appending to it, and reading positions back.
+//
+// A block is `block` positions of a page (a multiple of 16 that divides the page); a value is code * scale of its block and head.  Codes
+// are int8 (whole numbers up to 127) or e4m3 (up to 448).  A call finds the rows that it brings to a block, whatever their order, and
+// takes scale = max |x| / largest code over them.  A block whose first position is among them begins anew; any other keeps what it
+// holds, its scale only grows, and where it does the codes that the call does not write are rounded once more, by old / new scale.
+//
+// A workgroup takes a chunk of rows of the call (a row whose block an earlier row has is left to that row's workgroup), keys or
+// values, and some heads: it looks up its block's rows among all of the call's, takes the largest magnitude per head, then the codes.
+// Values are read twice rather than kept: a block of 64 positions of one head alone is 8192 values.
+#pragma once
+#include "sp_paged.h"
+
+namespace paged {
+
+constexpr int MOST_BLOCK = 128;                                        // positions of a block at most
+constexpr int BLOCK_HEADS = 64;                                        // heads of a workgroup at most
+constexpr float MOST_SCALE = 0x1p60f;                                  // (scales within 2^-60 .. 2^60: attention takes their products)
+
+struct BlockAppendArgs : AppendArgs {                                  // ks, vs are not used; units, tail, vecs are a head's
+    float *kscale, *vscale;                                            // [n_pages][nkv][per_page]
+    int block, per_page;
+    PageDivisor by_block, by_page;
+    int chunk, chunks, splits, heads;                                  // rows of a workgroup, their number; workgroups over heads, heads of each
+    Divisor by_key, by_value;                                          // vectors of a slot: keys (pairs of them where rotated), values
+    uint32_t angles_at;                                                // LDS bytes before the angles [block][rot / 2]
+};
+struct ReadArgs {
+    const void *kc, *vc;
+    void *k_out, *v_out;
+    int64_t k_row, k_head, v_row, v_head;
+    const float *ks, *vs;                                              // scales per head, per block, or NULL
+    const int *seq, *at, *table;
+    int rows, nkv, kv_dt, per_block, vecs, per_row;
+    int n_seq, max_pages, n_pages, page_size, block, per_page;         // block 0: scales per head
+    int64_t page_stride, head_stride, row_stride;
+    Divisor by_row, by_vecs;
+};
+
+__attribute__((visibility("hidden"))) void launch_block_items(int dtype, int kv_dtype, int HD, const BlockArgs &a, int grid, hipStream_t st);
+__attribute__((visibility("hidden"))) void launch_block_append(int dtype, bool wide, const BlockAppendArgs &a, int query_blocks, size_t lds, hipStream_t st);
+__attribute__((visibility("hidden"))) void launch_read(int dtype, bool wide, const ReadArgs &a, hipStream_t st);
+
+// ------------------------------------------------------------------------------------------------ codes
+// N fp32 values (already over their scale) as codes of kind I8 or e4m3, and codes as fp32.
+template <bool I8, int N>
+__device__ __forceinline__ void store_codes(uint8_t *p, const float *v) {
+    if constexpr (!I8) {
+        store_values<N>(p, 0, SP_DT_E4M3, v);
+    } else {
+        int c[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = (int)rintf(fminf(fmaxf(v[i], -127.f), 127.f));
+        if constexpr (N == 1) p[0] = (uint8_t)c[0];
+        else {
+            u32x2 w;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                w[i] = (c[4 * i] & 0xff) | (c[4 * i + 1] & 0xff) << 8 | (c[4 * i + 2] & 0xff) << 16 | (uint32_t)c[4 * i + 3] << 24;
+            *(u32x2 *)p = w;
+        }
+    }
+}
+__device__ __forceinline__ float e4m3_value(uint32_t code) { return __builtin_amdgcn_cvt_f32_fp8(code, 0); }
+template <bool I8, int N>
+__device__ __forceinline__ void load_codes(const uint8_t *p, float *v) {
+    if constexpr (N == 1) {
+        v[0] = I8 ? (float)(int8_t)p[0] : e4m3_value(p[0]);
+    } else {
+        const u32x2 w = *(const u32x2 *)p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t c = w[i / 4] >> (8 * (i % 4));
+            v[i] = I8 ? (float)(int8_t)c : e4m3_value(c & 0xff);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ append
+struct BlockShared {
+    int slot[MOST_BLOCK];                                              // the row that brings each position of the block (the last one), -1
+    uint32_t most[BLOCK_HEADS];                                        // bits of the largest magnitude
+    float scale[BLOCK_HEADS], keep[BLOCK_HEADS];                       // 1 / new scale; old / new (1: codes stay)
+    int earlier;
+};
+
+// The largest magnitude of N values, as bits: a NaN is above all (int8), or left out (e4m3, which holds it as itself).
+template <bool I8, int N>
+__device__ __forceinline__ uint32_t magnitude(const float *v, uint32_t most) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+        most = I8 || b <= 0x7f800000u ? max(most, b) : most;
+    }
+    return most;
+}
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    return v;
+}
+
+template <class T, int VEC, bool I8>
+__device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, bool keys, int head0, BlockShared &sh, float2 *cs) {
+    const int tid = threadIdx.x, s = a.seq[r], p = a.at[r];
+    if (s < 0 || s >= a.n_seq || p < 0 || p >= (1 << 30)) return;
+    const int b = p / a.by_block, page = p / a.by_page;
+    auto same = [&](int i) { const int q = a.at[i]; return a.seq[i] == s && q >= 0 && q < (1 << 30) && q / a.by_block == b; };
+    if (page >= a.max_pages || (r > 0 && same(r - 1))) return;
+    const int e = a.table[(int64_t)s * a.max_pages + page];
+    if (e < 0 || e >= a.n_pages) return;
+    __syncthreads();                                                   // the block before has been written
+    for (int i = tid; i < a.block; i += blockDim.x) sh.slot[i] = -1;
+    if (tid < a.heads) sh.most[tid] = 0;
+    if (tid == 0) sh.earlier = 0;
+    __syncthreads();
+    for (int i = tid; i < a.rows; i += blockDim.x) {
+        if (!same(i)) continue;
+        if (i < r) sh.earlier = 1;
+        else atomicMax(&sh.slot[a.at[i] - b * a.block], i);
+    }
+    __syncthreads();
+    if (sh.earlier) return;
+    const int heads = min(a.heads, a.nkv - head0), half = a.rot.rot >> 1;
+    const int64_t block_of_page = b - (int64_t)page * a.per_page;
+    float *const scale = (keys ? a.kscale : a.vscale) + ((int64_t)e * a.nkv + head0) * a.per_page + block_of_page;      // of head h: at h * per_page
+    const float old = tid < heads ? scale[(int64_t)tid * a.per_page] : 0.f;
+    const bool begun = sh.slot[0] >= 0;
+    if (keys && half) {
+        for (int k = tid; k < a.block * half; k += blockDim.x) {
+            const int i = k / a.by_half, row = sh.slot[i];
+            if (row >= 0) cs[k] = turn_of(a.rot, a.pos[row], k - i * half);
+        }
+        __syncthreads();
+    }
+    // item i: slot and vector of it (keys: a rotated pair of vectors, or one of the rest)
+    const Divisor by = keys ? a.by_key : a.by_value;
+    const int per = keys ? a.units + a.tail : a.vecs, total = a.block * per;
+    uint8_t *const pool = (uint8_t *)(keys ? a.kc : a.vc) + e * a.page_stride + head0 * a.head_stride +
+                          (int64_t)(p - page * a.page_size - (p - b * a.block)) * a.row_stride;
+    auto offsets = [&](int u, int &at1, int &at2) -> bool {
+        if (keys && u < a.units) { unit_offsets<VEC>(a.rot, u, at1, at2); return true; }
+        at1 = at2 = keys ? a.rot.rot + (u - a.units) * VEC : u * VEC;
+        return false;
+    };
+    auto fetch = [&](int row, int h, int i, int u, int at1, int at2, bool two, float *v1, float *v2) {
+        const T *src = keys ? (const T *)a.k + (int64_t)row * a.k_row + (int64_t)(head0 + h) * a.k_head
+                            : (const T *)a.v + (int64_t)row * a.v_row + (int64_t)(head0 + h) * a.v_head;
+        load_values<T, VEC>(src + at1, v1);
+        load_values<T, VEC>(src + at2, v2);
+        if (two) turn_unit<VEC>(a.rot, cs + i * half + u * VEC, v1, v2);
+    };
+    float v1[VEC], v2[VEC];
+    for (int k0 = 0; k0 < total; k0 += blockDim.x) {
+        const int k = min(k0 + tid, total - 1), i = k / by, u = k - i * per, row = sh.slot[i];
+        int at1, at2;
+        const bool two = offsets(u, at1, at2);
+        for (int h = 0; h < heads; ++h) {
+            uint32_t most = 0;
+            if (row >= 0) {
+                fetch(row, h, i, u, at1, at2, two, v1, v2);
+                most = magnitude<I8, VEC>(v2, magnitude<I8, VEC>(v1, 0));
+            }
+            most = wave_umax(most);
+            if ((tid & 63) == 0 && most) atomicMax(&sh.most[h], most);
+        }
+    }
+    __syncthreads();
+    if (tid < heads) {
+        const float most = __uint_as_float(sh.most[tid]);
+        const float made = most > MOST_SCALE * (I8 ? 127.f : 448.f) ? MOST_SCALE : most * (I8 ? 1.f / 127.f : 1.f / 448.f);
+        // (comparisons that leave a NaN where it is: of int8's new values, or held since the block began)
+        float grown = made < LEAST_SCALE ? LEAST_SCALE : made;
+        if (!begun && !(old <= grown)) grown = grown != grown ? grown : old;
+        sh.scale[tid] = 1.f / grown;
+        sh.keep[tid] = begun || grown == old ? 1.f : old / grown;
+        scale[(int64_t)tid * a.per_page] = grown;
+    }
+    __syncthreads();
+    for (int k = tid; k < total; k += blockDim.x) {
+        const int i = k / by, u = k - i * per, row = sh.slot[i];
+        int at1, at2;
+        const bool two = offsets(u, at1, at2);
+        for (int h = 0; h < heads; ++h) {
+            uint8_t *const to = pool + h * a.head_stride + i * a.row_stride;
+            const float f = row >= 0 ? sh.scale[h] : sh.keep[h];
+            if (row >= 0) {
+                fetch(row, h, i, u, at1, at2, two, v1, v2);
+            } else {
+                if (f == 1.f) continue;
+                load_codes<I8, VEC>(to + at1, v1);
+                load_codes<I8, VEC>(to + at2, v2);
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) { v1[j] *= f; v2[j] *= f; }
+            store_codes<I8, VEC>(to + at1, v1);
+            if (two) store_codes<I8, VEC>(to + at2, v2);
+        }
+    }
+}
+
+// Blocks: chunks x (keys, values) x splits of the heads, then the queries' rows.
+template <class T, int VEC, bool I8>
+__global__ void __launch_bounds__(ROT_THREADS) k_append_blocks(BlockAppendArgs a) {
+    extern __shared__ __align__(16) unsigned char block_smem[];
+    __shared__ BlockShared sh;
+    const int parts = 2 * a.splits, n = a.chunks * parts;
+    if ((int)blockIdx.x >= n) {
+        append_rows<T, VEC>(a, blockIdx.x - n, block_smem);
+        return;
+    }
+    const int chunk = blockIdx.x / parts, part = blockIdx.x - chunk * parts;
+    const int r0 = chunk * a.chunk, r1 = min(r0 + a.chunk, a.rows);
+    for (int r = r0; r < r1; ++r) append_block<T, VEC, I8>(a, r, part < a.splits, part % a.splits * a.heads, sh, (float2 *)block_smem);
+}
+
+// ------------------------------------------------------------------------------------------------ read
+// Rows of a cache as dense values: row r's keys and values at position at[r] of sequence seq[r]; zeros where it has no place.
+template <class C, int N>
+__device__ __forceinline__ void load_cached(const void *p, int64_t at, int kv_dt, float *v) {
+    if (kv_dt == SP_DT_I8) load_codes<true, N>((const uint8_t *)p + at, v);
+    else if (kv_dt == SP_DT_E4M3) load_codes<false, N>((const uint8_t *)p + at, v);
+    else if (kv_dt == SP_DT_F16) load_values<f16, N>((const f16 *)p + at, v);
+    else load_values<bf16, N>((const bf16 *)p + at, v);
+}
+template <class T, int VEC>
+__global__ void __launch_bounds__(ROT_THREADS) k_paged_read(ReadArgs a) {
+    __shared__ int64_t from[ROT_THREADS];                              // [rows of the block]: element offset in the pools, or -1
+    __shared__ int64_t scale_at[ROT_THREADS];
+    const int row0 = blockIdx.x * a.per_block, n = min(a.per_block, a.rows - row0), total = n * a.per_row;
+    for (int k = threadIdx.x; k < n; k += blockDim.x) {
+        const int s = a.seq[row0 + k], p = a.at[row0 + k];
+        int64_t at = -1, sc = 0;
+        if (s >= 0 && s < a.n_seq && p >= 0 && p / a.page_size < a.max_pages) {
+            const int e = a.table[(int64_t)s * a.max_pages + p / a.page_size];
+            if (e >= 0 && e < a.n_pages) {
+                at = e * a.page_stride + (p % a.page_size) * a.row_stride;
+                if (a.block) sc = (int64_t)e * a.nkv * a.per_page + p % a.page_size / a.block;
+            }
+        }
+        from[k] = at;
+        scale_at[k] = sc;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < total; i += blockDim.x) {
+        const int r = i / a.by_row, k = i - r * a.per_row, w = k / a.by_vecs, at = (k - w * a.vecs) * VEC;
+        const bool keys = w < a.nkv;
+        const int h = keys ? w : w - a.nkv;
+        float v[VEC];
+        if (from[r] < 0) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+        } else {
+            load_cached<T, VEC>(keys ? a.kc : a.vc, from[r] + h * a.head_stride + at, a.kv_dt, v);
+            const float *scales = keys ? a.ks : a.vs;
+            if (scales) {
+                const float f = scales[scale_at[r] + (a.block ? (int64_t)h * a.per_page : h)];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[j] *= f;
+            }
+        }
+        const int64_t row = row0 + r;
+        store_values<VEC>(keys ? a.k_out : a.v_out, (keys ? row * a.k_row + h * a.k_head : row * a.v_row + h * a.v_head) + at, dtype_of<T>(), v);
+    }
+}
+
+}  // namespace paged

@@ -72,6 +72,17 @@ struct AttnArgs {
     f32x4 *ml;
 };
 
+// What a cache holds: the queries' type, e4m3 with a scale per K/V head, and e4m3 or int8 with a scale per block of positions and head.
+enum { KV_16 = 0, KV_E4M3 = 1, KV_E4M3_BLOCKS = 2, KV_I8_BLOCKS = 3 };
+constexpr bool in_blocks(int kv) { return kv >= KV_E4M3_BLOCKS; }
+struct BlockArgs : AttnArgs {         // ks, vs: [n_pages][n_kv][per_page]
+    int per_page;                     // blocks of a page
+    PageDivisor by_block;
+};
+template <int KV> using ArgsOf = std::conditional_t<in_blocks(KV), BlockArgs, AttnArgs>;
+constexpr int SCALE_KEYS = 16;        // blocks are whole runs of this many positions
+constexpr float LEAST_SCALE = 0x1p-60f;
+
 template <class T> struct Mma;
 template <> struct Mma<f16> {
     typedef f16x8 frag;
@@ -96,6 +107,28 @@ template <> struct Mma<bf16> {
 template <class T>
 __device__ __forceinline__ typename Mma<T>::frag from_e4m3(u32x2 c) {       // exact: e4m3 is a subset of fp16 and of bf16
     const u32x4 w = {Mma<T>::pair(c.x, false), Mma<T>::pair(c.x, true), Mma<T>::pair(c.y, false), Mma<T>::pair(c.y, true)};
+    return __builtin_bit_cast(typename Mma<T>::frag, w);
+}
+
+// int8 codes, exact in both types: fp16 from bytes under the exponent of 1024 (q8_pair), bf16, whose 8 bits of fraction do not hold
+// that sum, by way of fp32 (the upper half is the value).
+template <class T>
+__device__ __forceinline__ typename Mma<T>::frag from_i8(u32x2 c) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (std::is_same<T, f16>::value) {
+            const uint32_t u = c[i] ^ 0x80808080u;
+            w[2 * i] = __builtin_bit_cast(uint32_t, q8_pair(u, 0x04010400u));
+            w[2 * i + 1] = __builtin_bit_cast(uint32_t, q8_pair(u, 0x04030402u));
+        } else {
+            uint32_t f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = __float_as_uint((float)(int8_t)(c[i] >> (8 * j)));
+            w[2 * i] = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);
+            w[2 * i + 1] = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
+        }
+    }
     return __builtin_bit_cast(typename Mma<T>::frag, w);
 }
 
@@ -130,6 +163,7 @@ __device__ __forceinline__ float half_sum(float v) {
 // key waves' (m, l).  Two blocks share a CU (8 waves: one block's loads and exponentials beside the other's matrix products).
 constexpr int TABLE_KEYS = 2048;
 constexpr int TILE_SMEM = 65536;
+template <int KV> constexpr int attn_smem = TILE_SMEM + (in_blocks(KV) ? TABLE_KEYS / SCALE_KEYS * 16 : 0);
 struct AttnShared {                                                    // beside the tiles
     uint32_t rows[TABLE_KEYS];                                         // pool row of each position (0 where there is none)
     uint32_t seen[TABLE_KEYS / 32];                                    // which positions exist
@@ -168,8 +202,9 @@ __device__ __forceinline__ __attribute__((address_space(3))) V *lds_at(uint32_t 
     return (__attribute__((address_space(3))) V *)(size_t)address;
 }
 
-template <class T, bool KV8, int HD, int WM>
-__device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsigned char *smem, AttnShared &sh) {
+template <class T, int KV, int HD, int WM>
+__device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, unsigned char *smem, AttnShared &sh) {
+    constexpr bool KV8 = KV != KV_16, BLOCKS = in_blocks(KV), I8 = KV == KV_I8_BLOCKS;
     typedef AttnTile<KV8, HD, WM> TL;
     typedef Mma<T> M;
     typedef typename M::frag frag;
@@ -187,7 +222,10 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     auto page_of = [&](int key) { return key / a.by_page; };           // (of no meaning behind the last key, where it is not used)
     auto entry_of = [&](int key, int page) { return key < w.k1 && w.seq < a.n_seq && page < a.max_pages ? table[page] : -1; };
     if (threadIdx.x == 0) sh.nonfinite = 0;
-    const int key0 = w.k0 + (int)threadIdx.x, page0 = page_of(key0), entry0 = entry_of(key0, page0);
+    // (with blocks the tiles begin on whole SCALE_KEYS; positions before the item's first do not exist for it)
+    const int k0 = BLOCKS ? w.k0 & -SCALE_KEYS : w.k0;
+    f32x4 *const scales = (f32x4 *)(smem + TILE_SMEM);                 // of each SCALE_KEYS positions of the table: see scale_terms
+    const int key0 = k0 + (int)threadIdx.x, page0 = page_of(key0), entry0 = entry_of(key0, page0);
 
     const int row = rw * 32 + col;
     // (a captured call may meet tables set later: its own sizes bound every access)
@@ -210,7 +248,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     const int lim = live ? min(w.k1, w.pos0 + tok + 1) : w.k1;
     const int lo = min(w.k1, w.pos0 + (rw * 32) / a.by_g + 1);
     const int hi = rw * 32 < w.ntok * a.G ? min(w.k1, w.pos0 + min(w.ntok - 1, (rw * 32 + 31) / a.by_g) + 1) : 0;
-    const float sc = KV8 ? a.scale * a.ks[w.kvh] : a.scale;
+    const float sc = KV == KV_E4M3 ? a.scale * a.ks[w.kvh] : a.scale;
 
     const int swz = piece_swap<NCH>(col);
     const int tg = (lane >> 4) & 1, ti = lane & 15;                    // which 16 of 32 dims; lane within them
@@ -249,9 +287,9 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     // Values that a weight of 0 may meet must be finite (each wave its own copies): those without a position, which are row 0 of
     // the pool, become zeros; so do infinities and NaNs of the border's tiles, which hold keys that some rows see and some
     // do not, and the rows that see them get them at the end.
-    const int border = w.ntok > 1 ? w.k0 + max(min(w.k1, w.pos0 + 1) - w.k0, 0) / KT * KT : w.k1;
+    const int border = w.ntok > 1 ? k0 + max(min(w.k1, w.pos0 + 1) - k0, 0) / KT * KT : w.k1;
     auto clear_values = [&](int vb, int t, int t0, uint32_t all) {
-        if (all == ~0u && t0 < border) return;
+        if (I8 || (all == ~0u && t0 < border)) return;                 // (every int8 code is finite)
         const int ln = opaque(lane);
 #pragma unroll 1
         for (int c = 0; c < TL::COPIES; ++c) {
@@ -300,7 +338,8 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     // operands as LDS gives them, and as the products take them: e4m3 is converted when it is used, after the wait for it
     typedef std::conditional_t<KV8, u32x2, u32x4> raw;
     auto cooked = [&](raw x) -> frag {
-        if constexpr (KV8) return from_e4m3<T>(x);
+        if constexpr (I8) return from_i8<T>(x);
+        else if constexpr (KV8) return from_e4m3<T>(x);
         else return __builtin_bit_cast(frag, x);
     };
     auto value_raw = [&](int vb, int y, int d) -> raw {           // keys 16 y .. + 15
@@ -328,8 +367,28 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
 #pragma unroll
         for (int p = 0; p < NS; ++p) s = M::run(cooked(k[p]), qf[p], s);
     };
+    // With blocks: a key's score is s kc, its weight times its values' scale is 2^(s kc + lv), and that weight over the scale is the
+    // weight itself.  Exponents are taken of s kc + lv: then what is rounded to T for the product with the values is at most 1
+    // however the scales of a row's blocks differ, and the sum of weights takes the scale out again (iv) in fp32.
+    struct Terms { f32x4 c[SUB][2]; };                                 // kc, lv, iv of keys 0 .. 15 and 16 .. 31
+    auto terms_of = [&](int t) {
+        Terms x;
+        if constexpr (BLOCKS) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) x.c[u][y] = scales[t * (KT / SCALE_KEYS) + 2 * u + y];
+        }
+        return x;
+    };
     // masks a tile's scores, positions from t0, and brings the running maximum up to date; returns the exponent's base
-    auto maxima = [&](f32x16 (&s)[SUB], int t0, const uint32_t (&seen)[SUB]) -> float {
+    auto maxima = [&](f32x16 (&s)[SUB], int t0, const uint32_t (&seen)[SUB], const Terms &x) -> float {
+        if constexpr (BLOCKS) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[u][j] = __builtin_fmaf(s[u][j], x.c[u][j / 8][0], x.c[u][j / 8][1]);
+        }
         if (t0 + KT > lo || (seen[0] & seen[SUB - 1]) != ~0u) {
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
@@ -347,7 +406,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
             for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[u][j]);
-        mx = fmaxf(m, half_max(mx) * sc);
+        mx = fmaxf(m, BLOCKS ? half_max(mx) : half_max(mx) * sc);
         // weights are taken from the base m.  With bf16 weights it follows the maximum only when that has grown by more than
         // 2^8, and the outputs need no rescaling up to there; with fp16 weights it is the maximum, whose weight is then
         // exactly 1 (outputs 2.4e-4 from the 64-bit result, 3.3e-4 by the other rule).  (A row that has seen nothing stays empty.)
@@ -362,23 +421,24 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
         }
         return m == -INFINITY ? 0.f : m;
     };
-    auto weights = [&](const f32x16 &s, float base, frag (&pf)[2], int j0, int n) {
+    auto weights = [&](const f32x16 &s, float base, const f32x4 (&x)[2], frag (&pf)[2], int j0, int n) {
 #pragma unroll
         for (int j = j0; j < j0 + n; ++j) {
-            const float p = __builtin_amdgcn_exp2f(s[j] * sc - base);
-            l += p;
+            const float p = __builtin_amdgcn_exp2f(BLOCKS ? s[j] - base : s[j] * sc - base);
+            if constexpr (BLOCKS) l = __builtin_fmaf(p, x[j / 8][2], l);
+            else l += p;
             pf[j / 8][j % 8] = (T)p;
         }
     };
     // The tile's weights and outputs; v0: the values of its first 16 keys.  Operands are read a group of products ahead, and the
     // second half's exponentials stand between the first half's products: left to itself the compiler reads each product's
     // operands right before it and waits for them.
-    auto tile_outputs = [&](int vb, raw (&v0)[ND], const f32x16 (&s)[SUB], float base) {
+    auto tile_outputs = [&](int vb, raw (&v0)[ND], const f32x16 (&s)[SUB], float base, const Terms &x) {
         raw v1[ND];
         frag pf[SUB][2];
         read_values(vb, 1, v1);
         __builtin_amdgcn_sched_barrier(0);
-        weights(s[0], base, pf[0], 0, 16);
+        weights(s[0], base, x.c[0], pf[0], 0, 16);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (SUB == 2) {
             constexpr int PER = 16 / (2 * ND);
@@ -389,7 +449,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                     raw &v = y ? v1[d] : v0[d];
                     o[d] = M::run(cooked(v), pf[0][y], o[d]);
                     v = value_raw(vb + 32 * RB, y, d);
-                    weights(s[1], base, pf[1], (y * ND + d) * PER, PER);
+                    weights(s[1], base, x.c[1], pf[1], (y * ND + d) * PER, PER);
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
@@ -399,16 +459,29 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
             for (int d = 0; d < ND; ++d) o[d] = M::run(cooked(y ? v1[d] : v0[d]), pf[SUB - 1][y], o[d]);
     };
 
-    for (int c0 = w.k0; c0 < w.k1; c0 += TABLE_KEYS) {
+    for (int c0 = k0; c0 < w.k1; c0 += TABLE_KEYS) {
         // the pool rows of the next positions (row 0 where there is none), and which exist
-        const bool first = c0 == w.k0;
+        const bool first = c0 == k0;
         if (!first) lds_barrier();
         const int tid = opaque(threadIdx.x);
 #pragma unroll 1
         for (int j = tid; j < TABLE_KEYS && c0 + j - tid < w.k1 + 64; j += 256) {  // (a tile past the end reads up to 63 rows past it)
             const int key = c0 + j, page = first && j == tid ? page0 : page_of(key);
             const int e = first && j == tid ? entry0 : entry_of(key, page);
-            const bool ok = e >= 0 && e < a.n_pages;
+            const bool in_pool = e >= 0 && e < a.n_pages, ok = in_pool && (!BLOCKS || key >= w.k0);
+            if constexpr (BLOCKS) {
+                if (key % SCALE_KEYS == 0) {
+                    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                    if (in_pool) {
+                        const int64_t i = ((int64_t)e * (a.NH / a.G) + w.kvh) * a.per_page + (key - page * a.page_size) / a.by_block;
+                        const float ks = a.ks[i], vs = a.vs[i];
+                        // (a scale of 0, of pages that were never written, stands for the least one; a NaN reaches the rows that see it)
+                        const float v = vs < LEAST_SCALE ? LEAST_SCALE : vs;
+                        x = (f32x4){ks * a.scale, __builtin_amdgcn_logf(v), v < INFINITY ? 1.f / v : 0.f, 0.f};
+                    }
+                    scales[j / SCALE_KEYS] = x;
+                }
+            }
             sh.rows[j] = ok ? (uint32_t)e * a.page_rows + (uint32_t)w.kvh * a.head_rows + (uint32_t)(key - page * a.page_size) * a.slot_rows : 0u;
             const uint64_t b = __ballot(ok);
             if ((tid & 63) == 0) *(uint64_t *)&sh.seen[j / 32] = b;
@@ -435,6 +508,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 copies_wait<TL::COPIES>();
                 f32x16 s[SUB];
                 raw k[SUB][NS], v0[ND];
+                const Terms x = terms_of(t);
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) read_keys(kb + u * 32 * RB, k[u]);
                 __builtin_amdgcn_sched_barrier(0);
@@ -442,12 +516,12 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 for (int u = 0; u < SUB; ++u) scores(k[u], s[u]);
                 lds_wait();
                 if (more) copy_tile(a.k, t + WK, lds0);
-                const float base = maxima(s, c0 + t * KT, seen);
+                const float base = maxima(s, c0 + t * KT, seen, x);
                 if (more) copies_wait<TL::COPIES>();
                 else copies_wait<0>();
                 clear_values(vb, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
                 read_values(vb, 0, v0);
-                tile_outputs(vb, v0, s, base);
+                tile_outputs(vb, v0, s, base, x);
                 lds_wait();
                 if (more) copy_tile(a.v, t + WK, lds0 + TL::TILE);
             }
@@ -494,6 +568,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                 }
                 f32x16 s[SUB];
                 raw k[SUB][NS], v0[ND];
+                const Terms x = terms_of(t);
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) read_keys(kb + u * 32 * RB, k[u]);
                 __builtin_amdgcn_sched_barrier(0);
@@ -503,7 +578,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
                     copies(u);
                 }
                 read_values(vb, 0, v0);
-                tile_outputs(vb, v0, s, maxima(s, c0 + t * KT, seen));
+                tile_outputs(vb, v0, s, maxima(s, c0 + t * KT, seen, x), x);
             };
             for (int i = 0; i < rounds; i += 2) {
                 step(i, std::integral_constant<int, 0>{});
@@ -555,7 +630,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     }
     if (nonfinite) {
 #pragma unroll 1
-        for (int key = border; key < w.k1; ++key) {
+        for (int key = max(border, w.k0); key < w.k1; ++key) {
             const int page = page_of(key), e = entry_of(key, page);
             if (e < 0 || e >= a.n_pages || key >= lim) continue;
             const uint8_t *v = a.v + (uint64_t)((uint32_t)e * a.page_rows + (uint32_t)w.kvh * a.head_rows + (uint32_t)(key - page * a.page_size) * a.slot_rows) * RB +
@@ -576,7 +651,7 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     const int row2 = rw * 32 + (opaque(lane) & 31), tok2 = row2 / a.by_g;
     if (row2 < w.ntok * a.G && (w.rec >= 0 || w.tok0 + tok2 < a.rows)) {       // (records have room for every row of the plan)
         const int hh2 = row2 - tok2 * a.G;
-        const float vs = KV8 ? a.vs[w.kvh] : 1.f;
+        const float vs = KV == KV_E4M3 ? a.vs[w.kvh] : 1.f;
         if (w.rec < 0) {
             const float il = l > 0.f ? vs / l : 0.f;                   // a row that sees nothing: zeros
             const int64_t head = w.kvh * a.G + hh2;
@@ -598,17 +673,17 @@ __device__ __forceinline__ void run_item(const AttnArgs &a, const Item &w, unsig
     }
 }
 
-template <class T, bool KV8, int HD>
-__global__ void __launch_bounds__(256, 2) k_paged_attn(AttnArgs a) {
-    extern __shared__ __align__(1024) unsigned char smem[];            // TILE_SMEM
+template <class T, int KV, int HD>
+__global__ void __launch_bounds__(256, 2) k_paged_attn(ArgsOf<KV> a) {
+    extern __shared__ __align__(1024) unsigned char smem[];            // attn_smem<KV>
     __shared__ __align__(16) AttnShared sh;
     const int n = a.n_items ? *a.n_items : gridDim.x;
     for (int it = blockIdx.x; it < n; it += gridDim.x) {
         const Item w = a.items[it];
         if (it != (int)blockIdx.x) lds_barrier();                      // LDS is free of the item before
-        if (w.kind == 0) run_item<T, KV8, HD, 1>(a, w, smem, sh);
-        else if (w.kind == 1) run_item<T, KV8, HD, 2>(a, w, smem, sh);
-        else run_item<T, KV8, HD, 4>(a, w, smem, sh);
+        if (w.kind == 0) run_item<T, KV, HD, 1>(a, w, smem, sh);
+        else if (w.kind == 1) run_item<T, KV, HD, 2>(a, w, smem, sh);
+        else run_item<T, KV, HD, 4>(a, w, smem, sh);
     }
 }
 

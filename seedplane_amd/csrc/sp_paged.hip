@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "sp_host.h"
+#include "sp_blocks.h"
 #include "sp_paged.h"
 #include "sp_paged_plan.h"
 #include "sp_rotate.h"
@@ -40,7 +41,7 @@ bool is_capturing(hipStream_t st) {
     return cs != hipStreamCaptureStatusNone;
 }
 
-int bytes_of(int dt) { return dt == SP_DT_F32 ? 4 : dt == SP_DT_E4M3 ? 1 : 2; }
+int bytes_of(int dt) { return dt == SP_DT_F32 ? 4 : dt == SP_DT_E4M3 || dt == SP_DT_I8 ? 1 : 2; }
 bool aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 Rotation rotation_of(const sp_rotary *r, int hd) {
@@ -53,9 +54,9 @@ Rotation rotation_of(const sp_rotary *r, int hd) {
     return Rotation{r->inv_freq_dev, r->rot_dim, r->layout == SP_ROPE_INTERLEAVED, r->factor};
 }
 
-// Vectors of 8 values are used where every vector of the operands is aligned to 16 bytes (8 for e4m3).
+// Vectors of 8 values are used where every vector of the operands is aligned to 16 bytes (8 for a type of 8 bits).
 bool wide_ok(const void *p, int dt, int64_t row, int64_t head) {
-    return aligned(p, dt == SP_DT_E4M3 ? 8 : 16) && row % 8 == 0 && head % 8 == 0;
+    return aligned(p, bytes_of(dt) == 1 ? 8 : 16) && row % 8 == 0 && head % 8 == 0;
 }
 
 // The bytes of [rows][heads][hd] values at strides row and head (elements); empty where there are none.
@@ -117,8 +118,9 @@ void for_input(int dt, bool wide, F &&fn) {
 
 void check_cache(const sp_paged_kv *kv) {
     require(kv && kv->k_dev && kv->v_dev, SP_EINVAL, "NULL cache");
-    require(kv->dtype == SP_DT_F16 || kv->dtype == SP_DT_BF16 || kv->dtype == SP_DT_E4M3, SP_EINVAL,
-            "the cache's dtype must be SP_DT_F16, SP_DT_BF16 or SP_DT_E4M3");
+    const bool codes = kv->dtype == SP_DT_E4M3 || kv->dtype == SP_DT_I8;
+    require(kv->dtype == SP_DT_F16 || kv->dtype == SP_DT_BF16 || codes, SP_EINVAL,
+            "the cache's dtype must be SP_DT_F16, SP_DT_BF16, SP_DT_E4M3 or SP_DT_I8");
     require(kv->n_pages >= 1 && kv->page_size >= 1 && kv->n_kv_heads >= 1 && kv->head_dim >= 2, SP_EINVAL,
             "the cache's sizes must be positive");
     require((kv->n_pages == 1 || kv->page_stride >= kv->head_dim) && (kv->n_kv_heads == 1 || kv->head_stride >= kv->head_dim) &&
@@ -129,8 +131,52 @@ void check_cache(const sp_paged_kv *kv) {
     for (const auto &d : dims)
         require(!__builtin_mul_overflow(d[0] - 1, d[1], &more) && more < ((int64_t)1 << 60) && (reach += more) < ((int64_t)1 << 60),
                 SP_EINVAL, "the cache is too large");
-    require((kv->dtype == SP_DT_E4M3) == (kv->k_scale_dev != nullptr) && (kv->dtype == SP_DT_E4M3) == (kv->v_scale_dev != nullptr),
-            SP_EINVAL, "an e4m3 cache has k_scale_dev and v_scale_dev, others have none");
+    require(codes == (kv->k_scale_dev != nullptr) && codes == (kv->v_scale_dev != nullptr),
+            SP_EINVAL, "a cache of 8 bits has k_scale_dev and v_scale_dev, others have none");
+    require(kv->scale_block >= 0 && (kv->scale_block == 0 || codes), SP_EINVAL, "only caches of 8 bits have a scale_block");
+    require(kv->dtype != SP_DT_I8 || kv->scale_block, SP_EINVAL, "an int8 cache has a scale_block");
+    require(kv->scale_block % SCALE_KEYS == 0 && kv->scale_block <= MOST_BLOCK && (!kv->scale_block || kv->page_size % kv->scale_block == 0),
+            SP_EINVAL, "scale_block must be a multiple of 16 up to 128 that divides page_size");
+    require(!kv->scale_block || (double)kv->n_pages * kv->n_kv_heads * (kv->page_size / kv->scale_block) < 1e15, SP_EINVAL, "the cache is too large");
+}
+
+// The scales of a cache in blocks, of keys or of values.
+Span scales_of(const sp_paged_kv *kv, const float *p) {
+    Span s;
+    s.lo = (uintptr_t)p;
+    s.hi = s.lo + (uintptr_t)kv->n_pages * kv->n_kv_heads * (kv->page_size / kv->scale_block) * sizeof(float);
+    return s;
+}
+
+// Rows of blocks with scales of their own: see sp_blocks.h.  a: the append's arguments as for other caches.
+void append_blocks(const sp_paged_kv *kv, AppendArgs &a, int dtype, bool wide, hipStream_t st) {
+    BlockAppendArgs b{};
+    (AppendArgs &)b = a;
+    b.kscale = kv->k_scale_dev; b.vscale = kv->v_scale_dev;
+    b.block = kv->scale_block; b.per_page = kv->page_size / kv->scale_block;
+    b.by_block = PageDivisor(b.block); b.by_page = PageDivisor(kv->page_size);
+    b.by_key = Divisor(a.units + a.tail); b.by_value = Divisor(a.vecs);
+    // a step brings a row or a few to each block and has a workgroup for each row; of longer calls most rows follow one of the same block
+    b.chunk = std::max(1, std::min(16, a.rows / 256));
+    b.chunks = (a.rows + b.chunk - 1) / b.chunk;
+    // heads are split while a call's blocks are too few to fill the chip
+    const int runs = std::max(1, a.rows / b.block);
+    b.splits = std::max((a.nkv + BLOCK_HEADS - 1) / BLOCK_HEADS, std::min(a.nkv, 256 / runs));
+    b.heads = (a.nkv + b.splits - 1) / b.splits;
+    b.splits = (a.nkv + b.heads - 1) / b.heads;
+    // the queries' rows are the plain append's, without keys and values
+    b.turned = a.nq * a.units;
+    b.rest = a.nq * a.tail;
+    b.per_row = b.turned + b.rest;
+    int query_blocks = 0;
+    size_t lds = (size_t)b.block * (a.rot.rot / 2) * sizeof(float2);
+    if (a.nq) {
+        b.by_row = Divisor(b.per_row);
+        b.per_block = std::max(1, std::min(a.rows, 256 / b.per_row));
+        query_blocks = (a.rows + b.per_block - 1) / b.per_block;
+        lds = std::max(lds, (size_t)b.per_block * (sizeof(int64_t) + (a.rot.rot / 2) * sizeof(float2)));
+    }
+    launch_block_append(dtype, wide, b, query_blocks, lds, st);
 }
 
 }  // namespace
@@ -213,14 +259,14 @@ void tables_of(int NH, int NKV, int HD, int n_seq, const int32_t *q_len, const i
     }
 }
 
-template <class T, bool KV8, int HD>
+template <class T, int KV, int HD>
 void launch_items(const AttnArgs &a, int grid, hipStream_t st) {
-    hipLaunchKernelGGL((k_paged_attn<T, KV8, HD>), dim3(grid), dim3(256), TILE_SMEM, st, a);
+    hipLaunchKernelGGL((k_paged_attn<T, KV, HD>), dim3(grid), dim3(256), attn_smem<KV>, st, a);
 }
 template <class T>
 void launch_typed(bool kv8, int HD, const AttnArgs &a, int grid, hipStream_t st) {
-    if (kv8) { if (HD == 128) launch_items<T, true, 128>(a, grid, st); else launch_items<T, true, 64>(a, grid, st); }
-    else { if (HD == 128) launch_items<T, false, 128>(a, grid, st); else launch_items<T, false, 64>(a, grid, st); }
+    if (kv8) { if (HD == 128) launch_items<T, KV_E4M3, 128>(a, grid, st); else launch_items<T, KV_E4M3, 64>(a, grid, st); }
+    else { if (HD == 128) launch_items<T, KV_16, 128>(a, grid, st); else launch_items<T, KV_16, 64>(a, grid, st); }
 }
 // A wave joins a (token, head) whose records it has in flight at once; more are shared by the block's four waves (15 records of 96
 // tokens x 28 heads: 8.1 us by four, 5.1 by one).
@@ -297,6 +343,8 @@ int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t d
                 "q_out_dtype must be SP_DT_F32, SP_DT_F16 or SP_DT_BF16");
         require(n_seq >= 1 && max_pages >= 1, SP_EINVAL, "n_seq and max_pages must be positive");
         const Rotation rot = rotation_of(rotary, hd);
+        require(!kv->scale_block || (kv->scale_block * (int64_t)rot.rot <= 16384 && kv->scale_block * (int64_t)hd < (1 << 16)), SP_EINVAL,
+                "scale_block * rot_dim must be at most 16384 and scale_block * head_dim below 65536");
         if (n_rows == 0) return;
         require(k_dev && v_dev && seq_dev && at_dev && table_dev && (!rotary || pos_dev), SP_EINVAL, "NULL pointer");
         require(kv->k_dev != kv->v_dev, SP_EINVAL, "keys and values need memory of their own");
@@ -307,6 +355,17 @@ int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t d
                         (!q_dev || (!may_overlap(pool, q_dev, dtype, n_rows, nq, hd, q_row, q_head) &&
                                     !may_overlap(pool, q_out_dev, q_out_dtype, n_rows, nq, hd, q_out_row, q_out_head))),
                     SP_EINVAL, "the queries, keys or values overlap the cache");
+        }
+        if (kv->scale_block) {
+            const Span ks = scales_of(kv, kv->k_scale_dev), vs = scales_of(kv, kv->v_scale_dev);
+            require(!overlap(ks, vs), SP_EINVAL, "keys' and values' scales need memory of their own");
+            for (const Span &s : {ks, vs})
+                require(!overlap(s, pool_of(kv, kv->k_dev)) && !overlap(s, pool_of(kv, kv->v_dev)) &&
+                            !may_overlap(s, k_dev, dtype, n_rows, kv->n_kv_heads, hd, k_row, k_head) &&
+                            !may_overlap(s, v_dev, dtype, n_rows, kv->n_kv_heads, hd, v_row, v_head) &&
+                            (!q_dev || (!may_overlap(s, q_dev, dtype, n_rows, nq, hd, q_row, q_head) &&
+                                        !may_overlap(s, q_out_dev, q_out_dtype, n_rows, nq, hd, q_out_row, q_out_head))),
+                        SP_EINVAL, "the scales overlap the cache, queries, keys or values");
         }
         if (q_dev) {
             const bool in_place = q_dev == q_out_dev && q_out_dtype == dtype && q_row == q_out_row && q_head == q_out_head;
@@ -342,6 +401,10 @@ int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t d
         a.per_row = a.turned + a.rest + a.nkv * a.vecs;
         a.by_row = Divisor(a.per_row); a.by_units = Divisor(a.units); a.by_tail = Divisor(a.tail); a.by_vecs = Divisor(a.vecs);
         a.by_half = Divisor(rot.rot / 2);
+        if (kv->scale_block) {
+            append_blocks(kv, a, dtype, wide, (hipStream_t)stream);
+            return;
+        }
         int threads;
         shape_of(a.per_row, n_rows, a.per_block, threads);
         for_input(dtype, wide, [&](auto *t, auto v) {
@@ -350,6 +413,46 @@ int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t d
                                (size_t)a.per_block * (sizeof(int64_t) + (rot.rot / 2) * sizeof(float2)), (hipStream_t)stream, a);
         });
         HIPCHK(hipGetLastError());
+    });
+}
+
+int sp_op_paged_read(const sp_paged_kv *kv, int32_t dtype, int32_t n_rows, const int32_t *seq_dev, const int32_t *at_dev,
+                     const int32_t *table_dev, int32_t n_seq, int32_t max_pages, void *k_out_dev, int64_t k_row, int64_t k_head,
+                     void *v_out_dev, int64_t v_row, int64_t v_head, void *stream) {
+    return guarded([&] {
+        check_cache(kv);
+        require(dtype == SP_DT_F32 || dtype == SP_DT_F16 || dtype == SP_DT_BF16, SP_EINVAL,
+                "dtype must be SP_DT_F32, SP_DT_F16 or SP_DT_BF16");
+        const int hd = kv->head_dim, nkv = kv->n_kv_heads;
+        require(n_rows >= 0 && n_seq >= 1 && max_pages >= 1 && hd <= 1024 && 2 * (int64_t)nkv * hd < (1 << 16), SP_EINVAL,
+                "n_rows must not be negative, n_seq and max_pages positive, head_dim at most 1024 and the values of a row below 2^16");
+        if (n_rows == 0) return;
+        require(seq_dev && at_dev && table_dev && k_out_dev && v_out_dev, SP_EINVAL, "NULL pointer");
+        const Span k = span_of(k_out_dev, dtype, n_rows, nkv, hd, k_row, k_head), v = span_of(v_out_dev, dtype, n_rows, nkv, hd, v_row, v_head);
+        check_output(k);
+        check_output(v);
+        require(!overlap(k, v), SP_EINVAL, "the outputs overlap each other");
+        for (const Span &s : {k, v})
+            require(!overlap(s, pool_of(kv, kv->k_dev)) && !overlap(s, pool_of(kv, kv->v_dev)) &&
+                        (!kv->scale_block || (!overlap(s, scales_of(kv, kv->k_scale_dev)) && !overlap(s, scales_of(kv, kv->v_scale_dev)))),
+                    SP_EINVAL, "an output overlaps the cache");
+        ReadArgs a{};
+        a.kc = kv->k_dev; a.vc = kv->v_dev; a.k_out = k_out_dev; a.v_out = v_out_dev;
+        a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
+        a.ks = kv->k_scale_dev; a.vs = kv->v_scale_dev;
+        a.seq = seq_dev; a.at = at_dev; a.table = table_dev;
+        a.rows = n_rows; a.nkv = nkv; a.kv_dt = kv->dtype;
+        a.n_seq = n_seq; a.max_pages = max_pages; a.n_pages = kv->n_pages; a.page_size = kv->page_size;
+        a.block = kv->scale_block; a.per_page = a.block ? kv->page_size / a.block : 0;
+        a.page_stride = kv->page_stride; a.head_stride = kv->head_stride; a.row_stride = kv->row_stride;
+        const bool wide = wide_ok(k_out_dev, dtype, k_row, k_head) && wide_ok(v_out_dev, dtype, v_row, v_head) &&
+                          wide_ok(kv->k_dev, kv->dtype, kv->page_stride, kv->head_stride) &&
+                          wide_ok(kv->v_dev, kv->dtype, kv->row_stride, 0) && hd % 8 == 0;
+        a.vecs = hd / (wide ? 8 : 1);
+        a.per_row = 2 * nkv * a.vecs;
+        a.per_block = std::max(1, std::min(n_rows, ROT_THREADS / a.per_row));
+        a.by_row = Divisor(a.per_row); a.by_vecs = Divisor(a.vecs);
+        launch_read(dtype, wide, a, (hipStream_t)stream);
     });
 }
 
@@ -456,7 +559,7 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         require(p != nullptr, SP_EINVAL, "plan is NULL");
         check_cache(kv);
         require(dtype == SP_DT_F16 || dtype == SP_DT_BF16, SP_EINVAL, "dtype must be SP_DT_F16 or SP_DT_BF16");
-        require(kv->dtype == dtype || kv->dtype == SP_DT_E4M3, SP_EINVAL, "the cache's dtype must be the queries' or SP_DT_E4M3");
+        require(kv->dtype == dtype || bytes_of(kv->dtype) == 1, SP_EINVAL, "the cache's dtype must be the queries', SP_DT_E4M3 or SP_DT_I8");
         require(kv->n_kv_heads == p->NKV && kv->head_dim == p->HD, SP_EINVAL, "the cache's heads are not the plan's");
         require(scale > 0.f && std::isfinite(scale), SP_EINVAL, "scale must be positive");
         require(p->set, SP_ESTATE, "the plan has no lengths: call sp_attn_plan_set first");
@@ -483,13 +586,15 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
             const Span to = span_of(out_dev, dtype, n_rows, p->NH, p->HD, out_row, out_head);
             check_output(to);
             require(!may_overlap(to, q_dev, dtype, n_rows, p->NH, p->HD, q_row, q_head), SP_EINVAL, "the output overlaps the queries");
-            require(!overlap(to, pool_of(kv, kv->k_dev)) && !overlap(to, pool_of(kv, kv->v_dev)), SP_EINVAL, "the output overlaps the cache");
+            require(!overlap(to, pool_of(kv, kv->k_dev)) && !overlap(to, pool_of(kv, kv->v_dev)) &&
+                        (!kv->scale_block || (!overlap(to, scales_of(kv, kv->k_scale_dev)) && !overlap(to, scales_of(kv, kv->v_scale_dev)))),
+                    SP_EINVAL, "the output overlaps the cache");
         }
         require(aligned(out_dev, 8) && out_row % 4 == 0 && out_head % 4 == 0, SP_EINVAL, "outputs must be aligned to 8 bytes");
         require(aligned(kv->k_dev, 16) && aligned(kv->v_dev, 16) && kv->head_dim * bytes_of(kv->dtype) % 16 == 0,
                 SP_EINVAL, "the cache's pages must be aligned to 16 bytes");
         require(aligned(workspace_dev, 16), SP_EINVAL, "the workspace must be aligned to 16 bytes");
-        AttnArgs a{};
+        BlockArgs a{};
         a.q = q_dev; a.out = out_dev; a.lse = lse_dev;
         a.q_row = q_row; a.q_head = q_head; a.out_row = out_row; a.out_head = out_head;
         a.k = (const uint8_t *)kv->k_dev; a.v = (const uint8_t *)kv->v_dev; a.ks = kv->k_scale_dev; a.vs = kv->v_scale_dev;
@@ -508,7 +613,11 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         a.items = (const Item *)(p->dev + p->item_at);
         a.n_items = capturing ? p->dev : nullptr;
         const int grid = capturing ? CAPTURED_GRID : p->n_items;
-        if (grid) {
+        if (grid && kv->scale_block) {
+            a.per_page = kv->page_size / kv->scale_block;
+            a.by_block = PageDivisor(kv->scale_block);
+            launch_block_items(dtype, kv->dtype, p->HD, a, grid, st);
+        } else if (grid) {
             if (dtype == SP_DT_F16) launch_typed<f16>(kv8, p->HD, a, grid, st);
             else launch_typed<bf16>(kv8, p->HD, a, grid, st);
             HIPCHK(hipGetLastError());

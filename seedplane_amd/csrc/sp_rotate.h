@@ -218,11 +218,10 @@ struct AppendArgs {
 // Units of a row: the rotated parts of the query and key heads, their unrotated rests, the value heads.  A row whose
 // sequence, position or page is out of range writes nothing.
 template <class T, int VEC>
-__global__ void __launch_bounds__(ROT_THREADS) k_append(AppendArgs a) {
-    extern __shared__ __align__(16) unsigned char rot_smem[];
+__device__ __forceinline__ void append_rows(const AppendArgs &a, int block, unsigned char *rot_smem) {
     int64_t *dst = (int64_t *)rot_smem;                                // [rows of the block]: element offset in the pools, or -1
     float2 *cs = (float2 *)(dst + a.per_block);                        // [rows of the block][rot / 2]
-    const int row0 = blockIdx.x * a.per_block, n = min(a.per_block, a.rows - row0), half = a.rot.rot >> 1;
+    const int row0 = block * a.per_block, n = min(a.per_block, a.rows - row0), half = a.rot.rot >> 1;
     const int total = n * a.per_row;
     float v1[VEC], v2[VEC];
     int at1 = 0, at2 = 0, r = 0, head = 0, u = 0;
@@ -293,6 +292,12 @@ __global__ void __launch_bounds__(ROT_THREADS) k_append(AppendArgs a) {
         i += blockDim.x;
         if (i < total) fetch(i);
     }
+}
+
+template <class T, int VEC>
+__global__ void __launch_bounds__(ROT_THREADS) k_append(AppendArgs a) {
+    extern __shared__ __align__(16) unsigned char rot_smem[];
+    append_rows<T, VEC>(a, blockIdx.x, rot_smem);
 }
 
 }  // namespace paged

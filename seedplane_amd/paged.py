@@ -1,7 +1,7 @@
 """Paged K/V cache operators on MI355X: rotary embedding, append, and attention over pages with shared prefixes.
 
 For servers that hold their K/V in pages rather than in `Qwen2Engine`'s rings, and for other models than Qwen2: rotary layouts
-and scaled position tables, fp16 / bf16 / e4m3 caches, head ratios up to 32.  A page holds `page_size` positions of one
+and scaled position tables, fp16 / bf16 / e4m3 / int8 caches, head ratios up to 32.  A page holds `page_size` positions of one
 sequence for every K/V head; a table (int32 [sequences, most pages]) names each sequence's pages in order.  Sequences that
 start with the same tokens may name the same pages, and `AttentionPlan` then reads those once for all of them:
 
@@ -28,9 +28,10 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.SP_DT_F32, torch.float16: _lib.SP_DT_F16, torch.bfloat16: _lib.SP_DT_BF16,
-           torch.float8_e4m3fn: _lib.SP_DT_E4M3}
+           torch.float8_e4m3fn: _lib.SP_DT_E4M3, torch.int8: _lib.SP_DT_I8}
 _INT32 = torch.int32
-_FLOATS = {t: code for t, code in _DTYPES.items() if t != torch.float8_e4m3fn}
+_CODES = (torch.float8_e4m3fn, torch.int8)
+_FLOATS = {t: code for t, code in _DTYPES.items() if t not in _CODES}
 
 
 def rotary_frequencies(rot_dim, theta=10000.0, scaling=None, length=None):
@@ -210,10 +211,11 @@ class Rotary:
 
 
 class PagedKV:
-    """One layer's pages: `k` and `v` [n_pages, kv_heads, page_size, head_dim], fp16, bf16 or float8_e4m3fn, or views of that
+    """One layer's pages: `k` and `v` [n_pages, kv_heads, page_size, head_dim], fp16, bf16, float8_e4m3fn or int8, or views of that
     shape (`pool.transpose(1, 2)` of a [n_pages, page_size, kv_heads, head_dim] pool, halves of one allocation, ...) with the
-    same strides for both and the values of a row side by side.  An e4m3 cache holds value / scale, with fp32 scales per K/V
-    head."""
+    same strides for both and the values of a row side by side.  A cache of 8 bits holds value / scale, with fp32 scales: [kv_heads]
+    (e4m3), or for each block of positions [n_pages, kv_heads, page_size / block] (int8 or e4m3; blocks of 16 to 128 positions, whole
+    16s), which `append` writes from the values themselves."""
 
     _lease = None                 # of an engine's pool (Qwen2Engine.paged_kv): what holds and dates its memory
 
@@ -221,16 +223,24 @@ class PagedKV:
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
             raise ValueError('k and v must be [n_pages, kv_heads, page_size, head_dim] of one shape, type, device and layout')
         if k.dtype not in _DTYPES or k.dtype == torch.float32:
-            raise ValueError('the cache must be fp16, bf16 or float8_e4m3fn')
+            raise ValueError('the cache must be fp16, bf16, float8_e4m3fn or int8')
         n, nkv, page, hd = k.shape
         if 0 in k.shape or k.stride(3) != 1 or any(m > 1 and s < hd for m, s in zip(k.shape[:3], k.stride())):
             raise ValueError('the values of a row must lie side by side and rows must not overlap')
-        e4m3 = k.dtype == torch.float8_e4m3fn
+        codes, self.scale_block = k.dtype in _CODES, 0
         for s in (k_scale, v_scale):
-            if (s is not None) != e4m3:
-                raise ValueError('an e4m3 cache has k_scale and v_scale, others have none')
-            if s is not None and (s.shape != (nkv,) or s.dtype != torch.float32 or s.device != k.device or not s.is_contiguous()):
-                raise ValueError('scales must be fp32 [kv_heads] on the device of the cache')
+            if (s is not None) != codes:
+                raise ValueError('a cache of 8 bits has k_scale and v_scale, others have none')
+            if s is None:
+                continue
+            if s.dtype != torch.float32 or s.device != k.device or not s.is_contiguous() or s.shape != k_scale.shape:
+                raise ValueError('scales must be contiguous fp32 tensors of one shape on the device of the cache')
+            if s.dim() == 3 and s.shape[:2] == (n, nkv) and s.shape[2] and page % s.shape[2] == 0:
+                self.scale_block = page // s.shape[2]
+                if self.scale_block % 16 or self.scale_block > 128:
+                    raise ValueError('blocks of a scale must be of 16, 32, .. 128 positions')
+            elif s.shape != (nkv,) or k.dtype == torch.int8:
+                raise ValueError('scales must be [kv_heads] (e4m3) or [n_pages, kv_heads, page_size / block]')
         _lib.require_gpu()
         self.lib = _lib.load()
         self.device = k.device
@@ -239,8 +249,9 @@ class PagedKV:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, nkv, page, hd
         self.dtype = k.dtype
-        self.desc = _lib.PagedKVDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if e4m3 else None,
-                                     v_scale.data_ptr() if e4m3 else None, *self._strides(), _DTYPES[k.dtype], n, page, nkv, hd, 0)
+        self.desc = _lib.PagedKVDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if codes else None,
+                                     v_scale.data_ptr() if codes else None, *self._strides(), _DTYPES[k.dtype], n, page, nkv, hd,
+                                     self.scale_block)
         self._ref = ctypes.addressof(self.desc)
 
     def _strides(self):
@@ -255,8 +266,16 @@ class PagedKV:
             raise ValueError('the page table is of an older pool, another engine or other pages: call page_table() again')
 
     @classmethod
-    def allocate(cls, n_pages, page_size, n_kv_heads, head_dim, dtype=torch.float16, k_scale=None, v_scale=None, device='cuda'):
+    def allocate(cls, n_pages, page_size, n_kv_heads, head_dim, dtype=torch.float16, k_scale=None, v_scale=None, device='cuda',
+                 scale_block=None):
+        """Cleared pages; scale_block: positions of a block, whose scales are allocated too."""
         shape, device = (n_pages, n_kv_heads, page_size, head_dim), _device(device)
+        if scale_block is not None:
+            if scale_block < 1 or page_size % scale_block:
+                raise ValueError('scale_block must divide page_size')
+            if k_scale is not None or v_scale is not None:
+                raise ValueError('scales of blocks are allocated here')
+            k_scale, v_scale = (torch.zeros((n_pages, n_kv_heads, page_size // scale_block), device=device) for _ in range(2))
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device), k_scale, v_scale)
 
     def append(self, k, v, seq, pos, table, rotary=None, q=None, q_out=None, rotary_pos=None):
@@ -295,6 +314,31 @@ class PagedKV:
             if rotary is not None:
                 rotary._used()
         return q_out
+
+
+    def read(self, seq, pos, table, dtype=torch.float16, out=None):
+        """Keys and values at positions pos[r] of sequences seq[r] (int32 [rows]) as dense tensors [rows, kv_heads, head_dim] of
+        `dtype` (fp32, fp16 or bf16), or into out, a pair of such; zeros where a row has no place."""
+        if self._lease is not None:
+            self._check_lease(table)
+        dev, nkv, hd = self.device, self.n_kv_heads, self.head_dim
+        if seq.dim() != 1:
+            raise ValueError('seq must be [rows]')
+        rows = seq.shape[0]
+        s, p, t = _ints(seq, 'seq', dev, rows), _ints(pos, 'pos', dev, rows), _table(table, dev)
+        if out is None:
+            if dtype not in _FLOATS:
+                raise ValueError('dtype must be fp32, fp16 or bf16')
+            out = torch.empty((2, rows, nkv, hd), dtype=dtype, device=dev).unbind(0)
+        k, v = out
+        dt, k_rows, k_row, k_head, k_addr = _heads(k, 'k', dev, nkv, hd)
+        v_dt, v_rows, v_row, v_head, v_addr = _heads(v, 'v', dev, nkv, hd)
+        if v_dt != dt or k_rows != rows or v_rows != rows:
+            raise ValueError('out must be two tensors of one type, a row for each of seq')
+        if rows:
+            _call(self.lib.sp_op_paged_read, dev, self._ref, dt, rows, s, p, t, table.shape[0], table.shape[1], k_addr, k_row, k_head,
+                  v_addr, v_row, v_head)
+        return k, v
 
 
 class AttentionPlan:
