@@ -498,6 +498,57 @@ int sp_op_paged_attention(const sp_attn_plan *plan, const sp_paged_kv *kv, int32
                           void *out_dev, int64_t out_row, int64_t out_head, float *lse_dev, void *workspace_dev,
                           void *hip_stream);
 
+/* ---------------------------------------------------------------- pages of sequences, beams
+ * No counterpart in the reference (one tensor per sequence, no beams).  All calls are asynchronous on hip_stream, allocate nothing and may
+ * be captured into a graph; calls on one pool must not overlap. */
+
+/* The pages of the layers' caches and the sequences that hold them, all in device memory that the caller owns: a program may read
+ * the tables between calls, and set them to any state that follows the rules.  Pool i (keys or values of a layer) is at pools_dev[i],
+ * laid out as a sp_paged_kv's, its blocks' scales at scales_dev[i].  Row s of the table names the pages of sequence s's
+ * lengths_dev[s] positions in order, -1 behind them.  holders_dev[e]: how many entries of the table name page e, and 1 more for each
+ * time that the caller keeps it; 0: free.  A sequence's last page, where it is not full, has one holder.  missing_dev[0] counts the
+ * pages that were wanted and not found (their entries are -1, which hides the positions) and sequences cut at the table's width. */
+typedef struct sp_page_pool {
+    const uint64_t *pools_dev, *scales_dev;   /* device [n_pools] addresses; scales_dev NULL without scale_block */
+    int32_t *table_dev, *lengths_dev;         /* device [max_seqs][max_pages], [max_seqs] */
+    int32_t *holders_dev, *missing_dev;       /* device [n_pages], [1] */
+    void *workspace_dev;                      /* sp_pages_workspace bytes, cleared once before the first call */
+    int64_t page_stride, head_stride, row_stride;      /* elements */
+    int32_t n_pools, dtype, n_pages, page_size, n_kv_heads, head_dim, scale_block;
+    int32_t max_seqs, max_pages;
+    int32_t aligned16;                        /* 1: every address in pools_dev is a multiple of 16 */
+} sp_page_pool;
+size_t sp_pages_workspace(int32_t max_seqs, int32_t max_pages, int32_t n_pages);
+
+/* Every sequence s continues parents_dev[s] (int32 [max_seqs], each a sequence, itself included; anything else: none, s is empty
+ * afterwards).  Full pages are held in common; of a last page that is not full the first child keeps it, and each other gets a page
+ * of its own with its rows, in every pool (the lowest free pages, in the order of sequences).  Pages that nobody holds any more are free. */
+int sp_op_pages_fork(const sp_page_pool *pool, const int32_t *parents_dev, void *hip_stream);
+/* counts_dev[s] more positions for each sequence (int32 [max_seqs]; 0 or less: none), with pages for them: the lowest free ones, in the
+ * order of sequences and positions. */
+int sp_op_pages_grow(const sp_page_pool *pool, const int32_t *counts_dev, void *hip_stream);
+/* Sequences seqs_dev[0 .. n_seqs) end; entries that are no sequence, or are there twice, do nothing. */
+int sp_op_pages_free(const sp_page_pool *pool, int32_t n_seqs, const int32_t *seqs_dev, void *hip_stream);
+/* Held pages move to the lowest places, in every pool: with n of them held, those at or behind n go to the free ones before it, both in
+ * order.  places_dev (may be NULL): int32 [n_pages], each page's place afterwards (for what the caller keeps). */
+int sp_op_pages_compact(const sp_page_pool *pool, int32_t *places_dev, void *hip_stream);
+/* Pages src_dev[i] to dst_dev[i] in every pool, the whole of them with their scales; pairs outside the pool are left out.  A page must
+ * not be a destination twice, nor both a source and a destination. */
+int sp_op_pages_copy(const sp_page_pool *pool, int32_t n_copies, const int32_t *src_dev, const int32_t *dst_dev, void *hip_stream);
+
+/* Beam search's selection.  Request b's beam k has the logits of row b n_beams + k (dtype F32, F16 or BF16, rows ld apart) and the
+ * score scores_dev[b][k]; a continuation of it by token t scores scores[b][k] + logits[t] - log sum exp logits.  out_*: the n best of
+ * each request in order (ties: the lowest beam, then token) as [n_batch][n]: score, beam, token.  next_*: those of them whose token is
+ * none of eos (host, n_eos of them), the first n_beams, as [n_batch][n_beams]: score, row b n_beams + beam, token.  Places without a
+ * continuation hold -infinity, -1, -1: logits of -infinity are none, nor has a beam one whose score is -infinity or NaN, or whose logits hold
+ * NaN or +infinity.  Totals are compared in 64 bits; a row's sum of exponentials is held in 32.  n_beams <= n <= 64 (with n_eos ends,
+ * (n_eos + 1) n_beams is enough for n_beams that go on). */
+size_t sp_op_beam_select_workspace(int32_t n_batch, int32_t n_beams, int32_t vocab, int32_t n);
+int sp_op_beam_select(int32_t dtype, const void *logits_dev, int64_t ld, int32_t n_batch, int32_t n_beams, int32_t vocab,
+                      const float *scores_dev, int32_t n, int32_t n_eos, const int32_t *eos, float *out_scores_dev,
+                      int32_t *out_beams_dev, int32_t *out_tokens_dev, float *next_scores_dev, int32_t *next_rows_dev,
+                      int32_t *next_tokens_dev, void *workspace_dev, void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -54,6 +54,13 @@ class PagedKVDesc(ctypes.Structure):
                 ('scale_block', c_int32)]
 
 
+class PagePoolDesc(ctypes.Structure):
+    _fields_ = [('pools', c_void_p), ('scales', c_void_p), ('table', c_void_p), ('lengths', c_void_p), ('holders', c_void_p),
+                ('missing', c_void_p), ('workspace', c_void_p), ('page_stride', c_int64), ('head_stride', c_int64), ('row_stride', c_int64),
+                ('n_pools', c_int32), ('dtype', c_int32), ('n_pages', c_int32), ('page_size', c_int32), ('n_kv_heads', c_int32),
+                ('head_dim', c_int32), ('scale_block', c_int32), ('max_seqs', c_int32), ('max_pages', c_int32), ('aligned16', c_int32)]
+
+
 # the same layout as a numpy structured dtype (columns built in bulk)
 TOKEN_DTYPE = np.dtype([(name, np.int32 if ctype is c_int32 else np.uint64) for name, ctype in Token._fields_])
 assert TOKEN_DTYPE.itemsize == 40 and all(TOKEN_DTYPE.fields[n][1] == getattr(Token, n).offset for n, _ in Token._fields_)
@@ -128,6 +135,15 @@ SIGNATURES = {
     'sp_attn_plan_workspace': (c_size_t, [c_void_p]),
     'sp_op_paged_attention': (c_int, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_int32,
                                       c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    'sp_pages_workspace': (c_size_t, [c_int32, c_int32, c_int32]),
+    'sp_op_pages_fork': (c_int, [c_void_p, c_void_p, c_void_p]),
+    'sp_op_pages_grow': (c_int, [c_void_p, c_void_p, c_void_p]),
+    'sp_op_pages_free': (c_int, [c_void_p, c_int32, c_void_p, c_void_p]),
+    'sp_op_pages_compact': (c_int, [c_void_p, c_void_p, c_void_p]),
+    'sp_op_pages_copy': (c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
+    'sp_op_beam_select_workspace': (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
+    'sp_op_beam_select': (c_int, [c_int32, c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_int32, c_int32, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     'sp_library_release': (c_int, []),
     'sp_engine_kv_layer': (c_int, [c_void_p, c_int32, ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p)]),
 }

@@ -1,0 +1,73 @@
+"""Beam search's selection on MI355X: the best continuations of each request's beams, in one pass over the logits.
+
+    step = beam_select(logits, scores, eos=eos)             # logits [requests * beams, vocabulary], scores [requests, beams]
+    pool.fork(step.next_rows.view(-1))                      # the beams' pages follow (seedplane_amd.pages)
+    scores, tokens = step.next_scores, step.next_tokens
+
+Everything runs on torch's current stream of the logits' device, without waiting for it, and may be captured into a graph.  The reference
+samples one continuation (seedplane/qwen_engine.py:138-153); it has no beams.
+"""
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .paged import _FLOATS, _call
+
+MOST = 64                                                   # beams, and continuations asked for
+
+
+class BeamStep(NamedTuple):
+    """The best continuations of each request in order, [requests, n], and those of them that go on, [requests, beams]: fp32 scores,
+    int32 beams or rows of the logits, int32 tokens; -infinity and -1 in places without one."""
+    scores: torch.Tensor
+    beams: torch.Tensor
+    tokens: torch.Tensor
+    next_scores: torch.Tensor
+    next_rows: torch.Tensor
+    next_tokens: torch.Tensor
+
+    @classmethod
+    def allocate(cls, requests, beams, n, device='cuda'):
+        f = torch.empty((requests, n + beams), dtype=torch.float32, device=device).view(-1)
+        i = torch.empty((2, requests, n + beams), dtype=torch.int32, device=device).view(2, -1)
+        cut = requests * n
+        best, go = (requests, n), (requests, beams)
+        return cls(f[:cut].view(best), i[0, :cut].view(best), i[1, :cut].view(best), f[cut:].view(go), i[0, cut:].view(go), i[1, cut:].view(go))
+
+
+def beam_select(logits, scores, n=None, eos=None, out=None):
+    """The n best of scores[b, k] + log_softmax(logits[b * beams + k]) over beams and vocabulary of each request b, and the best of
+    them that do not end, as many as there are beams.
+
+    logits: [requests * beams, vocabulary], fp32, fp16 or bf16, the values of a row side by side; scores: fp32 [requests, beams],
+    -infinity for beams that do not live (all but one in a first step).  eos: a token or a list of up to 8 that end a sequence.
+    n: default beams * (1 + number of eos), enough for as many to go on as there are beams; at most 64.  Ties go to the lowest beam, then token; logits
+    of -infinity, and beams whose logits hold NaN or +infinity, have no continuation.  out: a BeamStep to fill."""
+    if logits.dim() != 2 or logits.dtype not in _FLOATS or (logits.shape[1] > 1 and logits.stride(1) != 1) or logits.device.type != 'cuda':
+        raise ValueError('logits must be an fp32, fp16 or bf16 GPU tensor [requests * beams, vocabulary], the values of a row side by side')
+    dev, (rows, vocab), ld = logits.device, logits.shape, logits.stride(0)
+    if scores.dtype != torch.float32 or scores.dim() != 2 or scores.device != dev or not scores.is_contiguous() or scores.numel() != rows:
+        raise ValueError(f'scores must be a contiguous fp32 tensor [requests, beams] on {dev}, one for each row of the logits')
+    requests, beams = scores.shape
+    ends = () if eos is None else (eos,) if isinstance(eos, int) else tuple(eos)
+    if n is None:
+        n = beams * (1 + len(ends))
+    if not 1 <= beams <= n <= MOST:
+        raise ValueError(f'beams must be in [1, n] and n at most {MOST}; got {beams} and {n}')
+    if out is None:
+        out = BeamStep.allocate(requests, beams, n, dev)
+    else:
+        for i, x in enumerate(out):
+            if x.shape != (requests, n if i < 3 else beams) or x.dtype != (torch.int32 if i % 3 else torch.float32) or x.device != dev \
+                    or not x.is_contiguous():
+                raise ValueError('out must be a BeamStep of these requests, beams and n (BeamStep.allocate)')
+    if not requests:
+        return out
+    lib = _lib.load()
+    workspace = torch.empty(lib.sp_op_beam_select_workspace(requests, beams, vocab, n), dtype=torch.uint8, device=dev)
+    _call(lib.sp_op_beam_select, dev, _FLOATS[logits.dtype], logits.data_ptr(), ld if rows > 1 else vocab, requests, beams, vocab,
+          scores.data_ptr(), n, len(ends), (ctypes.c_int32 * len(ends))(*ends) if ends else None, *(x.data_ptr() for x in out),
+          workspace.data_ptr())
+    return out

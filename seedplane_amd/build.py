@@ -10,7 +10,7 @@ import tempfile
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
-SOURCES = [PKG / 'csrc' / name for name in ('sp_engine.hip', 'sp_paged.hip', 'sp_blocks.hip')]
+SOURCES = [PKG / 'csrc' / name for name in ('sp_engine.hip', 'sp_paged.hip', 'sp_blocks.hip', 'sp_pages.hip', 'sp_beam.hip')]
 OUT = PKG / 'libseedplane_hip.so'
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 

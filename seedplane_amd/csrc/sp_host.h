@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <new>
 #include <string>
 
 #include "../../include/seedplane_hip.h"
@@ -44,6 +45,24 @@ T *dev_alloc(size_t count, uint64_t *acct = nullptr) {
 }
 [[maybe_unused]] inline void dev_free(void *p) {
     if (p) (void)hipFree(p);
+}
+
+// What a C entry does: no exception passes it.
+template <class F>
+int guarded(F &&fn) {
+    try {
+        fn();
+        return SP_OK;
+    } catch (const Fail &f) {
+        sp_call_error() = f.msg;
+        return f.code;
+    } catch (const std::bad_alloc &) {
+        sp_call_error() = "out of host memory";
+        return SP_ENOMEM;
+    } catch (const std::exception &ex) {
+        sp_call_error() = ex.what();
+        return SP_EHIP;
+    }
 }
 
 }  // namespace

@@ -18,23 +18,6 @@ using namespace paged;
 
 namespace {
 
-template <class F>
-int guarded(F &&fn) {
-    try {
-        fn();
-        return SP_OK;
-    } catch (const Fail &f) {
-        sp_call_error() = f.msg;
-        return f.code;
-    } catch (const std::bad_alloc &) {
-        sp_call_error() = "out of host memory";
-        return SP_ENOMEM;
-    } catch (const std::exception &ex) {
-        sp_call_error() = ex.what();
-        return SP_EHIP;
-    }
-}
-
 bool is_capturing(hipStream_t st) {
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     HIPCHK(hipStreamIsCapturing(st, &cs));

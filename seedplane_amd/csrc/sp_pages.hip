@@ -1,0 +1,125 @@
+// C ABI (include/seedplane_hip.h) of the page pool: forks, growth, ends and compaction of paged sequences.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "sp_host.h"
+#include "sp_pages.h"
+
+namespace {
+
+size_t up(size_t n) { return (n + 15) / 16 * 16; }
+
+struct Places { size_t fresh, first, rows, list, moves, total; };
+Places places_of(int64_t S, int64_t width, int64_t n_pages) {
+    Places p{};
+    p.fresh = 64;
+    p.first = p.fresh + up(S * 4);
+    p.rows = p.first + up((S + 1) * 4);
+    p.list = p.rows + up(S * width * 4);
+    p.moves = p.list + up(n_pages * 4);
+    p.total = p.moves + up(std::max(S, n_pages) * sizeof(pages::Move));
+    return p;
+}
+bool sizes_ok(int64_t S, int64_t width, int64_t n_pages) {
+    return S >= 1 && S <= 65535 && width >= 1 && n_pages >= 1 && S * width < (1 << 30);
+}
+
+pages::Pool pool_args(const sp_page_pool *p) {
+    require(p != nullptr, SP_EINVAL, "pool is NULL");
+    require(sizes_ok(p->max_seqs, p->max_pages, p->n_pages), SP_EINVAL,
+            "max_seqs must be in [1, 65535], max_pages and n_pages positive and max_seqs * max_pages below 2^30");
+    const int b = p->dtype == SP_DT_F16 || p->dtype == SP_DT_BF16 ? 2 : p->dtype == SP_DT_E4M3 || p->dtype == SP_DT_I8 ? 1 : 0;
+    require(b != 0, SP_EINVAL, "dtype must be SP_DT_F16, SP_DT_BF16, SP_DT_E4M3 or SP_DT_I8");
+    require(p->n_pools >= 1 && p->n_pools <= 65535 && p->page_size >= 1 && p->n_kv_heads >= 1 && p->head_dim >= 1, SP_EINVAL,
+            "the pool's sizes must be positive, n_pools at most 65535");
+    require((double)p->page_size * p->n_kv_heads * p->head_dim * b < (double)(1u << 31) && (double)p->max_pages * p->page_size < (double)(1u << 31),
+            SP_EINVAL, "a page must be below 2^31 bytes and a sequence below 2^31 positions");
+    require((p->n_pages == 1 || p->page_stride >= p->head_dim) && (p->n_kv_heads == 1 || p->head_stride >= p->head_dim) &&
+                (p->page_size == 1 || p->row_stride >= p->head_dim) && p->page_stride >= 0 && p->head_stride >= 0 && p->row_stride >= 0,
+            SP_EINVAL, "the pool's strides are smaller than a row");
+    require(p->pools_dev && p->table_dev && p->lengths_dev && p->holders_dev && p->missing_dev && p->workspace_dev, SP_EINVAL, "NULL pointer");
+    require(((uintptr_t)p->workspace_dev & 15) == 0, SP_EINVAL, "the workspace must be aligned to 16 bytes");
+    require((p->scale_block > 0) == (p->scales_dev != nullptr) && p->scale_block >= 0 &&
+                (!p->scale_block || p->page_size % p->scale_block == 0), SP_EINVAL, "scales come with a scale_block that divides page_size");
+    pages::Pool a{};
+    a.pools = p->pools_dev; a.scales = p->scales_dev;
+    a.table = p->table_dev; a.lengths = p->lengths_dev; a.holders = p->holders_dev; a.missing = p->missing_dev;
+    a.page_bytes = p->page_stride * b; a.head_bytes = p->head_stride * b; a.row_bytes = p->row_stride * b;
+    a.n_pools = p->n_pools; a.n_pages = p->n_pages; a.page = p->page_size; a.nkv = p->n_kv_heads; a.width_bytes = p->head_dim * b;
+    a.block = p->scale_block; a.per_page = p->scale_block ? p->page_size / p->scale_block : 0;
+    a.S = p->max_seqs; a.width = p->max_pages;
+    a.aligned = p->aligned16 && (a.page_bytes | a.head_bytes | a.row_bytes | a.width_bytes) % 16 == 0;
+    const Places at = places_of(a.S, a.width, a.n_pages);
+    uint8_t *const w = (uint8_t *)p->workspace_dev;
+    a.arrived = (int *)w;
+    a.fresh = (int *)(w + at.fresh);
+    a.first = (int *)(w + at.first);
+    a.rows = (int *)(w + at.rows);
+    a.list = (int *)(w + at.list);
+    a.moves = (pages::Move *)(w + at.moves);
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sp_pages_workspace(int32_t max_seqs, int32_t max_pages, int32_t n_pages) {
+    return sizes_ok(max_seqs, max_pages, n_pages) ? places_of(max_seqs, max_pages, n_pages).total : 0;
+}
+
+int sp_op_pages_fork(const sp_page_pool *pool, const int32_t *parents_dev, void *stream) {
+    return guarded([&] {
+        const pages::Pool a = pool_args(pool);
+        require(parents_dev != nullptr, SP_EINVAL, "NULL pointer");
+        hipLaunchKernelGGL(pages::k_fork, dim3(a.S), dim3(pages::SCAN), 0, (hipStream_t)stream, a, parents_dev);
+        HIPCHK(hipGetLastError());
+        hipLaunchKernelGGL(pages::k_fork_copy, dim3(a.S, a.n_pools), dim3(pages::THREADS), 0, (hipStream_t)stream, a);
+        HIPCHK(hipGetLastError());
+    });
+}
+
+int sp_op_pages_grow(const sp_page_pool *pool, const int32_t *counts_dev, void *stream) {
+    return guarded([&] {
+        const pages::Pool a = pool_args(pool);
+        require(counts_dev != nullptr, SP_EINVAL, "NULL pointer");
+        hipLaunchKernelGGL(pages::k_grow, dim3(1), dim3(pages::SCAN), 0, (hipStream_t)stream, a, counts_dev);
+        HIPCHK(hipGetLastError());
+    });
+}
+
+int sp_op_pages_free(const sp_page_pool *pool, int32_t n_seqs, const int32_t *seqs_dev, void *stream) {
+    return guarded([&] {
+        const pages::Pool a = pool_args(pool);
+        require(n_seqs >= 0, SP_EINVAL, "n_seqs must not be negative");
+        if (n_seqs == 0) return;
+        require(seqs_dev != nullptr, SP_EINVAL, "NULL pointer");
+        hipLaunchKernelGGL(pages::k_free, dim3(n_seqs), dim3(pages::THREADS), 0, (hipStream_t)stream, a, seqs_dev);
+        HIPCHK(hipGetLastError());
+    });
+}
+
+int sp_op_pages_compact(const sp_page_pool *pool, int32_t *places_dev, void *stream) {
+    return guarded([&] {
+        const pages::Pool a = pool_args(pool);
+        hipLaunchKernelGGL(pages::k_compact, dim3(1), dim3(pages::SCAN), 0, (hipStream_t)stream, a, places_dev);
+        HIPCHK(hipGetLastError());
+        const int64_t most = std::max<int64_t>((int64_t)(a.n_pages / 2) * a.n_pools, 1);
+        hipLaunchKernelGGL(pages::k_compact_copy, dim3((int)std::min<int64_t>(most, 8192)), dim3(pages::THREADS), 0, (hipStream_t)stream, a);
+        HIPCHK(hipGetLastError());
+    });
+}
+
+int sp_op_pages_copy(const sp_page_pool *pool, int32_t n_copies, const int32_t *src_dev, const int32_t *dst_dev, void *stream) {
+    return guarded([&] {
+        const pages::Pool a = pool_args(pool);
+        require(n_copies >= 0, SP_EINVAL, "n_copies must not be negative");
+        if (n_copies == 0) return;
+        require(src_dev && dst_dev, SP_EINVAL, "NULL pointer");
+        hipLaunchKernelGGL(pages::k_copy, dim3(n_copies, a.n_pools), dim3(pages::THREADS), 0, (hipStream_t)stream, a, src_dev, dst_dev);
+        HIPCHK(hipGetLastError());
+    });
+}
+
+}  // extern "C"
