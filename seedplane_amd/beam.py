@@ -30,11 +30,8 @@ class BeamStep(NamedTuple):
 
     @classmethod
     def allocate(cls, requests, beams, n, device='cuda'):
-        f = torch.empty((requests, n + beams), dtype=torch.float32, device=device).view(-1)
-        i = torch.empty((2, requests, n + beams), dtype=torch.int32, device=device).view(2, -1)
-        cut = requests * n
-        best, go = (requests, n), (requests, beams)
-        return cls(f[:cut].view(best), i[0, :cut].view(best), i[1, :cut].view(best), f[cut:].view(go), i[0, cut:].view(go), i[1, cut:].view(go))
+        f, g = (torch.empty((3, requests, k), dtype=torch.int32, device=device).unbind(0) for k in (n, beams))
+        return cls(f[0].view(torch.float32), f[1], f[2], g[0].view(torch.float32), g[1], g[2])
 
 
 def beam_select(logits, scores, n=None, eos=None, out=None):

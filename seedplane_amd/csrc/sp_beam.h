@@ -5,10 +5,10 @@
 // forms the sums' logarithms, compares totals in 64 bits and writes the results in order (k_beam_merge).  Ties go to the lowest beam,
 // then token.
 //
-// The n best of a part: a block's waves take 8 values a thread at a time.  From the first chunk a border that at least n of its
-// values reach is known (each of 8 waves has ceil(n / 8) threads whose largest value does); values on the good side of it go to a
-// buffer in LDS, and when the buffer fills, its exact n best stay and the n-th becomes the border.  Later chunks bring few: a value
-// reaches the n best of what came before it n / (position) of the time.
+// The n best of a part: each thread streams its values, keeping their largest beside the sum.  The largest of all threads give a border
+// that at least n values reach and few others (each of 4 waves has ceil(n / 4) threads at or above it: about 2 n values of a part);
+// the few threads that have such values are listed, their values read once more by the whole block, and what reaches the border is put in order.
+// The stream has no barrier, no LDS and nothing but a maximum and an exponential for each value.
 #pragma once
 #include "sp_device.h"
 #include "sp_rotate.h"
@@ -17,11 +17,14 @@ namespace beam {
 
 using paged::bf16;
 
-constexpr int THREADS = 512, WAVES = THREADS / 64, VALUES = 8, CHUNK = THREADS * VALUES;
+constexpr int THREADS = 256, WAVES = THREADS / 64, VALUES = 8, CHUNK = THREADS * VALUES;
+constexpr int MERGE_THREADS = 512, MERGE_WAVES = MERGE_THREADS / 64;
 constexpr int MOST_N = 64, MOST_BEAMS = 64, MOST_EOS = 8, MOST_SPLITS = 64, LEAST_SPLITS = 4;
-constexpr int KEPT = 256;                  // entries of the buffer from which it is cut back to n
-constexpr int CAPACITY = KEPT + THREADS;   // one value of every thread fits behind them
-constexpr int LISTS = 512;                 // parts of a request's rows at most (splits are chosen so)
+constexpr int AHEAD = 2;                   // vectors of a thread in flight
+constexpr int CAPACITY = 1024;             // entries of the buffer
+constexpr int KEPT = CAPACITY - THREADS;   // entries to which one value of every thread can be added
+constexpr int LISTS = MERGE_THREADS;       // parts of a request's rows at most (splits are chosen so)
+constexpr int MERGED = 1024;               // entries that the merge puts in order at once
 
 struct Entry { float v; int i; };          // value, token
 struct Args {
@@ -30,7 +33,7 @@ struct Args {
     const float *scores;                   // [B][K]
     int B, K, V, n, splits, len;           // len: values of a part
     Entry *best;                           // [B K][splits][n], best first; i -1: none
-    float2 *sums;                          // [B K][splits]: maximum, sum of exponentials
+    float2 *sums;                          // [B K][splits]: m, the largest value, and sum e^(v - m)
     float *out_score, *next_score;
     int *out_beam, *out_token, *next_row, *next_token;
     int eos[MOST_EOS], n_eos;
@@ -39,20 +42,37 @@ struct Args {
 __device__ __forceinline__ bool better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 __device__ __forceinline__ bool alive(float score) { return score > -INFINITY; }       // (NaN: no)
 
+constexpr float LOG2E = 1.4426950408889634f;
+
+// The n-th largest of a wave's values (-infinity: there are fewer).  A border for more than the wave has only to be reached by n values,
+// so NaNs, which fmaxf leaves out, do not matter.
+__device__ __forceinline__ float nth_of_wave(float mine, int n) {
+    float w = -INFINITY;
+    for (int k = 0; k < n; ++k) {
+        w = wave_max_dpp(mine);
+        const uint64_t who = __ballot(mine == w);
+        if (who && (int)(threadIdx.x & 63) == __builtin_ctzll(who)) mine = -INFINITY;
+    }
+    return w;
+}
+
 struct RowShared {
     Entry buf[CAPACITY], top[MOST_N];
-    int count, overflow;
+    int count, threads, who[THREADS];
     float border[WAVES];
     float2 sum[WAVES];
 };
 
-// The exact n best of the buffer's count entries, in order, to its front.  Every thread calls; ends with a barrier.
+// The exact n best of the buffer's count entries, in order, to its front; the n-th becomes the border.  Every thread calls; ends with a
+// barrier.
 __device__ __forceinline__ int cut(RowShared &sh, int count, int n, float &bv, int &bi) {
-    for (int e = threadIdx.x; e < count; e += THREADS) {
+    for (int e = threadIdx.x / 4; e < count; e += THREADS / 4) {       // 4 threads an entry
         const Entry x = sh.buf[e];
         int rank = 0;
-        for (int j = 0; j < count; ++j) rank += better(sh.buf[j].v, sh.buf[j].i, x.v, x.i);
-        if (rank < n) sh.top[rank] = x;
+        for (int j = threadIdx.x & 3; j < count; j += 4) rank += better(sh.buf[j].v, sh.buf[j].i, x.v, x.i);
+        rank += __shfl_xor(rank, 1);
+        rank += __shfl_xor(rank, 2);
+        if ((threadIdx.x & 3) == 0 && rank < n) sh.top[rank] = x;
     }
     __syncthreads();
     const int left = min(count, n);
@@ -63,7 +83,8 @@ __device__ __forceinline__ int cut(RowShared &sh, int count, int n, float &bv, i
     return left;
 }
 
-template <class T, bool ALIGNED>
+// SHORT: rows of fewer values than a vector.
+template <class T, bool SHORT>
 __global__ void __launch_bounds__(THREADS) k_beam_rows(Args a) {
     __shared__ RowShared sh;
     const int split = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -75,91 +96,119 @@ __global__ void __launch_bounds__(THREADS) k_beam_rows(Args a) {
         return;
     }
     const T *const x = (const T *)a.logits + row * a.ld;
-    auto fetch = [&](int at, float (&v)[VALUES]) {
-        if (ALIGNED && at + VALUES <= hi) {
-            paged::load_values<T, VALUES>(x + at, v);
-        } else {
+    // A vector past the part's end is read from its last 8 values, and those before its own first are hidden: one load without a
+    // branch, wherever rows begin.
+    typedef T Vector __attribute__((ext_vector_type(VALUES), aligned(sizeof(T))));
+    auto place = [&](int own) { return SHORT ? own : min(own, hi - VALUES); };
+    auto fetch = [&](int own) -> Vector {
+        if constexpr (!SHORT) return *(const Vector *)(x + place(own));
+        Vector v;
 #pragma unroll
-            for (int j = 0; j < VALUES; ++j) v[j] = at + j < hi ? (float)x[at + j] : -INFINITY;
+        for (int j = 0; j < VALUES; ++j) v[j] = own + j < hi ? x[own + j] : (T)-INFINITY;
+        return v;
+    };
+    auto values = [&](const Vector &raw, int own, float (&v)[VALUES]) {
+        const int hidden = own - place(own);
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) v[j] = (float)raw[j];
+        if (hidden > 0) {
+#pragma unroll
+            for (int j = 0; j < VALUES; ++j) v[j] = j < hidden ? -INFINITY : v[j];
         }
     };
-    if (tid == 0) { sh.count = 0; sh.overflow = 0; }
-    float next[VALUES], v[VALUES];
-    fetch(lo + tid * VALUES, next);
+    if (tid == 0) { sh.count = 0; sh.threads = 0; }
+    // the thread's values: the largest, sum e^(v - m); AHEAD vectors at a time
     float m = -INFINITY, s = 0.f;
-    float bv = -INFINITY;                                              // a value is taken if it is better than (bv, bi)
-    int bi = -1, kept = 0;
-    for (int c = lo; c < hi; c += CHUNK) {
-        const int at = c + tid * VALUES;
+    for (int c = lo + tid * VALUES; c < hi; c += AHEAD * CHUNK) {
+        Vector raw[AHEAD];
 #pragma unroll
-        for (int j = 0; j < VALUES; ++j) v[j] = next[j];
-        if (c + CHUNK < hi) fetch(at + CHUNK, next);
-        float top = v[0];
+        for (int u = 0; u < AHEAD; ++u) raw[u] = fetch(c + u * CHUNK);
+        float v[AHEAD][VALUES], top = m;
 #pragma unroll
-        for (int j = 1; j < VALUES; ++j) top = fmaxf(top, v[j]);
-        if (top > m) {
-            s *= __builtin_amdgcn_exp2f((m - top) * 1.4426950408889634f);
-            m = top;
+        for (int u = 0; u < AHEAD; ++u) {
+            values(raw[u], c + u * CHUNK, v[u]);
+#pragma unroll
+            for (int j = 0; j < VALUES; ++j) top = fmaxf(top, v[u][j]);
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = top == -INFINITY ? 0.f : top;
+        s *= __builtin_amdgcn_exp2f((m - base) * LOG2E);
+        m = top;
+        // (a fused v LOG2E - m would save an instruction, but leave fp32's range for a type's lowest values)
 #pragma unroll
-        for (int j = 0; j < VALUES; ++j) s += __builtin_amdgcn_exp2f((v[j] - base) * 1.4426950408889634f);
-        if (c == lo) {
-            // each wave's ceil(n / WAVES)-th largest of its threads' largest values; the least of the waves'
-            float mine = top, w = -INFINITY;
-            for (int k = 0; k < a.n; k += WAVES) {
-                w = wave_max_dpp(mine);
-                const uint64_t who = __ballot(mine == w);
-                if (who && lane == __builtin_ctzll(who)) mine = -INFINITY;
-            }
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int j = 0; j < VALUES; ++j) s += __builtin_amdgcn_exp2f((v[u][j] - base) * LOG2E);
+    }
+    // A border that at least n values reach: ceil(n / waves) threads of every wave whose lanes all have a value, or, where some wave has
+    // too few, n threads of one wave.
+    const int waves = min(hi - lo, CHUNK) / (64 * VALUES);
+    float bv = -INFINITY;
+    if (waves > 0) {                                                   // (a part of fewer fits into the buffer as it is)
+        float w = nth_of_wave(m, (a.n + waves - 1) / waves);
+        if (lane == 0) sh.border[wv] = w;
+        __syncthreads();
+        bv = sh.border[0];
+        for (int k = 1; k < waves; ++k) bv = fminf(bv, sh.border[k]);
+        if (bv == -INFINITY) {
+            __syncthreads();
+            w = nth_of_wave(m, a.n);
             if (lane == 0) sh.border[wv] = w;
             __syncthreads();
-            bv = sh.border[0];
-#pragma unroll
-            for (int k = 1; k < WAVES; ++k) bv = fminf(bv, sh.border[k]);
-            bi = bv == -INFINITY ? -1 : 0x7fffffff;
+            for (int k = 0; k < waves; ++k) bv = fmaxf(bv, sh.border[k]);
         }
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < VALUES; ++j) mine += better(v[j], at + j, bv, bi);
-        if (mine) {
-            int to = atomicAdd(&sh.count, mine);
-            if (to + mine > CAPACITY) {
-                sh.overflow = 1;
-            } else {
-#pragma unroll
-                for (int j = 0; j < VALUES; ++j)
-                    if (better(v[j], at + j, bv, bi)) sh.buf[to++] = {v[j], at + j};
-            }
-        }
+    } else {
         __syncthreads();
-        const bool over = sh.overflow;
-        int count = sh.count;
+    }
+    // the threads that have such values, and their vectors again, one a thread
+    if (m >= bv && m > -INFINITY) sh.who[atomicAdd(&sh.threads, 1)] = tid;
+    __syncthreads();
+    const int chunks = (hi - lo + CHUNK - 1) / CHUNK, vectors = sh.threads * chunks;
+    for (int e = tid; e < vectors; e += THREADS) {
+        const int k = e / chunks, own = lo + (e - k * chunks) * CHUNK + sh.who[k] * VALUES;
+        if (own >= hi) continue;
+        float v[VALUES];
+        values(fetch(own), own, v);
+        uint32_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) mine |= (uint32_t)(v[j] >= bv && v[j] > -INFINITY) << j;
+        if (!mine) continue;
+        int to = atomicAdd(&sh.count, __popc(mine));
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j)
+            if ((mine >> j & 1) && to < CAPACITY) sh.buf[to++] = {v[j], place(own) + j};
+    }
+    __syncthreads();
+    int kept = sh.count, bi = -1;
+    if (kept <= CAPACITY) {
+        kept = cut(sh, kept, a.n, bv, bi);
+    } else {
+        // more of one value than the buffer holds: everything anew, a value of each thread at a time, and the lowest tokens stay
         __syncthreads();
-        if (over) {                                                    // the chunk again, one value of each thread at a time
-            if (tid == 0) { sh.count = kept; sh.overflow = 0; }
-            __syncthreads();
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        bv = -INFINITY;
+        for (int c = lo + tid * VALUES; c - tid * VALUES < hi; c += CHUNK) {
+            float v[VALUES];
+            values(fetch(min(c, hi)), min(c, hi), v);
 #pragma unroll 1
             for (int j = 0; j < VALUES; ++j) {
                 float mine = v[0];
 #pragma unroll
                 for (int k = 1; k < VALUES; ++k) mine = j == k ? v[k] : mine;
-                if (better(mine, at + j, bv, bi)) sh.buf[atomicAdd(&sh.count, 1)] = {mine, at + j};
+                const int token = place(min(c, hi)) + j;
+                if (better(mine, token, bv, bi)) sh.buf[atomicAdd(&sh.count, 1)] = {mine, token};
                 __syncthreads();
-                count = sh.count;
+                const int count = sh.count;
                 __syncthreads();
-                if (count > KEPT) count = cut(sh, count, a.n, bv, bi);
+                if (count > KEPT) cut(sh, count, a.n, bv, bi);
             }
-        } else if (count > KEPT) {
-            count = cut(sh, count, a.n, bv, bi);
         }
-        kept = count;
+        kept = cut(sh, sh.count, a.n, bv, bi);
     }
-    kept = cut(sh, kept, a.n, bv, bi);
     if (tid < a.n) best[tid] = tid < kept ? sh.buf[tid] : Entry{-INFINITY, -1};
     // the part's maximum and sum
-    const float wm = wave_max_dpp(m), wbase = wm == -INFINITY ? 0.f : wm;
-    const float ws = wave_sum_dpp(s * __builtin_amdgcn_exp2f((m - wbase) * 1.4426950408889634f));
+    const float wm = wave_max_dpp(m);
+    const float ws = wave_sum_dpp(s * __builtin_amdgcn_exp2f((m - (wm == -INFINITY ? 0.f : wm)) * LOG2E));
     if (lane == 0) sh.sum[wv] = make_float2(wm, ws);
     __syncthreads();
     if (tid == 0) {
@@ -168,104 +217,128 @@ __global__ void __launch_bounds__(THREADS) k_beam_rows(Args a) {
         for (int k = 1; k < WAVES; ++k) M = fmaxf(M, sh.sum[k].x);
         const float b = M == -INFINITY ? 0.f : M;
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) S += sh.sum[k].y * __builtin_amdgcn_exp2f((sh.sum[k].x - b) * 1.4426950408889634f);
+        for (int k = 0; k < WAVES; ++k) S += sh.sum[k].y * __builtin_amdgcn_exp2f((sh.sum[k].x - b) * LOG2E);
         a.sums[(int64_t)row * a.splits + split] = make_float2(M, S);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ merge
-struct Total { double v; int64_t i; };     // score, beam V + token
-__device__ __forceinline__ bool better(const Total &x, const Total &y) { return x.v > y.v || (x.v == y.v && x.i < y.i); }
+struct Total { double v; int beam, token; };
+__device__ __forceinline__ bool better(const Total &x, const Total &y) {
+    return x.v > y.v || (x.v == y.v && (x.beam < y.beam || (x.beam == y.beam && x.token < y.token)));
+}
+constexpr Total NONE = {-INFINITY, 0x7fffffff, 0x7fffffff};
 
 struct MergeShared {
     // a continuation's total is (logit - top) + shift: 64 bits would lose the shift beside a type's lowest values
     double top[MOST_BEAMS], shift[MOST_BEAMS];      // largest logit; score - log of the sum, NaN: a beam without continuations
-    Total head[LISTS], border, out[MOST_N];
-    int good[MOST_N];
-    int count;
-    Total buf[MOST_N * MOST_N];            // at most n lists have a head at or before the border, of n entries each
+    float border[MERGE_WAVES];
+    int lists, count, good[LISTS];
+    Total out[MOST_N], best[MERGE_WAVES], buf[MERGED];
 };
 
-__global__ void __launch_bounds__(THREADS) k_beam_merge(Args a) {
-    extern __shared__ __align__(16) unsigned char merge_smem[];
-    MergeShared &sh = *(MergeShared *)merge_smem;
+// One block a request.  The parts' lists are in order, so a list whose first entry is behind the border has nothing to give.  The border
+// is taken as in k_beam_rows, of the lists' first totals, rounded to fp32 (which keeps their order): every total that is at least
+// the n-th best of these passes it.
+__global__ void __launch_bounds__(MERGE_THREADS) k_beam_merge(Args a) {
+    __shared__ MergeShared sh;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int64_t row0 = (int64_t)b * a.K;
-    for (int k = wv; k < a.K; k += WAVES) {
+    const int lists = a.K * a.splits;                                  // at most LISTS: one a thread
+    const Entry *const best = a.best + row0 * a.splits * a.n;
+    const int list = lane * MERGE_WAVES + wv, beam = list / a.splits;  // (every wave has some of them)
+    const Entry head = list < lists ? best[(int64_t)list * a.n] : Entry{-INFINITY, -1};
+    if (tid == 0) { sh.lists = 0; sh.count = 0; }
+    for (int k = wv; k < a.K; k += MERGE_WAVES) {
         // (splits are at most a wave's lanes)
+        const float score = a.scores[row0 + k];
         const float2 p = lane < a.splits ? a.sums[(row0 + k) * a.splits + lane] : make_float2(-INFINITY, 0.f);
-        float bad = p.x != p.x || !(p.y < INFINITY) || p.x == INFINITY ? 1.f : 0.f;
-        bad = wave_max_dpp(bad);
+        const bool bad = __any(p.x != p.x || !(p.y < INFINITY) || p.x == INFINITY);
         const float M = wave_max_dpp(p.x);
-        double s = M > -INFINITY ? (double)p.y * exp((double)p.x - (double)M) : 0.0;
+        double s = M > -INFINITY ? (double)(p.y * __builtin_amdgcn_exp2f((p.x - M) * LOG2E)) : 0.0;
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
         if (lane == 0) {
-            const float score = a.scores[row0 + k];
             sh.top[k] = (double)M;
-            sh.shift[k] = bad > 0.f || !(s > 0.0) || !alive(score) ? (double)NAN : (double)score - log(s);
+            sh.shift[k] = bad || !(s > 0.0) || !alive(score) ? (double)NAN : (double)score - log(s);
         }
     }
-    if (tid == 0) { sh.count = 0; sh.border = {-INFINITY, -1}; }
     __syncthreads();
-    const int lists = a.K * a.splits;
-    const Entry *const best = a.best + row0 * a.splits * a.n;
-    auto total_of = [&](int list, int j) -> Total {
-        const int k = list / a.splits;
-        const Entry e = best[(int64_t)list * a.n + j];
+    auto total_of = [&](const Entry &e, int k) -> Total {
+        if (e.i < 0) return NONE;
         const double v = ((double)e.v - sh.top[k]) + sh.shift[k];
-        return e.i < 0 || v != v ? Total{-INFINITY, -1} : Total{v, (int64_t)k * a.V + e.i};
+        return v > -INFINITY ? Total{v, k, e.i} : NONE;
     };
-    for (int l = tid; l < lists; l += THREADS) {
-        Total h = total_of(l, 0);
-        if (h.i < 0) h.i = ((int64_t)1 << 62) + l;                     // lists without entries come last, in a definite order
-        sh.head[l] = h;
-    }
+    Total mine = list < lists ? total_of(head, beam) : NONE;
+    const float top = (float)mine.v;
+    const float w = nth_of_wave(top, (a.n + MERGE_WAVES - 1) / MERGE_WAVES);
+    if (lane == 0) sh.border[wv] = w;
     __syncthreads();
-    for (int l = tid; l < lists; l += THREADS) {
-        const Total h = sh.head[l];
-        int rank = 0;
-        for (int j = 0; j < lists; ++j) rank += better(sh.head[j], h);
-        if (rank < a.n) sh.good[rank] = l;
-        if (rank == a.n - 1 && h.v > -INFINITY) sh.border = h;
-    }
+    float border = sh.border[0];
+#pragma unroll
+    for (int k = 1; k < MERGE_WAVES; ++k) border = fminf(border, sh.border[k]);
+    if (top >= border && mine.v > -INFINITY) sh.good[atomicAdd(&sh.lists, 1)] = list;
     __syncthreads();
-    const int lists_in = min(lists, a.n);
-    const Total border = sh.border;
-    for (int e = tid; e < lists_in * a.n; e += THREADS) {
-        const int g = e / a.n;
-        const Total t = total_of(sh.good[g], e - g * a.n);
-        if (t.v > -INFINITY && !better(border, t)) sh.buf[atomicAdd(&sh.count, 1)] = t;
+    const int entries = sh.lists * a.n;
+    for (int e = tid; e < entries; e += MERGE_THREADS) {
+        const int g = sh.good[e / a.n];
+        const Total t = total_of(best[(int64_t)g * a.n + e % a.n], g / a.splits);
+        if ((float)t.v >= border && t.v > -INFINITY) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < MERGED) sh.buf[at] = t;
+        }
     }
     __syncthreads();
     const int count = sh.count, found = min(count, a.n);
-    for (int e = tid; e < count; e += THREADS) {
-        const Total t = sh.buf[e];
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += better(sh.buf[j], t);
-        if (rank < a.n) sh.out[rank] = t;
+    if (count <= MERGED) {
+        for (int e = tid / 8; e < count; e += MERGE_THREADS / 8) {     // 8 threads an entry
+            const Total t = sh.buf[e];
+            int rank = 0;
+            for (int j = tid & 7; j < count; j += 8) rank += better(sh.buf[j], t);
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor(rank, o);
+            if ((tid & 7) == 0 && rank < a.n) sh.out[rank] = t;
+        }
+        __syncthreads();
+    } else {                                                           // equal totals in most lists: one place after the other
+        int at = 0;
+        for (int place = 0; place < a.n; ++place) {
+            Total t = mine;
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) {
+                const Total u = {__shfl_xor(t.v, o), __shfl_xor(t.beam, o), __shfl_xor(t.token, o)};
+                if (better(u, t)) t = u;
+            }
+            if (lane == 0) sh.best[wv] = t;
+            __syncthreads();
+            t = sh.best[0];
+            for (int k = 1; k < MERGE_WAVES; ++k)
+                if (better(sh.best[k], t)) t = sh.best[k];
+            if (tid == 0) sh.out[place] = t;
+            if (mine.v > -INFINITY && mine.beam == t.beam && mine.token == t.token)
+                mine = ++at < a.n ? total_of(best[(int64_t)list * a.n + at], beam) : NONE;
+            __syncthreads();
+        }
     }
-    __syncthreads();
     if (wv != 0) return;
     // one wave: place i of the n best, and those among them that go on
     const bool have = lane < found;
-    const Total t = have ? sh.out[lane] : Total{-INFINITY, -1};
-    const int beam = have ? (int)(t.i / a.V) : -1, token = have ? (int)(t.i - (int64_t)beam * a.V) : -1;
+    const Total t = have ? sh.out[lane] : Total{-INFINITY, -1, -1};
     if (lane < a.n) {
         const int64_t o = (int64_t)b * a.n + lane;
         a.out_score[o] = (float)t.v;
-        a.out_beam[o] = beam;
-        a.out_token[o] = token;
+        a.out_beam[o] = t.beam;
+        a.out_token[o] = t.token;
     }
     bool on = have;
-    for (int k = 0; k < a.n_eos; ++k) on &= token != a.eos[k];
+    for (int k = 0; k < a.n_eos; ++k) on &= t.token != a.eos[k];
     const uint64_t going = __ballot(on);
     const int at = __popcll(going & (((uint64_t)1 << lane) - 1)), n = min(__popcll(going), a.K);
     if (on && at < a.K) {
         const int64_t o = row0 + at;
         a.next_score[o] = (float)t.v;
-        a.next_row[o] = (int)(row0 + beam);
-        a.next_token[o] = token;
+        a.next_row[o] = (int)(row0 + t.beam);
+        a.next_token[o] = t.token;
     }
     if (lane >= n && lane < a.K) {
         const int64_t o = row0 + lane;

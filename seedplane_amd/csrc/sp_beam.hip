@@ -8,10 +8,10 @@
 
 namespace {
 
-// Parts of a row: enough blocks to fill the chip twice, as many lists as the merge takes, at least a chunk each.
+// Parts of a row: blocks for every wave that the chip holds (8 a CU), as many lists as the merge takes, at least a chunk each.
 int splits_of(int64_t rows, int beams, int vocab) {
-    const int most = std::min({beam::MOST_SPLITS, beam::LISTS / beams, std::max(1, (vocab + beam::CHUNK / 2 - 1) / (beam::CHUNK / 2))});
-    return (int)std::max<int64_t>(1, std::min<int64_t>(most, std::max<int64_t>(beam::LEAST_SPLITS, 512 / rows)));
+    const int most = std::min({beam::MOST_SPLITS, beam::LISTS / beams, (vocab + beam::CHUNK - 1) / beam::CHUNK});
+    return (int)std::max<int64_t>(1, std::min<int64_t>(most, std::max<int64_t>(beam::LEAST_SPLITS, 2048 / rows)));
 }
 void check_beams(int batch, int beams, int vocab, int n) {
     require(batch >= 0 && beams >= 1 && beams <= beam::MOST_BEAMS && n >= beams && n <= beam::MOST_N, SP_EINVAL,
@@ -21,9 +21,9 @@ void check_beams(int batch, int beams, int vocab, int n) {
 }
 
 template <class T>
-void rows_of(bool aligned, const beam::Args &a, hipStream_t st) {
+void rows_of(const beam::Args &a, hipStream_t st) {
     const dim3 grid(a.splits, a.B * a.K), block(beam::THREADS);
-    if (aligned) hipLaunchKernelGGL((beam::k_beam_rows<T, true>), grid, block, 0, st, a);
+    if (a.V < beam::VALUES) hipLaunchKernelGGL((beam::k_beam_rows<T, true>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((beam::k_beam_rows<T, false>), grid, block, 0, st, a);
 }
 
@@ -56,22 +56,19 @@ int sp_op_beam_select(int32_t dtype, const void *logits_dev, int64_t ld, int32_t
         a.B = n_batch; a.K = n_beams; a.V = vocab; a.n = n;
         const int64_t rows = (int64_t)n_batch * n_beams;
         a.splits = splits_of(rows, n_beams, vocab);
-        a.len = ((vocab + a.splits - 1) / a.splits + 7) / 8 * 8;
+        a.len = ((vocab + a.splits - 1) / a.splits + beam::VALUES - 1) / beam::VALUES * beam::VALUES;
         a.best = (beam::Entry *)workspace_dev;
         a.sums = (float2 *)(a.best + rows * a.splits * n);
         a.out_score = out_scores_dev; a.out_beam = out_beams_dev; a.out_token = out_tokens_dev;
         a.next_score = next_scores_dev; a.next_row = next_rows_dev; a.next_token = next_tokens_dev;
         a.n_eos = n_eos;
         for (int i = 0; i < n_eos; ++i) a.eos[i] = eos[i];
-        const int b = dtype == SP_DT_F32 ? 4 : 2;
-        const bool aligned = ((uintptr_t)logits_dev & 15) == 0 && ld * b % 16 == 0;
         const hipStream_t st = (hipStream_t)stream;
-        if (dtype == SP_DT_F32) rows_of<float>(aligned, a, st);
-        else if (dtype == SP_DT_F16) rows_of<f16>(aligned, a, st);
-        else rows_of<paged::bf16>(aligned, a, st);
+        if (dtype == SP_DT_F32) rows_of<float>(a, st);
+        else if (dtype == SP_DT_F16) rows_of<f16>(a, st);
+        else rows_of<paged::bf16>(a, st);
         HIPCHK(hipGetLastError());
-        const size_t lds = offsetof(beam::MergeShared, buf) + sizeof(beam::Total) * std::min(n, n_beams * a.splits) * n;
-        hipLaunchKernelGGL(beam::k_beam_merge, dim3(n_batch), dim3(beam::THREADS), lds, st, a);
+        hipLaunchKernelGGL(beam::k_beam_merge, dim3(n_batch), dim3(beam::MERGE_THREADS), 0, st, a);
         HIPCHK(hipGetLastError());
     });
 }

@@ -7,7 +7,7 @@
 //
 // A workgroup takes a chunk of rows of the call (a row whose block an earlier row has is left to that row's workgroup), keys or
 // values, and some heads: it looks up its block's rows among all of the call's, takes the largest magnitude per head, then the codes.
-// Values are read twice rather than kept: a block of 64 positions of one head alone is 8192 values.
+// Values are read twice unless a thread has but one item of them: a block of 64 positions of one head alone is 8192 values.
 #pragma once
 #include "sp_paged.h"
 
@@ -15,6 +15,7 @@ namespace paged {
 
 constexpr int MOST_BLOCK = 128;                                        // positions of a block at most
 constexpr int BLOCK_HEADS = 64;                                        // heads of a workgroup at most
+constexpr int SEARCHED = 8;                                            // rows that a thread looks at at once
 constexpr float MOST_SCALE = 0x1p60f;                                  // (scales within 2^-60 .. 2^60: attention takes their products)
 
 struct BlockAppendArgs : AppendArgs {                                  // ks, vs are not used; units, tail, vecs are a head's
@@ -100,34 +101,49 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
     return v;
 }
 
+// Whether row i is of block b of sequence s.
+__device__ __forceinline__ bool of_block(const BlockAppendArgs &a, int seq, int at, int s, int b) {
+    return seq == s && at >= 0 && at < (1 << 30) && at / a.by_block == b;
+}
+
+// The block of row r, which does not follow a row of the same block.
 template <class T, int VEC, bool I8>
 __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, bool keys, int head0, BlockShared &sh, float2 *cs) {
     const int tid = threadIdx.x, s = a.seq[r], p = a.at[r];
     if (s < 0 || s >= a.n_seq || p < 0 || p >= (1 << 30)) return;
     const int b = p / a.by_block, page = p / a.by_page;
-    auto same = [&](int i) { const int q = a.at[i]; return a.seq[i] == s && q >= 0 && q < (1 << 30) && q / a.by_block == b; };
-    if (page >= a.max_pages || (r > 0 && same(r - 1))) return;
-    const int e = a.table[(int64_t)s * a.max_pages + page];
-    if (e < 0 || e >= a.n_pages) return;
+    if (page >= a.max_pages) return;
+    const int e = a.table[(int64_t)s * a.max_pages + page];            // (awaited after the search)
     __syncthreads();                                                   // the block before has been written
-    for (int i = tid; i < a.block; i += blockDim.x) sh.slot[i] = -1;
+    for (int i = tid; i < a.block; i += ROT_THREADS) sh.slot[i] = -1;
     if (tid < a.heads) sh.most[tid] = 0;
     if (tid == 0) sh.earlier = 0;
     __syncthreads();
-    for (int i = tid; i < a.rows; i += blockDim.x) {
-        if (!same(i)) continue;
-        if (i < r) sh.earlier = 1;
-        else atomicMax(&sh.slot[a.at[i] - b * a.block], i);
+    for (int i0 = tid; i0 < a.rows; i0 += ROT_THREADS * SEARCHED) {
+        int seq[SEARCHED], at[SEARCHED];
+#pragma unroll
+        for (int k = 0; k < SEARCHED; ++k) {
+            const int i = min(i0 + k * ROT_THREADS, a.rows - 1);
+            seq[k] = a.seq[i];
+            at[k] = a.at[i];
+        }
+#pragma unroll
+        for (int k = 0; k < SEARCHED; ++k) {
+            const int i = min(i0 + k * ROT_THREADS, a.rows - 1);
+            if (!of_block(a, seq[k], at[k], s, b)) continue;
+            if (i < r) sh.earlier = 1;
+            else atomicMax(&sh.slot[at[k] - b * a.block], i);
+        }
     }
     __syncthreads();
-    if (sh.earlier) return;
+    if (sh.earlier || e < 0 || e >= a.n_pages) return;
     const int heads = min(a.heads, a.nkv - head0), half = a.rot.rot >> 1;
     const int64_t block_of_page = b - (int64_t)page * a.per_page;
     float *const scale = (keys ? a.kscale : a.vscale) + ((int64_t)e * a.nkv + head0) * a.per_page + block_of_page;      // of head h: at h * per_page
     const float old = tid < heads ? scale[(int64_t)tid * a.per_page] : 0.f;
     const bool begun = sh.slot[0] >= 0;
     if (keys && half) {
-        for (int k = tid; k < a.block * half; k += blockDim.x) {
+        for (int k = tid; k < a.block * half; k += ROT_THREADS) {
             const int i = k / a.by_half, row = sh.slot[i];
             if (row >= 0) cs[k] = turn_of(a.rot, a.pos[row], k - i * half);
         }
@@ -151,7 +167,8 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, bo
         if (two) turn_unit<VEC>(a.rot, cs + i * half + u * VEC, v1, v2);
     };
     float v1[VEC], v2[VEC];
-    for (int k0 = 0; k0 < total; k0 += blockDim.x) {
+    const bool held = total <= ROT_THREADS && heads == 1;              // one item a thread: its values stay in registers
+    for (int k0 = 0; k0 < total; k0 += ROT_THREADS) {
         const int k = min(k0 + tid, total - 1), i = k / by, u = k - i * per, row = sh.slot[i];
         int at1, at2;
         const bool two = offsets(u, at1, at2);
@@ -177,7 +194,7 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, bo
         scale[(int64_t)tid * a.per_page] = grown;
     }
     __syncthreads();
-    for (int k = tid; k < total; k += blockDim.x) {
+    for (int k = tid; k < total; k += ROT_THREADS) {
         const int i = k / by, u = k - i * per, row = sh.slot[i];
         int at1, at2;
         const bool two = offsets(u, at1, at2);
@@ -185,7 +202,7 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, bo
             uint8_t *const to = pool + h * a.head_stride + i * a.row_stride;
             const float f = row >= 0 ? sh.scale[h] : sh.keep[h];
             if (row >= 0) {
-                fetch(row, h, i, u, at1, at2, two, v1, v2);
+                if (!held) fetch(row, h, i, u, at1, at2, two, v1, v2);
             } else {
                 if (f == 1.f) continue;
                 load_codes<I8, VEC>(to + at1, v1);
@@ -210,8 +227,15 @@ __global__ void __launch_bounds__(ROT_THREADS) k_append_blocks(BlockAppendArgs a
         return;
     }
     const int chunk = blockIdx.x / parts, part = blockIdx.x - chunk * parts;
-    const int r0 = chunk * a.chunk, r1 = min(r0 + a.chunk, a.rows);
-    for (int r = r0; r < r1; ++r) append_block<T, VEC, I8>(a, r, part < a.splits, part % a.splits * a.heads, sh, (float2 *)block_smem);
+    // the chunk's rows that begin a run of a block's rows (every wave finds the same)
+    const int r = chunk * a.chunk + (int)(threadIdx.x & 63);
+    bool begins = r < a.rows && r < (chunk + 1) * a.chunk;
+    if (begins && r > 0) {
+        const int s = a.seq[r], p = a.at[r];
+        begins = p < 0 || p >= (1 << 30) || !of_block(a, a.seq[r - 1], a.at[r - 1], s, p / a.by_block);
+    }
+    for (uint64_t runs = __ballot(begins); runs; runs &= runs - 1)
+        append_block<T, VEC, I8>(a, chunk * a.chunk + __builtin_ctzll(runs), part < a.splits, part % a.splits * a.heads, sh, (float2 *)block_smem);
 }
 
 // ------------------------------------------------------------------------------------------------ read

@@ -6,15 +6,20 @@
 // taken lowest first, in the order of sequences and positions, so results do not depend on the order in which blocks run.
 //
 // The tables are small and their updates a few dependent steps, bound by latency: one block does what needs an order (ranks of free
-// pages by scans), a block per sequence what does not, and the last of those to finish goes on as the one.  The copies are bound by
-// memory: 16 bytes a thread, a block per (page, layer's keys or values).
+// pages by scans), the rows of a fork too unless they are many.  The copies are bound by memory: 16 bytes a thread, a block per (page,
+// layer's keys or values).
 #pragma once
 #include "sp_device.h"
 
 namespace pages {
 
 constexpr int THREADS = 256;               // per sequence, and of copies
-constexpr int SCAN = 1024, PER = 8;        // threads of the ordered steps, pages of each at a time
+constexpr int PER = 8;                     // pages of each thread at a time in the ordered steps
+// Threads of the ordered steps: few where that does the tables and pages in a turn or two (a block of 16 waves starts later and its barriers
+// take longer), else as many as a block has.
+constexpr int FEW = 256, MANY = 1024;
+constexpr int ROWS_IN_ONE = 16384;         // sequences x pages up to which a fork's one block makes the rows too
+constexpr int SEQS_IN_ONE = 2048;
 
 struct Move { int src, dst, rows; };       // pages, rows of each head
 struct Pool {                              // see sp_page_pool
@@ -24,14 +29,15 @@ struct Pool {                              // see sp_page_pool
     int n_pools, n_pages, page, nkv, width_bytes, block, per_page, S, width;      // width_bytes: of a row's values
     bool aligned;                                                      // every row to 16 bytes
     // workspace
-    int *arrived;                          // [0] blocks that have finished, [1] moves
+    int *counts;                           // moves; held pages
     int *fresh, *first;                    // [S] new lengths; [S + 1] places of each sequence's pages among those wanted
     int *rows;                             // [S][width] new table
     int *list;                             // [n_pages] free pages taken
     Move *moves;                           // [max(S, n_pages)]
 };
 
-// Exclusive sum over the block of one value per thread, and the total.  SCAN threads.
+// Exclusive sum over the block's N threads of one value each, and the total.
+template <int N>
 __device__ __forceinline__ int block_rank(int v, int *wave_sums, int &total) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     int x = v;
@@ -46,7 +52,7 @@ __device__ __forceinline__ int block_rank(int v, int *wave_sums, int &total) {
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int k = 0; k < SCAN / 64; ++k) {
+    for (int k = 0; k < N / 64; ++k) {
         const int w = wave_sums[k];
         before += k < wv ? w : 0;
         total += w;
@@ -54,10 +60,11 @@ __device__ __forceinline__ int block_rank(int v, int *wave_sums, int &total) {
     return before + x - v;
 }
 
-// The lowest `want` free pages in order to list; returns how many there are.  SCAN threads.
+// The lowest `want` free pages in order to list; returns how many there are.
+template <int N>
 __device__ __forceinline__ int take_free(const int *holders, int n_pages, int want, int *list, int *wave_sums) {
     int found = 0;
-    for (int e0 = 0; e0 < n_pages && found < want; e0 += SCAN * PER) {
+    for (int e0 = 0; e0 < n_pages && found < want; e0 += N * PER) {
         const int at = e0 + (int)threadIdx.x * PER;
         bool free[PER];
         int mine = 0, total;
@@ -66,7 +73,7 @@ __device__ __forceinline__ int take_free(const int *holders, int n_pages, int wa
             free[j] = at + j < n_pages && holders[at + j] == 0;
             mine += free[j];
         }
-        int rank = found + block_rank(mine, wave_sums, total);
+        int rank = found + block_rank<N>(mine, wave_sums, total);
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             if (free[j] && rank < want) list[rank++] = at + j;
@@ -76,65 +83,82 @@ __device__ __forceinline__ int take_free(const int *holders, int n_pages, int wa
     return min(found, want);
 }
 
-// Whether this block is the last of gridDim.x to come here; its thread then sees what the others wrote.
-__device__ __forceinline__ bool last_block(int *arrived) {
-    __shared__ int last_s;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int n = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-        last_s = n == (int)gridDim.x - 1;
-        if (last_s) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (last_s) __threadfence();
-    return last_s;
-}
-
 // ------------------------------------------------------------------------------------------------ fork
-// A block per sequence: its new row, holders of what changes.  The last block then takes pages for the copies.
-__global__ void __launch_bounds__(SCAN) k_fork(Pool a, const int *parents) {
-    __shared__ int wave_sums[SCAN / 64], earlier;
-    const int s = blockIdx.x, tid = threadIdx.x;
-    {
-        const int p = parents[s];
-        const bool valid = p >= 0 && p < a.S;
-        const int len = valid ? min(a.lengths[p], a.width * a.page) : 0, full = len / a.page, rest = len - full * a.page;
-        if (tid == 0) earlier = 0;
-        __syncthreads();
-        if (valid && rest)
-            for (int i = tid; i < s; i += blockDim.x)
-                if (parents[i] == p) earlier = 1;
-        __syncthreads();
-        // (a last page that the parent does not have is missing in its children too)
-        const bool copy = earlier && a.table[(int64_t)p * a.width + full] >= 0;
-        const int keep = full + (rest && !copy);
-        for (int j = tid; j < a.width; j += blockDim.x) {
-            const int now = a.table[(int64_t)s * a.width + j], e = j < keep ? a.table[(int64_t)p * a.width + j] : -1;
-            a.rows[(int64_t)s * a.width + j] = e;
-            if (e != now) {
-                if (now >= 0 && now < a.n_pages) atomicSub(&a.holders[now], 1);
-                if (e >= 0 && e < a.n_pages) atomicAdd(&a.holders[e], 1);
-            }
-        }
-        if (tid == 0) {
-            a.fresh[s] = len;
-            a.first[s] = copy ? rest : 0;
-        }
+// A sequence's new row: its length, the pages that it holds in common with its parent, and rows of a last page to copy (0: none).
+// A last page that the parent does not have is missing in its children too.
+struct Child { int parent, len, keep, copy; };
+__device__ __forceinline__ Child child_of(const Pool &a, int p) {
+    if (p < 0 || p >= a.S) return {-1, 0, 0, 0};
+    const int len = min(max(a.lengths[p], 0), a.width * a.page), full = len / a.page, rest = len - full * a.page;
+    const bool has = rest && a.table[(int64_t)p * a.width + full] >= 0;
+    return {p, len, full + (rest > 0), has ? rest : 0};
+}
+// Entry (s, j): what the new row holds, and holders of what changes.
+__device__ __forceinline__ void fork_entry(const Pool &a, int s, int j, int parent, int keep) {
+    const int64_t at = (int64_t)s * a.width + j;
+    const int now = a.table[at], e = j < keep ? a.table[(int64_t)parent * a.width + j] : -1;
+    a.rows[at] = e;
+    if (e != now) {
+        if (now >= 0 && now < a.n_pages) atomicSub(&a.holders[now], 1);
+        if (e >= 0 && e < a.n_pages) atomicAdd(&a.holders[e], 1);
     }
-    if (!last_block(a.arrived)) return;
-    // places of the copies, in order of sequences
+}
+// A wave a sequence: the first child of a parent keeps its last page.
+__global__ void __launch_bounds__(THREADS) k_fork_rows(Pool a, const int *parents) {
+    const int s = blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (s >= a.S) return;
+    Child c = child_of(a, parents[s]);
+    bool earlier = false;
+    if (c.copy)
+        for (int i = lane; i < s; i += 64) earlier |= parents[i] == c.parent;
+    if (__any(earlier)) --c.keep;
+    else c.copy = 0;
+    for (int j = lane; j < a.width; j += 64) fork_entry(a, s, j, c.parent, c.keep);
+    if (lane == 0) {
+        a.fresh[s] = c.len;
+        a.first[s] = c.copy;
+    }
+}
+// Pages for the copies, in the order of sequences.  One block; ROWS: it makes the rows too.
+template <bool ROWS, int N>
+__global__ void __launch_bounds__(N) k_fork(Pool a, const int *parents) {
+    __shared__ int wave_sums[N / 64], first_s[ROWS ? SEQS_IN_ONE : 1], keep_s[ROWS ? SEQS_IN_ONE : 1];
+    const int tid = threadIdx.x;
+    if constexpr (ROWS) {
+        for (int s = tid; s < a.S; s += N) first_s[s] = a.S;
+        __syncthreads();
+        for (int s = tid; s < a.S; s += N) {
+            const Child c = child_of(a, parents[s]);
+            if (c.copy) atomicMin(&first_s[c.parent], s);
+            keep_s[s] = c.keep;
+            a.fresh[s] = c.len;
+            a.first[s] = c.copy;
+        }
+        __syncthreads();
+        for (int s = tid; s < a.S; s += N)
+            if (a.first[s]) {
+                if (first_s[parents[s]] == s) a.first[s] = 0;
+                else --keep_s[s];
+            }
+        __syncthreads();
+        const int entries = a.S * a.width;
+        for (int i = tid; i < entries; i += N) {
+            const int s = i / a.width;
+            fork_entry(a, s, i - s * a.width, parents[s], keep_s[s]);
+        }
+        __syncthreads();
+    }
     int wanted = 0;
-    for (int s0 = 0; s0 < a.S; s0 += SCAN) {
+    for (int s0 = 0; s0 < a.S; s0 += N) {
         const int s = s0 + tid, rest = s < a.S ? a.first[s] : 0;
         int total;
-        const int at = wanted + block_rank(rest > 0, wave_sums, total);
+        const int at = wanted + block_rank<N>(rest > 0, wave_sums, total);
         if (rest > 0) a.moves[at] = {s, -1, rest};
         wanted += total;
     }
     __syncthreads();
-    const int got = take_free(a.holders, a.n_pages, wanted, a.list, wave_sums);
-    for (int k = tid; k < wanted; k += SCAN) {
+    const int got = take_free<N>(a.holders, a.n_pages, wanted, a.list, wave_sums);
+    for (int k = tid; k < wanted; k += N) {
         const int s = a.moves[k].src, full = a.fresh[s] / a.page, p = parents[s];
         const int src = a.table[(int64_t)p * a.width + full], dst = k < got ? a.list[k] : -1;
         if (dst >= 0) a.holders[dst] = 1;
@@ -143,7 +167,7 @@ __global__ void __launch_bounds__(SCAN) k_fork(Pool a, const int *parents) {
         a.moves[k].dst = dst;
     }
     if (tid == 0) {
-        a.arrived[1] = got;
+        a.counts[0] = got;
         if (wanted > got) *a.missing += wanted - got;
     }
 }
@@ -202,16 +226,17 @@ __global__ void __launch_bounds__(THREADS) k_fork_copy(Pool a) {
         for (int j = threadIdx.x; j < a.width; j += blockDim.x) a.table[(int64_t)k * a.width + j] = a.rows[(int64_t)k * a.width + j];
         if (threadIdx.x == 0) a.lengths[k] = a.fresh[k];
     }
-    if (k < a.arrived[1]) copy_page(a, pool, a.moves[k]);
+    if (k < a.counts[0]) copy_page(a, pool, a.moves[k]);
 }
 
 // ------------------------------------------------------------------------------------------------ growth, ends
 // counts[s] new positions of each sequence: pages for those that have none yet.  One block.
-__global__ void __launch_bounds__(SCAN) k_grow(Pool a, const int *counts) {
-    __shared__ int wave_sums[SCAN / 64];
+template <int N>
+__global__ void __launch_bounds__(N) k_grow(Pool a, const int *counts) {
+    __shared__ int wave_sums[N / 64];
     const int tid = threadIdx.x;
     int wanted = 0;
-    for (int s0 = 0; s0 < a.S; s0 += SCAN) {
+    for (int s0 = 0; s0 < a.S; s0 += N) {
         const int s = s0 + tid;
         int need = 0, total;
         if (s < a.S) {
@@ -219,14 +244,14 @@ __global__ void __launch_bounds__(SCAN) k_grow(Pool a, const int *counts) {
             need = max(0, (int)((grown + a.page - 1) / a.page - (len + a.page - 1) / a.page));
             a.fresh[s] = (int)grown;
         }
-        const int at = wanted + block_rank(need, wave_sums, total);
+        const int at = wanted + block_rank<N>(need, wave_sums, total);
         if (s < a.S) a.first[s] = at;
         wanted += total;
     }
     if (tid == 0) a.first[a.S] = wanted;
     __syncthreads();
-    const int got = take_free(a.holders, a.n_pages, min(wanted, a.n_pages), a.list, wave_sums);
-    for (int s = tid >> 4; s < a.S; s += SCAN / 16) {                  // 16 threads a sequence
+    const int got = take_free<N>(a.holders, a.n_pages, min(wanted, a.n_pages), a.list, wave_sums);
+    for (int s = tid >> 4; s < a.S; s += N / 16) {                  // 16 threads a sequence
         const int at = a.first[s], n = a.first[s + 1] - at, have = (a.lengths[s] + a.page - 1) / a.page;
         for (int j = tid & 15; j < n; j += 16) {
             const int e = at + j < got ? a.list[at + j] : -1;
@@ -236,7 +261,7 @@ __global__ void __launch_bounds__(SCAN) k_grow(Pool a, const int *counts) {
     }
     __syncthreads();
     int over = 0;
-    for (int s = tid; s < a.S; s += SCAN) {
+    for (int s = tid; s < a.S; s += N) {
         over += max(a.lengths[s] + (int64_t)max(counts[s], 0) - a.fresh[s], (int64_t)0) > 0;
         a.lengths[s] = a.fresh[s];
     }
@@ -257,20 +282,21 @@ __global__ void __launch_bounds__(THREADS) k_free(Pool a, const int *seqs) {
 // ------------------------------------------------------------------------------------------------ compaction
 // Held pages at or behind U, the number of held pages, go to the free pages before it, in order.  One block.  places (may be NULL): where
 // each page is afterwards.
-__global__ void __launch_bounds__(SCAN) k_compact(Pool a, int *places) {
-    __shared__ int wave_sums[SCAN / 64];
+template <int N>
+__global__ void __launch_bounds__(N) k_compact(Pool a, int *places) {
+    __shared__ int wave_sums[N / 64];
     const int tid = threadIdx.x;
     int held = 0;
-    for (int e0 = 0; e0 < a.n_pages; e0 += SCAN * PER) {
+    for (int e0 = 0; e0 < a.n_pages; e0 += N * PER) {
         const int at = e0 + tid * PER;
         int mine = 0, total;
 #pragma unroll
         for (int j = 0; j < PER; ++j) mine += at + j < a.n_pages && a.holders[at + j] != 0;
-        block_rank(mine, wave_sums, total);
+        block_rank<N>(mine, wave_sums, total);
         held += total;
     }
     int moves = 0;
-    for (int e0 = held; e0 < a.n_pages; e0 += SCAN * PER) {
+    for (int e0 = held; e0 < a.n_pages; e0 += N * PER) {
         const int at = e0 + tid * PER;
         bool used[PER];
         int mine = 0, total;
@@ -279,31 +305,31 @@ __global__ void __launch_bounds__(SCAN) k_compact(Pool a, int *places) {
             used[j] = at + j < a.n_pages && a.holders[at + j] != 0;
             mine += used[j];
         }
-        int rank = moves + block_rank(mine, wave_sums, total);
+        int rank = moves + block_rank<N>(mine, wave_sums, total);
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             if (used[j]) a.moves[rank++].src = at + j;
         moves += total;
     }
-    const int low = take_free(a.holders, held, moves, a.list, wave_sums);         // (as many as there are moves)
-    for (int k = tid; k < low; k += SCAN) {
+    const int low = take_free<N>(a.holders, held, moves, a.list, wave_sums);         // (as many as there are moves)
+    for (int k = tid; k < low; k += N) {
         const int src = a.moves[k].src, dst = a.list[k];
         a.moves[k].dst = dst;
         a.moves[k].rows = a.page;
         a.holders[dst] = a.holders[src];
     }
     if (places)
-        for (int e = tid; e < a.n_pages; e += SCAN) places[e] = e;
+        for (int e = tid; e < a.n_pages; e += N) places[e] = e;
     __syncthreads();
     if (places)
-        for (int k = tid; k < low; k += SCAN) places[a.moves[k].src] = a.moves[k].dst;
-    for (int k = tid; k < low; k += SCAN) a.holders[a.moves[k].src] = 0;
-    if (tid == 0) { a.arrived[1] = low; a.arrived[2] = held; }
+        for (int k = tid; k < low; k += N) places[a.moves[k].src] = a.moves[k].dst;
+    for (int k = tid; k < low; k += N) a.holders[a.moves[k].src] = 0;
+    if (tid == 0) { a.counts[0] = low; a.counts[1] = held; }
 }
 // The compaction's copies, (pool, move) pairs over the grid, and the tables: a page behind the last held one is found among the moves,
 // whose sources are in order.
 __global__ void __launch_bounds__(THREADS) k_compact_copy(Pool a) {
-    const int moves = a.arrived[1], held = a.arrived[2];
+    const int moves = a.counts[0], held = a.counts[1];
     const int64_t entries = (int64_t)a.S * a.width, stride = (int64_t)gridDim.x * blockDim.x;
     if (moves == 0) return;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < entries; i += stride) {

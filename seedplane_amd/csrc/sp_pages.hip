@@ -52,7 +52,7 @@ pages::Pool pool_args(const sp_page_pool *p) {
     a.aligned = p->aligned16 && (a.page_bytes | a.head_bytes | a.row_bytes | a.width_bytes) % 16 == 0;
     const Places at = places_of(a.S, a.width, a.n_pages);
     uint8_t *const w = (uint8_t *)p->workspace_dev;
-    a.arrived = (int *)w;
+    a.counts = (int *)w;
     a.fresh = (int *)(w + at.fresh);
     a.first = (int *)(w + at.first);
     a.rows = (int *)(w + at.rows);
@@ -60,6 +60,8 @@ pages::Pool pool_args(const sp_page_pool *p) {
     a.moves = (pages::Move *)(w + at.moves);
     return a;
 }
+
+bool few(const pages::Pool &a) { return a.S <= pages::FEW && a.n_pages <= 2 * pages::FEW * pages::PER && (int64_t)a.S * a.width <= 8 * pages::FEW; }
 
 }  // namespace
 
@@ -73,7 +75,16 @@ int sp_op_pages_fork(const sp_page_pool *pool, const int32_t *parents_dev, void 
     return guarded([&] {
         const pages::Pool a = pool_args(pool);
         require(parents_dev != nullptr, SP_EINVAL, "NULL pointer");
-        hipLaunchKernelGGL(pages::k_fork, dim3(a.S), dim3(pages::SCAN), 0, (hipStream_t)stream, a, parents_dev);
+        const hipStream_t st = (hipStream_t)stream;
+        if ((int64_t)a.S * a.width <= pages::ROWS_IN_ONE && a.S <= pages::SEQS_IN_ONE) {
+            if (few(a)) hipLaunchKernelGGL((pages::k_fork<true, pages::FEW>), dim3(1), dim3(pages::FEW), 0, st, a, parents_dev);
+            else hipLaunchKernelGGL((pages::k_fork<true, pages::MANY>), dim3(1), dim3(pages::MANY), 0, st, a, parents_dev);
+        } else {
+            constexpr int per = pages::THREADS / 64;
+            hipLaunchKernelGGL(pages::k_fork_rows, dim3((a.S + per - 1) / per), dim3(pages::THREADS), 0, st, a, parents_dev);
+            HIPCHK(hipGetLastError());
+            hipLaunchKernelGGL((pages::k_fork<false, pages::MANY>), dim3(1), dim3(pages::MANY), 0, st, a, parents_dev);
+        }
         HIPCHK(hipGetLastError());
         hipLaunchKernelGGL(pages::k_fork_copy, dim3(a.S, a.n_pools), dim3(pages::THREADS), 0, (hipStream_t)stream, a);
         HIPCHK(hipGetLastError());
@@ -84,7 +95,8 @@ int sp_op_pages_grow(const sp_page_pool *pool, const int32_t *counts_dev, void *
     return guarded([&] {
         const pages::Pool a = pool_args(pool);
         require(counts_dev != nullptr, SP_EINVAL, "NULL pointer");
-        hipLaunchKernelGGL(pages::k_grow, dim3(1), dim3(pages::SCAN), 0, (hipStream_t)stream, a, counts_dev);
+        if (few(a)) hipLaunchKernelGGL(pages::k_grow<pages::FEW>, dim3(1), dim3(pages::FEW), 0, (hipStream_t)stream, a, counts_dev);
+        else hipLaunchKernelGGL(pages::k_grow<pages::MANY>, dim3(1), dim3(pages::MANY), 0, (hipStream_t)stream, a, counts_dev);
         HIPCHK(hipGetLastError());
     });
 }
@@ -103,10 +115,12 @@ int sp_op_pages_free(const sp_page_pool *pool, int32_t n_seqs, const int32_t *se
 int sp_op_pages_compact(const sp_page_pool *pool, int32_t *places_dev, void *stream) {
     return guarded([&] {
         const pages::Pool a = pool_args(pool);
-        hipLaunchKernelGGL(pages::k_compact, dim3(1), dim3(pages::SCAN), 0, (hipStream_t)stream, a, places_dev);
+        if (few(a)) hipLaunchKernelGGL(pages::k_compact<pages::FEW>, dim3(1), dim3(pages::FEW), 0, (hipStream_t)stream, a, places_dev);
+        else hipLaunchKernelGGL(pages::k_compact<pages::MANY>, dim3(1), dim3(pages::MANY), 0, (hipStream_t)stream, a, places_dev);
         HIPCHK(hipGetLastError());
+        // (a block for every one that the chip holds; each takes several)
         const int64_t most = std::max<int64_t>((int64_t)(a.n_pages / 2) * a.n_pools, 1);
-        hipLaunchKernelGGL(pages::k_compact_copy, dim3((int)std::min<int64_t>(most, 8192)), dim3(pages::THREADS), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(pages::k_compact_copy, dim3((int)std::min<int64_t>(most, 2048)), dim3(pages::THREADS), 0, (hipStream_t)stream, a);
         HIPCHK(hipGetLastError());
     });
 }
