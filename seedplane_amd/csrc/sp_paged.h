@@ -147,6 +147,10 @@ __device__ __forceinline__ int piece_swap(int k) {
 __device__ __forceinline__ void copy_to_lds(const void *g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds) : "memory");
 }
+// The same of 4 bytes a lane: lane i's land at lds + 4 i.
+__device__ __forceinline__ void copy_dword_to_lds(const void *g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds) : "memory");
+}
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // The other half's value of lane ^ 32, combined.
@@ -163,7 +167,7 @@ __device__ __forceinline__ float half_sum(float v) {
 // key waves' (m, l).  Two blocks share a CU (8 waves: one block's loads and exponentials beside the other's matrix products).
 constexpr int TABLE_KEYS = 2048;
 constexpr int TILE_SMEM = 65536;
-template <int KV> constexpr int attn_smem = TILE_SMEM + (in_blocks(KV) ? TABLE_KEYS / SCALE_KEYS * 16 : 0);
+template <int KV> constexpr int attn_smem = TILE_SMEM + (in_blocks(KV) ? TABLE_KEYS / SCALE_KEYS * 5 * 4 : 0);
 struct AttnShared {                                                    // beside the tiles
     uint32_t rows[TABLE_KEYS];                                         // pool row of each position (0 where there is none)
     uint32_t seen[TABLE_KEYS / 32];                                    // which positions exist
@@ -171,19 +175,22 @@ struct AttnShared {                                                    // beside
     float2 ml[4][32];
 };
 
-template <bool KV8, int HD, int WM>
+// WIDE: the tile is brought to 16 bits once for all row waves (WM > 1), behind its codes, which need one stage then.
+template <bool KV8, int HD, int WM, bool WIDE = false>
 struct AttnTile {
     static constexpr int WK = 4 / WM;                                  // waves over keys
     static constexpr int RB = HD * (KV8 ? 1 : 2), NCH = RB / 16;       // bytes and pieces of a row
     static constexpr int KT = WM == 2 || (WM == 1 && RB == 256) ? 32 : 64;      // keys of a tile (of one group of WM waves)
-    static constexpr int STAGES = WM == 1 ? 1 : 2;
+    static constexpr int STAGES = WM == 1 || WIDE ? 1 : 2;
     static constexpr int TILE = KT * RB;                               // bytes of a tile's keys (and of its values)
+    static constexpr int WIDE_TILE = WIDE ? KT * HD * 2 : 0;           // ... in 16 bits
+    static constexpr int GROUP = STAGES * 2 * TILE + 2 * WIDE_TILE;    // of the waves that share a tile
     static constexpr int ALL = KT * NCH / 64;                          // copies of a tile's keys, and of its values
     static constexpr int COPIES = ALL / WM;                            // ... of a wave
     static constexpr int QUADS = HD / 8;                               // 4-value pieces of a lane's half of a row
     static constexpr int JOIN = 4 * 32 * HD * 4;                       // LDS of the join over the key waves
     static_assert(ALL >= WM && ALL % WM == 0, "whole copies");
-    static_assert(WK * STAGES * 2 * TILE <= TILE_SMEM && JOIN <= TILE_SMEM, "LDS plan");
+    static_assert(WK * GROUP <= TILE_SMEM && JOIN <= TILE_SMEM, "LDS plan");
     static_assert(TABLE_KEYS % (WK * KT) == 0, "whole rounds of the row table");
 };
 
@@ -205,15 +212,18 @@ __device__ __forceinline__ __attribute__((address_space(3))) V *lds_at(uint32_t 
 template <class T, int KV, int HD, int WM>
 __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, unsigned char *smem, AttnShared &sh) {
     constexpr bool KV8 = KV != KV_16, BLOCKS = in_blocks(KV), I8 = KV == KV_I8_BLOCKS;
-    typedef AttnTile<KV8, HD, WM> TL;
+    constexpr bool WIDE = BLOCKS && WM > 1;
+    typedef AttnTile<KV8, HD, WM, WIDE> TL;
     typedef Mma<T> M;
     typedef typename M::frag frag;
     constexpr int KT = TL::KT, RB = TL::RB, NCH = TL::NCH, WK = TL::WK, NS = HD / 16, ND = HD / 32, SUB = KT / 32;
     constexpr int RPC = 64 / NCH;                                      // rows of one copy
+    constexpr bool OP8 = KV8 && !WIDE;                                 // what the products' operands are read from: codes,
+    constexpr int ORB = WIDE ? HD * 2 : RB, ONCH = ORB / 16;           // bytes and pieces of a row
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;                          // the lane's query row; its half of every 8 keys
     const int rw = wv % WM, kw = wv / WM;
-    unsigned char *const buf0 = smem + kw * (TL::STAGES * 2 * TL::TILE);       // [stage][keys, values] of this key wave
+    unsigned char *const buf0 = smem + kw * TL::GROUP;                 // [stage][keys, values] of this key wave, and in 16 bits
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
         (uint32_t)(size_t)((__attribute__((address_space(3))) unsigned char *)buf0));
 
@@ -224,7 +234,9 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     if (threadIdx.x == 0) sh.nonfinite = 0;
     // (with blocks the tiles begin on whole SCALE_KEYS; positions before the item's first do not exist for it)
     const int k0 = BLOCKS ? w.k0 & -SCALE_KEYS : w.k0;
-    f32x4 *const scales = (f32x4 *)(smem + TILE_SMEM);                 // of each SCALE_KEYS positions of the table: see scale_terms
+    // of each SCALE_KEYS positions of the table: (kc, lv) and iv (see make_terms), and the scales as they lie in the cache, keys', values'
+    constexpr int BLOCKS_OF = TABLE_KEYS / SCALE_KEYS;
+    float *const terms = (float *)(smem + TILE_SMEM), *const inverses = terms + 2 * BLOCKS_OF, *const raw_scales = inverses + BLOCKS_OF;
     const int key0 = k0 + (int)threadIdx.x, page0 = page_of(key0), entry0 = entry_of(key0, page0);
 
     const int row = rw * 32 + col;
@@ -250,7 +262,7 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     const int hi = rw * 32 < w.ntok * a.G ? min(w.k1, w.pos0 + min(w.ntok - 1, (rw * 32 + 31) / a.by_g) + 1) : 0;
     const float sc = KV == KV_E4M3 ? a.scale * a.ks[w.kvh] : a.scale;
 
-    const int swz = piece_swap<NCH>(col);
+    const int swz = piece_swap<ONCH>(col);
     const int tg = (lane >> 4) & 1, ti = lane & 15;                    // which 16 of 32 dims; lane within them
 
     f32x16 o[ND];
@@ -317,17 +329,18 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     // 32 keys at a time: scores (kb: their rows), then maxima, weights, outputs (vb: their rows).  The lane's operands: LDS addresses in
     // the wave's first tile, kb and vb constants beside them, so that reads need no address of their own
     uint32_t ka[NS], va[2][ND];
+    const uint32_t op0 = WIDE ? lds0 + 2 * TL::TILE : lds0;
 #pragma unroll
-    for (int p = 0; p < NS; ++p) ka[p] = lds0 + (KV8 ? col * RB + (((swz ^ p) << 4) | (h << 3)) : col * RB + ((h ^ swz ^ (2 * p)) << 4));
+    for (int p = 0; p < NS; ++p) ka[p] = op0 + (OP8 ? col * ORB + (((swz ^ p) << 4) | (h << 3)) : col * ORB + ((h ^ swz ^ (2 * p)) << 4));
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-        if constexpr (KV8) {
+        if constexpr (OP8) {
             const int rr = ti >> 1, key = 8 * (rr >> 2) + 4 * h + (rr & 3);
-            va[0][d] = va[1][d] = lds0 + key * RB + (((2 * d + tg) ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
+            va[0][d] = va[1][d] = op0 + key * ORB + (((2 * d + tg) ^ piece_swap<ONCH>(key)) << 4) + ((ti & 1) << 3);
         } else {
             const int key = 4 * h + (ti >> 2), c = 4 * d + 2 * tg + ((ti >> 1) & 1);
-            va[0][d] = lds0 + key * RB + ((c ^ piece_swap<NCH>(key)) << 4) + ((ti & 1) << 3);
-            va[1][d] = lds0 + (key + 8) * RB + ((c ^ piece_swap<NCH>(key + 8)) << 4) + ((ti & 1) << 3);
+            va[0][d] = op0 + key * ORB + ((c ^ piece_swap<ONCH>(key)) << 4) + ((ti & 1) << 3);
+            va[1][d] = op0 + (key + 8) * ORB + ((c ^ piece_swap<ONCH>(key + 8)) << 4) + ((ti & 1) << 3);
         }
     }
     // (sums for good: the compiler would add the wave's part again at every read)
@@ -336,19 +349,22 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
 #pragma unroll
     for (int d = 0; d < ND; ++d) asm volatile("" : "+v"(va[0][d]), "+v"(va[1][d]));
     // operands as LDS gives them, and as the products take them: e4m3 is converted when it is used, after the wait for it
-    typedef std::conditional_t<KV8, u32x2, u32x4> raw;
-    auto cooked = [&](raw x) -> frag {
+    typedef std::conditional_t<OP8, u32x2, u32x4> raw;
+    auto widened = [&](u32x2 x) -> frag {
         if constexpr (I8) return from_i8<T>(x);
-        else if constexpr (KV8) return from_e4m3<T>(x);
+        else return from_e4m3<T>(x);
+    };
+    auto cooked = [&](raw x) -> frag {
+        if constexpr (OP8) return widened(x);
         else return __builtin_bit_cast(frag, x);
     };
     auto value_raw = [&](int vb, int y, int d) -> raw {           // keys 16 y .. + 15
-        if constexpr (KV8) {
+        if constexpr (OP8) {
             return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                lds_at<i32x2>(va[0][d] + vb + 16 * y * RB)));
+                lds_at<i32x2>(va[0][d] + vb + 16 * y * ORB)));
         } else {
-            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(va[0][d] + vb + 16 * y * RB));
-            const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(va[1][d] + vb + 16 * y * RB));
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(va[0][d] + vb + 16 * y * ORB));
+            const s16x4 z = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(va[1][d] + vb + 16 * y * ORB));
             const u32x2 xx = __builtin_bit_cast(u32x2, x), zz = __builtin_bit_cast(u32x2, z);
             return (u32x4){xx.x, xx.y, zz.x, zz.y};
         }
@@ -370,24 +386,29 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     // With blocks: a key's score is s kc, its weight times its values' scale is 2^(s kc + lv), and that weight over the scale is the
     // weight itself.  Exponents are taken of s kc + lv: then what is rounded to T for the product with the values is at most 1
     // however the scales of a row's blocks differ, and the sum of weights takes the scale out again (iv) in fp32.
-    struct Terms { f32x4 c[SUB][2]; };                                 // kc, lv, iv of keys 0 .. 15 and 16 .. 31
-    auto terms_of = [&](int t) {
-        Terms x;
+    // A wave's own copies of scales, which have landed, as terms: 4 of each 256 positions of the table.
+    auto make_terms = [&]() {
         if constexpr (BLOCKS) {
-#pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) x.c[u][y] = scales[t * (KT / SCALE_KEYS) + 2 * u + y];
+            constexpr int PER = 64 / SCALE_KEYS, ROUND = 256 / SCALE_KEYS;
+            if (lane < TABLE_KEYS / 256 * PER) {
+                const int b = lane / PER * ROUND + wv * PER + lane % PER;
+                const float vs = raw_scales[BLOCKS_OF + b];
+                // (a scale of 0, of pages that were never written, stands for the least one; a NaN reaches the rows that see it)
+                const float v = vs < LEAST_SCALE ? LEAST_SCALE : vs;
+                *(float2 *)(terms + 2 * b) = make_float2(raw_scales[b] * a.scale, __builtin_amdgcn_logf(v));
+                inverses[b] = v < INFINITY ? 1.f / v : 0.f;
+            }
         }
-        return x;
     };
     // masks a tile's scores, positions from t0, and brings the running maximum up to date; returns the exponent's base
-    auto maxima = [&](f32x16 (&s)[SUB], int t0, const uint32_t (&seen)[SUB], const Terms &x) -> float {
+    auto maxima = [&](f32x16 (&s)[SUB], int t, int t0, const uint32_t (&seen)[SUB]) -> float {
         if constexpr (BLOCKS) {
 #pragma unroll
-            for (int u = 0; u < SUB; ++u)
+            for (int u = 0; u < SUB; ++u) {
+                const f32x4 x = *(const f32x4 *)(terms + 2 * (t * (KT / SCALE_KEYS) + 2 * u));       // of keys 0 .. 15, 16 .. 31
 #pragma unroll
-                for (int j = 0; j < 16; ++j) s[u][j] = __builtin_fmaf(s[u][j], x.c[u][j / 8][0], x.c[u][j / 8][1]);
+                for (int j = 0; j < 16; ++j) s[u][j] = __builtin_fmaf(s[u][j], x[j / 8 * 2], x[j / 8 * 2 + 1]);
+            }
         }
         if (t0 + KT > lo || (seen[0] & seen[SUB - 1]) != ~0u) {
 #pragma unroll
@@ -421,11 +442,12 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
         }
         return m == -INFINITY ? 0.f : m;
     };
-    auto weights = [&](const f32x16 &s, float base, const f32x4 (&x)[2], frag (&pf)[2], int j0, int n) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    auto weights = [&](const f32x16 &s, float base, f32x2 iv, frag (&pf)[2], int j0, int n) {
 #pragma unroll
         for (int j = j0; j < j0 + n; ++j) {
             const float p = __builtin_amdgcn_exp2f(BLOCKS ? s[j] - base : s[j] * sc - base);
-            if constexpr (BLOCKS) l = __builtin_fmaf(p, x[j / 8][2], l);
+            if constexpr (BLOCKS) l = __builtin_fmaf(p, iv[j / 8], l);
             else l += p;
             pf[j / 8][j % 8] = (T)p;
         }
@@ -433,12 +455,15 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     // The tile's weights and outputs; v0: the values of its first 16 keys.  Operands are read a group of products ahead, and the
     // second half's exponentials stand between the first half's products: left to itself the compiler reads each product's
     // operands right before it and waits for them.
-    auto tile_outputs = [&](int vb, raw (&v0)[ND], const f32x16 (&s)[SUB], float base, const Terms &x) {
+    auto tile_outputs = [&](int vb, raw (&v0)[ND], const f32x16 (&s)[SUB], float base, int t) {
         raw v1[ND];
         frag pf[SUB][2];
+        f32x2 iv[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) iv[u] = BLOCKS ? *(const f32x2 *)(inverses + t * (KT / SCALE_KEYS) + 2 * u) : (f32x2){};
         read_values(vb, 1, v1);
         __builtin_amdgcn_sched_barrier(0);
-        weights(s[0], base, x.c[0], pf[0], 0, 16);
+        weights(s[0], base, iv[0], pf[0], 0, 16);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (SUB == 2) {
             constexpr int PER = 16 / (2 * ND);
@@ -448,8 +473,8 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                 for (int d = 0; d < ND; ++d) {
                     raw &v = y ? v1[d] : v0[d];
                     o[d] = M::run(cooked(v), pf[0][y], o[d]);
-                    v = value_raw(vb + 32 * RB, y, d);
-                    weights(s[1], base, x.c[1], pf[1], (y * ND + d) * PER, PER);
+                    v = value_raw(vb + 32 * ORB, y, d);
+                    weights(s[1], base, iv[1], pf[1], (y * ND + d) * PER, PER);
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
@@ -469,17 +494,14 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
             const int key = c0 + j, page = first && j == tid ? page0 : page_of(key);
             const int e = first && j == tid ? entry0 : entry_of(key, page);
             const bool in_pool = e >= 0 && e < a.n_pages, ok = in_pool && (!BLOCKS || key >= w.k0);
-            if constexpr (BLOCKS) {
-                if (key % SCALE_KEYS == 0) {
-                    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                    if (in_pool) {
-                        const int64_t i = ((int64_t)e * (a.NH / a.G) + w.kvh) * a.per_page + (key - page * a.page_size) / a.by_block;
-                        const float ks = a.ks[i], vs = a.vs[i];
-                        // (a scale of 0, of pages that were never written, stands for the least one; a NaN reaches the rows that see it)
-                        const float v = vs < LEAST_SCALE ? LEAST_SCALE : vs;
-                        x = (f32x4){ks * a.scale, __builtin_amdgcn_logf(v), v < INFINITY ? 1.f / v : 0.f, 0.f};
-                    }
-                    scales[j / SCALE_KEYS] = x;
+            if constexpr (BLOCKS) {                                    // lanes 0 .. 3: of the wave's 64 positions
+                const int b = lane < 64 / SCALE_KEYS ? lane : 0, eb = __shfl(in_pool ? e : -1, b * SCALE_KEYS);
+                const int kb = key - lane + b * SCALE_KEYS, pb = page_of(kb);
+                const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)((__attribute__((address_space(3))) float *)(raw_scales + j / SCALE_KEYS)));
+                if (lane < 64 / SCALE_KEYS && eb >= 0) {
+                    const int64_t at = ((int64_t)eb * (a.NH / a.G) + w.kvh) * a.per_page + (kb - pb * a.page_size) / a.by_block;
+                    copy_dword_to_lds(a.ks + at, to);
+                    copy_dword_to_lds(a.vs + at, to + BLOCKS_OF * 4);
                 }
             }
             sh.rows[j] = ok ? (uint32_t)e * a.page_rows + (uint32_t)w.kvh * a.head_rows + (uint32_t)(key - page * a.page_size) * a.slot_rows : 0u;
@@ -500,6 +522,14 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                 copy_tile(a.k, kw, lds0);
                 copy_tile(a.v, kw, lds0 + TL::TILE);
             }
+            if constexpr (BLOCKS) {                                    // (a wave's tiles are the positions whose scales it copied)
+                static_assert(!BLOCKS || (KT == 64 && WK == 4), "tiles of a wave");
+                if (kw < n) {
+                    copies_wait<TL::COPIES>();
+                    make_terms();
+                    lds_wait();
+                }
+            }
             for (int t = kw; t < n; t += WK) {
                 const bool more = t + WK < n;
                 uint32_t seen[SUB];
@@ -508,20 +538,19 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                 copies_wait<TL::COPIES>();
                 f32x16 s[SUB];
                 raw k[SUB][NS], v0[ND];
-                const Terms x = terms_of(t);
 #pragma unroll
-                for (int u = 0; u < SUB; ++u) read_keys(kb + u * 32 * RB, k[u]);
+                for (int u = 0; u < SUB; ++u) read_keys(kb + u * 32 * ORB, k[u]);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) scores(k[u], s[u]);
                 lds_wait();
                 if (more) copy_tile(a.k, t + WK, lds0);
-                const float base = maxima(s, c0 + t * KT, seen, x);
+                const float base = maxima(s, t, c0 + t * KT, seen);
                 if (more) copies_wait<TL::COPIES>();
                 else copies_wait<0>();
                 clear_values(vb, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
                 read_values(vb, 0, v0);
-                tile_outputs(vb, v0, s, base, x);
+                tile_outputs(vb, v0, s, base, t);
                 lds_wait();
                 if (more) copy_tile(a.v, t + WK, lds0 + TL::TILE);
             }
@@ -533,12 +562,16 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
             uint32_t seen_next[SUB];
 #pragma unroll
             for (int u = 0; u < SUB; ++u) seen_next[u] = seen_of(kw * SUB + u);
+            if constexpr (BLOCKS) {
+                copies_wait<0>();
+                make_terms();
+            }
             auto step = [&](int i, auto stage_of) {
                 constexpr int ST = decltype(stage_of)::value * 2 * TL::TILE;
                 const int t = i * WK + kw;
                 const bool more = i + 1 < rounds;
-                constexpr int kb = ST, vb = ST + TL::TILE;
-                const uint32_t to = lds0 + (2 * TL::TILE - ST);
+                constexpr int kb = WIDE ? 0 : ST, vb = WIDE ? TL::WIDE_TILE : ST + TL::TILE;
+                const uint32_t to = WIDE ? lds0 : lds0 + (2 * TL::TILE - ST);
                 uint32_t seen[SUB], r[TL::COPIES];
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) seen[u] = seen_next[u];
@@ -548,7 +581,22 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                     for (int u = 0; u < SUB; ++u) seen_next[u] = seen_of((t + WK) * SUB + u);
                 }
                 copies_wait<0>();
-                clear_values(vb, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
+                clear_values(ST + TL::TILE, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
+                if constexpr (WIDE) {
+                    // each wave brings what it copied to 16 bits, when all are done with the tile before
+                    lds_barrier();
+                    const int ln = opaque(lane);
+#pragma unroll
+                    for (int c = 0; c < TL::COPIES; ++c)
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            const int kr = (rw * TL::COPIES + c) * RPC + ln / NCH, piece = (ln % NCH) ^ piece_swap<NCH>(kr);
+                            const u32x4 x = *lds_at<u32x4>(lds0 + v * TL::TILE + (rw * TL::COPIES + c) * 1024 + ln * 16);
+                            const uint32_t at = op0 + v * TL::WIDE_TILE + kr * ORB;
+                            *lds_at<frag>(at + (((2 * piece) ^ piece_swap<ONCH>(kr)) << 4)) = widened((u32x2){x.x, x.y});
+                            *lds_at<frag>(at + (((2 * piece + 1) ^ piece_swap<ONCH>(kr)) << 4)) = widened((u32x2){x.z, x.w});
+                        }
+                }
                 lds_barrier();
                 // the next tile's copies are issued behind matrix products: a CU takes one in 16 cycles, and four waves that
                 // issue theirs together wait for each other
@@ -568,9 +616,8 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                 }
                 f32x16 s[SUB];
                 raw k[SUB][NS], v0[ND];
-                const Terms x = terms_of(t);
 #pragma unroll
-                for (int u = 0; u < SUB; ++u) read_keys(kb + u * 32 * RB, k[u]);
+                for (int u = 0; u < SUB; ++u) read_keys(kb + u * 32 * ORB, k[u]);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) {
@@ -578,14 +625,19 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                     copies(u);
                 }
                 read_values(vb, 0, v0);
-                tile_outputs(vb, v0, s, maxima(s, c0 + t * KT, seen, x), x);
+                tile_outputs(vb, v0, s, maxima(s, t, c0 + t * KT, seen), t);
             };
-            for (int i = 0; i < rounds; i += 2) {
-                step(i, std::integral_constant<int, 0>{});
-                if (i + 1 < rounds) step(i + 1, std::integral_constant<int, 1>{});
+            if constexpr (WIDE) {
+                for (int i = 0; i < rounds; ++i) step(i, std::integral_constant<int, 0>{});
+            } else {
+                for (int i = 0; i < rounds; i += 2) {
+                    step(i, std::integral_constant<int, 0>{});
+                    if (i + 1 < rounds) step(i + 1, std::integral_constant<int, 1>{});
+                }
             }
         }
     }
+    if constexpr (BLOCKS) copies_wait<0>();                            // (scales of a wave without tiles)
     l = half_sum(l);
     if (w.ntok > 1) lds_barrier();
     const bool nonfinite = w.ntok > 1 && __builtin_amdgcn_readfirstlane(sh.nonfinite);
