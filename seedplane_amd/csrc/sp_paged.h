@@ -175,22 +175,20 @@ struct AttnShared {                                                    // beside
     float2 ml[4][32];
 };
 
-// WIDE: the tile is brought to 16 bits once for all row waves (WM > 1), behind its codes, which need one stage then.
+// WIDE: codes are brought to 16 bits on the way, once for all row waves.
 template <bool KV8, int HD, int WM, bool WIDE = false>
 struct AttnTile {
     static constexpr int WK = 4 / WM;                                  // waves over keys
     static constexpr int RB = HD * (KV8 ? 1 : 2), NCH = RB / 16;       // bytes and pieces of a row
     static constexpr int KT = WM == 2 || (WM == 1 && RB == 256) ? 32 : 64;      // keys of a tile (of one group of WM waves)
-    static constexpr int STAGES = WM == 1 || WIDE ? 1 : 2;
-    static constexpr int TILE = KT * RB;                               // bytes of a tile's keys (and of its values)
-    static constexpr int WIDE_TILE = WIDE ? KT * HD * 2 : 0;           // ... in 16 bits
-    static constexpr int GROUP = STAGES * 2 * TILE + 2 * WIDE_TILE;    // of the waves that share a tile
+    static constexpr int STAGES = WM == 1 ? 1 : 2;
+    static constexpr int TILE = KT * (WIDE ? HD * 2 : RB);             // LDS bytes of a tile's keys (and of its values)
     static constexpr int ALL = KT * NCH / 64;                          // copies of a tile's keys, and of its values
     static constexpr int COPIES = ALL / WM;                            // ... of a wave
     static constexpr int QUADS = HD / 8;                               // 4-value pieces of a lane's half of a row
     static constexpr int JOIN = 4 * 32 * HD * 4;                       // LDS of the join over the key waves
     static_assert(ALL >= WM && ALL % WM == 0, "whole copies");
-    static_assert(WK * GROUP <= TILE_SMEM && JOIN <= TILE_SMEM, "LDS plan");
+    static_assert(WK * STAGES * 2 * TILE <= TILE_SMEM && JOIN <= TILE_SMEM, "LDS plan");
     static_assert(TABLE_KEYS % (WK * KT) == 0, "whole rounds of the row table");
 };
 
@@ -212,7 +210,7 @@ __device__ __forceinline__ __attribute__((address_space(3))) V *lds_at(uint32_t 
 template <class T, int KV, int HD, int WM>
 __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, unsigned char *smem, AttnShared &sh) {
     constexpr bool KV8 = KV != KV_16, BLOCKS = in_blocks(KV), I8 = KV == KV_I8_BLOCKS;
-    constexpr bool WIDE = BLOCKS && WM > 1;
+    constexpr bool WIDE = I8 && WM > 1;
     typedef AttnTile<KV8, HD, WM, WIDE> TL;
     typedef Mma<T> M;
     typedef typename M::frag frag;
@@ -223,7 +221,7 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;                          // the lane's query row; its half of every 8 keys
     const int rw = wv % WM, kw = wv / WM;
-    unsigned char *const buf0 = smem + kw * TL::GROUP;                 // [stage][keys, values] of this key wave, and in 16 bits
+    unsigned char *const buf0 = smem + kw * (TL::STAGES * 2 * TL::TILE);       // [stage][keys, values] of this key wave
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
         (uint32_t)(size_t)((__attribute__((address_space(3))) unsigned char *)buf0));
 
@@ -329,18 +327,17 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     // 32 keys at a time: scores (kb: their rows), then maxima, weights, outputs (vb: their rows).  The lane's operands: LDS addresses in
     // the wave's first tile, kb and vb constants beside them, so that reads need no address of their own
     uint32_t ka[NS], va[2][ND];
-    const uint32_t op0 = WIDE ? lds0 + 2 * TL::TILE : lds0;
 #pragma unroll
-    for (int p = 0; p < NS; ++p) ka[p] = op0 + (OP8 ? col * ORB + (((swz ^ p) << 4) | (h << 3)) : col * ORB + ((h ^ swz ^ (2 * p)) << 4));
+    for (int p = 0; p < NS; ++p) ka[p] = lds0 + (OP8 ? col * ORB + (((swz ^ p) << 4) | (h << 3)) : col * ORB + ((h ^ swz ^ (2 * p)) << 4));
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
         if constexpr (OP8) {
             const int rr = ti >> 1, key = 8 * (rr >> 2) + 4 * h + (rr & 3);
-            va[0][d] = va[1][d] = op0 + key * ORB + (((2 * d + tg) ^ piece_swap<ONCH>(key)) << 4) + ((ti & 1) << 3);
+            va[0][d] = va[1][d] = lds0 + key * ORB + (((2 * d + tg) ^ piece_swap<ONCH>(key)) << 4) + ((ti & 1) << 3);
         } else {
             const int key = 4 * h + (ti >> 2), c = 4 * d + 2 * tg + ((ti >> 1) & 1);
-            va[0][d] = op0 + key * ORB + ((c ^ piece_swap<ONCH>(key)) << 4) + ((ti & 1) << 3);
-            va[1][d] = op0 + (key + 8) * ORB + ((c ^ piece_swap<ONCH>(key + 8)) << 4) + ((ti & 1) << 3);
+            va[0][d] = lds0 + key * ORB + ((c ^ piece_swap<ONCH>(key)) << 4) + ((ti & 1) << 3);
+            va[1][d] = lds0 + (key + 8) * ORB + ((c ^ piece_swap<ONCH>(key + 8)) << 4) + ((ti & 1) << 3);
         }
     }
     // (sums for good: the compiler would add the wave's part again at every read)
@@ -385,29 +382,35 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     };
     // With blocks: a key's score is s kc, its weight times its values' scale is 2^(s kc + lv), and that weight over the scale is the
     // weight itself.  Exponents are taken of s kc + lv: then what is rounded to T for the product with the values is at most 1
-    // however the scales of a row's blocks differ, and the sum of weights takes the scale out again (iv) in fp32.
+    // however the scales of a row's blocks differ, and the sum of weights takes the scale out again (iv) in fp32.  As kc is positive a
+    // block's largest s is that of its exponents too.
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    struct Terms { f32x2 kc[SUB], lv[SUB], iv[SUB]; };                 // of keys 0 .. 15 and 16 .. 31
     // A wave's own copies of scales, which have landed, as terms: 4 of each 256 positions of the table.
     auto make_terms = [&]() {
         if constexpr (BLOCKS) {
             constexpr int PER = 64 / SCALE_KEYS, ROUND = 256 / SCALE_KEYS;
-            if (lane < TABLE_KEYS / 256 * PER) {
-                const int b = lane / PER * ROUND + wv * PER + lane % PER;
+            const int ln = opaque(lane);
+            if (ln < TABLE_KEYS / 256 * PER) {
+                const int b = ln / PER * ROUND + wv * PER + ln % PER;
                 const float vs = raw_scales[BLOCKS_OF + b];
                 // (a scale of 0, of pages that were never written, stands for the least one; a NaN reaches the rows that see it)
                 const float v = vs < LEAST_SCALE ? LEAST_SCALE : vs;
-                *(float2 *)(terms + 2 * b) = make_float2(raw_scales[b] * a.scale, __builtin_amdgcn_logf(v));
+                const float ks = raw_scales[b], k = ks < LEAST_SCALE ? LEAST_SCALE : ks;
+                *(float2 *)(terms + 2 * b) = make_float2(k * a.scale, __builtin_amdgcn_logf(v));
                 inverses[b] = v < INFINITY ? 1.f / v : 0.f;
             }
         }
     };
     // masks a tile's scores, positions from t0, and brings the running maximum up to date; returns the exponent's base
-    auto maxima = [&](f32x16 (&s)[SUB], int t, int t0, const uint32_t (&seen)[SUB]) -> float {
+    auto maxima = [&](f32x16 (&s)[SUB], int t, int t0, const uint32_t (&seen)[SUB], Terms &x) -> float {
         if constexpr (BLOCKS) {
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
-                const f32x4 x = *(const f32x4 *)(terms + 2 * (t * (KT / SCALE_KEYS) + 2 * u));       // of keys 0 .. 15, 16 .. 31
-#pragma unroll
-                for (int j = 0; j < 16; ++j) s[u][j] = __builtin_fmaf(s[u][j], x[j / 8 * 2], x[j / 8 * 2 + 1]);
+                const f32x4 y = *(const f32x4 *)(terms + 2 * (t * (KT / SCALE_KEYS) + 2 * u));
+                x.kc[u] = (f32x2){y.x, y.z};
+                x.lv[u] = (f32x2){y.y, y.w};
+                x.iv[u] = *(const f32x2 *)(inverses + t * (KT / SCALE_KEYS) + 2 * u);
             }
         }
         if (t0 + KT > lo || (seen[0] & seen[SUB - 1]) != ~0u) {
@@ -418,15 +421,31 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const int kk = 8 * (j / 4) + j % 4;
-                    s[u][j] = kk < left && ((mine >> kk) & 1) ? s[u][j] : -INFINITY;
+                    // (a hidden key's terms may be anything)
+                    const float v = BLOCKS ? __builtin_fmaf(s[u][j], x.kc[u][j / 8], x.lv[u][j / 8]) : s[u][j];
+                    s[u][j] = kk < left && ((mine >> kk) & 1) ? v : -INFINITY;
+                }
+                if constexpr (BLOCKS) {
+                    x.kc[u] = (f32x2){1.f, 1.f};
+                    x.lv[u] = (f32x2){0.f, 0.f};
                 }
             }
         }
-        float mx = s[0][0];
+        float mx = BLOCKS ? -INFINITY : s[0][0];
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
+            if constexpr (BLOCKS) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[u][j]);
+                for (int y = 0; y < 2; ++y) {
+                    float b = s[u][8 * y];
+#pragma unroll
+                    for (int j = 1; j < 8; ++j) b = fmaxf(b, s[u][8 * y + j]);
+                    mx = fmaxf(mx, __builtin_fmaf(b, x.kc[u][y], x.lv[u][y]));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[u][j]);
+            }
         mx = fmaxf(m, BLOCKS ? half_max(mx) : half_max(mx) * sc);
         // weights are taken from the base m.  With bf16 weights it follows the maximum only when that has grown by more than
         // 2^8, and the outputs need no rescaling up to there; with fp16 weights it is the maximum, whose weight is then
@@ -442,12 +461,11 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
         }
         return m == -INFINITY ? 0.f : m;
     };
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    auto weights = [&](const f32x16 &s, float base, f32x2 iv, frag (&pf)[2], int j0, int n) {
+    auto weights = [&](const f32x16 &s, float base, const Terms &x, int u, frag (&pf)[2], int j0, int n) {
 #pragma unroll
         for (int j = j0; j < j0 + n; ++j) {
-            const float p = __builtin_amdgcn_exp2f(BLOCKS ? s[j] - base : s[j] * sc - base);
-            if constexpr (BLOCKS) l = __builtin_fmaf(p, iv[j / 8], l);
+            const float p = __builtin_amdgcn_exp2f(BLOCKS ? __builtin_fmaf(s[j], x.kc[u][j / 8], x.lv[u][j / 8]) : s[j] * sc - base);
+            if constexpr (BLOCKS) l = __builtin_fmaf(p, x.iv[u][j / 8], l);
             else l += p;
             pf[j / 8][j % 8] = (T)p;
         }
@@ -455,15 +473,16 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     // The tile's weights and outputs; v0: the values of its first 16 keys.  Operands are read a group of products ahead, and the
     // second half's exponentials stand between the first half's products: left to itself the compiler reads each product's
     // operands right before it and waits for them.
-    auto tile_outputs = [&](int vb, raw (&v0)[ND], const f32x16 (&s)[SUB], float base, int t) {
+    auto tile_outputs = [&](int vb, raw (&v0)[ND], const f32x16 (&s)[SUB], float base, Terms &x) {
         raw v1[ND];
         frag pf[SUB][2];
-        f32x2 iv[SUB];
+        if constexpr (BLOCKS) {
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) iv[u] = BLOCKS ? *(const f32x2 *)(inverses + t * (KT / SCALE_KEYS) + 2 * u) : (f32x2){};
+            for (int u = 0; u < SUB; ++u) x.lv[u] = (f32x2){x.lv[u].x - base, x.lv[u].y - base};
+        }
         read_values(vb, 1, v1);
         __builtin_amdgcn_sched_barrier(0);
-        weights(s[0], base, iv[0], pf[0], 0, 16);
+        weights(s[0], base, x, 0, pf[0], 0, 16);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (SUB == 2) {
             constexpr int PER = 16 / (2 * ND);
@@ -474,7 +493,7 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                     raw &v = y ? v1[d] : v0[d];
                     o[d] = M::run(cooked(v), pf[0][y], o[d]);
                     v = value_raw(vb + 32 * ORB, y, d);
-                    weights(s[1], base, iv[1], pf[1], (y * ND + d) * PER, PER);
+                    weights(s[1], base, x, 1, pf[1], (y * ND + d) * PER, PER);
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
@@ -495,10 +514,10 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
             const int e = first && j == tid ? entry0 : entry_of(key, page);
             const bool in_pool = e >= 0 && e < a.n_pages, ok = in_pool && (!BLOCKS || key >= w.k0);
             if constexpr (BLOCKS) {                                    // lanes 0 .. 3: of the wave's 64 positions
-                const int b = lane < 64 / SCALE_KEYS ? lane : 0, eb = __shfl(in_pool ? e : -1, b * SCALE_KEYS);
-                const int kb = key - lane + b * SCALE_KEYS, pb = page_of(kb);
+                const int ln = tid & 63, b = ln < 64 / SCALE_KEYS ? ln : 0, eb = __shfl(in_pool ? e : -1, b * SCALE_KEYS);
+                const int kb = key - ln + b * SCALE_KEYS, pb = page_of(kb);
                 const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)((__attribute__((address_space(3))) float *)(raw_scales + j / SCALE_KEYS)));
-                if (lane < 64 / SCALE_KEYS && eb >= 0) {
+                if (ln < 64 / SCALE_KEYS && eb >= 0) {
                     const int64_t at = ((int64_t)eb * (a.NH / a.G) + w.kvh) * a.per_page + (kb - pb * a.page_size) / a.by_block;
                     copy_dword_to_lds(a.ks + at, to);
                     copy_dword_to_lds(a.vs + at, to + BLOCKS_OF * 4);
@@ -522,14 +541,6 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                 copy_tile(a.k, kw, lds0);
                 copy_tile(a.v, kw, lds0 + TL::TILE);
             }
-            if constexpr (BLOCKS) {                                    // (a wave's tiles are the positions whose scales it copied)
-                static_assert(!BLOCKS || (KT == 64 && WK == 4), "tiles of a wave");
-                if (kw < n) {
-                    copies_wait<TL::COPIES>();
-                    make_terms();
-                    lds_wait();
-                }
-            }
             for (int t = kw; t < n; t += WK) {
                 const bool more = t + WK < n;
                 uint32_t seen[SUB];
@@ -543,70 +554,103 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) scores(k[u], s[u]);
+                if constexpr (BLOCKS) {                                // (a wave's tiles are the positions whose scales it copied, before them)
+                    static_assert(!BLOCKS || (KT == 64 && WK == 4), "tiles of a wave");
+                    if (t == kw) make_terms();
+                }
                 lds_wait();
                 if (more) copy_tile(a.k, t + WK, lds0);
-                const float base = maxima(s, t, c0 + t * KT, seen);
+                Terms x;
+                const float base = maxima(s, t, c0 + t * KT, seen, x);
                 if (more) copies_wait<TL::COPIES>();
                 else copies_wait<0>();
                 clear_values(vb, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
                 read_values(vb, 0, v0);
-                tile_outputs(vb, v0, s, base, t);
+                tile_outputs(vb, v0, s, base, x);
                 lds_wait();
                 if (more) copy_tile(a.v, t + WK, lds0 + TL::TILE);
             }
         } else {
             // the row waves share a tile; the next one is copied meanwhile
             const int rounds = (nt + WK - 1) / WK;
-            copy_tile(a.k, kw, lds0);
-            copy_tile(a.v, kw, lds0 + TL::TILE);
+            // WIDE: codes go through registers, a tile ahead of the one that is brought to 16 bits and written behind matrix products
+            u32x4 codes[2][WIDE ? TL::COPIES : 1];
+            auto fetch_codes = [&](int t) {
+                uint32_t r[TL::COPIES];
+                rows_of(t, r);
+#pragma unroll
+                for (int c = 0; c < TL::COPIES; ++c) {
+                    const uint64_t at = offset_of(r[c], c);
+                    codes[0][c] = *(const u32x4 *)(a.k + at);
+                    codes[1][c] = *(const u32x4 *)(a.v + at);
+                }
+            };
+            // (the place of the lane's first codes in a tile; the others' differ by constants, as piece_swap of a sum of such rows is
+            // the xor of the rows' own)
+            const int wide_piece = (lane % NCH) ^ piece_swap<NCH>(copy0);
+            const uint32_t wide0 = copy0 * ORB + (((2 * wide_piece) ^ piece_swap<ONCH>(copy0)) << 4);
+            auto put_codes = [&](uint32_t to, int v) {
+#pragma unroll
+                for (int c = 0; c < TL::COPIES; ++c) {
+                    const uint32_t swap = ((2 * piece_swap<NCH>(c * RPC)) ^ piece_swap<ONCH>(c * RPC)) << 4;
+                    const uint32_t at = to + v * TL::TILE + c * RPC * ORB;
+                    const u32x4 x = codes[v][c];
+                    *lds_at<frag>(at + (wide0 ^ swap)) = widened((u32x2){x.x, x.y});
+                    *lds_at<frag>(at + (wide0 ^ swap ^ 16)) = widened((u32x2){x.z, x.w});
+                }
+            };
+            if constexpr (WIDE) {
+                fetch_codes(kw);
+                copies_wait<0>();
+                make_terms();
+                put_codes(lds0, 0);
+                put_codes(lds0, 1);
+                if (rounds > 1) fetch_codes(kw + WK);
+            } else {
+                copy_tile(a.k, kw, lds0);
+                copy_tile(a.v, kw, lds0 + TL::TILE);
+                if constexpr (BLOCKS) {
+                    copies_wait<0>();
+                    make_terms();
+                }
+            }
             uint32_t seen_next[SUB];
 #pragma unroll
             for (int u = 0; u < SUB; ++u) seen_next[u] = seen_of(kw * SUB + u);
-            if constexpr (BLOCKS) {
-                copies_wait<0>();
-                make_terms();
-            }
             auto step = [&](int i, auto stage_of) {
                 constexpr int ST = decltype(stage_of)::value * 2 * TL::TILE;
                 const int t = i * WK + kw;
                 const bool more = i + 1 < rounds;
-                constexpr int kb = WIDE ? 0 : ST, vb = WIDE ? TL::WIDE_TILE : ST + TL::TILE;
-                const uint32_t to = WIDE ? lds0 : lds0 + (2 * TL::TILE - ST);
+                constexpr int kb = ST, vb = ST + TL::TILE;
+                const uint32_t to = lds0 + (2 * TL::TILE - ST);
                 uint32_t seen[SUB], r[TL::COPIES];
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) seen[u] = seen_next[u];
                 if (more) {                                            // (read ahead of the barrier)
-                    rows_of(t + WK, r);
+                    if constexpr (!WIDE) rows_of(t + WK, r);
 #pragma unroll
                     for (int u = 0; u < SUB; ++u) seen_next[u] = seen_of((t + WK) * SUB + u);
                 }
-                copies_wait<0>();
-                clear_values(ST + TL::TILE, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
-                if constexpr (WIDE) {
-                    // each wave brings what it copied to 16 bits, when all are done with the tile before
-                    lds_barrier();
-                    const int ln = opaque(lane);
-#pragma unroll
-                    for (int c = 0; c < TL::COPIES; ++c)
-#pragma unroll
-                        for (int v = 0; v < 2; ++v) {
-                            const int kr = (rw * TL::COPIES + c) * RPC + ln / NCH, piece = (ln % NCH) ^ piece_swap<NCH>(kr);
-                            const u32x4 x = *lds_at<u32x4>(lds0 + v * TL::TILE + (rw * TL::COPIES + c) * 1024 + ln * 16);
-                            const uint32_t at = op0 + v * TL::WIDE_TILE + kr * ORB;
-                            *lds_at<frag>(at + (((2 * piece) ^ piece_swap<ONCH>(kr)) << 4)) = widened((u32x2){x.x, x.y});
-                            *lds_at<frag>(at + (((2 * piece + 1) ^ piece_swap<ONCH>(kr)) << 4)) = widened((u32x2){x.z, x.w});
-                        }
+                if constexpr (!WIDE) {
+                    copies_wait<0>();
+                    clear_values(vb, t, c0 + t * KT, seen[0] & seen[SUB - 1]);
                 }
                 lds_barrier();
                 // the next tile's copies are issued behind matrix products: a CU takes one in 16 cycles, and four waves that
                 // issue theirs together wait for each other
                 auto copies = [&](int part) {
                     if (!more) return;
+                    if constexpr (WIDE) {
 #pragma unroll
-                    for (int c = part; c < TL::COPIES; c += SUB) {
-                        const uint64_t at = offset_of(r[c], c);
-                        copy_row(a.k, at, to, c);
-                        copy_row(a.v, at, to + TL::TILE, c);
+                        for (int v = part; v < 2; v += SUB) put_codes(to, v);
+                        if (part == SUB - 1 && i + 2 < rounds) fetch_codes(t + 2 * WK);
+                    } else {
+#pragma unroll
+                        for (int c = part; c < TL::COPIES; c += SUB) {
+                            const uint64_t at = offset_of(r[c], c);
+                            copy_row(a.k, at, to, c);
+                            copy_row(a.v, at, to + TL::TILE, c);
+                        }
                     }
                 };
                 if (c0 + t * KT >= hi) {
@@ -625,15 +669,13 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
                     copies(u);
                 }
                 read_values(vb, 0, v0);
-                tile_outputs(vb, v0, s, maxima(s, t, c0 + t * KT, seen), t);
+                Terms x;
+                const float base = maxima(s, t, c0 + t * KT, seen, x);
+                tile_outputs(vb, v0, s, base, x);
             };
-            if constexpr (WIDE) {
-                for (int i = 0; i < rounds; ++i) step(i, std::integral_constant<int, 0>{});
-            } else {
-                for (int i = 0; i < rounds; i += 2) {
-                    step(i, std::integral_constant<int, 0>{});
-                    if (i + 1 < rounds) step(i + 1, std::integral_constant<int, 1>{});
-                }
+            for (int i = 0; i < rounds; i += 2) {
+                step(i, std::integral_constant<int, 0>{});
+                if (i + 1 < rounds) step(i + 1, std::integral_constant<int, 1>{});
             }
         }
     }
