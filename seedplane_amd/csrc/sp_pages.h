@@ -33,6 +33,7 @@ struct Pool {                              // see sp_page_pool
     int *fresh, *first;                    // [S] new lengths; [S + 1] places of each sequence's pages among those wanted
     int *rows;                             // [S][width] new table
     int *list;                             // [n_pages] free pages taken
+    int *to;                               // [n_pages] where the pages of a compaction's moves go
     Move *moves;                           // [max(S, n_pages)]
 };
 
@@ -219,14 +220,20 @@ __device__ __forceinline__ void copy_page(const Pool &a, int pool, const Move &m
         }
     }
 }
-// A fork's copies: block (copy, pool); the first pool's blocks write the tables too.
-__global__ void __launch_bounds__(THREADS) k_fork_copy(Pool a) {
-    const int pool = blockIdx.y, k = blockIdx.x;
-    if (pool == 0) {
-        for (int j = threadIdx.x; j < a.width; j += blockDim.x) a.table[(int64_t)k * a.width + j] = a.rows[(int64_t)k * a.width + j];
-        if (threadIdx.x == 0) a.lengths[k] = a.fresh[k];
+// The moves' copies, (move, pool) pairs over the grid's blocks.
+__device__ __forceinline__ void copy_moves(const Pool &a, int moves) {
+    const int64_t total = (int64_t)moves * a.n_pools;
+    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
+        const int k = (int)(w / a.n_pools);
+        copy_page(a, (int)(w - (int64_t)k * a.n_pools), a.moves[k]);
     }
-    if (k < a.counts[0]) copy_page(a, pool, a.moves[k]);
+}
+// A fork's copies, and its tables.
+__global__ void __launch_bounds__(THREADS) k_fork_copy(Pool a) {
+    const int64_t entries = (int64_t)a.S * a.width, stride = (int64_t)gridDim.x * THREADS, first = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+    for (int64_t i = first; i < entries; i += stride) a.table[i] = a.rows[i];
+    for (int64_t s = first; s < a.S; s += stride) a.lengths[s] = a.fresh[s];
+    copy_moves(a, a.counts[0]);
 }
 
 // ------------------------------------------------------------------------------------------------ growth, ends
@@ -316,6 +323,7 @@ __global__ void __launch_bounds__(N) k_compact(Pool a, int *places) {
         const int src = a.moves[k].src, dst = a.list[k];
         a.moves[k].dst = dst;
         a.moves[k].rows = a.page;
+        a.to[src] = dst;
         a.holders[dst] = a.holders[src];
     }
     if (places)
@@ -326,28 +334,16 @@ __global__ void __launch_bounds__(N) k_compact(Pool a, int *places) {
     for (int k = tid; k < low; k += N) a.holders[a.moves[k].src] = 0;
     if (tid == 0) { a.counts[0] = low; a.counts[1] = held; }
 }
-// The compaction's copies, (pool, move) pairs over the grid, and the tables: a page behind the last held one is found among the moves,
-// whose sources are in order.
+// The compaction's copies, and the pages behind the last held one in the tables.
 __global__ void __launch_bounds__(THREADS) k_compact_copy(Pool a) {
     const int moves = a.counts[0], held = a.counts[1];
-    const int64_t entries = (int64_t)a.S * a.width, stride = (int64_t)gridDim.x * blockDim.x;
+    const int64_t entries = (int64_t)a.S * a.width, stride = (int64_t)gridDim.x * THREADS;
     if (moves == 0) return;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < entries; i += stride) {
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < entries; i += stride) {
         const int e = a.table[i];
-        if (e < held || e >= a.n_pages) continue;
-        int lo = 0, hi = moves - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (a.moves[mid].src < e) lo = mid + 1;
-            else hi = mid;
-        }
-        if (a.moves[lo].src == e) a.table[i] = a.moves[lo].dst;
+        if (e >= held && e < a.n_pages) a.table[i] = a.to[e];
     }
-    const int64_t total = (int64_t)moves * a.n_pools;
-    for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-        const int k = (int)(w / a.n_pools);
-        copy_page(a, (int)(w - (int64_t)k * a.n_pools), a.moves[k]);
-    }
+    copy_moves(a, moves);
 }
 // Whole pages by lists.
 __global__ void __launch_bounds__(THREADS) k_copy(Pool a, const int *src, const int *dst) {

@@ -10,14 +10,15 @@ namespace {
 
 size_t up(size_t n) { return (n + 15) / 16 * 16; }
 
-struct Places { size_t fresh, first, rows, list, moves, total; };
+struct Places { size_t fresh, first, rows, list, to, moves, total; };
 Places places_of(int64_t S, int64_t width, int64_t n_pages) {
     Places p{};
     p.fresh = 64;
     p.first = p.fresh + up(S * 4);
     p.rows = p.first + up((S + 1) * 4);
     p.list = p.rows + up(S * width * 4);
-    p.moves = p.list + up(n_pages * 4);
+    p.to = p.list + up(n_pages * 4);
+    p.moves = p.to + up(n_pages * 4);
     p.total = p.moves + up(std::max(S, n_pages) * sizeof(pages::Move));
     return p;
 }
@@ -57,10 +58,13 @@ pages::Pool pool_args(const sp_page_pool *p) {
     a.first = (int *)(w + at.first);
     a.rows = (int *)(w + at.rows);
     a.list = (int *)(w + at.list);
+    a.to = (int *)(w + at.to);
     a.moves = (pages::Move *)(w + at.moves);
     return a;
 }
 
+// Blocks of up to `moves` copies in every pool: those that the chip holds, each of which takes several.
+int copy_blocks(const pages::Pool &a, int64_t moves) { return (int)std::min<int64_t>(std::max<int64_t>(moves * a.n_pools, 1), 2048); }
 bool few(const pages::Pool &a) { return a.S <= pages::FEW && a.n_pages <= 2 * pages::FEW * pages::PER && (int64_t)a.S * a.width <= 8 * pages::FEW; }
 
 }  // namespace
@@ -86,7 +90,7 @@ int sp_op_pages_fork(const sp_page_pool *pool, const int32_t *parents_dev, void 
             hipLaunchKernelGGL((pages::k_fork<false, pages::MANY>), dim3(1), dim3(pages::MANY), 0, st, a, parents_dev);
         }
         HIPCHK(hipGetLastError());
-        hipLaunchKernelGGL(pages::k_fork_copy, dim3(a.S, a.n_pools), dim3(pages::THREADS), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(pages::k_fork_copy, dim3(copy_blocks(a, a.S)), dim3(pages::THREADS), 0, st, a);
         HIPCHK(hipGetLastError());
     });
 }
@@ -118,9 +122,7 @@ int sp_op_pages_compact(const sp_page_pool *pool, int32_t *places_dev, void *str
         if (few(a)) hipLaunchKernelGGL(pages::k_compact<pages::FEW>, dim3(1), dim3(pages::FEW), 0, (hipStream_t)stream, a, places_dev);
         else hipLaunchKernelGGL(pages::k_compact<pages::MANY>, dim3(1), dim3(pages::MANY), 0, (hipStream_t)stream, a, places_dev);
         HIPCHK(hipGetLastError());
-        // (a block for every one that the chip holds; each takes several)
-        const int64_t most = std::max<int64_t>((int64_t)(a.n_pages / 2) * a.n_pools, 1);
-        hipLaunchKernelGGL(pages::k_compact_copy, dim3((int)std::min<int64_t>(most, 2048)), dim3(pages::THREADS), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(pages::k_compact_copy, dim3(copy_blocks(a, a.n_pages / 2)), dim3(pages::THREADS), 0, (hipStream_t)stream, a);
         HIPCHK(hipGetLastError());
     });
 }

@@ -41,8 +41,8 @@ def test_arguments_are_refused():
     assert lib.sp_op_pages_free(ref, 0, None, None) == _lib.SP_OK and lib.sp_op_pages_copy(ref, 0, None, None, None) == _lib.SP_OK
     assert lib.sp_pages_workspace(0, 1, 1) == 0 and lib.sp_pages_workspace(1, 1, 0) == 0
     for S, W, N in ((1, 1, 1), (128, 40, 5000), (65535, 16000, 1000000)):
-        need = 64 + 4 * (S + S + 1 + S * W + N) + 12 * max(S, N)
-        assert need <= lib.sp_pages_workspace(S, W, N) <= need + 5 * 16
+        need = 64 + 4 * (S + S + 1 + S * W + 2 * N) + 12 * max(S, N)
+        assert need <= lib.sp_pages_workspace(S, W, N) <= need + 6 * 16
 
 
 def select(dtype=0, logits=P, ld=100, B=2, K=3, V=100, scores=P, n=6, n_eos=1, eos=True, ws=P, outs=(P,) * 6):
