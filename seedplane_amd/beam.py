@@ -30,8 +30,9 @@ class BeamStep(NamedTuple):
 
     @classmethod
     def allocate(cls, requests, beams, n, device='cuda'):
-        f, g = (torch.empty((3, requests, k), dtype=torch.int32, device=device).unbind(0) for k in (n, beams))
-        return cls(f[0].view(torch.float32), f[1], f[2], g[0].view(torch.float32), g[1], g[2])
+        a, b, c = torch.empty((3, requests, n), dtype=torch.int32, device=device).unbind(0)
+        d, e, f = torch.empty((3, requests, beams), dtype=torch.int32, device=device).unbind(0)
+        return cls(a.view(torch.float32), b, c, d.view(torch.float32), e, f)
 
 
 def beam_select(logits, scores, n=None, eos=None, out=None):
@@ -42,10 +43,11 @@ def beam_select(logits, scores, n=None, eos=None, out=None):
     -infinity for beams that do not live (all but one in a first step).  eos: a token or a list of up to 8 that end a sequence.
     n: default beams * (1 + number of eos), enough for as many to go on as there are beams; at most 64.  Ties go to the lowest beam, then token; logits
     of -infinity, and beams whose logits hold NaN or +infinity, have no continuation.  out: a BeamStep to fill."""
-    if logits.dim() != 2 or logits.dtype not in _FLOATS or (logits.shape[1] > 1 and logits.stride(1) != 1) or logits.device.type != 'cuda':
+    dt, shape, stride, dev = _FLOATS.get(logits.dtype), logits.shape, logits.stride(), logits.device
+    if dt is None or len(shape) != 2 or dev.type != 'cuda' or (stride[1] != 1 and shape[1] > 1):
         raise ValueError('logits must be an fp32, fp16 or bf16 GPU tensor [requests * beams, vocabulary], the values of a row side by side')
-    dev, (rows, vocab), ld = logits.device, logits.shape, logits.stride(0)
-    if scores.dtype != torch.float32 or scores.dim() != 2 or scores.device != dev or not scores.is_contiguous() or scores.numel() != rows:
+    rows, vocab = shape
+    if scores.dtype is not torch.float32 or scores.dim() != 2 or scores.device != dev or not scores.is_contiguous() or scores.numel() != rows:
         raise ValueError(f'scores must be a contiguous fp32 tensor [requests, beams] on {dev}, one for each row of the logits')
     requests, beams = scores.shape
     ends = () if eos is None else (eos,) if isinstance(eos, int) else tuple(eos)
@@ -64,7 +66,8 @@ def beam_select(logits, scores, n=None, eos=None, out=None):
         return out
     lib = _lib.load()
     workspace = torch.empty(lib.sp_op_beam_select_workspace(requests, beams, vocab, n), dtype=torch.uint8, device=dev)
-    _call(lib.sp_op_beam_select, dev, _FLOATS[logits.dtype], logits.data_ptr(), ld if rows > 1 else vocab, requests, beams, vocab,
-          scores.data_ptr(), n, len(ends), (ctypes.c_int32 * len(ends))(*ends) if ends else None, *(x.data_ptr() for x in out),
-          workspace.data_ptr())
+    a, b, c, d, e, f = out
+    _call(lib.sp_op_beam_select, dev, dt, logits.data_ptr(), stride[0] if rows > 1 else vocab, requests, beams, vocab, scores.data_ptr(), n,
+          len(ends), (ctypes.c_int32 * len(ends))(*ends) if ends else None, a.data_ptr(), b.data_ptr(), c.data_ptr(), d.data_ptr(),
+          e.data_ptr(), f.data_ptr(), workspace.data_ptr())
     return out

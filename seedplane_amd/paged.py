@@ -327,14 +327,18 @@ class PagedKV:
         rows = seq.shape[0]
         s, p, t = _ints(seq, 'seq', dev, rows), _ints(pos, 'pos', dev, rows), _table(table, dev)
         if out is None:
-            if dtype not in _FLOATS:
+            dt = _FLOATS.get(dtype)
+            if dt is None:
                 raise ValueError('dtype must be fp32, fp16 or bf16')
-            out = torch.empty((2, rows, nkv, hd), dtype=dtype, device=dev).unbind(0)
-        k, v = out
-        dt, k_rows, k_row, k_head, k_addr = _heads(k, 'k', dev, nkv, hd)
-        v_dt, v_rows, v_row, v_head, v_addr = _heads(v, 'v', dev, nkv, hd)
-        if v_dt != dt or k_rows != rows or v_rows != rows:
-            raise ValueError('out must be two tensors of one type, a row for each of seq')
+            k, v = torch.empty((2, rows, nkv, hd), dtype=dtype, device=dev).unbind(0)
+            k_row, k_head, k_addr = nkv * hd, hd, k.data_ptr()
+            v_row, v_head, v_addr = k_row, k_head, v.data_ptr()
+        else:
+            k, v = out
+            dt, k_rows, k_row, k_head, k_addr = _heads(k, 'k', dev, nkv, hd)
+            v_dt, v_rows, v_row, v_head, v_addr = _heads(v, 'v', dev, nkv, hd)
+            if v_dt != dt or k_rows != rows or v_rows != rows:
+                raise ValueError('out must be two tensors of one type, a row for each of seq')
         if rows:
             _call(self.lib.sp_op_paged_read, dev, self._ref, dt, rows, s, p, t, table.shape[0], table.shape[1], k_addr, k_row, k_head,
                   v_addr, v_row, v_head)

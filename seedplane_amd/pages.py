@@ -38,6 +38,7 @@ class PagePool:
             raise ValueError('the caches must have one shape, type, device, layout and scale block')
         self.lib, self.device = kv.lib, kv.device
         self.caches, self.max_seqs, self.max_pages = caches, int(max_seqs), int(max_pages)
+        self._leases = [c._lease for c in caches if c._lease is not None]      # of an engine's pool, which may move
         if not 1 <= self.max_seqs <= 65535 or self.max_pages < 1 or self.max_seqs * self.max_pages >= 1 << 30:
             raise ValueError('max_seqs must be in [1, 65535], max_pages positive and their product below 2^30')
         ints = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=self.device)
@@ -57,9 +58,8 @@ class PagePool:
         self._ref = ctypes.addressof(self.desc)
 
     def _run(self, fn, *args):
-        for c in self.caches:
-            if c._lease is not None:
-                c._lease.check()
+        for lease in self._leases:
+            lease.check()
         _call(fn, self.device, self._ref, *args)
         return self
 

@@ -12,6 +12,7 @@ Additions over the reference API (batch and window support the reference does no
     positions (p - W, p] (the Hugging Face sliding-window rule) and positions may grow without bound.
   * `decode(tokens, caches)`: one batched decode step over independent sequences (ragged lengths).
   * `generate_batch(prompts, max_new_tokens)`: greedy decode of many requests as one batch.
+  * `generate_beams(prompt_ids, beams, max_new_tokens)`: beam search.
   * `QwenEngine` is an alias of `Qwen2Engine`.
 Quantized bundles (`quantization_config.quant_method == 'seedplane'`) carry int8 block-32 or int4 group-32 weights
 (`<name>.qweight/.scales/.qzeros`); float bundles are run with fp16 weights.
@@ -830,6 +831,81 @@ class Qwen2Engine:
             for i, seq in zip(live, ids):
                 out[i] += seq
         return out
+
+    @torch.inference_mode()
+    def generate_beams(self, prompt_ids, beams=4, max_new_tokens=128, eos_token_id=None, length_penalty=1.0, graph=True):
+        """Beam search: up to `beams` continuations as (ids, score), the best first; a score is the sum of the ids' log
+        probabilities over their number to the power length_penalty, an eos counted and kept.  A beam that ends is set aside;
+        the search is over after max_new_tokens, or when `beams` ended ones are at least as good as every live one by its
+        present length.  Each step selects on the GPU (beam.beam_select), and beams that continue another's copy the pages of
+        its K/V that they do not share yet into the ring of one that nobody continues (pages.PagePool.copy)."""
+        from .beam import MOST, beam_select
+        from .pages import PagePool
+        K, limit = int(beams), int(max_new_tokens)
+        ends = 0 if eos_token_id is None else 1
+        if not 1 <= K <= min(self.max_tokens, MOST // (1 + ends)):
+            raise ValueError(f'beams must be in [1, {min(self.max_tokens, MOST // (1 + ends))}]')
+        if limit < 1:
+            raise ValueError('max_new_tokens must be positive')
+        n = len(prompt_ids)
+        if n + limit > self.config['max_position_embeddings']:
+            raise ValueError('the prompt and max_new_tokens exceed max_position_embeddings')
+        # (slots in whole pages where the pool is made for this call; a pool of other sizes has the pages that divide it)
+        slots = min(-(-(n + limit) // 64) * 64, self.config['max_position_embeddings'])
+        if self._pool_n == 0:
+            self.reserve(K, slots)
+        elif len(self._free) < K or self._pool_slots < n + limit:
+            self.grow(self._pool_n + max(0, K - len(self._free)), slots)
+        caches = [self.new_cache(n + limit) for _ in range(K)]
+        S = self._pool_slots
+        page = max(d for d in range(1, min(S, 64) + 1) if S % d == 0)
+        with torch.cuda.stream(self.stream):
+            pool = PagePool([self.paged_kv(layer, page) for layer in range(self.n_layers)], 1, 1)
+            first_page = {c.seq: c.seq * self.n_kv_heads * S // page for c in caches}
+            logits = torch.empty((K, self.vocab), dtype=torch.float32, device=self.device)
+            scores = torch.full((1, K), -torch.inf, dtype=torch.float32, device=self.device)
+            scores[0, 0] = 0
+            logits[0] = self.forward(prompt_ids, caches[0])[0][0]       # (the logits of beams that do not live are not read)
+            length, common = n, 0                                      # cached positions; those that are the same in every ring
+            ids, done = [[] for _ in range(K)], []
+            for step in range(limit):
+                best = beam_select(logits, scores, eos=eos_token_id)
+                if eos_token_id is not None:
+                    for total, beam, token in zip(*(x[0].tolist() for x in best[:3])):
+                        if token == eos_token_id:
+                            done.append((ids[beam] + [token], total / (step + 1) ** length_penalty))
+                    done = sorted(done, key=lambda d: -d[1])[:K]
+                scores = best.next_scores
+                totals, parents, tokens = scores[0].tolist(), best.next_rows[0].tolist(), best.next_tokens[0].tolist()
+                ids = [ids[p] + [t] if p >= 0 else [] for p, t in zip(parents, tokens)]
+                live = [t / (step + 1) ** length_penalty for t, p in zip(totals, parents) if p >= 0]
+                if not live or step + 1 == limit or (len(done) == K and max(live) <= done[-1][1]):
+                    done += [(i, t / (step + 1) ** length_penalty) for i, t, p in zip(ids, totals, parents) if p >= 0]
+                    break
+                # the first child of a beam keeps its ring, the others get those of beams without one
+                rings, kept = [None] * K, set()
+                for j, p in enumerate(parents):
+                    if p >= 0 and p not in kept:
+                        rings[j] = caches[p]
+                        kept.add(p)
+                spare, src, dst = [c for i, c in enumerate(caches) if i not in kept], [], []
+                for j, p in enumerate(parents):
+                    if rings[j] is None:
+                        rings[j] = spare.pop()
+                        if p >= 0:
+                            a, b = (first_page[c.seq] for c in (caches[p], rings[j]))
+                            part = range(common // page, -(-length // page))
+                            src += [a + i for i in part]
+                            dst += [b + i for i in part]
+                    rings[j].length = length
+                if src:
+                    pool.copy(*torch.tensor([src, dst], dtype=torch.int32).to(self.device).unbind(0))
+                if step == 0 and -1 not in parents:
+                    common = n
+                caches = rings
+                self.decode([max(t, 0) for t in tokens], caches, logits_out=logits, graph=graph)
+                length += 1
+        return sorted(done, key=lambda d: -d[1])[:K]
 
 
 QwenEngine = Qwen2Engine
