@@ -767,7 +767,8 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     }
 }
 
-template <class T, int KV, int HD>
+// LONE: every item is of kind 0.
+template <class T, int KV, int HD, bool LONE = false>
 __global__ void __launch_bounds__(256, 2) k_paged_attn(ArgsOf<KV> a) {
     extern __shared__ __align__(1024) unsigned char smem[];            // attn_smem<KV>
     __shared__ __align__(16) AttnShared sh;
@@ -775,7 +776,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(ArgsOf<KV> a) {
     for (int it = blockIdx.x; it < n; it += gridDim.x) {
         const Item w = a.items[it];
         if (it != (int)blockIdx.x) lds_barrier();                      // LDS is free of the item before
-        if (w.kind == 0) run_item<T, KV, HD, 1>(a, w, smem, sh);
+        if (LONE || w.kind == 0) run_item<T, KV, HD, 1>(a, w, smem, sh);
         else if (w.kind == 1) run_item<T, KV, HD, 2>(a, w, smem, sh);
         else run_item<T, KV, HD, 4>(a, w, smem, sh);
     }
