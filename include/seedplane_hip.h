@@ -435,7 +435,9 @@ typedef struct sp_paged_kv {
  * positions is lost.  The rows of a block may stand anywhere in the call; of two rows for the same place the later one
  * alone counts.
  * Magnitudes above 2^60 codes saturate; a NaN makes an int8 block's scale NaN until it begins anew, e4m3 keeps it to its place.
- * Here scale_block * rot_dim is at most 16384 and scale_block * head_dim below 65536. */
+ * Here scale_block * rot_dim is at most 16384, scale_block * head_dim below 65536 and max_pages * page_size at most 2^30.  Each block's
+ * rows are looked for among all of the call's (8 bytes a row): tens of thousands of rows are better given in several calls, each of whole
+ * blocks. */
 int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t n_heads,
                        const void *q_dev, int64_t q_row, int64_t q_head, const void *k_dev, int64_t k_row, int64_t k_head,
                        const void *v_dev, int64_t v_row, int64_t v_head, const int32_t *pos_dev, const int32_t *seq_dev,

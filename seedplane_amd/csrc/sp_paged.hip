@@ -328,6 +328,7 @@ int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t d
         const Rotation rot = rotation_of(rotary, hd);
         require(!kv->scale_block || (kv->scale_block * (int64_t)rot.rot <= 16384 && kv->scale_block * (int64_t)hd < (1 << 16)), SP_EINVAL,
                 "scale_block * rot_dim must be at most 16384 and scale_block * head_dim below 65536");
+        require(!kv->scale_block || (int64_t)max_pages * kv->page_size <= (1 << 30), SP_EINVAL, "a table over blocks must be of at most 2^30 positions");
         if (n_rows == 0) return;
         require(k_dev && v_dev && seq_dev && at_dev && table_dev && (!rotary || pos_dev), SP_EINVAL, "NULL pointer");
         require(kv->k_dev != kv->v_dev, SP_EINVAL, "keys and values need memory of their own");

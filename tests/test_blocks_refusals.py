@@ -16,11 +16,11 @@ def cache(dtype=I8, k=P, v=2 * P, ks=3 * P, vs=4 * P, stride=4 * 32 * 64, head=3
     return _lib.PagedKVDesc(k, v, ks, vs, stride, head, row, dtype, n, page, nkv, hd, block)
 
 
-def append(kv=None, rot=64, dtype=_lib.SP_DT_F16, rows=4, heads=8, q=8 * P, k=9 * P, v=10 * P, q_out=12 * P, hd=64):
+def append(kv=None, rot=64, dtype=_lib.SP_DT_F16, rows=4, heads=8, q=8 * P, k=9 * P, v=10 * P, q_out=12 * P, hd=64, width=4):
     kv = cache() if kv is None else kv
     r = _lib.RotaryDesc(P, rot, 0, 1.0, 0)
     return _lib.load().sp_op_paged_append(ctypes.byref(kv), ctypes.byref(r), dtype, rows, heads, q, 16 * hd, hd, k, 4 * hd, hd, v, 4 * hd, hd,
-                                          P, P, P, P, 2, 4, q_out, dtype, 8 * hd, hd, None)
+                                          P, P, P, P, 2, width, q_out, dtype, 8 * hd, hd, None)
 
 
 def read(kv=None, dtype=_lib.SP_DT_F16, rows=4, seq=P, at=P, table=P, n_seq=2, width=4, k=8 * P, k_row=256, k_head=64, v=9 * P):
@@ -41,7 +41,7 @@ def test_caches_are_refused_everywhere(kw):
 
 @pytest.mark.parametrize('kw', [
     dict(kv=cache(vs=3 * P)), dict(kv=cache(vs=3 * P + 64)), dict(kv=cache(ks=P + 64)), dict(kv=cache(vs=2 * P)), dict(k=3 * P),
-    dict(v=4 * P - 8), dict(q=3 * P), dict(q_out=4 * P),
+    dict(v=4 * P - 8), dict(q=3 * P), dict(q_out=4 * P), dict(width=(1 << 25) + 1),
     dict(kv=cache(page=128, block=128, hd=256, row=256, head=128 * 256, stride=4 * 128 * 256), rot=256, hd=256),
     dict(kv=cache(page=128, block=128, hd=512, row=512, head=128 * 512, stride=4 * 128 * 512), rot=64, hd=512, heads=1, q_out=14 * P),
 ])

@@ -335,6 +335,38 @@ def test_hidden_pages_and_poisoned_blocks(gpu_device, dtype, cache):
     assert float((lse - math.log(40)).abs().max()) <= 2.0 ** -15 * 5
 
 
+def test_pools_past_32_bits(gpu_device):
+    """Pages, codes and scales behind 2^32 bytes of a pool: append, read, attention and the page pool's copies."""
+    from seedplane_amd.pages import PagePool
+    g = torch.Generator().manual_seed(13)
+    nkv, page, hd, n = 2, 128, 128, 140000                    # 4.6 GB of keys, as much of values
+    pools = [torch.empty((n, nkv, page, hd), dtype=I8, device=gpu_device) for _ in range(2)]
+    scales = [torch.ones((n, nkv, page // 16), device=gpu_device) for _ in range(2)]
+    kv = PagedKV(*pools, *scales)
+    table = _int([[n - 1, 3, n - 2], [7, n - 3, 5]])
+    seq, at = _int([0] * 300 + [1] * 270), _int(list(range(300)) + list(range(270)))
+    x = torch.randn((570, 6, hd), generator=g).half().to(gpu_device)
+    q = kv.append(x[:, 2:4], x[:, 4:], seq, at, table, rotary=Rotary(hd, theta=1e6), q=x[:, :2])
+    lens = [300, 270]
+    plan = AttentionPlan(2, nkv, hd, 2, 2).set([1, 1], lens)
+    out = plan.run(q[[299, 569]].contiguous(), kv, table)
+    used = torch.unique(table.view(-1)).long()
+    small = torch.zeros_like(table)
+    for i, e in enumerate(used.tolist()):
+        small[table == e] = i
+    args = [t[used] for p in zip(pools, scales) for t in p]
+    want, _, bound = attend_blocks64(q[[299, 569]], *args, small, [1, 1], lens, hd ** -0.5)
+    _within(out, want, bound)
+    k, v = kv.read(seq, at, table, dtype=F32)
+    held = dense64(args[2], args[3])
+    pos = at.cpu().long()
+    _within(v, torch.stack([held[int(small[s, p // page]), :, p % page] for s, p in zip(seq.tolist(), pos.tolist())]), torch.full((570, nkv, hd), 1e-6, dtype=torch.float64))
+    pool = PagePool(kv, 2, 3)
+    pool.copy(_int([n - 1, 3]), _int([11, n - 9]))
+    for p in (pools[0], pools[1], scales[0], scales[1]):
+        assert torch.equal(p[11], p[n - 1]) and torch.equal(p[n - 9], p[3])
+
+
 def test_serving_run_captured(gpu_device):
     """A prompt appended, then steps of append and attention in a graph that follows positions on the device; every step against the
     64-bit form over what the cache holds, and against the eager calls in every bit."""
