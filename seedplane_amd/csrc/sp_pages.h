@@ -61,23 +61,33 @@ __device__ __forceinline__ int block_rank(int v, int *wave_sums, int &total) {
     return before + x - v;
 }
 
+// Holders of pages at .. at + PER - 1 (1 behind the last page).
+__device__ __forceinline__ void load_holders(const int *holders, int n_pages, int at, int (&h)[PER]) {
+    typedef int Vector __attribute__((ext_vector_type(PER), aligned(4)));
+    if (at + PER <= n_pages) {
+        const Vector v = *(const Vector *)(holders + at);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) h[j] = v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) h[j] = at + j < n_pages ? holders[at + j] : 1;
+    }
+}
+
 // The lowest `want` free pages in order to list; returns how many there are.
 template <int N>
 __device__ __forceinline__ int take_free(const int *holders, int n_pages, int want, int *list, int *wave_sums) {
     int found = 0;
     for (int e0 = 0; e0 < n_pages && found < want; e0 += N * PER) {
         const int at = e0 + (int)threadIdx.x * PER;
-        bool free[PER];
-        int mine = 0, total;
+        int h[PER], mine = 0, total;
+        load_holders(holders, n_pages, at, h);
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            free[j] = at + j < n_pages && holders[at + j] == 0;
-            mine += free[j];
-        }
+        for (int j = 0; j < PER; ++j) mine += h[j] == 0;
         int rank = found + block_rank<N>(mine, wave_sums, total);
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-            if (free[j] && rank < want) list[rank++] = at + j;
+            if (h[j] == 0 && rank < want) list[rank++] = at + j;
         found += total;
     }
     __syncthreads();
@@ -94,10 +104,8 @@ __device__ __forceinline__ Child child_of(const Pool &a, int p) {
     const bool has = rest && a.table[(int64_t)p * a.width + full] >= 0;
     return {p, len, full + (rest > 0), has ? rest : 0};
 }
-// Entry (s, j): what the new row holds, and holders of what changes.
-__device__ __forceinline__ void fork_entry(const Pool &a, int s, int j, int parent, int keep) {
-    const int64_t at = (int64_t)s * a.width + j;
-    const int now = a.table[at], e = j < keep ? a.table[(int64_t)parent * a.width + j] : -1;
+// Entry (s, j), where `now` was: e.
+__device__ __forceinline__ void fork_entry(const Pool &a, int64_t at, int now, int e) {
     a.rows[at] = e;
     if (e != now) {
         if (now >= 0 && now < a.n_pages) atomicSub(&a.holders[now], 1);
@@ -114,7 +122,10 @@ __global__ void __launch_bounds__(THREADS) k_fork_rows(Pool a, const int *parent
         for (int i = lane; i < s; i += 64) earlier |= parents[i] == c.parent;
     if (__any(earlier)) --c.keep;
     else c.copy = 0;
-    for (int j = lane; j < a.width; j += 64) fork_entry(a, s, j, c.parent, c.keep);
+    for (int j = lane; j < a.width; j += 64) {
+        const int64_t at = (int64_t)s * a.width + j;
+        fork_entry(a, at, a.table[at], j < c.keep ? a.table[(int64_t)c.parent * a.width + j] : -1);
+    }
     if (lane == 0) {
         a.fresh[s] = c.len;
         a.first[s] = c.copy;
@@ -123,7 +134,8 @@ __global__ void __launch_bounds__(THREADS) k_fork_rows(Pool a, const int *parent
 // Pages for the copies, in the order of sequences.  One block; ROWS: it makes the rows too.
 template <bool ROWS, int N>
 __global__ void __launch_bounds__(N) k_fork(Pool a, const int *parents) {
-    __shared__ int wave_sums[N / 64], first_s[ROWS ? SEQS_IN_ONE : 1], keep_s[ROWS ? SEQS_IN_ONE : 1];
+    constexpr int M = ROWS ? SEQS_IN_ONE : 1;
+    __shared__ int wave_sums[N / 64], parent_s[M], first_s[M], keep_s[M], full_s[M], copy_s[M];
     const int tid = threadIdx.x;
     if constexpr (ROWS) {
         for (int s = tid; s < a.S; s += N) first_s[s] = a.S;
@@ -131,41 +143,68 @@ __global__ void __launch_bounds__(N) k_fork(Pool a, const int *parents) {
         for (int s = tid; s < a.S; s += N) {
             const Child c = child_of(a, parents[s]);
             if (c.copy) atomicMin(&first_s[c.parent], s);
+            parent_s[s] = c.parent;
             keep_s[s] = c.keep;
+            full_s[s] = c.len / a.page;
+            copy_s[s] = c.copy;
             a.fresh[s] = c.len;
-            a.first[s] = c.copy;
         }
         __syncthreads();
         for (int s = tid; s < a.S; s += N)
-            if (a.first[s]) {
-                if (first_s[parents[s]] == s) a.first[s] = 0;
+            if (copy_s[s]) {
+                if (first_s[parent_s[s]] == s) copy_s[s] = 0;
                 else --keep_s[s];
             }
         __syncthreads();
+        constexpr int AT_ONCE = 4;
         const int entries = a.S * a.width;
-        for (int i = tid; i < entries; i += N) {
-            const int s = i / a.width;
-            fork_entry(a, s, i - s * a.width, parents[s], keep_s[s]);
+        for (int i0 = tid; i0 < entries; i0 += N * AT_ONCE) {
+            int now[AT_ONCE], e[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const int i = min(i0 + k * N, entries - 1), s = i / a.width, j = i - s * a.width;
+                now[k] = a.table[i];
+                e[k] = a.table[j < keep_s[s] ? parent_s[s] * a.width + j : i];
+                if (j >= keep_s[s]) e[k] = -1;
+            }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k)
+                if (i0 + k * N < entries) fork_entry(a, i0 + k * N, now[k], e[k]);
         }
         __syncthreads();
     }
+    // first_s / a.first: rows of a last page to copy, then the place of the sequence among those that copy
     int wanted = 0;
     for (int s0 = 0; s0 < a.S; s0 += N) {
-        const int s = s0 + tid, rest = s < a.S ? a.first[s] : 0;
+        const int s = s0 + tid, rest = s >= a.S ? 0 : ROWS ? copy_s[s] : a.first[s];
         int total;
         const int at = wanted + block_rank<N>(rest > 0, wave_sums, total);
-        if (rest > 0) a.moves[at] = {s, -1, rest};
+        if (s < a.S) {
+            if constexpr (ROWS) first_s[s] = at;
+            if (rest > 0) {
+                a.moves[at].rows = rest;
+                if constexpr (!ROWS) a.moves[at].src = s;
+            }
+        }
         wanted += total;
     }
     __syncthreads();
     const int got = take_free<N>(a.holders, a.n_pages, wanted, a.list, wave_sums);
-    for (int k = tid; k < wanted; k += N) {
-        const int s = a.moves[k].src, full = a.fresh[s] / a.page, p = parents[s];
+    auto place = [&](int s, int p, int full, int k) {
         const int src = a.table[(int64_t)p * a.width + full], dst = k < got ? a.list[k] : -1;
         if (dst >= 0) a.holders[dst] = 1;
         a.rows[(int64_t)s * a.width + full] = dst;
         a.moves[k].src = src;
         a.moves[k].dst = dst;
+    };
+    if constexpr (ROWS) {
+        for (int s = tid; s < a.S; s += N)
+            if (copy_s[s]) place(s, parent_s[s], full_s[s], first_s[s]);
+    } else {
+        for (int k = tid; k < wanted; k += N) {
+            const int s = a.moves[k].src;
+            place(s, parents[s], a.fresh[s] / a.page, k);
+        }
     }
     if (tid == 0) {
         a.counts[0] = got;
@@ -296,26 +335,27 @@ __global__ void __launch_bounds__(N) k_compact(Pool a, int *places) {
     int held = 0;
     for (int e0 = 0; e0 < a.n_pages; e0 += N * PER) {
         const int at = e0 + tid * PER;
-        int mine = 0, total;
+        int h[PER], mine = 0, total;
+        load_holders(a.holders, a.n_pages, at, h);
 #pragma unroll
-        for (int j = 0; j < PER; ++j) mine += at + j < a.n_pages && a.holders[at + j] != 0;
+        for (int j = 0; j < PER; ++j) mine += at + j < a.n_pages && h[j] != 0;
         block_rank<N>(mine, wave_sums, total);
         held += total;
     }
     int moves = 0;
     for (int e0 = held; e0 < a.n_pages; e0 += N * PER) {
         const int at = e0 + tid * PER;
-        bool used[PER];
-        int mine = 0, total;
+        int h[PER], mine = 0, total;
+        load_holders(a.holders, a.n_pages, at, h);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            used[j] = at + j < a.n_pages && a.holders[at + j] != 0;
-            mine += used[j];
+            h[j] = at + j < a.n_pages && h[j] != 0;
+            mine += h[j];
         }
         int rank = moves + block_rank<N>(mine, wave_sums, total);
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-            if (used[j]) a.moves[rank++].src = at + j;
+            if (h[j]) a.moves[rank++].src = at + j;
         moves += total;
     }
     const int low = take_free<N>(a.holders, held, moves, a.list, wave_sums);         // (as many as there are moves)
