@@ -23,6 +23,15 @@
 // exponential, scaling, sum, comparison and half a rounding against a product's 4 HD operations; LDS is used 24 % of the time, without
 // conflicts.  Tried, when this batch took 178 us: four tiles deep with 32 keys 243, sums of rounded weights by dot products 181,
 // priorities 172 to 182, blocks of 8 waves whose halves take turns multiplying and weighing 188.)
+//
+// Caches with a scale per block of positions and head (sp_blocks.h) run the same items: the scales of the table's positions come to LDS by
+// copies of 4 bytes in front of the tiles', each wave makes its own positions' terms of them behind the first scores, and a block's largest
+// score is scaled instead of every score.  64 sequences x 4096 positions, 28 / 4 heads of 128: int8 53.5 us, e4m3 52.4 (268 MB and 8 of
+// scales, 5.0 and 5.1 TB/s).  int8 takes five (fp16) or six (bf16) instructions for four codes where e4m3 takes two: a wave that shares a
+// tile's rows with others brings its part of the tile to 16 bits for all of them, codes going through registers a tile ahead and
+// being written behind products (6 prompts of 12 / 2 heads of 128 72 us, each wave for itself 80, a barrier more instead of the registers 77;
+// e4m3 each for itself 63, once for all 69; the same positions in 16 bits 55).  Tried for waves of their own: keys' codes left 1152 above their
+// values as operands, scores begun at what that adds: 8 sequences of 20000 to 40000 positions 65.0 -> 64.2 us then, not kept.
 #pragma once
 #include "sp_paged_plan.h"
 #include "sp_rotate.h"
