@@ -12,7 +12,10 @@
 //
 // A workgroup takes a chunk of rows of the call (a row whose block an earlier row has is left to that row's workgroup), keys or
 // values, and some heads: it looks up its block's rows among all of the call's, takes the largest magnitude per head, then the codes.
-// Values are read twice unless a thread has but one item of them: a block of 64 positions of one head alone is 8192 values.
+// Values are read twice unless a thread has but one item of them: a block of 64 positions of one head alone is 8192 values.  Long
+// calls (FIND) look up the rows of all a chunk's blocks at once.  They are bound by the blocks' chains of barriers (16384 rows of 28 / 4 / 4
+// heads 82 us, 49 of them without queries, where the bytes take 56 and 10), so their registers are held to those of 6 waves: with 4
+// waves, or more items in flight, the queries' rows behind them lose more (88 to 94 us) than the blocks gain (46).
 #pragma once
 #include "sp_paged.h"
 
@@ -21,6 +24,7 @@ namespace paged {
 constexpr int MOST_BLOCK = 128;                                        // positions of a block at most
 constexpr int BLOCK_HEADS = 64;                                        // heads of a workgroup at most
 constexpr int SEARCHED = 8;                                            // rows that a thread looks at at once
+constexpr int MOST_CHUNK = 256, MOST_FOUND = 512;                      // rows of a chunk; of the call that may be of its blocks
 constexpr float MOST_SCALE = 0x1p60f;                                  // (scales within 2^-60 .. 2^60: attention takes their products)
 
 struct BlockAppendArgs : AppendArgs {                                  // ks, vs are not used; units, tail, vecs are a head's
@@ -29,7 +33,8 @@ struct BlockAppendArgs : AppendArgs {                                  // ks, vs
     PageDivisor by_block, by_page;
     int chunk, chunks, splits, heads;                                  // rows of a workgroup, their number; workgroups over heads, heads of each
     Divisor by_key, by_value;                                          // vectors of a slot: keys (pairs of them where rotated), values
-    uint32_t angles_at;                                                // LDS bytes before the angles [block][rot / 2]
+    bool find;                                                         // rows of a chunk's blocks are looked up at once
+    PageDivisor by_keys, by_values;                                    // of a block of a head
 };
 struct ReadArgs {
     const void *kc, *vc;
@@ -88,6 +93,7 @@ struct BlockShared {
     uint32_t most[BLOCK_HEADS];                                        // bits of the largest magnitude
     float scale[BLOCK_HEADS], keep[BLOCK_HEADS];                       // 1 / new scale; old / new (1: codes stay)
     int earlier;
+    int found, row[MOST_FOUND], seq[MOST_FOUND], at[MOST_FOUND];       // the call's rows that may be of a block of the chunk (FIND)
 };
 
 // The largest magnitude of N values, as bits: a NaN is above all (int8), or left out (e4m3, which holds it as itself).
@@ -112,8 +118,8 @@ __device__ __forceinline__ bool of_block(const BlockAppendArgs &a, int seq, int 
 }
 
 // The block of row r, which does not follow a row of the same block.
-template <class T, int VEC, bool I8>
-__device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, bool keys, int head0, BlockShared &sh, float2 *cs) {
+template <class T, int VEC, bool I8, bool FIND, bool KEYS>
+__device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, int head0, BlockShared &sh, float2 *cs) {
     const int tid = threadIdx.x, s = a.seq[r], p = a.at[r];
     if (s < 0 || s >= a.n_seq || p < 0 || p >= (1 << 30)) return;
     const int b = p / a.by_block, page = p / a.by_page;
@@ -124,67 +130,95 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, bo
     if (tid < a.heads) sh.most[tid] = 0;
     if (tid == 0) sh.earlier = 0;
     __syncthreads();
-    for (int i0 = tid; i0 < a.rows; i0 += ROT_THREADS * SEARCHED) {
-        int seq[SEARCHED], at[SEARCHED];
+    auto look = [&](int i, int seq, int at) {
+        if (!of_block(a, seq, at, s, b)) return;
+        if (i < r) sh.earlier = 1;
+        else atomicMax(&sh.slot[at - b * a.block], i);
+    };
+    if (FIND && sh.found <= MOST_FOUND) {
+        for (int i = tid; i < sh.found; i += ROT_THREADS) look(sh.row[i], sh.seq[i], sh.at[i]);
+    } else {
+        for (int i0 = tid; i0 < a.rows; i0 += ROT_THREADS * SEARCHED) {
+            int seq[SEARCHED], at[SEARCHED];
 #pragma unroll
-        for (int k = 0; k < SEARCHED; ++k) {
-            const int i = min(i0 + k * ROT_THREADS, a.rows - 1);
-            seq[k] = a.seq[i];
-            at[k] = a.at[i];
-        }
+            for (int k = 0; k < SEARCHED; ++k) {
+                const int i = min(i0 + k * ROT_THREADS, a.rows - 1);
+                seq[k] = a.seq[i];
+                at[k] = a.at[i];
+            }
 #pragma unroll
-        for (int k = 0; k < SEARCHED; ++k) {
-            const int i = min(i0 + k * ROT_THREADS, a.rows - 1);
-            if (!of_block(a, seq[k], at[k], s, b)) continue;
-            if (i < r) sh.earlier = 1;
-            else atomicMax(&sh.slot[at[k] - b * a.block], i);
+            for (int k = 0; k < SEARCHED; ++k) look(min(i0 + k * ROT_THREADS, a.rows - 1), seq[k], at[k]);
         }
     }
     __syncthreads();
     if (sh.earlier || e < 0 || e >= a.n_pages) return;
     const int heads = min(a.heads, a.nkv - head0), half = a.rot.rot >> 1;
     const int64_t block_of_page = b - (int64_t)page * a.per_page;
-    float *const scale = (keys ? a.kscale : a.vscale) + ((int64_t)e * a.nkv + head0) * a.per_page + block_of_page;      // of head h: at h * per_page
+    float *const scale = (KEYS ? a.kscale : a.vscale) + ((int64_t)e * a.nkv + head0) * a.per_page + block_of_page;      // of head h: at h * per_page
     const float old = tid < heads ? scale[(int64_t)tid * a.per_page] : 0.f;
     const bool begun = sh.slot[0] >= 0;
-    if (keys && half) {
+    // item: head h, slot i and vector u of it (keys: a rotated pair of vectors, or one of the rest)
+    const Divisor by = KEYS ? a.by_key : a.by_value;
+    const PageDivisor by_head = KEYS ? a.by_keys : a.by_values;
+    const int per = KEYS ? a.units + a.tail : a.vecs, total = a.block * per, items = heads * total;
+    uint8_t *const pool = (uint8_t *)(KEYS ? a.kc : a.vc) + e * a.page_stride + head0 * a.head_stride +
+                          (int64_t)(p - page * a.page_size - (p - b * a.block)) * a.row_stride;
+    struct Item { int h, i, row, turn, at1, at2; bool two; };
+    auto item_of = [&](int k) -> Item {
+        Item x;
+        x.h = k / by_head;
+        k -= x.h * total;
+        x.i = k / by;
+        const int u = k - x.i * per;
+        x.row = sh.slot[x.i];
+        x.two = KEYS && u < a.units;
+        x.turn = x.i * half + u * VEC;
+        if (x.two) unit_offsets<VEC>(a.rot, u, x.at1, x.at2);
+        else x.at1 = x.at2 = KEYS ? a.rot.rot + (u - a.units) * VEC : u * VEC;
+        return x;
+    };
+    typedef T Vector __attribute__((ext_vector_type(VEC)));
+    Vector raw1, raw2;
+    float v1[VEC], v2[VEC];
+    // (a slot without a row reads row r's values and does not use them: loads without a branch)
+    auto fetch = [&](const Item &x) {
+        const int64_t row = x.row >= 0 ? x.row : r;
+        const T *src = KEYS ? (const T *)a.k + row * a.k_row + (int64_t)(head0 + x.h) * a.k_head
+                            : (const T *)a.v + row * a.v_row + (int64_t)(head0 + x.h) * a.v_head;
+        raw1 = *(const Vector *)(src + x.at1);
+        if constexpr (KEYS) raw2 = *(const Vector *)(src + x.at2);
+    };
+    auto values = [&](const Item &x) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            v1[i] = (float)raw1[i];
+            if constexpr (KEYS) v2[i] = (float)raw2[i];
+        }
+        if constexpr (KEYS)
+            if (x.two) turn_unit<VEC>(a.rot, cs + x.turn, v1, v2);
+    };
+    fetch(item_of(min(tid, items - 1)));
+    if (KEYS && half) {
         for (int k = tid; k < a.block * half; k += ROT_THREADS) {
             const int i = k / a.by_half, row = sh.slot[i];
             if (row >= 0) cs[k] = turn_of(a.rot, a.pos[row], k - i * half);
         }
         __syncthreads();
     }
-    // item i: slot and vector of it (keys: a rotated pair of vectors, or one of the rest)
-    const Divisor by = keys ? a.by_key : a.by_value;
-    const int per = keys ? a.units + a.tail : a.vecs, total = a.block * per;
-    uint8_t *const pool = (uint8_t *)(keys ? a.kc : a.vc) + e * a.page_stride + head0 * a.head_stride +
-                          (int64_t)(p - page * a.page_size - (p - b * a.block)) * a.row_stride;
-    auto offsets = [&](int u, int &at1, int &at2) -> bool {
-        if (keys && u < a.units) { unit_offsets<VEC>(a.rot, u, at1, at2); return true; }
-        at1 = at2 = keys ? a.rot.rot + (u - a.units) * VEC : u * VEC;
-        return false;
-    };
-    auto fetch = [&](int row, int h, int i, int u, int at1, int at2, bool two, float *v1, float *v2) {
-        const T *src = keys ? (const T *)a.k + (int64_t)row * a.k_row + (int64_t)(head0 + h) * a.k_head
-                            : (const T *)a.v + (int64_t)row * a.v_row + (int64_t)(head0 + h) * a.v_head;
-        load_values<T, VEC>(src + at1, v1);
-        load_values<T, VEC>(src + at2, v2);
-        if (two) turn_unit<VEC>(a.rot, cs + i * half + u * VEC, v1, v2);
-    };
-    float v1[VEC], v2[VEC];
-    const bool held = total <= ROT_THREADS && heads == 1;              // one item a thread: its values stay in registers
-    for (int k0 = 0; k0 < total; k0 += ROT_THREADS) {
-        const int k = min(k0 + tid, total - 1), i = k / by, u = k - i * per, row = sh.slot[i];
-        int at1, at2;
-        const bool two = offsets(u, at1, at2);
-        for (int h = 0; h < heads; ++h) {
-            uint32_t most = 0;
-            if (row >= 0) {
-                fetch(row, h, i, u, at1, at2, two, v1, v2);
-                most = magnitude<I8, VEC>(v2, magnitude<I8, VEC>(v1, 0));
-            }
+    for (int k0 = 0; k0 < items; k0 += ROT_THREADS) {
+        const Item x = item_of(min(k0 + tid, items - 1));
+        if (k0 > 0) fetch(x);
+        uint32_t most = 0;
+        if (x.row >= 0) {
+            values(x);
+            most = magnitude<I8, VEC>(v1, 0);
+            if constexpr (KEYS) most = magnitude<I8, VEC>(v2, most);
+        }
+        if (total % 64 == 0) {                                         // a wave's items are of one head
             most = wave_umax(most);
-            if ((tid & 63) == 0 && most) atomicMax(&sh.most[h], most);
+            if ((tid & 63) == 0 && most) atomicMax(&sh.most[x.h], most);
+        } else if (most) {
+            atomicMax(&sh.most[x.h], most);
         }
     }
     __syncthreads();
@@ -199,48 +233,105 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, bo
         scale[(int64_t)tid * a.per_page] = grown;
     }
     __syncthreads();
-    for (int k = tid; k < total; k += ROT_THREADS) {
-        const int i = k / by, u = k - i * per, row = sh.slot[i];
-        int at1, at2;
-        const bool two = offsets(u, at1, at2);
-        for (int h = 0; h < heads; ++h) {
-            uint8_t *const to = pool + h * a.head_stride + i * a.row_stride;
-            const float f = row >= 0 ? sh.scale[h] : sh.keep[h];
-            if (row >= 0) {
-                if (!held) fetch(row, h, i, u, at1, at2, two, v1, v2);
-            } else {
-                if (f == 1.f) continue;
-                load_codes<I8, VEC>(to + at1, v1);
-                load_codes<I8, VEC>(to + at2, v2);
-            }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) { v1[j] *= f; v2[j] *= f; }
-            store_codes<I8, VEC>(to + at1, v1);
-            if (two) store_codes<I8, VEC>(to + at2, v2);
+    for (int k = tid; k < items; k += ROT_THREADS) {
+        const Item x = item_of(k);
+        uint8_t *const to = pool + x.h * a.head_stride + x.i * a.row_stride;
+        const float f = x.row >= 0 ? sh.scale[x.h] : sh.keep[x.h];
+        if (x.row >= 0) {
+            if (items > ROT_THREADS) fetch(x);                         // (else its values are still here)
+            values(x);
+        } else {
+            if (f == 1.f) continue;
+            load_codes<I8, VEC>(to + x.at1, v1);
+            if constexpr (KEYS) load_codes<I8, VEC>(to + x.at2, v2);
         }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            v1[i] *= f;
+            if constexpr (KEYS) v2[i] *= f;
+        }
+        store_codes<I8, VEC>(to + x.at1, v1);
+        if constexpr (KEYS)
+            if (x.two) store_codes<I8, VEC>(to + x.at2, v2);
     }
 }
 
+// Rows of the call that are of the sequences and blocks between the least and largest of the chunk's, to sh.found.  (Every wave looks at the
+// chunk's rows itself.)
+__device__ __forceinline__ void find_rows(const BlockAppendArgs &a, int first, int last, BlockShared &sh) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    int s0 = 0x7fffffff, s1 = -1, p0 = 0x7fffffff, p1 = -1;
+    for (int r = first + lane; r < last; r += 64) {
+        const int s = a.seq[r], p = a.at[r];
+        if (s < 0 || s >= a.n_seq || p < 0 || p >= (1 << 30)) continue;
+        s0 = min(s0, s); s1 = max(s1, s);
+        p0 = min(p0, p); p1 = max(p1, p);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        s0 = min(s0, __shfl_xor(s0, o)); s1 = max(s1, __shfl_xor(s1, o));
+        p0 = min(p0, __shfl_xor(p0, o)); p1 = max(p1, __shfl_xor(p1, o));
+    }
+    if (tid == 0) sh.found = 0;
+    __syncthreads();
+    if (s1 < 0) return;
+    p0 = p0 / a.by_block * a.block;
+    p1 = p1 / a.by_block * a.block + (a.block - 1);
+    auto look = [&](int i, int seq, int at) {
+        if (seq < s0 || seq > s1 || at < p0 || at > p1) return;
+        const int k = atomicAdd(&sh.found, 1);
+        if (k < MOST_FOUND) { sh.row[k] = i; sh.seq[k] = seq; sh.at[k] = at; }
+    };
+    typedef int Four __attribute__((ext_vector_type(4), aligned(4)));
+    const int whole = a.rows / 4 * 4;
+    constexpr int STEP = ROT_THREADS * 4;
+    for (int i0 = tid * 4; i0 < whole; i0 += STEP * 4) {
+        Four seq[4], at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = min(i0 + k * STEP, whole - 4);
+            seq[k] = *(const Four *)(a.seq + i);
+            at[k] = *(const Four *)(a.at + i);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i0 + k * STEP >= whole) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) look(i0 + k * STEP + j, seq[k][j], at[k][j]);
+        }
+    }
+    if (whole + tid < a.rows) look(whole + tid, a.seq[whole + tid], a.at[whole + tid]);
+    __syncthreads();
+}
+
 // Blocks: chunks x (keys, values) x splits of the heads, then the queries' rows.
-template <class T, int VEC, bool I8>
-__global__ void __launch_bounds__(ROT_THREADS) k_append_blocks(BlockAppendArgs a) {
+template <class T, int VEC, bool I8, bool FIND>
+__global__ void __launch_bounds__(ROT_THREADS, FIND ? 6 : 1) k_append_blocks(BlockAppendArgs a) {
     extern __shared__ __align__(16) unsigned char block_smem[];
     __shared__ BlockShared sh;
     const int parts = 2 * a.splits, n = a.chunks * parts;
-    if ((int)blockIdx.x >= n) {
-        append_rows<T, VEC>(a, blockIdx.x - n, block_smem);
+    const int block = blockIdx.x;
+    if (block >= n) {
+        append_rows<T, VEC>(a, block - n, block_smem);
         return;
     }
-    const int chunk = blockIdx.x / parts, part = blockIdx.x - chunk * parts;
+    const int chunk = block / parts, part = block - chunk * parts;
+    const int first = chunk * a.chunk, last = min(a.rows, first + a.chunk), head0 = part % a.splits * a.heads;
+    if constexpr (FIND) find_rows(a, first, last, sh);
     // the chunk's rows that begin a run of a block's rows (every wave finds the same)
-    const int r = chunk * a.chunk + (int)(threadIdx.x & 63);
-    bool begins = r < a.rows && r < (chunk + 1) * a.chunk;
-    if (begins && r > 0) {
-        const int s = a.seq[r], p = a.at[r];
-        begins = p < 0 || p >= (1 << 30) || !of_block(a, a.seq[r - 1], a.at[r - 1], s, p / a.by_block);
+    for (int r0 = first; r0 < last; r0 += 64) {
+        const int r = r0 + (int)(threadIdx.x & 63);
+        bool begins = r < last;
+        if (begins && r > 0) {
+            const int s = a.seq[r], p = a.at[r];
+            begins = p < 0 || p >= (1 << 30) || !of_block(a, a.seq[r - 1], a.at[r - 1], s, p / a.by_block);
+        }
+        for (uint64_t runs = __ballot(begins); runs; runs &= runs - 1) {
+            const int at = r0 + __builtin_ctzll(runs);
+            if (part < a.splits) append_block<T, VEC, I8, FIND, true>(a, at, head0, sh, (float2 *)block_smem);
+            else append_block<T, VEC, I8, FIND, false>(a, at, head0, sh, (float2 *)block_smem);
+        }
     }
-    for (uint64_t runs = __ballot(begins); runs; runs &= runs - 1)
-        append_block<T, VEC, I8>(a, chunk * a.chunk + __builtin_ctzll(runs), part < a.splits, part % a.splits * a.heads, sh, (float2 *)block_smem);
 }
 
 // ------------------------------------------------------------------------------------------------ read

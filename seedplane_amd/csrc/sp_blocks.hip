@@ -22,10 +22,15 @@ void typed_items(bool i8, int HD, bool lone, const BlockArgs &a, int grid, hipSt
     else if (lone) items_of<T, KV_I8_BLOCKS, true>(HD, a, grid, st);
     else items_of<T, KV_I8_BLOCKS>(HD, a, grid, st);
 }
+template <class T, int VEC, bool I8>
+void append_codes(const BlockAppendArgs &a, int grid, size_t lds, hipStream_t st) {
+    if (a.find) hipLaunchKernelGGL((k_append_blocks<T, VEC, I8, true>), dim3(grid), dim3(ROT_THREADS), lds, st, a);
+    else hipLaunchKernelGGL((k_append_blocks<T, VEC, I8, false>), dim3(grid), dim3(ROT_THREADS), lds, st, a);
+}
 template <class T, int VEC>
 void append_of(const BlockAppendArgs &a, int grid, size_t lds, hipStream_t st) {
-    if (a.kv_dt == SP_DT_I8) hipLaunchKernelGGL((k_append_blocks<T, VEC, true>), dim3(grid), dim3(ROT_THREADS), lds, st, a);
-    else hipLaunchKernelGGL((k_append_blocks<T, VEC, false>), dim3(grid), dim3(ROT_THREADS), lds, st, a);
+    if (a.kv_dt == SP_DT_I8) append_codes<T, VEC, true>(a, grid, lds, st);
+    else append_codes<T, VEC, false>(a, grid, lds, st);
 }
 template <class T>
 void read_of(bool wide, const ReadArgs &a, hipStream_t st) {
