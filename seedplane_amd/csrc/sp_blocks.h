@@ -6,16 +6,17 @@
 // holds, its scale only grows, and where it does the codes that the call does not write are rounded once more, by old / new scale.
 //
 // What bounds it: a step is a chain of dependent accesses (row, table entry beside the search, values, scale, codes): 16 rows of 12 / 2 / 2
-// heads of 128 take 7 us, their reading back 3.5, where an empty launch takes 2.3; a prompt of 1777 rows of 28 / 4 / 4 heads, 26 MB of
-// values, takes 14 us, most of it the queries' rows, which the plain append's loop rotates (sp_rotate.h says what bounds that); its
+// heads of 128 take 6.1 us, their reading back 3.5, where an empty launch takes 2.3; a prompt of 1777 rows of 28 / 4 / 4 heads, 26 MB of
+// values, takes 15 us, most of it the queries' rows, which the plain append's loop rotates (sp_rotate.h says what bounds that); its
 // reading back 4.4 (14 MB).
 //
 // A workgroup takes a chunk of rows of the call (a row whose block an earlier row has is left to that row's workgroup), keys or
 // values, and some heads: it looks up its block's rows among all of the call's, takes the largest magnitude per head, then the codes.
 // Values are read twice unless a thread has but one item of them: a block of 64 positions of one head alone is 8192 values.  Long
 // calls (FIND) look up the rows of all a chunk's blocks at once.  They are bound by the blocks' chains of barriers (16384 rows of 28 / 4 / 4
-// heads 82 us, 49 of them without queries, where the bytes take 56 and 10), so their registers are held to those of 6 waves: with 4
-// waves, or more items in flight, the queries' rows behind them lose more (88 to 94 us) than the blocks gain (46).
+// heads 78 us, 41 of them without queries, where the bytes take 56 and 10), so their registers are held to those of 6 waves: with 5
+// waves the blocks gain less than the queries' rows behind them lose (83).  Keys and values have loops of their own: one for both
+// had more uniform values than scalar registers hold (16 rows 7.0 us instead of 6.1, 16384 89 instead of 78).
 #pragma once
 #include "sp_paged.h"
 
@@ -23,7 +24,7 @@ namespace paged {
 
 constexpr int MOST_BLOCK = 128;                                        // positions of a block at most
 constexpr int BLOCK_HEADS = 64;                                        // heads of a workgroup at most
-constexpr int SEARCHED = 8;                                            // rows that a thread looks at at once
+constexpr int SEARCHED = 4;                                            // rows that a thread looks at at once
 constexpr int MOST_CHUNK = 256, MOST_FOUND = 512;                      // rows of a chunk; of the call that may be of its blocks
 constexpr float MOST_SCALE = 0x1p60f;                                  // (scales within 2^-60 .. 2^60: attention takes their products)
 
@@ -88,12 +89,13 @@ __device__ __forceinline__ void load_codes(const uint8_t *p, float *v) {
 }
 
 // ------------------------------------------------------------------------------------------------ append
+template <bool FIND>
 struct BlockShared {
     int slot[MOST_BLOCK];                                              // the row that brings each position of the block (the last one), -1
     uint32_t most[BLOCK_HEADS];                                        // bits of the largest magnitude
     float scale[BLOCK_HEADS], keep[BLOCK_HEADS];                       // 1 / new scale; old / new (1: codes stay)
     int earlier;
-    int found, row[MOST_FOUND], seq[MOST_FOUND], at[MOST_FOUND];       // the call's rows that may be of a block of the chunk (FIND)
+    int found, row[FIND ? MOST_FOUND : 1], seq[FIND ? MOST_FOUND : 1], at[FIND ? MOST_FOUND : 1];       // the call's rows that may be of a block of the chunk (FIND)
 };
 
 // The largest magnitude of N values, as bits: a NaN is above all (int8), or left out (e4m3, which holds it as itself).
@@ -119,7 +121,7 @@ __device__ __forceinline__ bool of_block(const BlockAppendArgs &a, int seq, int 
 
 // The block of row r, which does not follow a row of the same block.
 template <class T, int VEC, bool I8, bool FIND, bool KEYS>
-__device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, int head0, BlockShared &sh, float2 *cs) {
+__device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, int head0, BlockShared<FIND> &sh, float2 *cs) {
     const int tid = threadIdx.x, s = a.seq[r], p = a.at[r];
     if (s < 0 || s >= a.n_seq || p < 0 || p >= (1 << 30)) return;
     const int b = p / a.by_block, page = p / a.by_page;
@@ -197,7 +199,6 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
         if constexpr (KEYS)
             if (x.two) turn_unit<VEC>(a.rot, cs + x.turn, v1, v2);
     };
-    fetch(item_of(min(tid, items - 1)));
     if (KEYS && half) {
         for (int k = tid; k < a.block * half; k += ROT_THREADS) {
             const int i = k / a.by_half, row = sh.slot[i];
@@ -207,7 +208,7 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
     }
     for (int k0 = 0; k0 < items; k0 += ROT_THREADS) {
         const Item x = item_of(min(k0 + tid, items - 1));
-        if (k0 > 0) fetch(x);
+        fetch(x);
         uint32_t most = 0;
         if (x.row >= 0) {
             values(x);
@@ -239,7 +240,7 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
         const float f = x.row >= 0 ? sh.scale[x.h] : sh.keep[x.h];
         if (x.row >= 0) {
             if (items > ROT_THREADS) fetch(x);                         // (else its values are still here)
-            values(x);
+            if (FIND || items > ROT_THREADS) values(x);                // (FIND: turned again, for the registers)
         } else {
             if (f == 1.f) continue;
             load_codes<I8, VEC>(to + x.at1, v1);
@@ -258,7 +259,7 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
 
 // Rows of the call that are of the sequences and blocks between the least and largest of the chunk's, to sh.found.  (Every wave looks at the
 // chunk's rows itself.)
-__device__ __forceinline__ void find_rows(const BlockAppendArgs &a, int first, int last, BlockShared &sh) {
+__device__ __forceinline__ void find_rows(const BlockAppendArgs &a, int first, int last, BlockShared<true> &sh) {
     const int tid = threadIdx.x, lane = tid & 63;
     int s0 = 0x7fffffff, s1 = -1, p0 = 0x7fffffff, p1 = -1;
     for (int r = first + lane; r < last; r += 64) {
@@ -304,19 +305,9 @@ __device__ __forceinline__ void find_rows(const BlockAppendArgs &a, int first, i
     __syncthreads();
 }
 
-// Blocks: chunks x (keys, values) x splits of the heads, then the queries' rows.
-template <class T, int VEC, bool I8, bool FIND>
-__global__ void __launch_bounds__(ROT_THREADS, FIND ? 6 : 1) k_append_blocks(BlockAppendArgs a) {
-    extern __shared__ __align__(16) unsigned char block_smem[];
-    __shared__ BlockShared sh;
-    const int parts = 2 * a.splits, n = a.chunks * parts;
-    const int block = blockIdx.x;
-    if (block >= n) {
-        append_rows<T, VEC>(a, block - n, block_smem);
-        return;
-    }
-    const int chunk = block / parts, part = block - chunk * parts;
-    const int first = chunk * a.chunk, last = min(a.rows, first + a.chunk), head0 = part % a.splits * a.heads;
+template <class T, int VEC, bool I8, bool FIND, bool KEYS>
+__device__ __forceinline__ void append_chunk(const BlockAppendArgs &a, int chunk, int split, BlockShared<FIND> &sh, float2 *cs) {
+    const int first = chunk * a.chunk, last = min(a.rows, first + a.chunk);
     if constexpr (FIND) find_rows(a, first, last, sh);
     // the chunk's rows that begin a run of a block's rows (every wave finds the same)
     for (int r0 = first; r0 < last; r0 += 64) {
@@ -326,12 +317,25 @@ __global__ void __launch_bounds__(ROT_THREADS, FIND ? 6 : 1) k_append_blocks(Blo
             const int s = a.seq[r], p = a.at[r];
             begins = p < 0 || p >= (1 << 30) || !of_block(a, a.seq[r - 1], a.at[r - 1], s, p / a.by_block);
         }
-        for (uint64_t runs = __ballot(begins); runs; runs &= runs - 1) {
-            const int at = r0 + __builtin_ctzll(runs);
-            if (part < a.splits) append_block<T, VEC, I8, FIND, true>(a, at, head0, sh, (float2 *)block_smem);
-            else append_block<T, VEC, I8, FIND, false>(a, at, head0, sh, (float2 *)block_smem);
-        }
+        for (uint64_t runs = __ballot(begins); runs; runs &= runs - 1)
+            append_block<T, VEC, I8, FIND, KEYS>(a, r0 + __builtin_ctzll(runs), split * a.heads, sh, cs);
     }
+}
+
+// Blocks: chunks x (keys, values) x splits of the heads, then the queries' rows.
+template <class T, int VEC, bool I8, bool FIND>
+__global__ void __launch_bounds__(ROT_THREADS, FIND ? 6 : 1) k_append_blocks(BlockAppendArgs a) {
+    extern __shared__ __align__(16) unsigned char block_smem[];
+    __shared__ BlockShared<FIND> sh;
+    const int parts = 2 * a.splits, n = a.chunks * parts;
+    const int block = blockIdx.x;
+    if (block >= n) {
+        append_rows<T, VEC>(a, block - n, block_smem);
+        return;
+    }
+    const int chunk = block / parts, part = block - chunk * parts;
+    if (part < a.splits) append_chunk<T, VEC, I8, FIND, true>(a, chunk, part, sh, (float2 *)block_smem);
+    else append_chunk<T, VEC, I8, FIND, false>(a, chunk, part - a.splits, sh, (float2 *)block_smem);
 }
 
 // ------------------------------------------------------------------------------------------------ read
