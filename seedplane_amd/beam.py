@@ -55,6 +55,8 @@ def beam_select(logits, scores, n=None, eos=None, out=None):
         n = beams * (1 + len(ends))
     if not 1 <= beams <= n <= MOST:
         raise ValueError(f'beams must be in [1, n] and n at most {MOST}; got {beams} and {n}')
+    if any(not 0 <= e < 1 << 31 for e in ends):
+        raise ValueError('eos must be tokens')
     if out is None:
         out = BeamStep.allocate(requests, beams, n, dev)
     else:

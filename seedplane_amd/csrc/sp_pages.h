@@ -278,6 +278,8 @@ __global__ void __launch_bounds__(THREADS) k_fork_copy(Pool a) {
 }
 
 // ------------------------------------------------------------------------------------------------ growth, ends
+// A length as the table can hold it: what a program set there never leads outside the table.
+__device__ __forceinline__ int length_of(const Pool &a, int s) { return min(max(a.lengths[s], 0), a.width * a.page); }
 // counts[s] new positions of each sequence: pages for those that have none yet.  One block.
 template <int N>
 __global__ void __launch_bounds__(N) k_grow(Pool a, const int *counts) {
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(N) k_grow(Pool a, const int *counts) {
         const int s = s0 + tid;
         int need = 0, total;
         if (s < a.S) {
-            const int64_t len = a.lengths[s], grown = min(len + max(counts[s], 0), (int64_t)a.width * a.page);
+            const int64_t len = length_of(a, s), grown = min(len + max(counts[s], 0), (int64_t)a.width * a.page);
             need = max(0, (int)((grown + a.page - 1) / a.page - (len + a.page - 1) / a.page));
             a.fresh[s] = (int)grown;
         }
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(N) k_grow(Pool a, const int *counts) {
     __syncthreads();
     const int got = take_free<N>(a.holders, a.n_pages, min(wanted, a.n_pages), a.list, wave_sums);
     for (int s = tid >> 4; s < a.S; s += N / 16) {                  // 16 threads a sequence
-        const int at = a.first[s], n = a.first[s + 1] - at, have = (a.lengths[s] + a.page - 1) / a.page;
+        const int at = a.first[s], n = a.first[s + 1] - at, have = (int)(((int64_t)length_of(a, s) + a.page - 1) / a.page);
         for (int j = tid & 15; j < n; j += 16) {
             const int e = at + j < got ? a.list[at + j] : -1;
             a.table[(int64_t)s * a.width + have + j] = e;
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(N) k_grow(Pool a, const int *counts) {
     __syncthreads();
     int over = 0;
     for (int s = tid; s < a.S; s += N) {
-        over += max(a.lengths[s] + (int64_t)max(counts[s], 0) - a.fresh[s], (int64_t)0) > 0;
+        over += length_of(a, s) + (int64_t)max(counts[s], 0) > a.fresh[s];
         a.lengths[s] = a.fresh[s];
     }
     if (over) atomicAdd(a.missing, over);

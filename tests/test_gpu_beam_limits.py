@@ -1,0 +1,88 @@
+"""Calls at the edges of the page pool and of beam search's selection."""
+import numpy as np
+import pytest
+import torch
+
+from seedplane_amd.beam import beam_select
+from seedplane_amd.pages import PagePool
+from test_gpu_pages import Both, F16, I8, _caches, _int
+
+pytestmark = pytest.mark.gpu
+
+
+def test_lengths_outside_the_table_stay_in_it(gpu_device):
+    """A program may set the tables; a length below 0 counts as 0, one past the table's width as the width."""
+    g = torch.Generator().manual_seed(0)
+    pool = PagePool(_caches(g, 1, 12, 1, 16, 16, F16), 3, 3)
+    guard = pool.table.clone()
+    pool.lengths.copy_(_int([-(1 << 31), 1 << 30, -17]))
+    pool.grow(_int([20, 0, 0]))
+    assert pool.lengths.tolist() == [20, 48, 0]
+    guard[0, :2] = _int([0, 1])
+    assert torch.equal(pool.table, guard) and pool.holders.tolist() == [1, 1] + [0] * 10 and pool.missing.tolist() == [0]
+    pool.lengths[2] = -5
+    pool.fork(_int([2, 0, 1]))
+    assert pool.lengths.tolist() == [0, 20, 48] and pool.table[1].tolist() == [0, 1, -1] and pool.table[0].tolist() == [-1] * 3
+
+
+def test_counts_past_every_width(gpu_device):
+    """The largest counts fill the table's width and are counted."""
+    g = torch.Generator().manual_seed(1)
+    pool = PagePool(_caches(g, 1, 8, 1, 16, 16, I8, 16), 3, 4)
+    pool.grow(_int([2 ** 31 - 1, -2 ** 31, 5]))
+    assert pool.lengths.tolist() == [64, 0, 5] and pool.missing.tolist() == [1]
+    assert pool.table.tolist() == [[0, 1, 2, 3], [-1] * 4, [4, -1, -1, -1]]
+
+
+@pytest.mark.parametrize('page,nkv,hd', [(1, 1, 2), (1, 3, 16), (5, 2, 6), (128, 1, 64)])
+def test_lives_on_other_pages(gpu_device, page, nkv, hd):
+    """Pages of one position (no last page is ever shared), odd ones, large ones."""
+    g = torch.Generator().manual_seed(page)
+    rng = np.random.default_rng(page)
+    both = Both(_caches(g, 2, 40, nkv, page, hd, F16), 5, 9)
+    for _ in range(12):
+        both.do('grow', rng.integers(0, 2 * page + 1, 5).tolist())
+        both.do('fork', rng.integers(-1, 5, 5).tolist())
+        both.do('compact')
+        both.do('free', [int(rng.integers(0, 5))])
+
+
+def test_steps_into_the_scores_that_they_read(gpu_device):
+    """A step's buffers taken for the next one: its scores are read before they are written."""
+    g = torch.Generator().manual_seed(2)
+    x = [(4 * torch.randn((15, 700), generator=g)).to(gpu_device) for _ in range(4)]
+    scores = torch.zeros((3, 5), device=gpu_device)
+    want, step = scores, None
+    for logits in x:
+        apart = beam_select(logits, want, eos=3)
+        want = apart.next_scores
+        step = beam_select(logits, scores if step is None else step.next_scores, eos=3, out=step)
+        for a, b in zip(apart, step):
+            assert torch.equal(a, b)
+
+
+def test_selections_side_by_side(gpu_device):
+    """Two streams at once: each call has a workspace of its own."""
+    g = torch.Generator().manual_seed(3)
+    x = [torch.randn((24, 30000), generator=g).to(gpu_device) for _ in range(2)]
+    scores = torch.zeros((3, 8), device=gpu_device)
+    want = [beam_select(t, scores) for t in x]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(beam_select(x[i], scores))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for step in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(step, want[i]))
+
+
+def test_ends_that_are_no_tokens_are_refused(gpu_device):
+    x, s = torch.zeros((2, 9), device=gpu_device), torch.zeros((1, 2), device=gpu_device)
+    for eos in (-1, 1 << 31, 1 << 40, [3, -2]):
+        with pytest.raises(ValueError):
+            beam_select(x, s, eos=eos)
+    assert beam_select(x, s, eos=(1 << 31) - 1).next_tokens.tolist() == [[0, 1]]
