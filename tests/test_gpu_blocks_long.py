@@ -1,11 +1,12 @@
-"""Appends of many rows to paged caches with a scale per block: workgroups that take several blocks and look their rows up at once, or,
-where too many rows are near, block by block.  Tolerances: tests/blocks_ref.py."""
+"""Long calls over paged caches with a scale per block.  Appends of many rows: workgroups that take several blocks and look their rows up at once, or,
+where too many rows are near, block by block.  Attention: items of more positions than their tables hold.  Tolerances: tests/blocks_ref.py."""
 import pytest
 import torch
 
+from blocks_ref import attend_blocks64
 from paged_ref import rotate64, rotate_bound
-from seedplane_amd.paged import PagedKV, Rotary
-from test_gpu_blocks import BF16, E4M3, F16, F32, I8, _cache, _check_append, _int
+from seedplane_amd.paged import AttentionPlan, PagedKV, Rotary
+from test_gpu_blocks import BF16, E4M3, F16, F32, I8, _cache, _check_append, _int, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +79,24 @@ def test_long_append_order_does_not_matter(gpu_device, n_seq, far):
         got = of([order])
         for a, b in zip((want.k, want.v, want.k_scale, want.v_scale), (got.k, got.v, got.k_scale, got.v_scale)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('cache', [I8, E4M3])
+@pytest.mark.parametrize('q_len,n_seq,hd,dtype', [(4, 600, 128, F16), (8, 600, 128, BF16), (8, 560, 64, F16), (3, 600, 64, BF16), (1, 1100, 128, BF16)])
+def test_items_longer_than_their_table(gpu_device, q_len, n_seq, hd, dtype, cache):
+    """So many sequences that none is cut: each item brings the rows of its positions to LDS several times, of tiles of 32, 64 and
+    128 rows.  All sequences name the same pages, in orders of their own, and a few of them are compared."""
+    print(f'long items {q_len} {n_seq} {hd} {dtype} {cache}', flush=True)
+    g = torch.Generator().manual_seed(q_len + hd)
+    nh, page, n = 16, 64, 4500
+    width = -(-n // page)
+    kv = _cache(g, gpu_device, width, 1, page, hd, cache, 16)
+    table = torch.stack([torch.randperm(width, generator=g) for _ in range(n_seq)]).int()
+    lens = [n - int(i) for i in torch.randint(0, 60, (n_seq,), generator=g)]
+    q = torch.randn((n_seq * q_len, nh, hd), generator=g).to(dtype).to(gpu_device)
+    plan = AttentionPlan(nh, 1, hd, max_rows=n_seq * q_len, max_seqs=n_seq).set([q_len] * n_seq, lens)
+    out = plan.run(q, kv, table.to(gpu_device))
+    for s in (0, n_seq // 2, n_seq - 1):
+        rows = slice(s * q_len, (s + 1) * q_len)
+        want, _, bound = attend_blocks64(q[rows], kv.k, kv.k_scale, kv.v, kv.v_scale, table[s:s + 1], [q_len], [lens[s]], hd ** -0.5)
+        _within(out[rows], want, bound)
