@@ -56,6 +56,7 @@ int sp_op_beam_select(int32_t dtype, const void *logits_dev, int64_t ld, int32_t
         a.B = n_batch; a.K = n_beams; a.V = vocab; a.n = n;
         const int64_t rows = (int64_t)n_batch * n_beams;
         a.splits = splits_of(rows, n_beams, vocab);
+        a.by_splits = paged::Divisor(a.splits); a.by_n = paged::Divisor(n);
         a.len = ((vocab + a.splits - 1) / a.splits + beam::VALUES - 1) / beam::VALUES * beam::VALUES;
         a.best = (beam::Entry *)workspace_dev;
         a.sums = (float2 *)(a.best + rows * a.splits * n);
