@@ -8,10 +8,12 @@
 // The n best of a part: each thread streams its values, keeping their largest beside the sum.  The largest of all threads give a border
 // that at least n values reach and few others (each of 4 waves has ceil(n / 4) threads at or above it: about 2 n values of a part);
 // the few threads that have such values are listed, their values read once more by the whole block, and what reaches the border is put in order.
-// The stream has no barrier, no LDS and nothing but a maximum and an exponential for each value.
+// The stream has no barrier, no LDS and nothing but a maximum and an exponential for each value.  Where more values reach the border than
+// the buffer holds (masks of a type's lowest value, padded vocabularies, ordered rows), borders with a token follow until they fit.
 //
 // What bounds it: few rows, the two launches' chains (4 beams x 151936 in fp32: 6.5 + 4.8 us); many, the stream: 256 rows in bf16, 78 MB, take
-// 23.5 us of which 15.3 are the bytes at a large copy's rate; the blocks all run at once, and what each does behind its stream (border, the
+// 22.4 us of which 15.3 are the bytes at a large copy's rate, 43 to 54 if masked to the lowest value, padded or ordered (by single values
+// past a border, in order, 546 to 666); the blocks all run at once, and what each does behind its stream (border, the
 // few values again, their order) has no other's stream beside it, but more blocks cost more than that (4096 33.9, 8192 42.8 us a call
 // against 29.8 by 2048; 1024 blocks of 512 threads 33.7).  With a buffer in LDS that took every value past a running border, chunk by chunk
 // between barriers, the call took 51 us.
@@ -27,10 +29,9 @@ constexpr int THREADS = 256, WAVES = THREADS / 64, VALUES = 8, CHUNK = THREADS *
 constexpr int MERGE_THREADS = 512, MERGE_WAVES = MERGE_THREADS / 64;
 constexpr int MOST_N = 64, MOST_BEAMS = 64, MOST_EOS = 8, MOST_SPLITS = 64, LEAST_SPLITS = 4;
 constexpr int AHEAD = 2;                   // vectors of a thread in flight
-constexpr int CAPACITY = 1024;             // entries of the buffer
-constexpr int KEPT = CAPACITY - THREADS;   // entries to which one value of every thread can be added
+constexpr int CAPACITY = THREADS;          // entries of the buffer
 constexpr int LISTS = MERGE_THREADS;       // parts of a request's rows at most (splits are chosen so)
-constexpr int MERGED = 1024;               // entries that the merge puts in order at once
+constexpr int MERGED = 512;                // entries that the merge puts in order at once
 
 struct Entry { float v; int i; };          // value, token
 struct Args {
@@ -46,7 +47,15 @@ struct Args {
     paged::Divisor by_splits, by_n;
 };
 
-__device__ __forceinline__ bool better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+// A value and its token as one number that grows with the value, then with lower tokens (v + 0: zeros are equal).
+__device__ __forceinline__ uint64_t key_of(float v, int i) {
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return (uint64_t)(u ^ (uint32_t)((int)u >> 31 | 0x80000000)) << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ Entry entry_of(uint64_t key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return {__uint_as_float(u ^ (u >> 31 ? 0x80000000u : ~0u)), (int)~(uint32_t)key};
+}
 __device__ __forceinline__ bool alive(float score) { return score > -INFINITY; }       // (NaN: no)
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -71,30 +80,40 @@ __device__ __forceinline__ float nth_of_wave(float mine, int n) {
 }
 
 struct RowShared {
-    Entry buf[CAPACITY], top[MOST_N];
+    __align__(16) uint64_t buf[CAPACITY], own[THREADS];
+    uint64_t top[MOST_N];
     int count, threads, who[THREADS];
     float border[WAVES];
     float2 sum[WAVES];
 };
 
-// The exact n best of the buffer's count entries, in order, to its front; the n-th becomes the border.  Every thread calls; ends with a
-// barrier.
-__device__ __forceinline__ int cut(RowShared &sh, int count, int n, float &bv, int &bi) {
-    for (int e = threadIdx.x / 4; e < count; e += THREADS / 4) {       // 4 threads an entry
-        const Entry x = sh.buf[e];
+// The n best of count keys (room for THREADS of them) in order to top.  Every thread calls; begins and ends with a barrier.
+__device__ __forceinline__ void put_in_order(uint64_t *keys, int count, uint64_t *top, int n) {
+    const int tid = threadIdx.x;
+    if (count <= THREADS / 4) {                                        // 4 threads a key
+        __syncthreads();
+        if (tid / 4 < count) {
+            const uint64_t x = keys[tid / 4];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = tid & 3; j < count; j += 4) rank += keys[j] > x;
+            rank += __shfl_xor(rank, 1);
+            rank += __shfl_xor(rank, 2);
+            if ((tid & 3) == 0 && rank < n) top[rank] = x;
+        }
+    } else {
+        if (tid == 0 && count % 2) keys[count] = 0;
+        __syncthreads();
+        const uint64_t x = keys[tid];
         int rank = 0;
-        for (int j = threadIdx.x & 3; j < count; j += 4) rank += better(sh.buf[j].v, sh.buf[j].i, x.v, x.i);
-        rank += __shfl_xor(rank, 1);
-        rank += __shfl_xor(rank, 2);
-        if ((threadIdx.x & 3) == 0 && rank < n) sh.top[rank] = x;
+#pragma unroll 4
+        for (int j = 0; j < count; j += 2) {
+            const ulonglong2 y = *(const ulonglong2 *)(keys + j);
+            rank += (y.x > x) + (y.y > x);
+        }
+        if (tid < count && rank < n) top[rank] = x;
     }
     __syncthreads();
-    const int left = min(count, n);
-    if ((int)threadIdx.x < left) sh.buf[threadIdx.x] = sh.top[threadIdx.x];
-    if (threadIdx.x == 0) sh.count = left;
-    if (count >= n) { bv = sh.top[n - 1].v; bi = sh.top[n - 1].i; }
-    __syncthreads();
-    return left;
 }
 
 // SHORT: rows of fewer values than a vector.
@@ -173,53 +192,71 @@ __global__ void __launch_bounds__(THREADS) k_beam_rows(Args a) {
     } else {
         __syncthreads();
     }
-    // the threads that have such values, and their vectors again, one a thread
-    if (m >= bv && m > -INFINITY) sh.who[atomicAdd(&sh.threads, 1)] = tid;
-    __syncthreads();
-    const int chunks = (hi - lo + CHUNK - 1) / CHUNK, vectors = sh.threads * chunks;
-    for (int e = tid; e < vectors; e += THREADS) {
-        const int k = e / chunks, own = lo + (e - k * chunks) * CHUNK + sh.who[k] * VALUES;
-        if (own >= hi) continue;
+    // (past the buffer's end only that there are more matters)
+    auto full = [&]() { return __hip_atomic_load(&sh.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > CAPACITY; };
+    // a vector's values from the border (its token: the last one of equal values) to the buffer
+    auto collect = [&](const Vector &raw, int own, float border, int token) {
         float v[VALUES];
-        values(fetch(own), own, v);
+        values(raw, own, v);
         uint32_t mine = 0;
 #pragma unroll
-        for (int j = 0; j < VALUES; ++j) mine |= (uint32_t)(v[j] >= bv && v[j] > -INFINITY) << j;
-        if (!mine) continue;
+        for (int j = 0; j < VALUES; ++j)
+            mine |= (uint32_t)(v[j] > -INFINITY && (v[j] > border || (v[j] == border && place(own) + j <= token))) << j;
+        if (!mine || full()) return;
         int to = atomicAdd(&sh.count, __popc(mine));
 #pragma unroll
         for (int j = 0; j < VALUES; ++j)
-            if ((mine >> j & 1) && to < CAPACITY) sh.buf[to++] = {v[j], place(own) + j};
+            if ((mine >> j & 1) && to < CAPACITY) sh.buf[to++] = key_of(v[j], place(own) + j);
+    };
+    // the threads that have such values, and their vectors again, one a thread
+    if (m >= bv && m > -INFINITY) sh.who[atomicAdd(&sh.threads, 1)] = tid;
+    __syncthreads();
+    const int listed = sh.threads, vectors = listed * ((hi - lo + CHUNK - 1) / CHUNK);
+    for (int e = tid; e < vectors && !full(); e += THREADS) {
+        const int c = e / listed, own = lo + c * CHUNK + sh.who[e - c * listed] * VALUES;
+        if (own < hi) collect(fetch(own), own, bv, a.V);
     }
     __syncthreads();
-    int kept = sh.count, bi = -1;
-    if (kept <= CAPACITY) {
-        kept = cut(sh, kept, a.n, bv, bi);
-    } else {
-        // more of one value than the buffer holds: everything anew, a value of each thread at a time, and the lowest tokens stay
-        __syncthreads();
+    // Equal values, or the best side by side, may be more than that.  The n-th best of the threads' best (values, then tokens) leaves those of
+    // n threads at most, few of each; if that is not few enough, or not n threads have a value, the n-th best of those in the buffer leaves
+    // fewer every time.
+    int kept = sh.count;
+    for (bool first = true; kept > CAPACITY; first = false) {
+        uint64_t last = 0;
+        if (first) {
+            int token = -1;
+            for (int c = lo + tid * VALUES; m > -INFINITY && token < 0 && c < hi; c += CHUNK) {
+                float v[VALUES];
+                values(fetch(c), c, v);
+#pragma unroll
+                for (int j = VALUES - 1; j >= 0; --j) token = v[j] == m ? place(c) + j : token;
+            }
+            sh.own[tid] = token < 0 ? 0 : key_of(m, token);
+            if (tid < a.n) sh.top[tid] = 0;
+            put_in_order(sh.own, THREADS, sh.top, a.n);
+            last = sh.top[a.n - 1];
+        }
+        if (last == 0) {
+            __syncthreads();
+            put_in_order(sh.buf, CAPACITY, sh.top, a.n);
+            last = sh.top[a.n - 1];
+        }
+        const Entry border = entry_of(last);
         if (tid == 0) sh.count = 0;
         __syncthreads();
-        bv = -INFINITY;
-        for (int c = lo + tid * VALUES; c - tid * VALUES < hi; c += CHUNK) {
-            float v[VALUES];
-            values(fetch(min(c, hi)), min(c, hi), v);
-#pragma unroll 1
-            for (int j = 0; j < VALUES; ++j) {
-                float mine = v[0];
+        if (m >= border.v)
+            for (int c = lo + tid * VALUES; c < hi && !full(); c += AHEAD * CHUNK) {
+                Vector raw[AHEAD];
 #pragma unroll
-                for (int k = 1; k < VALUES; ++k) mine = j == k ? v[k] : mine;
-                const int token = place(min(c, hi)) + j;
-                if (better(mine, token, bv, bi)) sh.buf[atomicAdd(&sh.count, 1)] = {mine, token};
-                __syncthreads();
-                const int count = sh.count;
-                __syncthreads();
-                if (count > KEPT) cut(sh, count, a.n, bv, bi);
+                for (int u = 0; u < AHEAD; ++u) raw[u] = fetch(c + u * CHUNK);
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) collect(raw[u], c + u * CHUNK, border.v, border.i);
             }
-        }
-        kept = cut(sh, sh.count, a.n, bv, bi);
+        __syncthreads();
+        kept = sh.count;
     }
-    if (tid < a.n) best[tid] = tid < kept ? sh.buf[tid] : Entry{-INFINITY, -1};
+    put_in_order(sh.buf, kept, sh.top, a.n);
+    if (tid < a.n) best[tid] = tid < kept ? entry_of(sh.top[tid]) : Entry{-INFINITY, -1};
     // the part's maximum and sum
     const float wm = wave_max_dpp(m);
     const float ws = wave_sum_dpp(s * __builtin_amdgcn_exp2f((m - (wm == -INFINITY ? 0.f : wm)) * LOG2E));
@@ -237,18 +274,21 @@ __global__ void __launch_bounds__(THREADS) k_beam_rows(Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ merge
-struct Total { double v; int beam, token; };
-__device__ __forceinline__ bool better(const Total &x, const Total &y) {
-    return x.v > y.v || (x.v == y.v && (x.beam < y.beam || (x.beam == y.beam && x.token < y.token)));
-}
-constexpr Total NONE = {-INFINITY, 0x7fffffff, 0x7fffffff};
+struct Total {
+    double v;
+    uint64_t at;                           // beam, token
+    __device__ int beam() const { return (int)(at >> 32); }
+    __device__ int token() const { return (int)(uint32_t)at; }
+};
+__device__ __forceinline__ bool better(const Total &x, const Total &y) { return (x.v > y.v) | ((x.v == y.v) & (x.at < y.at)); }
+constexpr Total NONE = {-INFINITY, ~0ull};
 
 struct MergeShared {
     // a continuation's total is (logit - top) + shift: 64 bits would lose the shift beside a type's lowest values
     double top[MOST_BEAMS], shift[MOST_BEAMS];      // largest logit; score - log of the sum, NaN: a beam without continuations
     float border[MERGE_WAVES];
     int lists, count, good[LISTS];
-    Total out[MOST_N], best[MERGE_WAVES], buf[MERGED];
+    Total out[MOST_N], buf[MERGED];
 };
 
 // One block a request.  The parts' lists are in order, so a list whose first entry is behind the border has nothing to give.  For the border
@@ -295,7 +335,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) k_beam_merge(Args a) {
     auto total_of = [&](const Entry &e, int k) -> Total {
         if (e.i < 0) return NONE;
         const double v = ((double)e.v - sh.top[k]) + sh.shift[k];
-        return v > -INFINITY ? Total{v, k, e.i} : NONE;
+        return v > -INFINITY ? Total{v, (uint64_t)k << 32 | (uint32_t)e.i} : NONE;
     };
     Total mine = list < lists ? total_of(head, beam) : NONE;
     float at_depth = (float)mine.v;
@@ -315,77 +355,68 @@ __global__ void __launch_bounds__(MERGE_THREADS) k_beam_merge(Args a) {
     for (int k = 1; k < MERGE_WAVES; ++k) border = spread ? fminf(border, sh.border[k]) : fmaxf(border, sh.border[k]);
     if ((float)mine.v >= border && mine.v > -INFINITY) sh.good[atomicAdd(&sh.lists, 1)] = list;
     __syncthreads();
+    // totals from the border on; where equal ones are more than the buffer holds, those from the n-th best of the first MERGED / 2 on, again
     const int entries = sh.lists * a.n;
-    for (int e0 = tid; e0 < entries; e0 += MERGE_THREADS * 4) {
-        Entry x[4];
-        int g[4];
+    Total last = NONE;
+    int count;
+    for (bool again = false;; again = true) {
+        for (int e0 = tid; e0 < entries; e0 += MERGE_THREADS * 4) {
+            Entry x[4];
+            int g[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int e = min(e0 + u * MERGE_THREADS, entries - 1), o = e / a.by_n;
-            g[u] = sh.good[o];
-            x[u] = best[(int64_t)g[u] * a.n + (e - o * a.n)];
-        }
+            for (int u = 0; u < 4; ++u) {
+                const int e = min(e0 + u * MERGE_THREADS, entries - 1), o = e / a.by_n;
+                g[u] = sh.good[o];
+                x[u] = best[(int64_t)g[u] * a.n + (e - o * a.n)];
+            }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (e0 + u * MERGE_THREADS >= entries) break;
-            const Total t = total_of(x[u], g[u] / a.by_splits);
-            if ((float)t.v >= border && t.v > -INFINITY) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < MERGED) sh.buf[at] = t;
+            for (int u = 0; u < 4; ++u) {
+                if (e0 + u * MERGE_THREADS >= entries) break;
+                const Total t = total_of(x[u], g[u] / a.by_splits);
+                if (t.v > -INFINITY && (again ? !better(last, t) : (float)t.v >= border)) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < MERGED) sh.buf[at] = t;
+                }
             }
         }
-    }
-    __syncthreads();
-    const int count = sh.count, found = min(count, a.n);
-    if (count <= MERGED) {
-        for (int e = tid / 8; e < count; e += MERGE_THREADS / 8) {     // 8 threads an entry
+        __syncthreads();
+        count = sh.count;
+        const int some = count <= MERGED ? count : MERGED / 2;
+        for (int e = tid / 8; e < some; e += MERGE_THREADS / 8) {      // 8 threads an entry
             const Total t = sh.buf[e];
             int rank = 0;
-            for (int j = tid & 7; j < count; j += 8) rank += better(sh.buf[j], t);
+#pragma unroll 4
+            for (int j = tid & 7; j < some; j += 8) rank += better(sh.buf[j], t);
 #pragma unroll
             for (int o = 1; o < 8; o <<= 1) rank += __shfl_xor(rank, o);
             if ((tid & 7) == 0 && rank < a.n) sh.out[rank] = t;
         }
         __syncthreads();
-    } else {                                                           // equal totals in most lists: one place after the other
-        int at = 0;
-        for (int place = 0; place < a.n; ++place) {
-            Total t = mine;
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                const Total u = {__shfl_xor(t.v, o), __shfl_xor(t.beam, o), __shfl_xor(t.token, o)};
-                if (better(u, t)) t = u;
-            }
-            if (lane == 0) sh.best[wv] = t;
-            __syncthreads();
-            t = sh.best[0];
-            for (int k = 1; k < MERGE_WAVES; ++k)
-                if (better(sh.best[k], t)) t = sh.best[k];
-            if (tid == 0) sh.out[place] = t;
-            if (mine.v > -INFINITY && mine.beam == t.beam && mine.token == t.token)
-                mine = ++at < a.n ? total_of(best[(int64_t)list * a.n + at], beam) : NONE;
-            __syncthreads();
-        }
+        if (count <= MERGED) break;
+        last = sh.out[a.n - 1];
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
     }
+    const int found = min(count, a.n);
     if (wv != 0) return;
     // one wave: place i of the n best, and those among them that go on
     const bool have = lane < found;
-    const Total t = have ? sh.out[lane] : Total{-INFINITY, -1, -1};
+    const Total t = have ? sh.out[lane] : NONE;
     if (lane < a.n) {
         const int64_t o = (int64_t)b * a.n + lane;
         a.out_score[o] = (float)t.v;
-        a.out_beam[o] = t.beam;
-        a.out_token[o] = t.token;
+        a.out_beam[o] = t.beam();
+        a.out_token[o] = t.token();
     }
     bool on = have;
-    for (int k = 0; k < a.n_eos; ++k) on &= t.token != a.eos[k];
+    for (int k = 0; k < a.n_eos; ++k) on &= t.token() != a.eos[k];
     const uint64_t going = __ballot(on);
     const int at = __popcll(going & (((uint64_t)1 << lane) - 1)), n = min(__popcll(going), a.K);
     if (on && at < a.K) {
         const int64_t o = row0 + at;
         a.next_score[o] = (float)t.v;
-        a.next_row[o] = (int)(row0 + t.beam);
-        a.next_token[o] = t.token;
+        a.next_row[o] = (int)(row0 + t.beam());
+        a.next_token[o] = t.token();
     }
     if (lane >= n && lane < a.K) {
         const int64_t o = row0 + lane;

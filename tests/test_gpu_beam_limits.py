@@ -5,6 +5,7 @@ import torch
 
 from seedplane_amd.beam import beam_select
 from seedplane_amd.pages import PagePool
+from test_gpu_beam import _check
 from test_gpu_pages import Both, F16, I8, _caches, _int
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +87,38 @@ def test_ends_that_are_no_tokens_are_refused(gpu_device):
         with pytest.raises(ValueError):
             beam_select(x, s, eos=eos)
     assert beam_select(x, s, eos=(1 << 31) - 1).next_tokens.tolist() == [[0, 1]]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('B,K,n,V', [(1, 4, 8, 40000), (2, 3, 64, 33001), (5, 8, 16, 9000), (1, 1, 1, 20000), (1, 16, 33, 5000)])
+@pytest.mark.parametrize('kind', ['equal', 'lowest', 'padded', 'falling', 'rising', 'one thread', 'few values', 'zeros', 'one beam', 'few'])
+def test_where_the_best_lie(gpu_device, kind, B, K, n, V, dtype):
+    """Rows in which more values than the buffers hold are as good as the n-th best, or the best lie side by side, at strides, at the end,
+    in one beam."""
+    print(f'selection {kind} {B} {K} {n} {V} {dtype}', flush=True)
+    g = torch.Generator().manual_seed(V + n)
+    x = torch.randn((B * K, V), generator=g)
+    at = torch.arange(V)
+    low = torch.finfo(dtype).min
+    scores = -torch.arange(K, dtype=torch.float32).repeat(B, 1) * 0.37
+    if kind == 'equal':
+        x.fill_(1.5)
+    elif kind == 'lowest':                                     # a mask of the type's lowest value, a few tokens allowed
+        x = torch.where(torch.rand((B * K, V), generator=g) < 30 / V, x, low)
+    elif kind == 'padded':
+        x[:, V // 3:] = -10000.0
+    elif kind == 'falling':
+        x = x.sort(1, descending=True).values
+    elif kind == 'rising':
+        x = x.sort(1).values
+    elif kind == 'one thread':                                 # 8 of every 2048 values
+        x = x + 10.0 * (at % 2048 < 8)
+    elif kind == 'few values':
+        x = torch.randint(0, 3, (B * K, V), generator=g).float()
+    elif kind == 'zeros':                                      # of both signs: equal
+        x = torch.where(torch.rand((B * K, V), generator=g) < 0.5, -0.0, 0.0)
+    elif kind == 'one beam':
+        scores = scores * 100
+    else:
+        x = torch.where(torch.rand((B * K, V), generator=g) < n / 2 / V, x, -torch.inf)
+    _check(x.to(dtype).to(gpu_device), scores.to(gpu_device), n=n)
