@@ -29,7 +29,7 @@ struct Pool {                              // see sp_page_pool
     int *table, *lengths, *holders, *missing;
     int64_t page_bytes, head_bytes, row_bytes;                         // strides
     int n_pools, n_pages, page, nkv, width_bytes, block, per_page, S, width;      // width_bytes: of a row's values
-    bool aligned;                                                      // every row to 16 bytes
+    int unit;                                                          // 16, 4 or 1: every row begins and ends on whole units of as many bytes
     // workspace
     int *counts;                           // moves; held pages
     int *fresh, *first;                    // [S] new lengths; [S + 1] places of each sequence's pages among those wanted
@@ -229,29 +229,26 @@ __device__ __forceinline__ void copy_page(const Pool &a, int pool, const Move &m
         const uint32_t h = r / m.rows;
         return h * a.head_bytes + (r - h * m.rows) * a.row_bytes;
     };
-    if (a.aligned) {
-        const uint32_t per = run / 16, total = per * runs;
+    auto copy = [&](auto unit) {
+        typedef decltype(unit) Unit;
+        const uint32_t per = run / sizeof(Unit), total = per * runs;
         for (uint32_t i0 = threadIdx.x; i0 < total; i0 += THREADS * 4) {
-            u32x4 v[4];
+            Unit v[4];
             int64_t at[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t i = min(i0 + k * THREADS, total - 1), r = i / per;
-                at[k] = place(r) + (i - r * per) * 16;
-                v[k] = *(const u32x4 *)(from + at[k]);
+                at[k] = place(r) + (i - r * per) * (uint32_t)sizeof(Unit);
+                v[k] = *(const Unit *)(from + at[k]);
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (i0 + k * THREADS < total) *(u32x4 *)(to + at[k]) = v[k];
+                if (i0 + k * THREADS < total) *(Unit *)(to + at[k]) = v[k];
         }
-    } else {
-        const uint32_t total = run * runs;
-        for (uint32_t i = threadIdx.x; i < total; i += THREADS) {
-            const uint32_t r = i / run;
-            const int64_t at = place(r) + (i - r * run);
-            to[at] = from[at];
-        }
-    }
+    };
+    if (a.unit == 16) copy(u32x4{});
+    else if (a.unit == 4) copy(uint32_t{});
+    else copy(uint8_t{});
     if (a.scales) {
         float *const s = (float *)a.scales[pool];
         const int blocks = (m.rows + a.block - 1) / a.block;

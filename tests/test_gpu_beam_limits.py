@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from seedplane_amd.beam import beam_select
+from seedplane_amd.paged import PagedKV
 from seedplane_amd.pages import PagePool
 from test_gpu_beam import _check
 from test_gpu_pages import Both, F16, I8, _caches, _int
@@ -46,6 +47,23 @@ def test_lives_on_other_pages(gpu_device, page, nkv, hd):
         both.do('fork', rng.integers(-1, 5, 5).tolist())
         both.do('compact')
         both.do('free', [int(rng.integers(0, 5))])
+
+
+@pytest.mark.parametrize('hd,dtype,first', [(6, I8, 0), (36, I8, 0), (40, I8, 0), (7, F16, 0), (32, F16, 1), (32, I8, 4)])
+def test_copies_of_rows_of_any_width(gpu_device, hd, dtype, first):
+    """Rows of bytes, of 4 bytes, and pools that begin `first` values behind an aligned address."""
+    g = torch.Generator().manual_seed(hd)
+    caches = []
+    for _ in range(2):
+        base = [torch.randint(0, 100, (first + 20 * 2 * 16 * hd,), generator=g, dtype=torch.int8).to(gpu_device).to(dtype) for _ in range(2)]
+        pools = [b[first:].view(20, 2, 16, hd) for b in base]
+        scales = [torch.rand((20, 2, 1), generator=g).to(gpu_device) for _ in range(2)] if dtype == I8 else [None, None]
+        caches.append(PagedKV(*pools, *scales))
+    both = Both(caches, 4, 5)
+    both.do('grow', [21, 3, 0, 33])
+    both.do('fork', [0, 0, 3, 0])
+    both.do('free', [1])
+    both.do('compact')
 
 
 def test_steps_into_the_scores_that_they_read(gpu_device):
