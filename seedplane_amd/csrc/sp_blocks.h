@@ -49,7 +49,7 @@ struct ReadArgs {
     Divisor by_row, by_vecs;
 };
 
-__attribute__((visibility("hidden"))) void launch_block_items(int dtype, int kv_dtype, int HD, bool lone, const BlockArgs &a, int grid, hipStream_t st);
+__attribute__((visibility("hidden"))) void launch_block_items(int dtype, int kv_dtype, int HD, const BlockArgs &a, int grid, hipStream_t st);
 __attribute__((visibility("hidden"))) void launch_block_append(int dtype, bool wide, const BlockAppendArgs &a, int query_blocks, size_t lds, hipStream_t st);
 __attribute__((visibility("hidden"))) void launch_read(int dtype, bool wide, const ReadArgs &a, hipStream_t st);
 

@@ -9,18 +9,15 @@
 namespace paged {
 namespace {
 
-template <class T, int KV, bool LONE = false>
+template <class T, int KV>
 void items_of(int HD, const BlockArgs &a, int grid, hipStream_t st) {
-    if (HD == 128) hipLaunchKernelGGL((k_paged_attn<T, KV, 128, LONE>), dim3(grid), dim3(256), attn_smem<KV>, st, a);
-    else hipLaunchKernelGGL((k_paged_attn<T, KV, 64, LONE>), dim3(grid), dim3(256), attn_smem<KV>, st, a);
+    if (HD == 128) hipLaunchKernelGGL((k_paged_attn<T, KV, 128>), dim3(grid), dim3(256), attn_smem<KV>, st, a);
+    else hipLaunchKernelGGL((k_paged_attn<T, KV, 64>), dim3(grid), dim3(256), attn_smem<KV>, st, a);
 }
-// lone: every item is a row tile of its own.  The int8 kernel for all kinds has values in scratch memory because of the larger ones' loops:
-// 8 sequences of 20000 to 40000 positions take 58.5 us without those, 65 with them.  (e4m3's has none: 57.)
 template <class T>
-void typed_items(bool i8, int HD, bool lone, const BlockArgs &a, int grid, hipStream_t st) {
-    if (!i8) items_of<T, KV_E4M3_BLOCKS>(HD, a, grid, st);
-    else if (lone) items_of<T, KV_I8_BLOCKS, true>(HD, a, grid, st);
-    else items_of<T, KV_I8_BLOCKS>(HD, a, grid, st);
+void typed_items(bool i8, int HD, const BlockArgs &a, int grid, hipStream_t st) {
+    if (i8) items_of<T, KV_I8_BLOCKS>(HD, a, grid, st);
+    else items_of<T, KV_E4M3_BLOCKS>(HD, a, grid, st);
 }
 template <class T, int VEC, bool I8>
 void append_codes(const BlockAppendArgs &a, int grid, size_t lds, hipStream_t st) {
@@ -41,10 +38,10 @@ void read_of(bool wide, const ReadArgs &a, hipStream_t st) {
 
 }  // namespace
 
-void launch_block_items(int dtype, int kv_dtype, int HD, bool lone, const BlockArgs &a, int grid, hipStream_t st) {
+void launch_block_items(int dtype, int kv_dtype, int HD, const BlockArgs &a, int grid, hipStream_t st) {
     const bool i8 = kv_dtype == SP_DT_I8;
-    if (dtype == SP_DT_F16) typed_items<f16>(i8, HD, lone, a, grid, st);
-    else typed_items<bf16>(i8, HD, lone, a, grid, st);
+    if (dtype == SP_DT_F16) typed_items<f16>(i8, HD, a, grid, st);
+    else typed_items<bf16>(i8, HD, a, grid, st);
     HIPCHK(hipGetLastError());
 }
 

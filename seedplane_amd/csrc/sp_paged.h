@@ -26,10 +26,10 @@
 //
 // Caches with a scale per block of positions and head (sp_blocks.h) run the same items: the scales of the table's positions come to LDS by
 // copies of 4 bytes in front of the tiles', each wave makes its own positions' terms of them behind the first scores, and a block's largest
-// score is scaled instead of every score.  64 sequences x 4096 positions, 28 / 4 heads of 128: int8 53.5 us, e4m3 52.4 (268 MB and 8 of
-// scales, 5.0 and 5.1 TB/s).  int8 takes five (fp16) or six (bf16) instructions for four codes where e4m3 takes two: a wave that shares a
+// score is scaled instead of every score.  64 sequences x 4096 positions, 28 / 4 heads of 128: int8 52.7 us, e4m3 51.2 (268 MB and 8 of
+// scales, 5.2 and 5.4 TB/s).  int8 takes five (fp16) or six (bf16) instructions for four codes where e4m3 takes two: a wave that shares a
 // tile's rows with others brings its part of the tile to 16 bits for all of them, codes going through registers a tile ahead and
-// being written behind products (6 prompts of 12 / 2 heads of 128 72 us, each wave for itself 80, a barrier more instead of the registers 77;
+// being written behind products (6 prompts of 12 / 2 heads of 128 70 us; before other steps 73, each wave for itself 80, a barrier more instead of the registers 77;
 // e4m3 each for itself 63, once for all 69; the same positions in 16 bits 55).  Tried for waves of their own: keys' codes left 1152 above their
 // values as operands, scores begun at what that adds: 8 sequences of 20000 to 40000 positions 65.0 -> 64.2 us then, not kept.
 #pragma once
@@ -227,7 +227,10 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     constexpr int RPC = 64 / NCH;                                      // rows of one copy
     constexpr bool OP8 = KV8 && !WIDE;                                 // what the products' operands are read from: codes,
     constexpr int ORB = WIDE ? HD * 2 : RB, ONCH = ORB / 16;           // bytes and pieces of a row
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // (blocks: what is computed from it stays inside the item, else the values that all kinds share are kept over the loop of items and int8's
+    // larger tiles, with codes in registers, go to scratch memory: a captured step of 64 x 4096 56.3 us instead of 51.6)
+    const int tid0 = BLOCKS ? opaque(threadIdx.x) : threadIdx.x;
+    const int lane = tid0 & 63, wv = __builtin_amdgcn_readfirstlane(tid0 >> 6);
     const int col = lane & 31, h = lane >> 5;                          // the lane's query row; its half of every 8 keys
     const int rw = wv % WM, kw = wv / WM;
     unsigned char *const buf0 = smem + kw * (TL::STAGES * 2 * TL::TILE);       // [stage][keys, values] of this key wave
@@ -776,8 +779,7 @@ __device__ __forceinline__ void run_item(const ArgsOf<KV> &a, const Item &w, uns
     }
 }
 
-// LONE: every item is of kind 0.
-template <class T, int KV, int HD, bool LONE = false>
+template <class T, int KV, int HD>
 __global__ void __launch_bounds__(256, 2) k_paged_attn(ArgsOf<KV> a) {
     extern __shared__ __align__(1024) unsigned char smem[];            // attn_smem<KV>
     __shared__ __align__(16) AttnShared sh;
@@ -785,7 +787,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(ArgsOf<KV> a) {
     for (int it = blockIdx.x; it < n; it += gridDim.x) {
         const Item w = a.items[it];
         if (it != (int)blockIdx.x) lds_barrier();                      // LDS is free of the item before
-        if (LONE || w.kind == 0) run_item<T, KV, HD, 1>(a, w, smem, sh);
+        if (w.kind == 0) run_item<T, KV, HD, 1>(a, w, smem, sh);
         else if (w.kind == 1) run_item<T, KV, HD, 2>(a, w, smem, sh);
         else run_item<T, KV, HD, 4>(a, w, smem, sh);
     }

@@ -180,7 +180,7 @@ struct sp_attn_plan {
     bool used[2] = {};
     int turn = 0;
     // the last set()
-    bool set = false, joined = false, lone = false;
+    bool set = false, joined = false;
     int n_items = 0, n_tok = 0, n_seq = 0, max_kv = 0, most_parts = 0;
 
     void release() {
@@ -513,7 +513,6 @@ int sp_attn_plan_set(sp_attn_plan *p, int32_t n_seq, const int32_t *q_len, const
         p->n_seq = n_seq;
         p->max_kv = t.max_kv;
         p->joined = t.joined;
-        p->lone = std::all_of(t.items.begin(), t.items.end(), [](const Item &i) { return i.kind == 0; });
         p->set = true;
     });
 }
@@ -606,7 +605,7 @@ int sp_op_paged_attention(const sp_attn_plan *p, const sp_paged_kv *kv, int32_t 
         if (grid && kv->scale_block) {
             a.per_page = kv->page_size / kv->scale_block;
             a.by_block = PageDivisor(kv->scale_block);
-            launch_block_items(dtype, kv->dtype, p->HD, !capturing && p->lone, a, grid, st);
+            launch_block_items(dtype, kv->dtype, p->HD, a, grid, st);
         } else if (grid) {
             if (dtype == SP_DT_F16) launch_typed<f16>(kv8, p->HD, a, grid, st);
             else launch_typed<bf16>(kv8, p->HD, a, grid, st);
