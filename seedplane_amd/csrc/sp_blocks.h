@@ -6,17 +6,19 @@
 // holds, its scale only grows, and where it does the codes that the call does not write are rounded once more, by old / new scale.
 //
 // What bounds it: a step is a chain of dependent accesses (row, table entry beside the search, values, scale, codes): 16 rows of 12 / 2 / 2
-// heads of 128 take 6.1 us, their reading back 3.5, where an empty launch takes 2.3; a prompt of 1777 rows of 28 / 4 / 4 heads, 26 MB of
+// heads of 128 take 6.0 us, their reading back 3.5, where an empty launch takes 2.3; a prompt of 1777 rows of 28 / 4 / 4 heads, 26 MB of
 // values, takes 15 us, most of it the queries' rows, which the plain append's loop rotates (sp_rotate.h says what bounds that); its
 // reading back 4.4 (14 MB).
 //
 // A workgroup takes a chunk of rows of the call (a row whose block an earlier row has is left to that row's workgroup), keys or
-// values, and some heads: it looks up its block's rows among all of the call's, takes the largest magnitude per head, then the codes.
+// values, and some heads: it looks up its block's rows among all of the call's, lists the slots that have one, takes the largest magnitude per
+// head, then the codes (a step of 1024 sequences on blocks of 128: 24 us, by all slots 88; 16384 rows of prompts, whose slots all have one, 2 us
+// more than without the list).
 // Values are read twice unless a thread has but one item of them: a block of 64 positions of one head alone is 8192 values.  Long
 // calls (FIND) look up the rows of all a chunk's blocks at once.  They are bound by the blocks' chains of barriers (16384 rows of 28 / 4 / 4
-// heads 78 us, 41 of them without queries, where the bytes take 56 and 10), so their registers are held to those of 6 waves: with 5
+// heads 80 us, 45 of them without queries, where the bytes take 56 and 10), so their registers are held to those of 6 waves: with 5
 // waves the blocks gain less than the queries' rows behind them lose (83).  Keys and values have loops of their own: one for both
-// had more uniform values than scalar registers hold (16 rows 7.0 us instead of 6.1, 16384 89 instead of 78).
+// had more uniform values than scalar registers hold (16 rows 7.0 us instead of 6.0, 16384 89 instead of 78).
 #pragma once
 #include "sp_paged.h"
 
@@ -33,9 +35,8 @@ struct BlockAppendArgs : AppendArgs {                                  // ks, vs
     int block, per_page;
     PageDivisor by_block, by_page;
     int chunk, chunks, splits, heads;                                  // rows of a workgroup, their number; workgroups over heads, heads of each
-    Divisor by_key, by_value;                                          // vectors of a slot: keys (pairs of them where rotated), values
+    PageDivisor by_key, by_value;                                      // vectors of a slot: keys (pairs of them where rotated), values
     bool find;                                                         // rows of a chunk's blocks are looked up at once
-    PageDivisor by_keys, by_values;                                    // of a block of a head
 };
 struct ReadArgs {
     const void *kc, *vc;
@@ -94,7 +95,8 @@ struct BlockShared {
     int slot[MOST_BLOCK];                                              // the row that brings each position of the block (the last one), -1
     uint32_t most[BLOCK_HEADS];                                        // bits of the largest magnitude
     float scale[BLOCK_HEADS], keep[BLOCK_HEADS];                       // 1 / new scale; old / new (1: codes stay)
-    int earlier;
+    int earlier, moved;                                                // rows before the workgroup's own; whether codes that stay move
+    int here, list[MOST_BLOCK];                                        // slots that have a row
     int found, row[FIND ? MOST_FOUND : 1], seq[FIND ? MOST_FOUND : 1], at[FIND ? MOST_FOUND : 1];       // the call's rows that may be of a block of the chunk (FIND)
 };
 
@@ -130,7 +132,7 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
     __syncthreads();                                                   // the block before has been written
     for (int i = tid; i < a.block; i += ROT_THREADS) sh.slot[i] = -1;
     if (tid < a.heads) sh.most[tid] = 0;
-    if (tid == 0) sh.earlier = 0;
+    if (tid == 0) { sh.earlier = 0; sh.moved = 0; sh.here = 0; }
     __syncthreads();
     auto look = [&](int i, int seq, int at) {
         if (!of_block(a, seq, at, s, b)) return;
@@ -159,19 +161,30 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
     float *const scale = (KEYS ? a.kscale : a.vscale) + ((int64_t)e * a.nkv + head0) * a.per_page + block_of_page;      // of head h: at h * per_page
     const float old = tid < heads ? scale[(int64_t)tid * a.per_page] : 0.f;
     const bool begun = sh.slot[0] >= 0;
-    // item: head h, slot i and vector u of it (keys: a rotated pair of vectors, or one of the rest)
-    const Divisor by = KEYS ? a.by_key : a.by_value;
-    const PageDivisor by_head = KEYS ? a.by_keys : a.by_values;
-    const int per = KEYS ? a.units + a.tail : a.vecs, total = a.block * per, items = heads * total;
+    if (tid < MOST_BLOCK) {                                            // (whole waves)
+        const bool here = tid < a.block && sh.slot[tid] >= 0;
+        const uint64_t who = __ballot(here);
+        int first = 0;
+        if ((tid & 63) == 0) first = atomicAdd(&sh.here, __popcll(who));
+        first = __builtin_amdgcn_readfirstlane(first);
+        if (here) sh.list[first + __popcll(who & (((uint64_t)1 << (tid & 63)) - 1))] = tid;
+    }
+    __syncthreads();
+    // item: head h, slot i that has a row, and vector u of it (keys: a rotated pair of vectors, or one of the rest)
+    const int here = __builtin_amdgcn_readfirstlane(sh.here);          // (at least row r's)
+    Divisor by_here;
+    by_here.d = here;
+    by_here.inverse = 0xffffffffu / here + 1;                          // (rounded up, as the constructor's; not used for 1)
+    const PageDivisor by = KEYS ? a.by_key : a.by_value;
+    const int per = KEYS ? a.units + a.tail : a.vecs, total = here * per, items = heads * total;
     uint8_t *const pool = (uint8_t *)(KEYS ? a.kc : a.vc) + e * a.page_stride + head0 * a.head_stride +
                           (int64_t)(p - page * a.page_size - (p - b * a.block)) * a.row_stride;
     struct Item { int h, i, row, turn, at1, at2; bool two; };
     auto item_of = [&](int k) -> Item {
         Item x;
-        x.h = k / by_head;
-        k -= x.h * total;
-        x.i = k / by;
-        const int u = k - x.i * per;
+        const int q = k / by, u = k - q * per;
+        x.h = q / by_here;
+        x.i = sh.list[q - x.h * here];
         x.row = sh.slot[x.i];
         x.two = KEYS && u < a.units;
         x.turn = x.i * half + u * VEC;
@@ -182,9 +195,8 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
     typedef T Vector __attribute__((ext_vector_type(VEC)));
     Vector raw1, raw2;
     float v1[VEC], v2[VEC];
-    // (a slot without a row reads row r's values and does not use them: loads without a branch)
     auto fetch = [&](const Item &x) {
-        const int64_t row = x.row >= 0 ? x.row : r;
+        const int64_t row = x.row;
         const T *src = KEYS ? (const T *)a.k + row * a.k_row + (int64_t)(head0 + x.h) * a.k_head
                             : (const T *)a.v + row * a.v_row + (int64_t)(head0 + x.h) * a.v_head;
         raw1 = *(const Vector *)(src + x.at1);
@@ -200,21 +212,18 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
             if (x.two) turn_unit<VEC>(a.rot, cs + x.turn, v1, v2);
     };
     if (KEYS && half) {
-        for (int k = tid; k < a.block * half; k += ROT_THREADS) {
-            const int i = k / a.by_half, row = sh.slot[i];
-            if (row >= 0) cs[k] = turn_of(a.rot, a.pos[row], k - i * half);
+        for (int k = tid; k < here * half; k += ROT_THREADS) {
+            const int o = k / a.by_half, j = k - o * half, i = sh.list[o];
+            cs[i * half + j] = turn_of(a.rot, a.pos[sh.slot[i]], j);
         }
         __syncthreads();
     }
     for (int k0 = 0; k0 < items; k0 += ROT_THREADS) {
-        const Item x = item_of(min(k0 + tid, items - 1));
+        const Item x = item_of(min(k0 + tid, items - 1));              // (past the last: the last again, its largest does not change)
         fetch(x);
-        uint32_t most = 0;
-        if (x.row >= 0) {
-            values(x);
-            most = magnitude<I8, VEC>(v1, 0);
-            if constexpr (KEYS) most = magnitude<I8, VEC>(v2, most);
-        }
+        values(x);
+        uint32_t most = magnitude<I8, VEC>(v1, 0);
+        if constexpr (KEYS) most = magnitude<I8, VEC>(v2, most);
         if (total % 64 == 0) {                                         // a wave's items are of one head
             most = wave_umax(most);
             if ((tid & 63) == 0 && most) atomicMax(&sh.most[x.h], most);
@@ -230,30 +239,42 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
         float grown = made < LEAST_SCALE ? LEAST_SCALE : made;
         if (!begun && !(old <= grown)) grown = grown != grown ? grown : old;
         sh.scale[tid] = 1.f / grown;
-        sh.keep[tid] = begun || grown == old ? 1.f : old / grown;
+        const float keep = begun || grown == old ? 1.f : old / grown;
+        sh.keep[tid] = keep;
+        if (keep != 1.f) sh.moved = 1;
         scale[(int64_t)tid * a.per_page] = grown;
     }
     __syncthreads();
-    for (int k = tid; k < items; k += ROT_THREADS) {
-        const Item x = item_of(k);
-        uint8_t *const to = pool + x.h * a.head_stride + x.i * a.row_stride;
-        const float f = x.row >= 0 ? sh.scale[x.h] : sh.keep[x.h];
-        if (x.row >= 0) {
-            if (items > ROT_THREADS) fetch(x);                         // (else its values are still here)
-            if (FIND || items > ROT_THREADS) values(x);                // (FIND: turned again, for the registers)
-        } else {
-            if (f == 1.f) continue;
-            load_codes<I8, VEC>(to + x.at1, v1);
-            if constexpr (KEYS) load_codes<I8, VEC>(to + x.at2, v2);
-        }
+    auto scaled = [&](uint8_t *to, float f, int at1, int at2, bool two) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             v1[i] *= f;
             if constexpr (KEYS) v2[i] *= f;
         }
-        store_codes<I8, VEC>(to + x.at1, v1);
+        store_codes<I8, VEC>(to + at1, v1);
         if constexpr (KEYS)
-            if (x.two) store_codes<I8, VEC>(to + x.at2, v2);
+            if (two) store_codes<I8, VEC>(to + at2, v2);
+    };
+    for (int k = tid; k < items; k += ROT_THREADS) {
+        const Item x = item_of(k);
+        if (items > ROT_THREADS) fetch(x);                             // (else its values are still here)
+        if (FIND || items > ROT_THREADS) values(x);                    // (FIND: turned again, for the registers)
+        scaled(pool + x.h * a.head_stride + x.i * a.row_stride, sh.scale[x.h], x.at1, x.at2, x.two);
+    }
+    // what the call does not write, of heads whose scale has grown (vectors of a whole head, whatever turns)
+    if (sh.moved) {
+        const int vecs = a.vecs, all = heads * a.block * vecs;
+        for (int k = tid; k < all; k += ROT_THREADS) {
+            const int q = k / a.by_value, h = q / a.by_block, i = q - h * a.block;
+            const float f = sh.keep[h];
+            if (sh.slot[i] >= 0 || f == 1.f) continue;
+            uint8_t *const to = pool + h * a.head_stride + i * a.row_stride + (k - q * vecs) * VEC;
+            float v[VEC];
+            load_codes<I8, VEC>(to, v);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] *= f;
+            store_codes<I8, VEC>(to, v);
+        }
     }
 }
 

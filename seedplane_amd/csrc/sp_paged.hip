@@ -138,13 +138,12 @@ void append_blocks(const sp_paged_kv *kv, AppendArgs &a, int dtype, bool wide, h
     b.kscale = kv->k_scale_dev; b.vscale = kv->v_scale_dev;
     b.block = kv->scale_block; b.per_page = kv->page_size / kv->scale_block;
     b.by_block = PageDivisor(b.block); b.by_page = PageDivisor(kv->page_size);
-    b.by_key = Divisor(a.units + a.tail); b.by_value = Divisor(a.vecs);
-    b.by_keys = PageDivisor(b.block * (a.units + a.tail)); b.by_values = PageDivisor(b.block * a.vecs);
+    b.by_key = PageDivisor(a.units + a.tail); b.by_value = PageDivisor(a.vecs);
     // Blocks that the call is likely to write: of many sequences (a step) one each, else its rows side by side.  Where there is one for every
     // other row a workgroup looks at one row, else at several, most of which follow one of the same block; heads are split while the
-    // blocks are too few to fill the chip.  (A step of 1024 sequences, 28 / 4 heads of 128: 17.9 us a call; by 4 rows and single heads twice that.)
+    // blocks are too few to fill the chip.  (A step of 1024 sequences, 28 / 4 heads of 128: 14.8 us a call; by 4 rows and single heads twice that.)
     // More than 4096 rows: the search of all rows for each block comes to count, so that a workgroup takes several blocks with one search
-    // (131072 rows of 16 sequences 570 us, by single searches 1154; 8192 35 and 40; 1777 18 and 14).
+    // (131072 rows of 16 sequences 595 us, by single searches 1154; 8192 38 and 40; 1777 18 and 14).
     const int runs = std::max(1, std::min(a.rows, std::max(a.rows / b.block, a.n_seq)));
     b.find = a.rows > 4096;
     b.chunk = b.find ? std::min(MOST_CHUNK, std::max(b.block, a.rows / 512)) : 2 * (int64_t)runs >= a.rows ? 1 : std::max(1, a.rows / 256);
