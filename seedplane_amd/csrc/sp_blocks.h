@@ -24,6 +24,7 @@
 
 namespace paged {
 
+constexpr int READ_AHEAD = 4;                                          // vectors of a thread in flight, reading back
 constexpr int MOST_BLOCK = 128;                                        // positions of a block at most
 constexpr int BLOCK_HEADS = 64;                                        // heads of a workgroup at most
 constexpr int SEARCHED = 4;                                            // rows that a thread looks at at once
@@ -387,25 +388,36 @@ __global__ void __launch_bounds__(ROT_THREADS) k_paged_read(ReadArgs a) {
         scale_at[k] = sc;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < total; i += blockDim.x) {
-        const int r = i / a.by_row, k = i - r * a.per_row, w = k / a.by_vecs, at = (k - w * a.vecs) * VEC;
-        const bool keys = w < a.nkv;
-        const int h = keys ? w : w - a.nkv;
-        float v[VEC];
-        if (from[r] < 0) {
+    for (int i0 = threadIdx.x; i0 < total; i0 += ROT_THREADS * READ_AHEAD) {
+        float v[READ_AHEAD][VEC], f[READ_AHEAD];
+        int64_t to[READ_AHEAD];
+        bool keys[READ_AHEAD];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = 0.f;
-        } else {
-            load_cached<T, VEC>(keys ? a.kc : a.vc, from[r] + h * a.head_stride + at, a.kv_dt, v);
-            const float *scales = keys ? a.ks : a.vs;
-            if (scales) {
-                const float f = scales[scale_at[r] + (a.block ? (int64_t)h * a.per_page : h)];
+        for (int u = 0; u < READ_AHEAD; ++u) {
+            const int i = i0 + u * ROT_THREADS;
+            if (i >= total) break;
+            const int r = i / a.by_row, k = i - r * a.per_row, w = k / a.by_vecs, at = (k - w * a.vecs) * VEC;
+            keys[u] = w < a.nkv;
+            const int h = keys[u] ? w : w - a.nkv;
+            const int64_t row = row0 + r;
+            to[u] = (keys[u] ? row * a.k_row + h * a.k_head : row * a.v_row + h * a.v_head) + at;
+            f[u] = 1.f;
+            if (from[r] < 0) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] *= f;
+                for (int j = 0; j < VEC; ++j) v[u][j] = 0.f;
+            } else {
+                load_cached<T, VEC>(keys[u] ? a.kc : a.vc, from[r] + h * a.head_stride + at, a.kv_dt, v[u]);
+                const float *scales = keys[u] ? a.ks : a.vs;
+                if (scales) f[u] = scales[scale_at[r] + (a.block ? (int64_t)h * a.per_page : h)];
             }
         }
-        const int64_t row = row0 + r;
-        store_values<VEC>(keys ? a.k_out : a.v_out, (keys ? row * a.k_row + h * a.k_head : row * a.v_row + h * a.v_head) + at, dtype_of<T>(), v);
+#pragma unroll
+        for (int u = 0; u < READ_AHEAD; ++u) {
+            if (i0 + u * ROT_THREADS >= total) break;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[u][j] *= f[u];
+            store_values<VEC>(keys[u] ? a.k_out : a.v_out, to[u], dtype_of<T>(), v[u]);
+        }
     }
 }
 
