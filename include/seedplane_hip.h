@@ -506,7 +506,8 @@ int sp_op_paged_attention(const sp_attn_plan *plan, const sp_paged_kv *kv, int32
 
 /* The pages of the layers' caches and the sequences that hold them, all in device memory that the caller owns: a program may read
  * the tables between calls, and set them to any state that follows the rules.  Pool i (keys or values of a layer) is at pools_dev[i],
- * laid out as a sp_paged_kv's, its blocks' scales at scales_dev[i].  Row s of the table names the pages of sequence s's
+ * laid out as a sp_paged_kv's, its blocks' scales at scales_dev[i].  Pages must not lie on each other (taken from the smallest stride on,
+ * each dimension steps over all that those before it reach): other pools can only copy, the other calls refuse them.  Row s of the table names the pages of sequence s's
  * lengths_dev[s] positions in order, -1 behind them.  holders_dev[e]: how many entries of the table name page e, and 1 more for each
  * time that the caller keeps it; 0: free.  A sequence's last page, where it is not full, has one holder.  missing_dev[0] counts the
  * pages that were wanted and not found (their entries are -1, which hides the positions) and sequences cut at the table's width. */

@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "sp_host.h"
 #include "sp_pages.h"
@@ -26,7 +27,21 @@ bool sizes_ok(int64_t S, int64_t width, int64_t n_pages) {
     return S >= 1 && S <= 65535 && width >= 1 && n_pages >= 1 && S * width < (1 << 30);
 }
 
-pages::Pool pool_args(const sp_page_pool *p) {
+// Whether no two rows of the pool share a byte: taken from the smallest stride on, each dimension steps over all that those before it reach.
+bool rows_apart(const sp_page_pool *p) {
+    std::pair<int64_t, int> dims[] = {{p->page_stride, p->n_pages}, {p->head_stride, p->n_kv_heads}, {p->row_stride, p->page_size}};
+    std::sort(std::begin(dims), std::end(dims));
+    __int128 reach = p->head_dim;
+    for (const auto &[stride, n] : dims) {
+        if (n == 1) continue;
+        if (stride < reach) return false;
+        reach += (__int128)stride * (n - 1);
+    }
+    return true;
+}
+
+// gives: the call gives pages to sequences or takes them back, by their numbers alone.
+pages::Pool pool_args(const sp_page_pool *p, bool gives = true) {
     require(p != nullptr, SP_EINVAL, "pool is NULL");
     require(sizes_ok(p->max_seqs, p->max_pages, p->n_pages), SP_EINVAL,
             "max_seqs must be in [1, 65535], max_pages and n_pages positive and max_seqs * max_pages below 2^30");
@@ -39,6 +54,7 @@ pages::Pool pool_args(const sp_page_pool *p) {
     require((p->n_pages == 1 || p->page_stride >= p->head_dim) && (p->n_kv_heads == 1 || p->head_stride >= p->head_dim) &&
                 (p->page_size == 1 || p->row_stride >= p->head_dim) && p->page_stride >= 0 && p->head_stride >= 0 && p->row_stride >= 0,
             SP_EINVAL, "the pool's strides are smaller than a row");
+    require(!gives || rows_apart(p), SP_EINVAL, "the pool's pages lie on each other: it can only copy");
     require(p->pools_dev && p->table_dev && p->lengths_dev && p->holders_dev && p->missing_dev && p->workspace_dev, SP_EINVAL, "NULL pointer");
     require(((uintptr_t)p->workspace_dev & 15) == 0, SP_EINVAL, "the workspace must be aligned to 16 bytes");
     require((p->scale_block > 0) == (p->scales_dev != nullptr) && p->scale_block >= 0 &&
@@ -131,7 +147,7 @@ int sp_op_pages_compact(const sp_page_pool *pool, int32_t *places_dev, void *str
 
 int sp_op_pages_copy(const sp_page_pool *pool, int32_t n_copies, const int32_t *src_dev, const int32_t *dst_dev, void *stream) {
     return guarded([&] {
-        const pages::Pool a = pool_args(pool);
+        const pages::Pool a = pool_args(pool, false);
         require(n_copies >= 0, SP_EINVAL, "n_copies must not be negative");
         if (n_copies == 0) return;
         require(src_dev && dst_dev, SP_EINVAL, "NULL pointer");

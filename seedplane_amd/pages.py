@@ -22,7 +22,8 @@ from .paged import _DTYPES, _call, _ints
 
 class PagePool:
     """The pages of `caches` (a PagedKV, or a list of them: the layers, alike in all but their memory) and `max_seqs` sequences of up to
-    `max_pages` pages.
+    `max_pages` pages.  Where pages lie on each other, and over an engine's rings (Qwen2Engine.paged_kv), whose pages belong to its own
+    caches, there are none to give: such a pool only copies, other calls raise ValueError.
 
     Tensors, which a program may read between calls: table int32 [max_seqs, max_pages] (-1 behind a sequence's pages), lengths int32
     [max_seqs], holders int32 [n_pages] (how many table entries name a page; add 1 to keep one that no sequence holds), missing int32
@@ -63,22 +64,27 @@ class PagePool:
         _call(fn, self.device, self._ref, *args)
         return self
 
+    def _give(self, fn, *args):
+        if self._leases:
+            raise ValueError("the pages are of an engine's rings: a pool over them can only copy")
+        return self._run(fn, *args)
+
     def fork(self, parents):
         """Sequence s continues parents[s] (int32 [max_seqs]: any sequence, itself included; -1: s ends)."""
-        return self._run(self.lib.sp_op_pages_fork, _ints(parents, 'parents', self.device, self.max_seqs))
+        return self._give(self.lib.sp_op_pages_fork, _ints(parents, 'parents', self.device, self.max_seqs))
 
     def grow(self, counts):
         """counts[s] more positions for each sequence (int32 [max_seqs]), with pages for them; they are the caller's to write."""
-        return self._run(self.lib.sp_op_pages_grow, _ints(counts, 'counts', self.device, self.max_seqs))
+        return self._give(self.lib.sp_op_pages_grow, _ints(counts, 'counts', self.device, self.max_seqs))
 
     def free(self, seqs):
         """Sequences seqs (int32 [n]) end; their pages are free unless others hold them."""
         n = seqs.numel()
-        return self._run(self.lib.sp_op_pages_free, n, _ints(seqs, 'seqs', self.device, n))
+        return self._give(self.lib.sp_op_pages_free, n, _ints(seqs, 'seqs', self.device, n))
 
     def compact(self, places=None):
         """Held pages move to the lowest places.  places: int32 [n_pages], filled with each page's place afterwards."""
-        return self._run(self.lib.sp_op_pages_compact, None if places is None else _ints(places, 'places', self.device, self.holders.numel()))
+        return self._give(self.lib.sp_op_pages_compact, None if places is None else _ints(places, 'places', self.device, self.holders.numel()))
 
     def copy(self, src, dst):
         """Pages src[i] to dst[i] (int32 [n]) in every cache, with their scales; pairs outside the pool are left out.  A page is not a
