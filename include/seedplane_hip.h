@@ -430,7 +430,7 @@ typedef struct sp_paged_kv {
  * stays NaN.  Two rows of one call must not name the same place (nor two positions share a page that the call writes): whose
  * values it then holds is not defined.
  * With scale_block a block's scale becomes the largest magnitude of a head's new values in it over the largest code (127 or 448), at
- * least the scale that it has; where it grows, the codes that the call does not write are rounded once more, by old / new scale.  A
+ * least the scale that it has, and a code is the fp32 quotient of value and scale, rounded (halves to even); where the scale grows, the codes that the call does not write are rounded once more, by old / new scale.  A
  * block whose first position is among the rows begins anew: its scale is that of the new values alone, and what it held at other
  * positions is lost.  The rows of a block may stand anywhere in the call; of two rows for the same place the later one
  * alone counts.

@@ -95,7 +95,7 @@ template <bool FIND>
 struct BlockShared {
     int slot[MOST_BLOCK];                                              // the row that brings each position of the block (the last one), -1
     uint32_t most[BLOCK_HEADS];                                        // bits of the largest magnitude
-    float scale[BLOCK_HEADS], keep[BLOCK_HEADS];                       // 1 / new scale; old / new (1: codes stay)
+    float scale[BLOCK_HEADS], inverse[BLOCK_HEADS], keep[BLOCK_HEADS]; // new scale, 1 / scale; old / new (1: codes stay)
     int earlier, moved;                                                // rows before the workgroup's own; whether codes that stay move
     int here, list[MOST_BLOCK];                                        // slots that have a row
     int found, row[FIND ? MOST_FOUND : 1], seq[FIND ? MOST_FOUND : 1], at[FIND ? MOST_FOUND : 1];       // the call's rows that may be of a block of the chunk (FIND)
@@ -235,22 +235,31 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
     __syncthreads();
     if (tid < heads) {
         const float most = __uint_as_float(sh.most[tid]);
-        const float made = most > MOST_SCALE * (I8 ? 127.f : 448.f) ? MOST_SCALE : most * (I8 ? 1.f / 127.f : 1.f / 448.f);
+        const float made = most > MOST_SCALE * (I8 ? 127.f : 448.f) ? MOST_SCALE : most / (I8 ? 127.f : 448.f);
         // (comparisons that leave a NaN where it is: of int8's new values, or held since the block began)
         float grown = made < LEAST_SCALE ? LEAST_SCALE : made;
         if (!begun && !(old <= grown)) grown = grown != grown ? grown : old;
-        sh.scale[tid] = 1.f / grown;
+        sh.scale[tid] = grown;
+        sh.inverse[tid] = 1.f / grown;
         const float keep = begun || grown == old ? 1.f : old / grown;
         sh.keep[tid] = keep;
         if (keep != 1.f) sh.moved = 1;
         scale[(int64_t)tid * a.per_page] = grown;
     }
     __syncthreads();
-    auto scaled = [&](uint8_t *to, float f, int at1, int at2, bool two) {
+    // Quotients by the scale: the product with its reciprocal alone, rounded twice, puts values half way between two codes to either side; what is
+    // left of the value behind it (one fused step, exact), taken in once more, gives the rounded quotient.  (Bounded in between, so that infinities
+    // leave infinity, not NaN.  It costs 16384 rows 1.7 us of 79, a division of the compiler's 2.8.)
+    auto scaled = [&](uint8_t *to, int h, int at1, int at2, bool two) {
+        const float s = sh.scale[h], inverse = sh.inverse[h];
+        auto quotient = [&](float v) {
+            const float q = fminf(fmaxf(v * inverse, -512.f), 512.f);
+            return __builtin_fmaf(__builtin_fmaf(-q, s, v), inverse, q);
+        };
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            v1[i] *= f;
-            if constexpr (KEYS) v2[i] *= f;
+            v1[i] = quotient(v1[i]);
+            if constexpr (KEYS) v2[i] = quotient(v2[i]);
         }
         store_codes<I8, VEC>(to + at1, v1);
         if constexpr (KEYS)
@@ -260,7 +269,7 @@ __device__ __forceinline__ void append_block(const BlockAppendArgs &a, int r, in
         const Item x = item_of(k);
         if (items > ROT_THREADS) fetch(x);                             // (else its values are still here)
         if (FIND || items > ROT_THREADS) values(x);                    // (FIND: turned again, for the registers)
-        scaled(pool + x.h * a.head_stride + x.i * a.row_stride, sh.scale[x.h], x.at1, x.at2, x.two);
+        scaled(pool + x.h * a.head_stride + x.i * a.row_stride, x.h, x.at1, x.at2, x.two);
     }
     // what the call does not write, of heads whose scale has grown (vectors of a whole head, whatever turns)
     if (sh.moved) {
