@@ -528,7 +528,8 @@ size_t sp_pages_workspace(int32_t max_seqs, int32_t max_pages, int32_t n_pages);
  * of its own with its rows, in every pool (the lowest free pages, in the order of sequences).  Pages that nobody holds any more are free. */
 int sp_op_pages_fork(const sp_page_pool *pool, const int32_t *parents_dev, void *hip_stream);
 /* counts_dev[s] more positions for each sequence (int32 [max_seqs]; 0 or less: none), with pages for them: the lowest free ones, in the
- * order of sequences and positions. */
+ * order of sequences and positions.  Where a program has lowered a sequence's length (positions that it takes back, drafts for instance), the
+ * pages that its row names behind are given back here as the growth comes to them, and by a fork or an end of the sequence. */
 int sp_op_pages_grow(const sp_page_pool *pool, const int32_t *counts_dev, void *hip_stream);
 /* Sequences seqs_dev[0 .. n_seqs) end; entries that are no sequence, or are there twice, do nothing. */
 int sp_op_pages_free(const sp_page_pool *pool, int32_t n_seqs, const int32_t *seqs_dev, void *hip_stream);

@@ -31,7 +31,7 @@ struct Pool {                              // see sp_page_pool
     int n_pools, n_pages, page, nkv, width_bytes, block, per_page, S, width;      // width_bytes: of a row's values
     int unit;                                                          // 16, 4 or 1: every row begins and ends on whole units of as many bytes
     // workspace
-    int *counts;                           // moves; held pages
+    int *counts;                           // moves; held pages; whether rows may have gaps (pages that were not found)
     int *fresh, *first;                    // [S] new lengths; [S + 1] places of each sequence's pages among those wanted
     int *rows;                             // [S][width] new table
     int *list;                             // [n_pages] free pages taken
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(N) k_fork(Pool a, const int *parents) {
     }
     if (tid == 0) {
         a.counts[0] = got;
-        if (wanted > got) *a.missing += wanted - got;
+        if (wanted > got) { *a.missing += wanted - got; a.counts[2] = 1; }
     }
 }
 
@@ -277,35 +277,51 @@ __global__ void __launch_bounds__(THREADS) k_fork_copy(Pool a) {
 // ------------------------------------------------------------------------------------------------ growth, ends
 // A length as the table can hold it: what a program set there never leads outside the table.
 __device__ __forceinline__ int length_of(const Pool &a, int s) { return min(max(a.lengths[s], 0), a.width * a.page); }
+__device__ __forceinline__ int pages_of(const Pool &a, int len) { return (int)(((uint32_t)len + a.page - 1) / (uint32_t)a.page); }
 // counts[s] new positions of each sequence: pages for those that have none yet.  One block.
 template <int N>
 __global__ void __launch_bounds__(N) k_grow(Pool a, const int *counts) {
-    __shared__ int wave_sums[N / 64];
-    const int tid = threadIdx.x;
+    __shared__ int wave_sums[N / 64], behind;
+    const int tid = threadIdx.x, gaps = a.counts[2];
+    if (tid == 0) behind = 0;
     int wanted = 0;
     for (int s0 = 0; s0 < a.S; s0 += N) {
         const int s = s0 + tid;
-        int need = 0, total;
+        int need = 0, now = -1, total;
         if (s < a.S) {
-            const int64_t len = length_of(a, s), grown = min(len + max(counts[s], 0), (int64_t)a.width * a.page);
-            need = max(0, (int)((grown + a.page - 1) / a.page - (len + a.page - 1) / a.page));
-            a.fresh[s] = (int)grown;
+            const int len = length_of(a, s), grown = len + min(max(counts[s], 0), a.width * a.page - len), have = pages_of(a, len);
+            need = pages_of(a, grown) - have;
+            a.fresh[s] = grown;
+            if (need) now = a.table[(int64_t)s * a.width + have];
         }
         const int at = wanted + block_rank<N>(need, wave_sums, total);
         if (s < a.S) a.first[s] = at;
+        if (now >= 0) behind = 1;
         wanted += total;
     }
     if (tid == 0) a.first[a.S] = wanted;
     __syncthreads();
-    const int got = take_free<N>(a.holders, a.n_pages, min(wanted, a.n_pages), a.list, wave_sums);
-    for (int s = tid >> 4; s < a.S; s += N / 16) {                  // 16 threads a sequence
-        const int at = a.first[s], n = a.first[s + 1] - at, have = (int)(((int64_t)length_of(a, s) + a.page - 1) / a.page);
-        for (int j = tid & 15; j < n; j += 16) {
-            const int e = at + j < got ? a.list[at + j] : -1;
-            a.table[(int64_t)s * a.width + have + j] = e;
-            if (e >= 0) a.holders[e] = 1;
+    auto each_new = [&](auto &&fn) {                                // fn(the place among those wanted, its entry); 16 threads a sequence
+        for (int s = tid >> 4; s < a.S; s += N / 16) {
+            const int at = a.first[s], n = a.first[s + 1] - at, have = pages_of(a, length_of(a, s));
+            for (int j = tid & 15; j < n; j += 16) fn(at + j, (int64_t)s * a.width + have + j);
         }
+    };
+    // Pages that the entries still name, where a program has lowered a sequence's length, are given back first.  (A row without gaps names one in
+    // the first of them if in any.)
+    if (behind || gaps) {
+        each_new([&](int, int64_t entry) {
+            const int e = a.table[entry];
+            if (e >= 0 && e < a.n_pages) atomicSub(&a.holders[e], 1);
+        });
+        __syncthreads();
     }
+    const int got = take_free<N>(a.holders, a.n_pages, min(wanted, a.n_pages), a.list, wave_sums);
+    each_new([&](int k, int64_t entry) {
+        const int e = k < got ? a.list[k] : -1;
+        a.table[entry] = e;
+        if (e >= 0) a.holders[e] = 1;
+    });
     __syncthreads();
     int over = 0;
     for (int s = tid; s < a.S; s += N) {
@@ -313,7 +329,7 @@ __global__ void __launch_bounds__(N) k_grow(Pool a, const int *counts) {
         a.lengths[s] = a.fresh[s];
     }
     if (over) atomicAdd(a.missing, over);
-    if (tid == 0 && wanted > got) atomicAdd(a.missing, wanted - got);
+    if (tid == 0 && wanted > got) { atomicAdd(a.missing, wanted - got); a.counts[2] = 1; }
 }
 // Sequences that end: a block each.  (The same one twice gives its pages back once.)
 __global__ void __launch_bounds__(THREADS) k_free(Pool a, const int *seqs) {

@@ -74,7 +74,9 @@ class PagePool:
         return self._give(self.lib.sp_op_pages_fork, _ints(parents, 'parents', self.device, self.max_seqs))
 
     def grow(self, counts):
-        """counts[s] more positions for each sequence (int32 [max_seqs]), with pages for them; they are the caller's to write."""
+        """counts[s] more positions for each sequence (int32 [max_seqs]), with pages for them; they are the caller's to write.  To take
+        positions back (rejected drafts) lower `lengths`, not into pages that other sequences hold too; the pages behind go with the next
+        growth over them, fork or end."""
         return self._give(self.lib.sp_op_pages_grow, _ints(counts, 'counts', self.device, self.max_seqs))
 
     def free(self, seqs):
