@@ -10,14 +10,15 @@
 
 A fork shares full pages and copies the rows of a last page that is not full, in every layer, so no sequence ever writes what another
 reads.  Every call runs on torch's current stream of the caches' device without waiting for it, allocates nothing and may be captured
-into a graph; calls on one pool follow each other.  The reference has one tensor per sequence (seedplane/qwen_engine.py:18-29).
+into a graph; calls on one pool follow each other (a stream other than the one it was made on waits for that first).  The reference has
+one tensor per sequence (seedplane/qwen_engine.py:18-29).
 """
 import ctypes
 
 import torch
 
 from . import _lib
-from .paged import _DTYPES, _call, _ints
+from .paged import _DTYPES, _call, _ints, _raw_stream
 
 
 class PagePool:
@@ -57,11 +58,19 @@ class PagePool:
                                       *kv._strides(), len(pools), _DTYPES[kv.dtype], kv.n_pages, kv.page_size, kv.n_kv_heads, kv.head_dim,
                                       kv.scale_block, self.max_seqs, self.max_pages, all(p % 16 == 0 for p in pools))
         self._ref = ctypes.addressof(self.desc)
+        self._stream = _raw_stream(self.device.index)
+        self._memory = [t for t in (self.table, self.lengths, self.holders, self.missing, self._workspace, self._pools, self._scales)
+                        if t is not None]
 
     def _run(self, fn, *args):
         for lease in self._leases:
             lease.check()
         _call(fn, self.device, self._ref, *args)
+        if _raw_stream(self.device.index) != self._stream:
+            # (the pool's memory is given back only after the calls on this stream)
+            stream = torch.cuda.current_stream(self.device)
+            for t in self._memory:
+                t.record_stream(stream)
         return self
 
     def _give(self, fn, *args):

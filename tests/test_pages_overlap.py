@@ -54,6 +54,7 @@ def _engine_pool(monkeypatch, nkv):
         raise _Reached
     monkeypatch.setattr(paged.PagedKV, '__init__', init)
     monkeypatch.setattr(pages, '_call', reached)
+    monkeypatch.setattr(pages, '_raw_stream', lambda device: 0)
     eng = Qwen2Engine.__new__(Qwen2Engine)
     eng.device, eng.n_layers, eng.n_kv_heads, eng.head_dim = torch.device('cpu'), 2, nkv, HD
     eng._pool_n, eng._pool_slots, eng._epoch, eng._pool_generation, eng._live = 2, SLOTS, 0, 1, weakref.WeakValueDictionary()
