@@ -415,11 +415,13 @@ int sp_op_rotate(const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t
  * sp_op_paged_append writes: within 2^-60 .. 2^60 (0, of memory that was cleared and never appended to, counts as 2^-60). */
 typedef struct sp_paged_kv {
     void *k_dev, *v_dev;
-    float *k_scale_dev, *v_scale_dev;         /* device [n_kv_heads], or [n_pages][n_kv_heads][page_size / scale_block]; NULL for 16 bits */
+    /* device [n_kv_heads], or [n_pages][n_kv_heads][page_size / scale_block]; NULL for 16 bits.  Read only, except that with scale_block
+     * sp_op_paged_append writes them: the memory is the caller's to have writable. */
+    const float *k_scale_dev, *v_scale_dev;
     int64_t page_stride, head_stride, row_stride;
     int32_t dtype;                            /* SP_DT_F16, SP_DT_BF16, SP_DT_E4M3, or SP_DT_I8 (with scale_block) */
     int32_t n_pages, page_size, n_kv_heads, head_dim;
-    int32_t scale_block;                      /* 0, or a multiple of 16 up to 128 that divides page_size */
+    int32_t scale_block;                      /* 0, or a multiple of 16 up to 128 that divides page_size (once reserved0: clear it) */
 } sp_paged_kv;
 
 /* Appends n_rows new tokens: row r's keys (rotated at pos_dev[r] unless rotary is NULL) and values go to position at_dev[r] of

@@ -135,7 +135,7 @@ Span scales_of(const sp_paged_kv *kv, const float *p) {
 void append_blocks(const sp_paged_kv *kv, AppendArgs &a, int dtype, bool wide, hipStream_t st) {
     BlockAppendArgs b{};
     (AppendArgs &)b = a;
-    b.kscale = kv->k_scale_dev; b.vscale = kv->v_scale_dev;
+    b.kscale = const_cast<float *>(kv->k_scale_dev); b.vscale = const_cast<float *>(kv->v_scale_dev);      // (written with scale_block alone)
     b.block = kv->scale_block; b.per_page = kv->page_size / kv->scale_block;
     b.by_block = PageDivisor(b.block); b.by_page = PageDivisor(kv->page_size);
     b.by_key = PageDivisor(a.units + a.tail); b.by_value = PageDivisor(a.vecs);
