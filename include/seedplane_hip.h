@@ -439,7 +439,8 @@ typedef struct sp_paged_kv {
  * Magnitudes above 2^60 codes saturate; a NaN makes an int8 block's scale NaN until it begins anew, e4m3 keeps it to its place.
  * Here scale_block * rot_dim is at most 16384, scale_block * head_dim below 65536 and max_pages * page_size at most 2^30.  Each block's
  * rows are looked for among all of the call's (8 bytes a row): tens of thousands of rows are better given in several calls, each of whole
- * blocks. */
+ * blocks, more than 4096 with a sequence's rows side by side (in order of time they take several times as long), and a prompt with a table of its
+ * own sequences' rows (n_seq says how many blocks a call is likely to write). */
 int sp_op_paged_append(const sp_paged_kv *kv, const sp_rotary *rotary, int32_t dtype, int32_t n_rows, int32_t n_heads,
                        const void *q_dev, int64_t q_row, int64_t q_head, const void *k_dev, int64_t k_row, int64_t k_head,
                        const void *v_dev, int64_t v_row, int64_t v_head, const int32_t *pos_dev, const int32_t *seq_dev,

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(THREADS) k_beam_rows(Args a) {
     // too few, n threads of one wave.
     const int waves = min(hi - lo, CHUNK) / (64 * VALUES);
     float bv = -INFINITY;
-    if (waves > 0) {                                                   // (a part of fewer fits into the buffer as it is)
+    if (waves > 0) {                                                   // (a part of fewer, 511 values at most, is listed whole: past 256 see below)
         float w = nth_of_wave(m, (a.n + waves - 1) / waves);
         if (lane == 0) sh.border[wv] = w;
         __syncthreads();
@@ -296,7 +296,9 @@ struct MergeShared {
 // or above a value, n totals are.  The largest such value is the border, and few more than n pass it, whether all beams are about as good or one
 // has nearly all of the best (by the lists' first totals alone: 32 x 16 beams, n 32, 146 us instead of 9; 64 beams, n 64, 173 instead of 23).
 // Rows of many parts spread their best over many lists: then the first totals are enough, of which each wave has an eighth (1 x 8 beams,
-// n 16, 64 parts: 6.2 us instead of 8.1; at most n n totals pass, hence not for large n).
+// n 16, 64 parts: 6.2 us instead of 8.1).  The least of the waves' borders counts, so lists of other waves may pass beyond the n best; where a
+// wave's parts are all masked every list does, with n totals each, which come to the buffer by turns (1 beam of 64 parts, n 16, every eighth
+// masked: 11.9 us, none 5.5), hence not for large n.
 __global__ void __launch_bounds__(MERGE_THREADS) k_beam_merge(Args a) {
     __shared__ MergeShared sh;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;

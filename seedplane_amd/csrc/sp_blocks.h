@@ -6,9 +6,10 @@
 // holds, its scale only grows, and where it does the codes that the call does not write are rounded once more, by old / new scale.
 //
 // What bounds it: a step is a chain of dependent accesses (row, table entry beside the search, values, scale, codes): 16 rows of 12 / 2 / 2
-// heads of 128 take 6.0 us, their reading back 3.5, where an empty launch takes 2.3; a prompt of 1777 rows of 28 / 4 / 4 heads, 26 MB of
-// values, takes 15 us, most of it the queries' rows, which the plain append's loop rotates (sp_rotate.h says what bounds that); its
-// reading back 4.4 (14 MB).
+// heads of 128 take 6.1 us, their reading back 3.6, where an empty launch takes 2.3; a prompt of 1777 rows of 28 / 4 / 4 heads, 26 MB of
+// values, takes 15.2 us, 13.3 of them without queries: the blocks' chains (the search of all rows, angles, which the workgroups of a block's single
+// heads form each for itself, largest magnitudes, codes, with barriers between), beside which the queries' rows run, one a workgroup (rotated alone
+// they take 5.8); its reading back 4.5 (14 MB).
 //
 // A workgroup takes a chunk of rows of the call (a row whose block an earlier row has is left to that row's workgroup), keys or
 // values, and some heads: it looks up its block's rows among all of the call's, lists the slots that have one, takes the largest magnitude per
@@ -16,9 +17,11 @@
 // more than without the list).
 // Values are read twice unless a thread has but one item of them: a block of 64 positions of one head alone is 8192 values.  Long
 // calls (FIND) look up the rows of all a chunk's blocks at once.  They are bound by the blocks' chains of barriers (16384 rows of 28 / 4 / 4
-// heads 80 us, 45 of them without queries, where the bytes take 56 and 10), so their registers are held to those of 6 waves: with 5
+// heads 79 us, 38 of them without queries, where the bytes take 56 and 10), so their registers are held to those of 6 waves: with 5
 // waves the blocks gain less than the queries' rows behind them lose (83).  Keys and values have loops of their own: one for both
 // had more uniform values than scalar registers hold (16 rows 7.0 us instead of 6.0, 16384 89 instead of 78).
+// Rows in order of time put more rows between a chunk's blocks than MOST_FOUND, and every run of a block's rows, here single rows, searches all
+// of them: 8192 rows of 4 sequences 74 us on blocks of 16 and 99 of 32 (by sequence 37, 35), of 64 sequences 200, 587, of 128 1740 (73).
 #pragma once
 #include "sp_paged.h"
 

@@ -141,7 +141,9 @@ void append_blocks(const sp_paged_kv *kv, AppendArgs &a, int dtype, bool wide, h
     b.by_key = PageDivisor(a.units + a.tail); b.by_value = PageDivisor(a.vecs);
     // Blocks that the call is likely to write: of many sequences (a step) one each, else its rows side by side.  Where there is one for every
     // other row a workgroup looks at one row, else at several, most of which follow one of the same block; heads are split while the
-    // blocks are too few to fill the chip.  (A step of 1024 sequences, 28 / 4 heads of 128: 14.8 us a call; by 4 rows and single heads twice that.)
+    // blocks are too few to fill the chip.  (A step of 1024 sequences, 28 / 4 heads of 128: 14.2 us a call; by 4 rows and single heads twice that.)
+    // The host knows a call's sequences only by the table's height, so that a prompt beside a tall table is laid out as a step: 1777 rows of one
+    // sequence 47 us with a table of 1024, 14.6 with its own row; 300 rows 20 and 13.
     // More than 4096 rows: the search of all rows for each block comes to count, so that a workgroup takes several blocks with one search
     // (131072 rows of 16 sequences 595 us, by single searches 1154; 8192 38 and 40; 1777 18 and 14).
     const int runs = std::max(1, std::min(a.rows, std::max(a.rows / b.block, a.n_seq)));
