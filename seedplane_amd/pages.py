@@ -58,19 +58,21 @@ class PagePool:
                                       *kv._strides(), len(pools), _DTYPES[kv.dtype], kv.n_pages, kv.page_size, kv.n_kv_heads, kv.head_dim,
                                       kv.scale_block, self.max_seqs, self.max_pages, all(p % 16 == 0 for p in pools))
         self._ref = ctypes.addressof(self.desc)
-        self._stream = _raw_stream(self.device.index)
+        self._streams = {_raw_stream(self.device.index)}       # that the pool's memory is noted for
         self._memory = [t for t in (self.table, self.lengths, self.holders, self.missing, self._workspace, self._pools, self._scales)
                         if t is not None]
 
     def _run(self, fn, *args):
         for lease in self._leases:
             lease.check()
-        _call(fn, self.device, self._ref, *args)
-        if _raw_stream(self.device.index) != self._stream:
-            # (the pool's memory is given back only after the calls on this stream)
+        raw = _raw_stream(self.device.index)
+        if raw not in self._streams:
+            # (given back only after the calls on this stream; a tensor keeps its streams for good)
             stream = torch.cuda.current_stream(self.device)
             for t in self._memory:
                 t.record_stream(stream)
+            self._streams.add(raw)
+        _call(fn, self.device, self._ref, *args)
         return self
 
     def _give(self, fn, *args):

@@ -23,14 +23,16 @@ def test_memory_is_noted_for_the_stream_of_a_call(monkeypatch):
     calls = [lambda: pool.fork(ints(0, 1, 2)), lambda: pool.grow(ints(1, 1, 1)), lambda: pool.free(ints(0)), lambda: pool.compact(),
              lambda: pool.copy(ints(0), ints(1))]
     own = {t.data_ptr() for t in (pool.table, pool.lengths, pool.holders, pool.missing, pool._workspace, pool._pools, pool._scales)}
-    for call in calls:
+    for i, call in enumerate(calls):
         now[0] = 7
         call()
         assert not noted
-        now[0] = 8
+        now[0] = 8 + i
         call()
-        assert own <= {p for p, s in noted if s == 'stream 8'}
+        assert own <= {p for p, s in noted if s == f'stream {8 + i}'}
         noted.clear()
+        call()                                               # (once is enough)
+        assert not noted
 
 
 @pytest.mark.gpu
