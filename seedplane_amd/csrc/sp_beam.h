@@ -3,9 +3,9 @@
 // A beam's order of continuations is its logits' order, so the softmax's sum is needed only to compare beams: one pass over the logits
 // takes the maximum, the sum of exponentials and the n best of a part of a row together (k_beam_rows), and a second, small launch
 // forms the sums' logarithms, compares totals in 64 bits and writes the results in order (k_beam_merge).  Ties go to the lowest beam,
-// then token.  The sums of a part are held in 32 bits, some V / 2048 + 40 terms after each other, off by 2^-24 of the sum each at most: the same
-// for all continuations of a beam, so that only beams whose totals lie closer than that may change places (64 bits would be two instructions
-// at a quarter of the rate for each logit).
+// then token.  The sums of a part are held in 32 bits, at most V / 1024 + 40 terms after each other, off by 2^-24 of the sum each at most: the
+// same for all continuations of a beam, so that only beams whose totals lie closer than that may change places (64 bits would be a conversion and
+// a 64-bit sum more for each logit).
 //
 // The n best of a part: each thread streams its values, keeping their largest beside the sum.  The largest of all threads give a border
 // that at least n values reach and few others (each of 4 waves has ceil(n / 4) threads at or above it: about 2 n values of a part);
